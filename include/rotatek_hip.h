@@ -500,6 +500,102 @@ int rk_spark_recover(const rk_tensor* k_prompt, const rk_tensor* k_pruned,
 int rk_channel_selection(const rk_tensor* keep_mask, const rk_tensor* R_out,
                          void* stream);
 
+/* ---- quantised rows of a KV cache (no counterpart in the reference, which
+ * stores the Keys and Values in the model's dtype).
+ *
+ * A row of D channels (1 <= D <= 128) is cut into blocks of 32, the last one
+ * filled up with zeros: W = 32 ceil(D / 32) channels are stored.  A block is
+ * a power of two 2^e and 32 element codes (a microscaling block):
+ *   e    = the smallest exponent that brings the block's largest magnitude to
+ *          at most the element type's largest value (RK_ROWS_MX8: e4m3, 448;
+ *          RK_ROWS_MX4: e2m1, 6), within -127 .. 127; an all-zero block has -127;
+ *   code = element(x 2^-e), rounded to nearest, ties to even.
+ * No value saturates, so every code is within half a step of x 2^-e (one that
+ * rounds up to 2^128 reads back as an infinity).  A block that holds an
+ * infinity or a NaN reads back as NaN.
+ *   codes  U8 [B,H,S,W] (RK_ROWS_MX4: [B,H,S,W/2], the even channel in the low
+ *          nibble); unit last stride, 16-byte aligned base and strides.
+ *   scales U8 [B,H,W/32,S'], S' >= 32 ceil(S / 32): e + 127, or 255 for NaN;
+ *          unit last stride, 8-byte aligned base and strides.  Block-major, so
+ *          that one load brings a block column's scales of eight tokens; the
+ *          bytes past S are padding, read and ignored. */
+typedef enum rk_rows_format {
+  RK_ROWS_PLAIN = 0, /* data [B,H,S,D] F16/BF16, no scales (attention only) */
+  RK_ROWS_MX8 = 1,   /* e4m3 codes, 33/32 bytes a channel */
+  RK_ROWS_MX4 = 2    /* e2m1 codes, 17/32 bytes a channel */
+} rk_rows_format;
+
+typedef struct rk_rows {
+  rk_tensor data;   /* codes as above, or plain rows */
+  rk_tensor scales; /* ignored for plain rows */
+  int64_t head_dim; /* D */
+  int32_t format;   /* rk_rows_format */
+} rk_rows;
+
+/* rows[b,h,t] = quantised x[b,h,t]; x [B,H,S,D] F16/BF16/F32, any strides. */
+int rk_mx_write(const rk_tensor* x, const rk_rows* rows, void* stream);
+
+/* The inverse: out [B,H,S,D] F16/BF16/F32 (any strides), each value code 2^e
+ * rounded once to out's dtype. */
+int rk_mx_read(const rk_rows* rows, const rk_tensor* out, void* stream);
+
+/* Append to a cache of quantised rows: k_new / v_new [B,H,T,D] are written to
+ * rows lens[b] .. lens[b] + T - 1 of k_rows / v_rows (lens: device int32 [B]);
+ * tokens past the capacity are dropped, and no other row is touched.  With
+ * `advance` lens[b] becomes min(lens[b] + T, capacity); without it the lengths
+ * stay (drafted tokens, counted once they are accepted).  v_new and v_rows may
+ * both be NULL.  K and V may differ in head_dim, not in format. */
+int rk_mx_append(const rk_tensor* k_new, const rk_tensor* v_new, const rk_rows* k_rows,
+                 const rk_rows* v_rows, int32_t* lens, int32_t advance, void* stream);
+
+/* RotateK or dense decode over quantised rows (the attention of
+ * rk_rotatek_decode, with the length and mask of rk_rotatek_decode_varlen):
+ * q [B,H_q,D] F16/BF16/F32; k_full, v_full [B,H_kv,S_f,*] and k_sparse,
+ * v_sparse [B,H_kv,S_v,*] quantised rows of one format, head_dim D (k_sparse:
+ * Dk); R_partial [B,H_kv,D,Dk], delta_mu [B,H_kv,D] or NULL in F16/BF16/F32.
+ * k_sparse, v_sparse and R_partial may all be NULL: the dense decode.
+ * mask_full [B,S_f] U8 or NULL; len_full device int32 [B] or NULL: only rows
+ * t < len_full[b] with mask_full[b,t] != 0 are attended; what the others hold
+ * (NaN too) does not matter.  out [B,H_q,D] in q's dtype; a row with nothing
+ * to attend is zero.
+ *   out = sum w v / (sum w + 1e-6),  w = exp(s - max s)
+ * The workspace (size from the _check variant, 256-byte aligned) needs no
+ * initialisation and holds nothing between calls; calls that overlap need one
+ * each.  Launches on `stream` only, and hipGraph-capturable: lengths are read
+ * on the device, the split depends on sizes alone. */
+int rk_quantized_decode_check(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
+                              const rk_rows* k_full, const rk_rows* v_full, const rk_tensor* mask_full,
+                              const rk_rows* k_sparse, const rk_rows* v_sparse, int64_t num_kv_groups,
+                              const rk_tensor* out, int32_t num_cus, size_t* workspace_bytes);
+int rk_quantized_decode(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
+                        const rk_rows* k_full, const rk_rows* v_full, const rk_tensor* mask_full,
+                        const int32_t* len_full, const rk_rows* k_sparse, const rk_rows* v_sparse,
+                        int64_t num_kv_groups, const rk_tensor* out, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Decode of a batch whose requests share a prompt and an image: the same
+ * attention over
+ *   k_prefix, v_prefix [1,H_kv,S_p,D]   full-width rows of every request,
+ *   k_sparse, v_sparse [1,H_kv,S_v,*]   the rotated span of every request, with
+ *                                       R_partial [1,H_kv,D,Dk] and delta_mu
+ *                                       [1,H_kv,D] (all NULL: none),
+ *   k_suffix, v_suffix [B,H_kv,S_s,D]   each request's own rows (both NULL:
+ *                                       none), t < len_suffix[b] (device int32
+ *                                       [B] or NULL) attended.
+ * The shared rows are read once for all the batch's queries (once per 64 on a
+ * KV head).  All rows are of one format: plain in q's dtype (F16, BF16; any
+ * strides), or quantised (q F16/BF16/F32).  Workspace and capture as above. */
+int rk_shared_prefix_decode_check(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
+                                  const rk_rows* k_prefix, const rk_rows* v_prefix, const rk_rows* k_sparse,
+                                  const rk_rows* v_sparse, const rk_rows* k_suffix, const rk_rows* v_suffix,
+                                  int64_t num_kv_groups, const rk_tensor* out, int32_t num_cus,
+                                  size_t* workspace_bytes);
+int rk_shared_prefix_decode(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
+                            const rk_rows* k_prefix, const rk_rows* v_prefix, const rk_rows* k_sparse,
+                            const rk_rows* v_sparse, const rk_rows* k_suffix, const rk_rows* v_suffix,
+                            const int32_t* len_suffix, int64_t num_kv_groups, const rk_tensor* out,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,7 @@ LIB_PATH = os.path.join(HERE, "librotatek_hip.so")
 
 RK_F16, RK_BF16, RK_F32, RK_F64, RK_U8, RK_I32, RK_I64 = range(7)
 RK_POLICY_PAPER, RK_POLICY_GQA = 0, 1
+RK_ROWS_PLAIN, RK_ROWS_MX8, RK_ROWS_MX4 = range(3)
 # rk_status (include/rotatek_hip.h)
 (RK_OK, RK_ERR_NULL, RK_ERR_RANK, RK_ERR_DTYPE, RK_ERR_SHAPE, RK_ERR_HEADS, RK_ERR_HEAD_DIM, RK_ERR_KEEP_DIM,
  RK_ERR_STRIDE, RK_ERR_WORKSPACE, RK_ERR_ARG, RK_ERR_HIP, RK_ERR_NO_DEVICE,
@@ -50,6 +51,15 @@ class RkTensor(ctypes.Structure):
     ]
 
 
+class RkRows(ctypes.Structure):
+    _fields_ = [
+        ("data", RkTensor),
+        ("scales", RkTensor),
+        ("head_dim", ctypes.c_int64),
+        ("format", ctypes.c_int32),
+    ]
+
+
 class RkDecodePlan(ctypes.Structure):
     _fields_ = [
         ("units", ctypes.c_int64),
@@ -69,6 +79,7 @@ class RkDecodePlan(ctypes.Structure):
 
 
 _P = ctypes.POINTER(RkTensor)
+_W = ctypes.POINTER(RkRows)
 _SIGNATURES = {
     "rk_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "rk_abi_version": (ctypes.c_int, []),
@@ -131,6 +142,17 @@ _SIGNATURES = {
     "rk_spark_recover_check": (ctypes.c_int, [_P, _P, _P, _P, _P, _P]),
     "rk_spark_recover": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, ctypes.c_void_p]),
     "rk_channel_selection": (ctypes.c_int, [_P, _P, ctypes.c_void_p]),
+    "rk_mx_write": (ctypes.c_int, [_P, _W, ctypes.c_void_p]),
+    "rk_mx_read": (ctypes.c_int, [_W, _P, ctypes.c_void_p]),
+    "rk_mx_append": (ctypes.c_int, [_P, _P, _W, _W, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]),
+    "rk_quantized_decode_check": (ctypes.c_int, [_P, _P, _P, _W, _W, _P, _W, _W, ctypes.c_int64, _P, ctypes.c_int32,
+                                                 ctypes.POINTER(ctypes.c_size_t)]),
+    "rk_quantized_decode": (ctypes.c_int, [_P, _P, _P, _W, _W, _P, ctypes.c_void_p, _W, _W, ctypes.c_int64, _P,
+                                           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "rk_shared_prefix_decode_check": (ctypes.c_int, [_P, _P, _P, _W, _W, _W, _W, _W, _W, ctypes.c_int64, _P,
+                                                     ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
+    "rk_shared_prefix_decode": (ctypes.c_int, [_P, _P, _P, _W, _W, _W, _W, _W, _W, ctypes.c_void_p, ctypes.c_int64,
+                                               _P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
 }
 
 _lib = None
@@ -200,6 +222,28 @@ def desc(t: torch.Tensor | None):
     pad = _PAD[4 - nd]
     return RkTensor.from_buffer_copy(_RK_TENSOR.pack(t.data_ptr() if t.numel() > 0 else 0, code, nd,
                                                      *t.shape, *pad, *t.stride(), *pad))
+
+
+_NO_TENSOR = _RK_TENSOR.pack(0, 0, 0, *([0] * 8))
+_RK_ROWS_TAIL = struct.Struct("=qii")
+
+
+def _pack(t: torch.Tensor) -> bytes:
+    nd = t.dim()
+    if nd > 4:
+        raise ValueError("tensors of rank > 4 are not supported")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {t.dtype}")
+    pad = _PAD[4 - nd]
+    return _RK_TENSOR.pack(t.data_ptr() if t.numel() > 0 else 0, code, nd, *t.shape, *pad, *t.stride(), *pad)
+
+
+def rows_desc(data: torch.Tensor, scales: torch.Tensor | None, head_dim: int, fmt: int) -> RkRows:
+    """rk_rows descriptor of quantised rows, or of plain ones (``scales``
+    None)."""
+    return RkRows.from_buffer_copy(_pack(data) + (_NO_TENSOR if scales is None else _pack(scales))
+                                   + _RK_ROWS_TAIL.pack(head_dim, fmt, 0))
 
 
 def ref(d):

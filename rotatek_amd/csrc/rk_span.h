@@ -1,0 +1,71 @@
+// rk_span.h -- one token's attention over spans of plain or quantised rows:
+// the argument block and launch geometry that the host code (rk_span.hip) and
+// the per-format kernel units (rk_span_{f16,bf16,mx8,mx4}.hip) share.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace rk {
+
+// One span of rows: K scores, V values, [B?, H_kv, S, *].  Strides in bytes
+// for quantised rows, in elements for plain ones.
+struct Span {
+  const void* k;
+  const void* v;
+  const uint8_t* ksc;  // scales [B?, H_kv, blocks, S'] of quantised rows
+  const uint8_t* vsc;
+  const int32_t* len;   // rows t < len[b] count (optional)
+  const uint8_t* mask;  // rows with mask[b, t] != 0 count (optional)
+  int64_t k_sb, k_sh, v_sb, v_sh;
+  int64_t ksc_sb, ksc_sh, vsc_sb, vsc_sh;
+  int64_t m_sb, m_ss;
+  uint32_t k_ss, k_sd, v_ss, v_sd;  // within a head: < 2^31 in all
+  uint32_t ksc_sn, vsc_sn;
+  int32_t S, chunk;  // tokens; tokens per workgroup
+  int32_t wgs;       // workgroups of a unit
+  int32_t np0;       // record number of the unit's first workgroup
+  int32_t width;     // stored channels of a score row (a multiple of 32, or D)
+};
+
+// Spans by what their rows score with.
+enum { kRotated = 0, kFull = 1, kTail = 2, kSpans = 3 };
+
+struct SpanArgs {
+  Span span[kSpans];
+  // units: (b, kv, row block) or, where the batch shares the span's rows,
+  // (kv, row block over the batch's queries)
+  int32_t units[kSpans], blocks[kSpans];
+  int32_t first[kSpans + 1];  // first workgroup of each span
+  const void* q;
+  void* out;
+  const uint16_t* qr;  // rotated queries in terms [row][terms][Dkp], 16 bits
+  const float* bias;   // q . delta_mu per row
+  float* acc;          // [row][np][DV] partial sums
+  float* ml;           // [row][np][2] running maximum and sum
+  int64_t q_sb, q_sh, q_sd, o_sb, o_sh, o_sd;
+  int32_t B, Hq, H, G, D, Dk, Dkp, np, shared;
+  int32_t q_dtype, o_dtype;
+  float scale_log2;  // log2(e) / sqrt(D)
+  // preparation of the rotated span's queries
+  const void* R;
+  const void* dm;
+  uint16_t* qr_w;
+  float* bias_w;
+  int64_t R_sb, R_sh, R_sd, R_sk, dm_sb, dm_sh, dm_sd;
+  int32_t r_dtype, dm_dtype, terms;
+};
+
+constexpr int kSpanThreads = 256;
+constexpr int kSpanWaves = 4;
+constexpr int kSpanBlk = 32;  // tokens of a wave's step
+
+// The split launch: kv = score blocks of 32 channels of the rotated span (0:
+// none, 1, 2 or 4), kf the full-width spans' (2: D <= 64, or 4), nr = blocks
+// of 16 queries per unit, terms = 16-bit terms that a query is exact in.
+hipError_t span_launch_f16(int kv, int kf, int nr, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_launch_bf16(int kv, int kf, int nr, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_launch_mx8(int kv, int kf, int nr, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_launch_mx4(int kv, int kf, int nr, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
+
+}  // namespace rk

@@ -1,0 +1,496 @@
+// rk_span.hip -- host side of the attention over quantised and shared spans
+// (rk_quantized_decode, rk_shared_prefix_decode of rotatek_hip.h): validation,
+// the split plan, and the two small kernels around the split launch
+// (rk_span_dev.h): the rotated span's queries before it, the join of a row's
+// partial sums after it.
+#include <hip/hip_runtime.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "rk_common.h"
+#include "rk_host.h"
+#include "rk_mx.h"
+#include "rk_span.h"
+#include "rotatek_hip.h"
+
+namespace {
+
+using rk::kFull;
+using rk::kRotated;
+using rk::kSpans;
+using rk::kTail;
+using rk::Span;
+using rk::SpanArgs;
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
+
+// ---------------------------------------------------------------- kernels
+
+// q R_partial and q . delta_mu of one query row per workgroup, fp32 sums; q R
+// is stored as a sum of `terms` 16-bit values (two hold 16 or more bits of it,
+// three an fp32's 24).
+template <class TT>
+__global__ void __launch_bounds__(128) span_queries_kernel(const SpanArgs a) {
+  __shared__ float s_q[128];
+  __shared__ float s_b[2];
+  const int c = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const int64_t b = row / a.Hq, h = row - b * a.Hq, kv = h / a.G, rb = a.shared ? 0 : b;
+  s_q[c] = c < a.D ? rk::load_any(a.q, b * a.q_sb + h * a.q_sh + c * a.q_sd, a.q_dtype) : 0.f;
+  __syncthreads();
+  if (c < a.Dkp) {
+    float v = 0.f;
+    if (c < a.Dk) {
+      const int64_t off = rb * a.R_sb + kv * a.R_sh + c * a.R_sk;
+      for (int d = 0; d < a.D; d += 16) {
+        float r[16];
+        rk::load_any_rows<16>(a.R, off, a.R_sd, a.r_dtype, d, a.D, r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (d + i < a.D) v = fmaf(s_q[d + i], r[i], v);
+      }
+    }
+    for (int t = 0; t < a.terms; ++t) {
+      const uint16_t w = TT::from_f32(v);
+      a.qr_w[(row * a.terms + t) * a.Dkp + c] = w;
+      v -= TT::to_f32(w);
+    }
+  }
+  float p = 0.f;
+  if (a.dm && c < a.D) p = s_q[c] * rk::load_any(a.dm, rb * a.dm_sb + kv * a.dm_sh + c * a.dm_sd, a.dm_dtype);
+  for (int d = 32; d; d >>= 1) p += rk::shfl_xor(p, d);
+  if ((c & 63) == 0) s_b[c >> 6] = p;
+  __syncthreads();
+  if (c == 0) a.bias_w[row] = s_b[0] + s_b[1];
+}
+
+// Joins a row's records: out = sum_p acc_p 2^(m_p - M) / (sum_p l_p 2^(m_p -
+// M) + 1e-6).  A wave per row: four groups of 16 lanes (DV / 16 channels a
+// lane) take every fourth record and are combined by lane exchange.
+template <int DV>
+__global__ void __launch_bounds__(256) span_merge_kernel(const SpanArgs a) {
+  constexpr int C = DV / 16;
+  const int lane = threadIdx.x & 63, s = lane >> 4, n = lane & 15;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.B * a.Hq) return;
+  const float* acc = a.acc + row * a.np * DV + n * C;
+  const float2* ml = (const float2*)a.ml + row * a.np;
+  float M = rk::kNegInit;
+  for (int p = lane; p < a.np; p += 64) M = fmaxf(M, ml[p].x);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, rk::shfl_xor(M, d));
+  float L = 0.f, A[C];
+#pragma unroll
+  for (int e = 0; e < C; ++e) A[e] = 0.f;
+  for (int p = s; p < a.np; p += 4) {
+    const float2 r = ml[p];
+    const float w = rk::fast_exp2(r.x - M);
+    L += r.y * w;
+#pragma unroll
+    for (int e = 0; e < C; e += 4) {
+      const float4 v = *(const float4*)(acc + (int64_t)p * DV + e);
+      A[e] += v.x * w; A[e + 1] += v.y * w; A[e + 2] += v.z * w; A[e + 3] += v.w * w;
+    }
+  }
+#pragma unroll
+  for (int d = 16; d < 64; d <<= 1) {
+    L += rk::shfl_xor(L, d);
+#pragma unroll
+    for (int e = 0; e < C; ++e) A[e] += rk::shfl_xor(A[e], d);
+  }
+  if (s != 0) return;
+  const int64_t b = row / a.Hq, h = row - b * a.Hq;
+  const int64_t off = b * a.o_sb + h * a.o_sh;
+  const float den = L + rk::kDenomEps;
+#pragma unroll
+  for (int e = 0; e < C; ++e) {
+    const int c = n * C + e;
+    if (c >= a.D) break;
+    const float v = A[e] / den;
+    const int64_t at = off + c * a.o_sd;
+    if (a.o_dtype == RK_F32)
+      ((float*)a.out)[at] = v;
+    else
+      ((uint16_t*)a.out)[at] = a.o_dtype == RK_F16 ? rk::F16::from_f32(v) : rk::BF16::from_f32(v);
+  }
+}
+
+// No tokens at all, or rotated rows without channels: what the kernels read
+// in their place is zero.
+__global__ void __launch_bounds__(256) span_zero_kernel(uint32_t* p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0u;
+}
+
+// ------------------------------------------------------------------- host
+
+// One call as the entry points give it; pairs may be null.
+struct Call {
+  const rk_tensor *q, *R, *dm, *mask, *out;
+  const rk_rows* k[kSpans];
+  const rk_rows* v[kSpans];
+  const int32_t* len[kSpans];
+  int64_t groups;
+  bool shared;
+};
+
+struct Plan {
+  int64_t B, Hq, H, G, D, Dk;
+  int format, kv, kf, nr, terms, rterms;  // terms of a query, of a rotated one
+  bool vec;
+  int64_t S[kSpans], chunk[kSpans], wgs[kSpans], units[kSpans], blocks[kSpans], np, grid, rows;
+  size_t qr, bias, zero, zero_bytes, acc, ml, total;
+};
+
+bool mx(const rk_rows* r) { return r->format != RK_ROWS_PLAIN; }
+
+// Rows of one span: shape [N, H, S, dim], one format and, if plain, q's dtype.
+int check_rows(const rk_rows* r, int format, int dtype, int64_t N, int64_t H, int64_t S, int64_t dim) {
+  if (!r) return RK_ERR_NULL;
+  if (r->format != format) return RK_ERR_DTYPE;
+  if (mx(r)) {
+    const int st = rk::check_mx(r);
+    if (st) return st;
+    if (r->head_dim != dim) return RK_ERR_SHAPE;
+  } else {
+    const int st = rk::check_desc(&r->data, 4);
+    if (st) return st;
+    if (r->data.dtype != dtype) return RK_ERR_DTYPE;
+    if (r->data.shape[3] != dim || r->head_dim != dim) return RK_ERR_SHAPE;
+    // 32-bit offsets inside a head
+    if ((S + 64) * r->data.stride[2] + dim * r->data.stride[3] >= (INT64_C(1) << 31)) return RK_ERR_STRIDE;
+  }
+  if (r->data.shape[0] != N || r->data.shape[1] != H || r->data.shape[2] != S) return RK_ERR_SHAPE;
+  return RK_OK;
+}
+
+int check_float(const rk_tensor* t, int ndim) {
+  const int st = rk::check_desc(t, ndim);
+  if (st) return st;
+  return rk::is_float_param(t->dtype) ? RK_OK : RK_ERR_DTYPE;
+}
+
+int make_plan(const Call& c, int cus, Plan* out) {
+  Plan p;
+  memset(&p, 0, sizeof(p));
+  int st = check_float(c.q, 3);
+  if (st) return st;
+  if (!c.k[kFull] || !c.v[kFull]) return RK_ERR_NULL;
+  p.B = c.q->shape[0];
+  p.Hq = c.q->shape[1];
+  p.D = c.q->shape[2];
+  if (p.D < 1 || p.D > 128) return RK_ERR_HEAD_DIM;
+  if (c.groups <= 0) return RK_ERR_ARG;
+  p.G = c.groups;
+  p.H = c.k[kFull]->data.ndim == 4 ? c.k[kFull]->data.shape[1] : 0;
+  if (p.H <= 0 || p.Hq != p.H * p.G) return RK_ERR_HEADS;
+  p.format = c.k[kFull]->format;
+  if (p.format != RK_ROWS_PLAIN && p.format != RK_ROWS_MX8 && p.format != RK_ROWS_MX4) return RK_ERR_ARG;
+  const bool quantised = p.format != RK_ROWS_PLAIN;
+  if (!quantised && (!c.shared || !rk::is_half(c.q->dtype))) return RK_ERR_DTYPE;
+  const int64_t N = c.shared ? 1 : p.B;
+  bool have[kSpans];
+  for (int i = 0; i < kSpans; ++i) {
+    have[i] = c.k[i] != nullptr;
+    if (have[i] != (c.v[i] != nullptr)) return RK_ERR_NULL;
+    if (have[i] && c.k[i]->data.ndim != 4) return RK_ERR_RANK;
+    p.S[i] = have[i] ? c.k[i]->data.shape[2] : 0;
+  }
+  if (have[kRotated]) {
+    if (!c.R) return RK_ERR_NULL;
+    if ((st = check_float(c.R, 4))) return st;
+    p.Dk = c.R->shape[3];
+    if (p.Dk < 0 || p.Dk > p.D) return RK_ERR_KEEP_DIM;
+    if (c.R->shape[0] != N || c.R->shape[1] != p.H || c.R->shape[2] != p.D) return RK_ERR_SHAPE;
+    if (c.dm) {
+      if ((st = check_float(c.dm, 3))) return st;
+      if (c.dm->shape[0] != N || c.dm->shape[1] != p.H || c.dm->shape[2] != p.D) return RK_ERR_SHAPE;
+    }
+  }
+  p.vec = true;
+  for (int i = 0; i < kSpans; ++i) {
+    if (!have[i]) continue;
+    const int64_t n = i == kTail ? p.B : N;
+    if ((st = check_rows(c.k[i], p.format, c.q->dtype, n, p.H, p.S[i], i == kRotated ? p.Dk : p.D))) return st;
+    if ((st = check_rows(c.v[i], p.format, c.q->dtype, n, p.H, p.S[i], p.D))) return st;
+    if (!quantised && p.S[i] > 0) {
+      const bool keys = i != kRotated || p.Dk > 0;
+      p.vec = p.vec && rk::vec_ok(&c.v[i]->data) && p.D % 8 == 0 &&
+              (!keys || (rk::vec_ok(&c.k[i]->data) && c.k[i]->data.shape[3] % 8 == 0));
+    }
+  }
+  if (c.mask) {
+    if ((st = rk::check_desc(c.mask, 2))) return st;
+    if (c.mask->dtype != RK_U8) return RK_ERR_DTYPE;
+    if (c.mask->shape[0] != p.B || c.mask->shape[1] != p.S[kFull]) return RK_ERR_SHAPE;
+  }
+  if (c.out) {
+    if ((st = rk::check_desc(c.out, 3))) return st;
+    if (c.out->dtype != c.q->dtype) return RK_ERR_DTYPE;
+    for (int i = 0; i < 3; ++i)
+      if (c.out->shape[i] != c.q->shape[i]) return RK_ERR_SHAPE;
+  }
+
+  p.kf = p.D <= 64 ? 2 : 4;
+  p.kv = p.S[kRotated] == 0 ? 0 : p.Dk <= 32 ? 1 : p.Dk <= 64 ? 2 : 4;
+  p.terms = quantised ? (c.q->dtype == RK_F32 ? 3 : 2) : 1;
+  p.rterms = std::max(p.terms, 2);
+  const int64_t rows = c.shared ? p.B * p.G : p.G;
+  // more than 16 queries on the same rows: 64 to a unit, for one read of K
+  // and V (element loads and fp32 queries stay at 16)
+  p.nr = rows > 16 && p.vec && p.terms < 3 ? 4 : 1;
+  p.rows = p.B * p.Hq;
+  const int64_t unit_rows = 16 * p.nr;
+  int64_t cost[kSpans], total = 0;  // channels read per token
+  for (int i = 0; i < kSpans; ++i) {
+    const bool per_request = !c.shared || i == kTail;
+    p.blocks[i] = cdiv(per_request ? p.G : p.B * p.G, unit_rows);
+    p.units[i] = p.H * p.blocks[i] * (per_request ? p.B : 1);
+    cost[i] = p.D + (i == kRotated ? p.Dk : p.D);
+    total += p.units[i] * p.S[i] * cost[i];
+  }
+  // equal shares of the channels to read for every workgroup of one round
+  const int64_t slots = (int64_t)cus * (p.nr > 1 ? 1 : 2);
+  const int64_t share = std::max<int64_t>(cdiv(total, slots), 1);
+  for (int i = 0; i < kSpans; ++i) {
+    if (p.S[i] == 0) continue;
+    p.chunk[i] = round_up(std::max<int64_t>(cdiv(share, cost[i]), 1), rk::kSpanWaves * rk::kSpanBlk);
+    p.wgs[i] = cdiv(p.S[i], p.chunk[i]);
+    p.np += p.wgs[i];
+    p.grid += p.wgs[i] * p.units[i];
+  }
+  if (p.grid >= (INT64_C(1) << 31) || p.rows >= (INT64_C(1) << 31) || p.rows * p.np >= (INT64_C(1) << 40))
+    return RK_ERR_SHAPE;
+  const int64_t dv = p.kf == 2 ? 64 : 128;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) & ~size_t(255);
+    return here;
+  };
+  p.qr = take(p.kv ? (size_t)p.rows * p.rterms * 32 * p.kv * 2 : 0);
+  p.bias = take(p.kv ? (size_t)p.rows * 4 : 0);
+  // rotated rows without channels: one zero row and its scales
+  p.zero_bytes = p.kv && p.Dk == 0 ? 256 + (size_t)round_up(p.S[kRotated], 32) : 0;
+  p.zero = take(p.zero_bytes);
+  p.acc = take((size_t)(p.rows * p.np) * dv * 4);
+  p.ml = take((size_t)(p.rows * p.np) * 8);
+  p.total = at;
+  *out = p;
+  return RK_OK;
+}
+
+int null_data(const Call& c, const Plan& p) {
+  if (!c.q->data || !c.out || !c.out->data) return RK_ERR_NULL;
+  for (int i = 0; i < kSpans; ++i) {
+    if (p.S[i] == 0) continue;
+    if (!c.v[i]->data.data || (p.format != RK_ROWS_PLAIN && !c.v[i]->scales.data)) return RK_ERR_NULL;
+    if (i == kRotated && p.Dk == 0) continue;
+    if (!c.k[i]->data.data || (p.format != RK_ROWS_PLAIN && !c.k[i]->scales.data)) return RK_ERR_NULL;
+  }
+  if (p.kv && p.Dk > 0 && !c.R->data) return RK_ERR_NULL;
+  if (p.kv && c.dm && !c.dm->data) return RK_ERR_NULL;
+  if (c.mask && p.S[kFull] > 0 && !c.mask->data) return RK_ERR_NULL;
+  return RK_OK;
+}
+
+Span make_span(const Call& c, const Plan& p, int i, char* ws) {
+  const rk_rows *k = c.k[i], *v = c.v[i];
+  Span s;
+  memset(&s, 0, sizeof(s));
+  const bool quantised = p.format != RK_ROWS_PLAIN;
+  s.v = v->data.data;
+  s.v_sb = v->data.stride[0]; s.v_sh = v->data.stride[1];
+  s.v_ss = (uint32_t)v->data.stride[2]; s.v_sd = (uint32_t)v->data.stride[3];
+  if (i == kRotated && p.Dk == 0) {
+    s.k = ws + p.zero;
+    s.ksc = (const uint8_t*)(ws + p.zero + 256);
+    s.k_sd = 1;
+  } else {
+    s.k = k->data.data;
+    s.k_sb = k->data.stride[0]; s.k_sh = k->data.stride[1];
+    s.k_ss = (uint32_t)k->data.stride[2]; s.k_sd = (uint32_t)k->data.stride[3];
+    s.width = (int32_t)(quantised ? rk::mx_width(k->head_dim) : k->head_dim);
+    if (quantised) {
+      s.ksc = (const uint8_t*)k->scales.data;
+      s.ksc_sb = k->scales.stride[0]; s.ksc_sh = k->scales.stride[1]; s.ksc_sn = (uint32_t)k->scales.stride[2];
+    }
+  }
+  if (quantised) {
+    s.vsc = (const uint8_t*)v->scales.data;
+    s.vsc_sb = v->scales.stride[0]; s.vsc_sh = v->scales.stride[1]; s.vsc_sn = (uint32_t)v->scales.stride[2];
+  }
+  s.len = c.len[i];
+  if (i == kFull && c.mask) {
+    s.mask = (const uint8_t*)c.mask->data;
+    s.m_sb = c.mask->stride[0]; s.m_ss = c.mask->stride[1];
+  }
+  s.S = (int32_t)p.S[i];
+  s.chunk = (int32_t)p.chunk[i];
+  s.wgs = (int32_t)p.wgs[i];
+  return s;
+}
+
+int resolve_cus(int num_cus, int* st) {
+  *st = RK_OK;
+  if (num_cus > 0) return num_cus;
+  const int cus = num_cus < 0 ? 0 : rk::current_device_cus(nullptr);
+  if (cus <= 0) *st = num_cus < 0 ? RK_ERR_ARG : RK_ERR_NO_DEVICE;
+  return cus;
+}
+
+int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
+  Plan p;
+  // everything but the split is checked before a device is asked for
+  int st = make_plan(c, 1, &p);
+  if (st) return st;
+  if (!c.out) return RK_ERR_NULL;
+  if (p.B == 0) return RK_OK;
+  if ((st = null_data(c, p))) return st;
+  const int cus = resolve_cus(0, &st);
+  if (st) return st;
+  if ((st = make_plan(c, cus, &p))) return st;
+  if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.total) return RK_ERR_WORKSPACE;
+  char* ws = (char*)workspace;
+  SpanArgs a;
+  memset(&a, 0, sizeof(a));
+  int64_t first = 0, np0 = 0;
+  for (int i = 0; i < kSpans; ++i) {
+    a.first[i] = (int32_t)first;
+    a.units[i] = (int32_t)std::max<int64_t>(p.units[i], 1);
+    a.blocks[i] = (int32_t)p.blocks[i];
+    if (p.S[i] == 0) continue;
+    a.span[i] = make_span(c, p, i, ws);
+    a.span[i].np0 = (int32_t)np0;
+    first += p.wgs[i] * p.units[i];
+    np0 += p.wgs[i];
+  }
+  a.first[kSpans] = (int32_t)first;
+  a.q = c.q->data;
+  a.q_sb = c.q->stride[0]; a.q_sh = c.q->stride[1]; a.q_sd = c.q->stride[2];
+  a.q_dtype = c.q->dtype;
+  a.out = c.out->data;
+  a.o_sb = c.out->stride[0]; a.o_sh = c.out->stride[1]; a.o_sd = c.out->stride[2];
+  a.o_dtype = c.out->dtype;
+  a.qr = a.qr_w = (uint16_t*)(ws + p.qr);
+  a.bias = a.bias_w = (float*)(ws + p.bias);
+  a.acc = (float*)(ws + p.acc);
+  a.ml = (float*)(ws + p.ml);
+  a.B = (int32_t)p.B; a.Hq = (int32_t)p.Hq; a.H = (int32_t)p.H; a.G = (int32_t)p.G;
+  a.D = (int32_t)p.D; a.Dk = (int32_t)p.Dk; a.Dkp = 32 * p.kv; a.np = (int32_t)p.np;
+  a.shared = c.shared;
+  a.terms = p.rterms;
+  a.scale_log2 = rk::kLog2e / sqrtf((float)p.D);
+  const hipStream_t s = (hipStream_t)stream;
+  hipError_t e = hipSuccess;
+  if (p.kv) {
+    if (p.zero_bytes)
+      hipLaunchKernelGGL(span_zero_kernel, dim3(64), dim3(256), 0, s, (uint32_t*)(ws + p.zero),
+                         (int64_t)(p.zero_bytes / 4));
+    a.R = c.R->data;
+    a.R_sb = c.R->stride[0]; a.R_sh = c.R->stride[1]; a.R_sd = c.R->stride[2]; a.R_sk = c.R->stride[3];
+    a.r_dtype = c.R->dtype;
+    if (c.dm) {
+      a.dm = c.dm->data;
+      a.dm_sb = c.dm->stride[0]; a.dm_sh = c.dm->stride[1]; a.dm_sd = c.dm->stride[2];
+      a.dm_dtype = c.dm->dtype;
+    }
+    if (p.format == RK_ROWS_PLAIN && c.q->dtype == RK_F16)
+      hipLaunchKernelGGL(span_queries_kernel<rk::F16>, dim3((unsigned)p.rows), dim3(128), 0, s, a);
+    else
+      hipLaunchKernelGGL(span_queries_kernel<rk::BF16>, dim3((unsigned)p.rows), dim3(128), 0, s, a);
+    if ((e = hipGetLastError()) != hipSuccess) return RK_ERR_HIP;
+  }
+  if (p.grid > 0) {
+    const unsigned grid = (unsigned)p.grid;
+    if (p.format == RK_ROWS_MX8)
+      e = rk::span_launch_mx8(p.kv, p.kf, p.nr, p.terms, a, grid, s);
+    else if (p.format == RK_ROWS_MX4)
+      e = rk::span_launch_mx4(p.kv, p.kf, p.nr, p.terms, a, grid, s);
+    else if (c.q->dtype == RK_F16)
+      e = rk::span_launch_f16(p.kv, p.kf, p.nr, p.vec, a, grid, s);
+    else
+      e = rk::span_launch_bf16(p.kv, p.kf, p.nr, p.vec, a, grid, s);
+    if (e != hipSuccess) return RK_ERR_HIP;
+  }
+  const dim3 mg((unsigned)cdiv(p.rows, 4));
+  if (p.kf == 2)
+    hipLaunchKernelGGL(span_merge_kernel<64>, mg, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(span_merge_kernel<128>, mg, dim3(256), 0, s, a);
+  return hipGetLastError() == hipSuccess ? RK_OK : RK_ERR_HIP;
+}
+
+int check_call(const Call& c, int32_t num_cus, size_t* bytes) {
+  Plan p;
+  int st = make_plan(c, 1, &p);
+  if (st) return st;
+  const int cus = resolve_cus(num_cus, &st);
+  if (st) return st;
+  if ((st = make_plan(c, cus, &p))) return st;
+  if (bytes) *bytes = p.total;
+  return RK_OK;
+}
+
+Call quantized_call(const rk_tensor* q, const rk_tensor* R, const rk_tensor* dm, const rk_rows* k_full,
+                    const rk_rows* v_full, const rk_tensor* mask, const int32_t* len, const rk_rows* k_sparse,
+                    const rk_rows* v_sparse, int64_t groups, const rk_tensor* out) {
+  Call c;
+  memset(&c, 0, sizeof(c));
+  c.q = q; c.R = R; c.dm = dm; c.mask = mask; c.out = out;
+  c.k[kFull] = k_full; c.v[kFull] = v_full; c.len[kFull] = len;
+  c.k[kRotated] = k_sparse; c.v[kRotated] = v_sparse;
+  c.groups = groups;
+  return c;
+}
+
+Call shared_call(const rk_tensor* q, const rk_tensor* R, const rk_tensor* dm, const rk_rows* k_prefix,
+                 const rk_rows* v_prefix, const rk_rows* k_sparse, const rk_rows* v_sparse, const rk_rows* k_suffix,
+                 const rk_rows* v_suffix, const int32_t* len, int64_t groups, const rk_tensor* out) {
+  Call c = quantized_call(q, R, dm, k_prefix, v_prefix, nullptr, nullptr, k_sparse, v_sparse, groups, out);
+  c.k[kTail] = k_suffix; c.v[kTail] = v_suffix; c.len[kTail] = len;
+  c.shared = true;
+  return c;
+}
+
+}  // namespace
+
+extern "C" int rk_quantized_decode_check(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
+                                         const rk_rows* k_full, const rk_rows* v_full, const rk_tensor* mask_full,
+                                         const rk_rows* k_sparse, const rk_rows* v_sparse, int64_t num_kv_groups,
+                                         const rk_tensor* out, int32_t num_cus, size_t* workspace_bytes) {
+  return check_call(quantized_call(q, R_partial, delta_mu, k_full, v_full, mask_full, nullptr, k_sparse, v_sparse,
+                                   num_kv_groups, out),
+                    num_cus, workspace_bytes);
+}
+
+extern "C" int rk_quantized_decode(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
+                                   const rk_rows* k_full, const rk_rows* v_full, const rk_tensor* mask_full,
+                                   const int32_t* len_full, const rk_rows* k_sparse, const rk_rows* v_sparse,
+                                   int64_t num_kv_groups, const rk_tensor* out, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  return run(quantized_call(q, R_partial, delta_mu, k_full, v_full, mask_full, len_full, k_sparse, v_sparse,
+                            num_kv_groups, out),
+             workspace, workspace_bytes, stream);
+}
+
+extern "C" int rk_shared_prefix_decode_check(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
+                                             const rk_rows* k_prefix, const rk_rows* v_prefix, const rk_rows* k_sparse,
+                                             const rk_rows* v_sparse, const rk_rows* k_suffix, const rk_rows* v_suffix,
+                                             int64_t num_kv_groups, const rk_tensor* out, int32_t num_cus,
+                                             size_t* workspace_bytes) {
+  return check_call(shared_call(q, R_partial, delta_mu, k_prefix, v_prefix, k_sparse, v_sparse, k_suffix, v_suffix,
+                                nullptr, num_kv_groups, out),
+                    num_cus, workspace_bytes);
+}
+
+extern "C" int rk_shared_prefix_decode(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
+                                       const rk_rows* k_prefix, const rk_rows* v_prefix, const rk_rows* k_sparse,
+                                       const rk_rows* v_sparse, const rk_rows* k_suffix, const rk_rows* v_suffix,
+                                       const int32_t* len_suffix, int64_t num_kv_groups, const rk_tensor* out,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+  return run(shared_call(q, R_partial, delta_mu, k_prefix, v_prefix, k_sparse, v_sparse, k_suffix, v_suffix,
+                         len_suffix, num_kv_groups, out),
+             workspace, workspace_bytes, stream);
+}

@@ -1,0 +1,13 @@
+// rk_span_f16.hip -- span attention over plain f16 rows (kernels in
+// rk_span_dev.h): queries exact in one term, probabilities in two.
+#include "rk_span_dev.h"
+
+namespace rk {
+
+hipError_t span_launch_f16(int kv, int kf, int nr, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s) {
+  using F = PlainFmt<F16>;
+  if (!vec) return pick_widths<F, 1, 2, false, 1>(kv, kf, a, grid, s);
+  return nr == 1 ? pick_widths<F, 1, 2, true, 1>(kv, kf, a, grid, s) : pick_widths<F, 1, 2, true, 4>(kv, kf, a, grid, s);
+}
+
+}  // namespace rk

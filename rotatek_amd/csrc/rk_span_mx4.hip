@@ -1,0 +1,15 @@
+// rk_span_mx4.hip -- span attention over quantised rows of 4-bit codes
+// (kernels in rk_span_dev.h).
+#include "rk_span_dev.h"
+
+namespace rk {
+
+// terms 2: bf16 and fp16 queries, exact in two bf16 terms, probabilities in
+// two; 3: fp32 ones, exact in three, probabilities in three.
+hipError_t span_launch_mx4(int kv, int kf, int nr, int terms, const SpanArgs& a, unsigned grid, hipStream_t s) {
+  if (terms == 3) return pick_widths<Mx4Fmt, 3, 3, true, 1>(kv, kf, a, grid, s);
+  return nr == 1 ? pick_widths<Mx4Fmt, 2, 2, true, 1>(kv, kf, a, grid, s)
+                 : pick_widths<Mx4Fmt, 2, 2, true, 4>(kv, kf, a, grid, s);
+}
+
+}  // namespace rk

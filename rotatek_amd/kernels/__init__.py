@@ -7,6 +7,10 @@
 Both families run the same hand-written HIP kernels (librotatek_hip.so);
 the variable only selects the work decomposition.  The value is read once
 at import and anything else raises ``ValueError``, as in the reference.
+
+The decodes over quantised rows (``rotatek_decode_quantized``,
+``full_channel_decode_quantized``) and over a prefix that the batch shares
+(``shared_prefix_decode``) have one decomposition whatever the variable says.
 """
 import os
 
@@ -30,4 +34,8 @@ def _pick():
 
 rotatek_decode, full_channel_decode = _pick()
 
-__all__ = ["ROTATEK_KERNEL", "rotatek_decode", "full_channel_decode"]
+from rotatek_amd.kernels.quantized_decode import full_channel_decode_quantized, rotatek_decode_quantized  # noqa: E402
+from rotatek_amd.kernels.shared_prefix import shared_prefix_decode  # noqa: E402
+
+__all__ = ["ROTATEK_KERNEL", "rotatek_decode", "full_channel_decode", "rotatek_decode_quantized",
+           "full_channel_decode_quantized", "shared_prefix_decode"]
