@@ -26,6 +26,7 @@ struct Span {
   int32_t wgs;       // workgroups of a unit
   int32_t np0;       // record number of the unit's first workgroup
   int32_t width;     // stored channels of a score row (a multiple of 32, or D)
+  int32_t k_row;     // bytes of a quantised score row
 };
 
 // Spans by what their rows score with.
@@ -36,24 +37,22 @@ struct SpanArgs {
   // units: (b, kv, row block) or, where the batch shares the span's rows,
   // (kv, row block over the batch's queries)
   int32_t units[kSpans], blocks[kSpans];
-  int32_t first[kSpans + 1];  // first workgroup of each span
+  int32_t first[kSpans];  // first workgroup of each span
   const void* q;
   void* out;
-  const uint16_t* qr;  // rotated queries in terms [row][terms][Dkp], 16 bits
-  const float* bias;   // q . delta_mu per row
-  float* acc;          // [row][np][DV] partial sums
-  float* ml;           // [row][np][2] running maximum and sum
+  float* acc;  // [row][np][DV] partial sums
+  float* ml;   // [row][np][2] running maximum and sum
   int64_t q_sb, q_sh, q_sd, o_sb, o_sh, o_sd;
-  int32_t B, Hq, H, G, D, Dk, Dkp, np, shared;
+  int32_t B, Hq, H, G, D, Dk, np, shared;
   int32_t q_dtype, o_dtype;
+  int32_t v_row;  // bytes of a quantised Value row
+  int32_t q_vec;  // queries in whole, 16-byte aligned pieces of eight channels
   float scale_log2;  // log2(e) / sqrt(D)
-  // preparation of the rotated span's queries
+  // the rotation of the rotated span's queries
   const void* R;
   const void* dm;
-  uint16_t* qr_w;
-  float* bias_w;
   int64_t R_sb, R_sh, R_sd, R_sk, dm_sb, dm_sh, dm_sd;
-  int32_t r_dtype, dm_dtype, terms;
+  int32_t r_dtype, dm_dtype;
 };
 
 constexpr int kSpanThreads = 256;
@@ -67,5 +66,12 @@ hipError_t span_launch_f16(int kv, int kf, int nr, bool vec, const SpanArgs& a, 
 hipError_t span_launch_bf16(int kv, int kf, int nr, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
 hipError_t span_launch_mx8(int kv, int kf, int nr, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
 hipError_t span_launch_mx4(int kv, int kf, int nr, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
+
+// The launch behind it where a shared call's suffix is short: the suffix rows
+// and the join of all records.
+hipError_t span_join_f16(int kf, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_join_bf16(int kf, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_join_mx8(int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_join_mx4(int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
 
 }  // namespace rk

@@ -1,8 +1,7 @@
 // rk_span.hip -- host side of the attention over quantised and shared spans
 // (rk_quantized_decode, rk_shared_prefix_decode of rotatek_hip.h): validation,
-// the split plan, and the two small kernels around the split launch
-// (rk_span_dev.h): the rotated span's queries before it, the join of a row's
-// partial sums after it.
+// the split plan, and the kernel behind the split launch
+// (rk_span_dev.h): the join of a row's partial sums after it.
 #include <hip/hip_runtime.h>
 #include <string.h>
 
@@ -28,77 +27,59 @@ int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
 // ---------------------------------------------------------------- kernels
 
-// q R_partial and q . delta_mu of one query row per workgroup, fp32 sums; q R
-// is stored as a sum of `terms` 16-bit values (two hold 16 or more bits of it,
-// three an fp32's 24).
-template <class TT>
-__global__ void __launch_bounds__(128) span_queries_kernel(const SpanArgs a) {
-  __shared__ float s_q[128];
-  __shared__ float s_b[2];
-  const int c = threadIdx.x;
-  const int64_t row = blockIdx.x;
-  const int64_t b = row / a.Hq, h = row - b * a.Hq, kv = h / a.G, rb = a.shared ? 0 : b;
-  s_q[c] = c < a.D ? rk::load_any(a.q, b * a.q_sb + h * a.q_sh + c * a.q_sd, a.q_dtype) : 0.f;
-  __syncthreads();
-  if (c < a.Dkp) {
-    float v = 0.f;
-    if (c < a.Dk) {
-      const int64_t off = rb * a.R_sb + kv * a.R_sh + c * a.R_sk;
-      for (int d = 0; d < a.D; d += 16) {
-        float r[16];
-        rk::load_any_rows<16>(a.R, off, a.R_sd, a.r_dtype, d, a.D, r);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (d + i < a.D) v = fmaf(s_q[d + i], r[i], v);
-      }
-    }
-    for (int t = 0; t < a.terms; ++t) {
-      const uint16_t w = TT::from_f32(v);
-      a.qr_w[(row * a.terms + t) * a.Dkp + c] = w;
-      v -= TT::to_f32(w);
-    }
-  }
-  float p = 0.f;
-  if (a.dm && c < a.D) p = s_q[c] * rk::load_any(a.dm, rb * a.dm_sb + kv * a.dm_sh + c * a.dm_sd, a.dm_dtype);
-  for (int d = 32; d; d >>= 1) p += rk::shfl_xor(p, d);
-  if ((c & 63) == 0) s_b[c >> 6] = p;
-  __syncthreads();
-  if (c == 0) a.bias_w[row] = s_b[0] + s_b[1];
-}
-
 // Joins a row's records: out = sum_p acc_p 2^(m_p - M) / (sum_p l_p 2^(m_p -
 // M) + 1e-6).  A wave per row: four groups of 16 lanes (DV / 16 channels a
-// lane) take every fourth record and are combined by lane exchange.
+// lane) fold every fourth record, four records' loads in flight, and are
+// combined by lane exchange.
 template <int DV>
 __global__ void __launch_bounds__(256) span_merge_kernel(const SpanArgs a) {
-  constexpr int C = DV / 16;
+  constexpr int C = DV / 16, NB = 4;
   const int lane = threadIdx.x & 63, s = lane >> 4, n = lane & 15;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)a.B * a.Hq) return;
   const float* acc = a.acc + row * a.np * DV + n * C;
   const float2* ml = (const float2*)a.ml + row * a.np;
-  float M = rk::kNegInit;
-  for (int p = lane; p < a.np; p += 64) M = fmaxf(M, ml[p].x);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, rk::shfl_xor(M, d));
-  float L = 0.f, A[C];
+  float M = rk::kNegInit, L = 0.f, A[C];
 #pragma unroll
   for (int e = 0; e < C; ++e) A[e] = 0.f;
-  for (int p = s; p < a.np; p += 4) {
-    const float2 r = ml[p];
-    const float w = rk::fast_exp2(r.x - M);
-    L += r.y * w;
+  for (int p = s; p < a.np; p += 4 * NB) {
+    float2 r[NB];
+    float4 v[NB][C / 4];
 #pragma unroll
-    for (int e = 0; e < C; e += 4) {
-      const float4 v = *(const float4*)(acc + (int64_t)p * DV + e);
-      A[e] += v.x * w; A[e + 1] += v.y * w; A[e + 2] += v.z * w; A[e + 3] += v.w * w;
+    for (int i = 0; i < NB; ++i) {
+      const int q = p + 4 * i < a.np ? p + 4 * i : p;  // past the last: a record again, with weight 0
+      r[i] = ml[q];
+#pragma unroll
+      for (int e = 0; e < C / 4; ++e) v[i][e] = *(const float4*)(acc + (int64_t)q * DV + 4 * e);
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) top = fmaxf(top, r[i].x);
+    const float f = rk::fast_exp2(M - top);
+    M = top;
+    L *= f;
+#pragma unroll
+    for (int e = 0; e < C; ++e) A[e] *= f;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      if (p + 4 * i >= a.np) break;
+      const float w = rk::fast_exp2(r[i].x - M);
+      L += r[i].y * w;
+#pragma unroll
+      for (int e = 0; e < C / 4; ++e) {
+        A[4 * e] += v[i][e].x * w; A[4 * e + 1] += v[i][e].y * w;
+        A[4 * e + 2] += v[i][e].z * w; A[4 * e + 3] += v[i][e].w * w;
+      }
     }
   }
 #pragma unroll
   for (int d = 16; d < 64; d <<= 1) {
-    L += rk::shfl_xor(L, d);
+    const float Mo = rk::shfl_xor(M, d), top = fmaxf(M, Mo);
+    const float f = rk::fast_exp2(M - top), fo = rk::fast_exp2(Mo - top);
+    L = L * f + rk::shfl_xor(L, d) * fo;
 #pragma unroll
-    for (int e = 0; e < C; ++e) A[e] += rk::shfl_xor(A[e], d);
+    for (int e = 0; e < C; ++e) A[e] = A[e] * f + rk::shfl_xor(A[e], d) * fo;
+    M = top;
   }
   if (s != 0) return;
   const int64_t b = row / a.Hq, h = row - b * a.Hq;
@@ -117,13 +98,18 @@ __global__ void __launch_bounds__(256) span_merge_kernel(const SpanArgs a) {
   }
 }
 
-// No tokens at all, or rotated rows without channels: what the kernels read
-// in their place is zero.
+// Rotated rows without channels: what the kernels read in their place is zero.
 __global__ void __launch_bounds__(256) span_zero_kernel(uint32_t* p, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0u;
 }
 
 // ------------------------------------------------------------------- host
+
+// Suffix rows up to this many are attended in the joining launch, one
+// workgroup per request and KV head; more are split like the other spans.
+constexpr int64_t kJoinTokens = 1024;
+// Bytes a workgroup streams at most.
+constexpr int64_t kMaxShare = INT64_C(512) << 10;
 
 // One call as the entry points give it; pairs may be null.
 struct Call {
@@ -137,10 +123,10 @@ struct Call {
 
 struct Plan {
   int64_t B, Hq, H, G, D, Dk;
-  int format, kv, kf, nr, terms, rterms;  // terms of a query, of a rotated one
-  bool vec;
+  int format, kv, kf, nr, terms;
+  bool vec, join;  // join: the suffix rows run in the launch that joins the records
   int64_t S[kSpans], chunk[kSpans], wgs[kSpans], units[kSpans], blocks[kSpans], np, grid, rows;
-  size_t qr, bias, zero, zero_bytes, acc, ml, total;
+  size_t zero, zero_bytes, acc, ml, total;
 };
 
 bool mx(const rk_rows* r) { return r->format != RK_ROWS_PLAIN; }
@@ -203,9 +189,11 @@ int make_plan(const Call& c, int cus, Plan* out) {
     p.Dk = c.R->shape[3];
     if (p.Dk < 0 || p.Dk > p.D) return RK_ERR_KEEP_DIM;
     if (c.R->shape[0] != N || c.R->shape[1] != p.H || c.R->shape[2] != p.D) return RK_ERR_SHAPE;
+    if (p.D * c.R->stride[2] + p.Dk * c.R->stride[3] >= (INT64_C(1) << 28)) return RK_ERR_STRIDE;
     if (c.dm) {
       if ((st = check_float(c.dm, 3))) return st;
       if (c.dm->shape[0] != N || c.dm->shape[1] != p.H || c.dm->shape[2] != p.D) return RK_ERR_SHAPE;
+      if (p.D * c.dm->stride[2] >= (INT64_C(1) << 28)) return RK_ERR_STRIDE;
     }
   }
   p.vec = true;
@@ -235,30 +223,46 @@ int make_plan(const Call& c, int cus, Plan* out) {
   p.kf = p.D <= 64 ? 2 : 4;
   p.kv = p.S[kRotated] == 0 ? 0 : p.Dk <= 32 ? 1 : p.Dk <= 64 ? 2 : 4;
   p.terms = quantised ? (c.q->dtype == RK_F32 ? 3 : 2) : 1;
-  p.rterms = std::max(p.terms, 2);
+  // more than 16 queries on the same rows: 32 to a unit, for one read of
+  // K and V (element loads and fp32 queries stay at 16)
   const int64_t rows = c.shared ? p.B * p.G : p.G;
-  // more than 16 queries on the same rows: 64 to a unit, for one read of K
-  // and V (element loads and fp32 queries stay at 16)
-  p.nr = rows > 16 && p.vec && p.terms < 3 ? 4 : 1;
+  p.nr = rows <= 16 || !p.vec || p.terms == 3 ? 1 : 2;
   p.rows = p.B * p.Hq;
   const int64_t unit_rows = 16 * p.nr;
-  int64_t cost[kSpans], total = 0;  // channels read per token
+  p.join = c.shared && p.S[kTail] > 0 && p.S[kTail] <= kJoinTokens;
+  int64_t cost[kSpans], total = 0;  // bytes of a token; of all units
   for (int i = 0; i < kSpans; ++i) {
     const bool per_request = !c.shared || i == kTail;
-    p.blocks[i] = cdiv(per_request ? p.G : p.B * p.G, unit_rows);
+    const int64_t r = p.join && i == kTail ? 16 : unit_rows;
+    p.blocks[i] = cdiv(per_request ? p.G : p.B * p.G, r);
     p.units[i] = p.H * p.blocks[i] * (per_request ? p.B : 1);
-    cost[i] = p.D + (i == kRotated ? p.Dk : p.D);
-    total += p.units[i] * p.S[i] * cost[i];
+    const int64_t kd = i == kRotated ? p.Dk : p.D;
+    cost[i] = quantised ? rk::mx_row_bytes(kd, p.format) + rk::mx_row_bytes(p.D, p.format) : 2 * (kd + p.D);
+    if (!(p.join && i == kTail)) total += p.units[i] * p.S[i] * cost[i];
   }
-  // equal shares of the channels to read for every workgroup of one round
-  const int64_t slots = (int64_t)cus * (p.nr > 1 ? 1 : 2);
-  const int64_t share = std::max<int64_t>(cdiv(total, slots), 1);
-  for (int i = 0; i < kSpans; ++i) {
-    if (p.S[i] == 0) continue;
-    p.chunk[i] = round_up(std::max<int64_t>(cdiv(share, cost[i]), 1), rk::kSpanWaves * rk::kSpanBlk);
-    p.wgs[i] = cdiv(p.S[i], p.chunk[i]);
-    p.np += p.wgs[i];
-    p.grid += p.wgs[i] * p.units[i];
+  // Equal shares of the bytes for every workgroup, of whole rounds of the
+  // workgroups that are resident at a time: the fewest rounds that keep a
+  // share at kMaxShare, and within them the largest grid that fits.
+  const int64_t slots = (int64_t)cus * (p.nr == 1 ? 3 : 2);
+  const int64_t rounds = std::max<int64_t>(cdiv(total, slots * kMaxShare), 1);
+  const int64_t align = rk::kSpanWaves * rk::kSpanBlk;
+  for (int64_t share = std::max<int64_t>(cdiv(total, slots * rounds), 1);; share += cdiv(share, 32)) {
+    p.np = p.grid = 0;
+    bool least = true;  // one workgroup per unit and span
+    for (int i = 0; i < kSpans; ++i) {
+      p.wgs[i] = p.chunk[i] = 0;
+      if (p.S[i] == 0 || (p.join && i == kTail)) continue;
+      p.chunk[i] = std::min(round_up(cdiv(share, cost[i]), align), round_up(p.S[i], align));
+      p.wgs[i] = cdiv(p.S[i], p.chunk[i]);
+      least = least && p.wgs[i] == 1;
+      p.np += p.wgs[i];
+      p.grid += p.wgs[i] * p.units[i];
+    }
+    if (least || p.grid <= slots * rounds) break;
+  }
+  if (p.join) {
+    p.chunk[kTail] = round_up(p.S[kTail], align);
+    p.wgs[kTail] = 1;
   }
   if (p.grid >= (INT64_C(1) << 31) || p.rows >= (INT64_C(1) << 31) || p.rows * p.np >= (INT64_C(1) << 40))
     return RK_ERR_SHAPE;
@@ -269,8 +273,6 @@ int make_plan(const Call& c, int cus, Plan* out) {
     at += (bytes + 255) & ~size_t(255);
     return here;
   };
-  p.qr = take(p.kv ? (size_t)p.rows * p.rterms * 32 * p.kv * 2 : 0);
-  p.bias = take(p.kv ? (size_t)p.rows * 4 : 0);
   // rotated rows without channels: one zero row and its scales
   p.zero_bytes = p.kv && p.Dk == 0 ? 256 + (size_t)round_up(p.S[kRotated], 32) : 0;
   p.zero = take(p.zero_bytes);
@@ -313,6 +315,7 @@ Span make_span(const Call& c, const Plan& p, int i, char* ws) {
     s.k_ss = (uint32_t)k->data.stride[2]; s.k_sd = (uint32_t)k->data.stride[3];
     s.width = (int32_t)(quantised ? rk::mx_width(k->head_dim) : k->head_dim);
     if (quantised) {
+      s.k_row = (int32_t)rk::mx_row_bytes(k->head_dim, p.format);
       s.ksc = (const uint8_t*)k->scales.data;
       s.ksc_sb = k->scales.stride[0]; s.ksc_sh = k->scales.stride[1]; s.ksc_sn = (uint32_t)k->scales.stride[2];
     }
@@ -363,24 +366,23 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
     if (p.S[i] == 0) continue;
     a.span[i] = make_span(c, p, i, ws);
     a.span[i].np0 = (int32_t)np0;
+    if (p.join && i == kTail) break;
     first += p.wgs[i] * p.units[i];
     np0 += p.wgs[i];
   }
-  a.first[kSpans] = (int32_t)first;
   a.q = c.q->data;
   a.q_sb = c.q->stride[0]; a.q_sh = c.q->stride[1]; a.q_sd = c.q->stride[2];
   a.q_dtype = c.q->dtype;
+  a.q_vec = rk::vec_ok(c.q) && p.D % 8 == 0;
   a.out = c.out->data;
   a.o_sb = c.out->stride[0]; a.o_sh = c.out->stride[1]; a.o_sd = c.out->stride[2];
   a.o_dtype = c.out->dtype;
-  a.qr = a.qr_w = (uint16_t*)(ws + p.qr);
-  a.bias = a.bias_w = (float*)(ws + p.bias);
   a.acc = (float*)(ws + p.acc);
   a.ml = (float*)(ws + p.ml);
   a.B = (int32_t)p.B; a.Hq = (int32_t)p.Hq; a.H = (int32_t)p.H; a.G = (int32_t)p.G;
-  a.D = (int32_t)p.D; a.Dk = (int32_t)p.Dk; a.Dkp = 32 * p.kv; a.np = (int32_t)p.np;
+  a.D = (int32_t)p.D; a.Dk = (int32_t)p.Dk; a.np = (int32_t)p.np;
   a.shared = c.shared;
-  a.terms = p.rterms;
+  a.v_row = p.format == RK_ROWS_PLAIN ? 0 : (int32_t)rk::mx_row_bytes(p.D, p.format);
   a.scale_log2 = rk::kLog2e / sqrtf((float)p.D);
   const hipStream_t s = (hipStream_t)stream;
   hipError_t e = hipSuccess;
@@ -396,10 +398,6 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
       a.dm_sb = c.dm->stride[0]; a.dm_sh = c.dm->stride[1]; a.dm_sd = c.dm->stride[2];
       a.dm_dtype = c.dm->dtype;
     }
-    if (p.format == RK_ROWS_PLAIN && c.q->dtype == RK_F16)
-      hipLaunchKernelGGL(span_queries_kernel<rk::F16>, dim3((unsigned)p.rows), dim3(128), 0, s, a);
-    else
-      hipLaunchKernelGGL(span_queries_kernel<rk::BF16>, dim3((unsigned)p.rows), dim3(128), 0, s, a);
     if ((e = hipGetLastError()) != hipSuccess) return RK_ERR_HIP;
   }
   if (p.grid > 0) {
@@ -413,6 +411,18 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
     else
       e = rk::span_launch_bf16(p.kv, p.kf, p.nr, p.vec, a, grid, s);
     if (e != hipSuccess) return RK_ERR_HIP;
+  }
+  if (p.join) {
+    const unsigned grid = (unsigned)p.units[kTail];
+    if (p.format == RK_ROWS_MX8)
+      e = rk::span_join_mx8(p.kf, p.terms, a, grid, s);
+    else if (p.format == RK_ROWS_MX4)
+      e = rk::span_join_mx4(p.kf, p.terms, a, grid, s);
+    else if (c.q->dtype == RK_F16)
+      e = rk::span_join_f16(p.kf, p.vec, a, grid, s);
+    else
+      e = rk::span_join_bf16(p.kf, p.vec, a, grid, s);
+    return e == hipSuccess ? RK_OK : RK_ERR_HIP;
   }
   const dim3 mg((unsigned)cdiv(p.rows, 4));
   if (p.kf == 2)

@@ -24,6 +24,12 @@
 // Quantised rows are widened to bf16, which holds code 2^e exactly, by the
 // conversion that applies the block's scale; queries then enter as one, two
 // or three bf16 terms, in which bf16, fp16 and fp32 are exact.
+//
+// Loads run ahead of the products: the K registers are reloaded with the
+// wave's next block as soon as the scores are formed, the V registers as soon
+// as V^T is.  All offsets of a lane are fixed; a block moves
+// the wave-uniform base alone.  The last block of a span starts 32 rows before
+// its end, its rows of the block before it left out.
 #pragma once
 
 #include <math.h>
@@ -65,9 +71,12 @@ struct Mx4Fmt {
   }
 };
 
-// A block's scale from its byte: the conversions read the exponent field, 255
-// makes NaN.
-__device__ __forceinline__ float mx_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+// The scale of byte r of w as the conversions take it: they read the exponent
+// field of the operand alone (255 makes NaN), so what else the shift leaves
+// does not matter.
+__device__ __forceinline__ float mx_scale(uint32_t w, int r) {
+  return __builtin_bit_cast(float, r < 3 ? w << (23 - 8 * r) : w >> 1);
+}
 
 // Eight channels as a matrix operand.
 template <class F>
@@ -79,16 +88,20 @@ __device__ __forceinline__ uint4 widen8(const uint32_t* w, float sc) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+typedef const __attribute__((address_space(1))) char* gptr;  // global memory
+#define RK_GLOBAL(T) const __attribute__((address_space(1))) T*
+
 template <int N>
-__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
+__device__ __forceinline__ void load_words(gptr p, uint32_t* w) {
   if constexpr (N == 4) {
-    const u32x4 v = *(const u32x4*)p;
+    const u32x4 v = *(RK_GLOBAL(u32x4))p;
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   } else if constexpr (N == 2) {
-    const uint2 v = *(const uint2*)p;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 v = *(RK_GLOBAL(u32x2))p;
     w[0] = v.x; w[1] = v.y;
   } else {
-    w[0] = *(const uint32_t*)p;
+    w[0] = *(RK_GLOBAL(uint32_t))p;
   }
 }
 
@@ -103,41 +116,92 @@ struct Block {
   uint2 vs;
 };
 
-struct SpanHead {  // a unit's rows of one span
-  const char* k;
-  const char* v;
-  const uint8_t* ksc;
+// A unit's rows of one tensor as a buffer: a load is descriptor + scalar
+// offset of the block + fixed 32-bit offset of the lane (an address needs two
+// registers and a 64-bit vector addition per load), and nothing past `bytes`
+// is read.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+__device__ __forceinline__ Rsrc make_rsrc(const void* p, uint32_t bytes) {
+  const uint64_t v = (uint64_t)p;
+  const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, (int)__builtin_amdgcn_readfirstlane((int)bytes), 0x00027000);
+}
+template <int N>
+__device__ __forceinline__ void load_words(Rsrc r, uint32_t off, uint32_t base, uint32_t* w) {
+  if constexpr (N == 4) {
+    const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, base, 0));
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, base, 0));
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, base, 0);
+  }
+}
+
+// A unit's rows of one span, and a lane's byte offsets in a block.
+template <int KB>
+struct SpanLane {
+  Rsrc k, v, ksc;
   const uint8_t* vsc;
+  uint32_t ko[2], kc[KB], so[2], vo[8], vso;
 };
 
-// Loads block `blk`; rows past the span are its last row.
-template <class F, int KB, int VB, bool VEC>
-__device__ __forceinline__ void load_block(const Span& sp, const SpanHead& hd, int D, int blk, int g, int n,
-                                           Block<F, KB, VB>& x) {
-  const uint32_t last = (uint32_t)sp.S - 1;
-  const uint32_t t0 = (uint32_t)blk * kSpanBlk;
+template <class F, int KB, int VB>
+__device__ __forceinline__ void lane_offsets(const Span& sp, int D, int g, int n, SpanLane<KB>& x) {
+  const uint32_t last = (uint32_t)sp.S - 1;  // a span of less than 32 rows repeats its last
+  const int cv = n * VB < D ? n * VB : 0;    // lanes past the head's channels: any will do
 #pragma unroll
   for (int tt = 0; tt < 2; ++tt) {
-    const uint32_t t = min(t0 + 8 * (n >> 2) + 4 * tt + (n & 3), last);
+    const uint32_t t = min((uint32_t)(8 * (n >> 2) + 4 * tt + (n & 3)), last);
     if constexpr (F::kMx) {
       // eight KB channels in one piece; past the row's width the first ones
       // stand in (the query is zero there)
       const uint32_t c = 8 * KB * g < sp.width ? 8 * KB * g : 0;
-      const char* p = hd.k + t * sp.k_ss + (F::kw == 2 ? c : c >> 1);
+      x.ko[tt] = t * sp.k_ss + (F::kw == 2 ? c : c >> 1);
+      x.so[tt] = (c >> 5) * sp.ksc_sn + t;
+    } else {
+      x.ko[tt] = 2 * t * sp.k_ss;
+    }
+  }
+  if constexpr (!F::kMx) {
+#pragma unroll
+    for (int j = 0; j < KB; ++j) x.kc[j] = 2 * (32 * j + 8 * g < sp.width ? 32 * j + 8 * g : 0);
+  }
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const uint32_t t = min((uint32_t)(8 * g + r), last);
+    if constexpr (F::kMx)
+      x.vo[r] = t * sp.v_ss + (F::kw == 2 ? cv : cv >> 1);
+    else
+      x.vo[r] = 2 * (t * sp.v_ss + (uint32_t)cv);
+  }
+  if constexpr (F::kMx) x.vso = (cv >> 5) * sp.vsc_sn + 8 * g;
+}
+
+// First row of a block: the span's last block ends with the span.
+__device__ __forceinline__ int block_row(const Span& sp, int blk) {
+  return min(blk * kSpanBlk, max(sp.S - kSpanBlk, 0));
+}
+
+template <class F, int KB, int VB, bool VEC>
+__device__ __forceinline__ void load_k(const Span& sp, const SpanLane<KB>& hd, int blk, int g, Block<F, KB, VB>& x) {
+  const uint32_t t0 = block_row(sp, blk), base = t0 * sp.k_ss * (F::kMx ? 1 : 2);
+#pragma unroll
+  for (int tt = 0; tt < 2; ++tt) {
+    if constexpr (F::kMx) {
       constexpr int kAll = KB * F::kw;
       if constexpr (kAll == 8) {
-        load_words<4>(p, x.k[tt]);
-        load_words<4>(p + 16, x.k[tt] + 4);
+        load_words<4>(hd.k, hd.ko[tt], base, x.k[tt]);
+        load_words<4>(hd.k, hd.ko[tt] + 16, base, x.k[tt] + 4);
       } else {
-        load_words<kAll>(p, x.k[tt]);
+        load_words<kAll>(hd.k, hd.ko[tt], base, x.k[tt]);
       }
-      x.ks[tt] = hd.ksc[(c >> 5) * sp.ksc_sn + t];
+      x.ks[tt] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(hd.ksc, hd.so[tt], t0, 0);
     } else if constexpr (VEC) {
 #pragma unroll
-      for (int j = 0; j < KB; ++j) {
-        const int c = 32 * j + 8 * g;
-        load_words<4>(hd.k + 2 * (t * sp.k_ss + (uint32_t)(c < sp.width ? c : 0)), x.k[tt] + 4 * j);
-      }
+      for (int j = 0; j < KB; ++j) load_words<4>(hd.k, hd.ko[tt] + hd.kc[j], base, x.k[tt] + 4 * j);
     } else {
 #pragma unroll
       for (int j = 0; j < KB; ++j) {
@@ -148,40 +212,48 @@ __device__ __forceinline__ void load_block(const Span& sp, const SpanHead& hd, i
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (c + 2 * w + e < sp.width)
-              v |= (uint32_t)((const uint16_t*)hd.k)[t * sp.k_ss + (c + 2 * w + e) * sp.k_sd] << (16 * e);
+              v |= (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
+                       hd.k, hd.ko[tt] + 2 * (uint32_t)(c + 2 * w + e) * sp.k_sd, base, 0)
+                   << (16 * e);
           x.k[tt][4 * j + w] = v;
         }
       }
     }
   }
-  const int cv = n * VB < D ? n * VB : 0;  // lanes past the head's channels: any will do
+}
+
+template <class F, int KB, int VB, bool VEC>
+__device__ __forceinline__ void load_v(const Span& sp, const SpanLane<KB>& hd, int D, int blk, int n,
+                                       Block<F, KB, VB>& x) {
+  const uint32_t t0 = block_row(sp, blk), base = t0 * sp.v_ss * (F::kMx ? 1 : 2);
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
-    const uint32_t t = min(t0 + 8 * g + r, last);
     if constexpr (F::kMx) {
       if constexpr (VB == 8)
-        load_words<F::kw>(hd.v + t * sp.v_ss + (F::kw == 2 ? cv : cv >> 1), x.v[r]);
+        load_words<F::kw>(hd.v, hd.vo[r], base, x.v[r]);
       else if constexpr (F::kw == 2)
-        load_words<1>(hd.v + t * sp.v_ss + cv, x.v[r]);
+        load_words<1>(hd.v, hd.vo[r], base, x.v[r]);
       else
-        x.v[r][0] = *(const uint16_t*)(hd.v + t * sp.v_ss + (cv >> 1));
+        x.v[r][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(hd.v, hd.vo[r], base, 0);
     } else if constexpr (VEC) {
-      load_words<VB / 2>(hd.v + 2 * (t * sp.v_ss + (uint32_t)cv), x.v[r]);
+      load_words<VB / 2>(hd.v, hd.vo[r], base, x.v[r]);
     } else {
+      const int cv = n * VB < D ? n * VB : 0;
 #pragma unroll
       for (int w = 0; w < VB / 2; ++w) {
         uint32_t v = 0;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           if (cv + 2 * w + e < D)
-            v |= (uint32_t)((const uint16_t*)hd.v)[t * sp.v_ss + (cv + 2 * w + e) * sp.v_sd] << (16 * e);
+            v |= (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
+                     hd.v, hd.vo[r] + 2 * ((uint32_t)(cv + 2 * w + e) * sp.v_sd - (uint32_t)cv), base, 0)
+                 << (16 * e);
         x.v[r][w] = v;
       }
     }
   }
-  // eight tokens' scales of the lane's block column; the column is padded to
-  // whole groups of 32
-  if constexpr (F::kMx) x.vs = *(const uint2*)(hd.vsc + (cv >> 5) * sp.vsc_sn + min(t0, last & ~31u) + 8 * g);
+  // eight tokens' scales of the lane's block column, at any byte address
+  if constexpr (F::kMx) __builtin_memcpy(&x.vs, hd.vsc + t0 + hd.vso, 8);
 }
 
 // Values as the products take them: x as the sum of NT 16-bit terms.
@@ -205,31 +277,61 @@ __device__ __forceinline__ void terms8(const float (&x)[8], uint4 (&o)[NT]) {
   }
 }
 
-// fp16 probabilities are formed as 2^14 p (at most 16384): those below 2^-28,
-// not 2^-14, fall into fp16's subnormals.  Sums carry the factor until the
-// workgroup's record, which is free of it.
+// The running maximum is raised (and the sums rescaled) only when a score
+// passes it by kSlack, in log2 units: a probability is then at most 2^kSlack,
+// and most blocks need no exchange between lanes.  fp16 probabilities are
+// formed as 2^kLift p (at most 2^15): those below 2^-24, not 2^-14, fall into
+// fp16's subnormals.  A workgroup's record is free of both.
 template <class TT>
-constexpr float kLift = TT::kRk == 0 ? 14.f : 0.f;
+constexpr float kLift = TT::kRk == 0 ? 10.f : 0.f;
+template <class TT>
+constexpr float kSlack = TT::kRk == 0 ? 5.f : 8.f;
 
-// The running state of one wave: NR blocks of 16 query rows.
+// The running state of one wave: NR blocks of 16 query rows.  m: the maximum
+// that the sums are relative to (0 until a token was `seen`, which all rows of
+// a block do together); top: the lane's largest score so far, relative to m
+// and lifted.  l: the sum of the probabilities, formed with the others as the
+// product of P with ones: every register of it is the sum.
 template <int NR, int VB>
 struct State {
-  float m[NR], l[NR];
-  f32x4 acc[NR][VB];
+  float m[NR], top[NR];
+  bool seen[NR];
+  f32x4 l[NR], acc[NR][VB];
 };
+// One instruction: fmaxf quiets each operand with another.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <class TT>
+__device__ __forceinline__ uint4 ones() {
+  const uint32_t w = TT::kRk == F16::kRk ? 0x3c003c00u : 0x3f803f80u;
+  return make_uint4(w, w, w, w);
+}
 
-// One chunk of one span: adds the wave's blocks to `st`.  sq: the unit's
-// queries in LDS, [term][row][stride] 16-bit, in the lane's channel order.
-template <class F, int KB, int VB, int NR, int NT, int NP, bool VEC>
-__device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, const SpanHead& hd, int b, int x, int wave,
+// One chunk of one span: adds the wave's blocks to `st`.  pre(): stages the
+// unit's queries in LDS, sq [term][row][stride] 16-bit in the lane's channel
+// order, while the first blocks are on their way.
+template <class F, int KB, int VB, int NR, int NT, int NP, bool VEC, class Pre>
+__device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, SpanLane<KB>& hd, int b, int chunk, int wave,
                                          int lane, const uint16_t* sq, int qstride, const float* sbias,
-                                         State<NR, VB>& st) {
+                                         State<NR, VB>& st, const Pre& pre) {
   using TT = typename F::TT;
   const int g = lane >> 4, n = lane & 15;
-  int lim = min(x * sp.chunk + sp.chunk, sp.S);
+  int lim = min(chunk * sp.chunk + sp.chunk, sp.S);
   if (sp.len) lim = min(lim, max(sp.len[b], 0));
-  const int blk0 = x * sp.chunk / kSpanBlk, nblk = (lim + kSpanBlk - 1) / kSpanBlk;
-  constexpr bool kRegQ = NR * NT * KB <= 16;  // queries held in registers
+  lim = __builtin_amdgcn_readfirstlane(lim);  // (a loaded length sits in a vector register)
+  const int blk0 = chunk * sp.chunk / kSpanBlk + wave, nblk = (lim + kSpanBlk - 1) / kSpanBlk;
+  const int nw = nblk > blk0 ? (nblk - blk0 - 1) / kSpanWaves + 1 : 0;
+  // past the wave's last block the ring reads that block again
+  auto blk_of = [&](int i) { return blk0 + kSpanWaves * min(i, max(nw - 1, 0)); };
+  lane_offsets<F, KB, VB>(sp, a.D, g, n, hd);
+  Block<F, KB, VB> buf;
+  load_k<F, KB, VB, VEC>(sp, hd, blk_of(0), g, buf);
+  load_v<F, KB, VB, VEC>(sp, hd, a.D, blk_of(0), n, buf);
+  pre();
+  constexpr bool kRegQ = NR * NT * KB <= (NR == 1 ? 12 : 8);  // queries held in registers
   uint4 qreg[kRegQ ? NR : 1][kRegQ ? NT : 1][kRegQ ? KB : 1];
   auto qload = [&](int nr, int t, int j) {
     const int c = F::kMx ? 8 * KB * g + 8 * j : 32 * j + 8 * g;
@@ -243,11 +345,13 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, cons
 #pragma unroll
         for (int j = 0; j < KB; ++j) qreg[nr][t][j] = qload(nr, t, j);
   }
-  float bias[NR];
+  // a score is one fused multiply-add: the bias, the maximum and the lift in
+  // its addend
+  float off[NR];
 #pragma unroll
-  for (int nr = 0; nr < NR; ++nr) bias[nr] = sbias ? sbias[nr * 16 + n] : 0.f;
+  for (int nr = 0; nr < NR; ++nr) off[nr] = (sbias ? sbias[nr * 16 + n] * a.scale_log2 : 0.f) + kLift<TT>;
 
-  auto compute = [&](const Block<F, KB, VB>& x, int blk) {
+  auto compute = [&](Block<F, KB, VB>& x, int blk, int next) {
     f32x4 s[2][NR];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
@@ -257,7 +361,7 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, cons
     for (int j = 0; j < KB; ++j)
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
-        uint4 kop = widen8<F>(x.k[tt] + j * F::kw, mx_scale(x.ks[tt]));
+        uint4 kop = widen8<F>(x.k[tt] + j * F::kw, mx_scale(x.ks[tt], 0));
         // plain rows narrower than KB blocks: no value of another channel
         // meets the query's zero (an infinity would make NaN)
         if constexpr (!F::kMx && VEC)
@@ -272,99 +376,111 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, cons
               s[tt][nr] = TT::mfma(kop, qload(nr, t, j), s[tt][nr]);
           }
       }
+    load_k<F, KB, VB, VEC>(sp, hd, next, g, x);
     // which of the lane's eight tokens count
-    const int t0 = blk * kSpanBlk + 8 * g;
+    const int t0 = block_row(sp, blk) + 8 * g;
     uint32_t on = 0xffu;
     const bool whole = (blk + 1) * kSpanBlk <= lim && !sp.mask;
     if (!whole) {
       on = 0;
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        bool ok = t0 + r < lim;
+        bool ok = t0 + r >= blk * kSpanBlk && t0 + r < lim;
         if (sp.mask && ok) ok = sp.mask[b * sp.m_sb + (t0 + r) * sp.m_ss] != 0;
         on |= (uint32_t)ok << r;
       }
     }
-    uint4 p[NR][NP];
+    // V^T of channel slots 2 w and 2 w + 1: eight tokens of each
+    auto turn = [&](int w, uint4& lo, uint4& hi) {
+      uint32_t y[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if constexpr (F::kMx) {
+          const float sc = mx_scale(r < 4 ? x.vs.x : x.vs.y, r & 3);
+          y[r] = w == 0   ? F::template pair<0>(x.v[r], sc)
+                 : w == 1 ? F::template pair<1>(x.v[r], sc)
+                 : w == 2 ? F::template pair<2>(x.v[r], sc)
+                          : F::template pair<3>(x.v[r], sc);
+        } else {
+          y[r] = x.v[r][w];
+        }
+        // rows that do not count hold anything: 0 x NaN must not reach the sum
+        if (!whole) y[r] = (on >> r) & 1u ? y[r] : 0u;
+      }
+      lo = make_uint4(pack_lo(y[0], y[1]), pack_lo(y[2], y[3]), pack_lo(y[4], y[5]), pack_lo(y[6], y[7]));
+      hi = make_uint4(pack_hi(y[0], y[1]), pack_hi(y[2], y[3]), pack_hi(y[4], y[5]), pack_hi(y[6], y[7]));
+    };
+    // several row blocks share V^T; one forms it as it goes
+    uint4 av[NR > 1 ? VB : 1];
+    if constexpr (NR > 1) {
+#pragma unroll
+      for (int w = 0; w < VB / 2; ++w) turn(w, av[2 * w], av[2 * w + 1]);
+      load_v<F, KB, VB, VEC>(sp, hd, a.D, next, n, x);
+    }
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
       float sc[8];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        sc[r] = (s[r >> 2][nr][r & 3] + bias[nr]) * a.scale_log2;
-        if (!((on >> r) & 1u)) sc[r] = -INFINITY;
-      }
-      float mx = sc[0];
+      for (int r = 0; r < 8; ++r) sc[r] = fmaf(s[r >> 2][nr][r & 3], a.scale_log2, off[nr]);
+      if (!whole) {
 #pragma unroll
-      for (int r = 1; r < 8; ++r) mx = fmaxf(mx, sc[r]);
-      mx = fmaxf(mx, shfl_xor(mx, 16));
-      mx = fmaxf(mx, shfl_xor(mx, 32));
-      const float m_new = fmaxf(st.m[nr], mx);
-      const float alpha = fast_exp2(st.m[nr] - m_new);
-      if (__any(m_new != st.m[nr])) {
+        for (int r = 0; r < 8; ++r) sc[r] = (on >> r) & 1u ? sc[r] : -INFINITY;
+      }
+      float mx = max3(sc[0], sc[1], sc[2]);
+      mx = max3(mx, sc[3], sc[4]);
+      mx = max3(mx, sc[5], sc[6]);
+      mx = max3(mx, sc[7], sc[7]);
+      st.top[nr] = max3(st.top[nr], mx, mx);
+      if (!st.seen[nr] || __any(mx > kSlack<TT> + kLift<TT>)) {
+        mx = fmaxf(mx, shfl_xor(mx, 16));
+        mx = fmaxf(mx, shfl_xor(mx, 32));
+        // how far the maximum rises; the first tokens set it
+        float up = mx - kLift<TT>;
+        if (st.seen[nr]) up = fmaxf(up, 0.f);
+        st.seen[nr] = st.seen[nr] || __any(mx > -INFINITY);
+        up = up > -INFINITY ? up : 0.f;
+        const float alpha = fast_exp2(-up);
 #pragma unroll
         for (int j = 0; j < VB; ++j) st.acc[nr][j] *= alpha;
-      }
-      st.m[nr] = m_new;
-      const float base = m_new - kLift<TT>;
-      float ps = 0.f;
+        st.l[nr] *= alpha;
+        st.m[nr] += up;
+        st.top[nr] -= up;
+        off[nr] -= up;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        sc[r] = fast_exp2(sc[r] - base);
-        ps += sc[r];
+        for (int r = 0; r < 8; ++r) sc[r] -= up;
       }
-      st.l[nr] = st.l[nr] * alpha + ps;
-      terms8<TT, NP>(sc, p[nr]);
-    }
-    // V^T: eight tokens of channel slot j
-    uint32_t vw[8][VB / 2];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      if constexpr (F::kMx) {
-        const float sc = mx_scale(((r < 4 ? x.vs.x : x.vs.y) >> (8 * (r & 3))) & 0xffu);
-        vw[r][0] = F::template pair<0>(x.v[r], sc);
-        vw[r][1] = F::template pair<1>(x.v[r], sc);
-        if constexpr (VB == 8) {
-          vw[r][2] = F::template pair<2>(x.v[r], sc);
-          vw[r][3] = F::template pair<3>(x.v[r], sc);
+      for (int r = 0; r < 8; ++r) sc[r] = fast_exp2(sc[r]);
+      uint4 p[NP];
+      terms8<TT, NP>(sc, p);
+#pragma unroll
+      for (int t = 0; t < NP; ++t) st.l[nr] = TT::mfma(ones<TT>(), p[t], st.l[nr]);
+      if constexpr (NR > 1) {
+#pragma unroll
+        for (int t = 0; t < NP; ++t)
+#pragma unroll
+          for (int j = 0; j < VB; ++j) st.acc[nr][j] = TT::mfma(av[j], p[t], st.acc[nr][j]);
+      } else {
+#pragma unroll
+        for (int w = 0; w < VB / 2; ++w) {
+          uint4 lo, hi;
+          __builtin_amdgcn_sched_barrier(0);  // one pair's registers at a time
+          turn(w, lo, hi);
+#pragma unroll
+          for (int t = 0; t < NP; ++t) {
+            st.acc[nr][2 * w] = TT::mfma(lo, p[t], st.acc[nr][2 * w]);
+            st.acc[nr][2 * w + 1] = TT::mfma(hi, p[t], st.acc[nr][2 * w + 1]);
+          }
         }
-      } else {
-#pragma unroll
-        for (int w = 0; w < VB / 2; ++w) vw[r][w] = x.v[r][w];
+        load_v<F, KB, VB, VEC>(sp, hd, a.D, next, n, x);
       }
-      // rows that do not count hold anything: 0 x NaN must not reach the sum
-      if (!whole) {
-        const bool ok = (on >> r) & 1u;
-#pragma unroll
-        for (int w = 0; w < VB / 2; ++w) vw[r][w] = ok ? vw[r][w] : 0u;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < VB; ++j) {
-      const int w = j >> 1;
-      uint4 av;
-      if (j & 1) {
-        av.x = pack_hi(vw[0][w], vw[1][w]); av.y = pack_hi(vw[2][w], vw[3][w]);
-        av.z = pack_hi(vw[4][w], vw[5][w]); av.w = pack_hi(vw[6][w], vw[7][w]);
-      } else {
-        av.x = pack_lo(vw[0][w], vw[1][w]); av.y = pack_lo(vw[2][w], vw[3][w]);
-        av.z = pack_lo(vw[4][w], vw[5][w]); av.w = pack_lo(vw[6][w], vw[7][w]);
-      }
-#pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-        for (int t = 0; t < NP; ++t) st.acc[nr][j] = TT::mfma(av, p[nr][t], st.acc[nr][j]);
     }
   };
 
-  Block<F, KB, VB> blk;
-  for (int i = blk0 + wave; i < nblk; i += kSpanWaves) {
-    load_block<F, KB, VB, VEC>(sp, hd, a.D, i, g, n, blk);
-    compute(blk, i);
-  }
+  for (int i = 0; i < nw; ++i) compute(buf, blk_of(i), blk_of(i + 1));
 }
 
-// Query row r of a unit: its batch row and head.
+// Query row R of a unit: its batch row and head.
 struct RowOf {
   int b, h;
 };
@@ -375,171 +491,353 @@ __device__ __forceinline__ RowOf row_of(const SpanArgs& a, bool shared, int b, i
   return o;
 }
 
-template <class F, int KV, int KF, int NR, int NT, int NP, bool VEC>
-__global__ void __launch_bounds__(kSpanThreads) span_kernel(const SpanArgs a) {
+// A unit's queries: thread i holds the i-th eight channels of every 256 of
+// them (16 to a row), as they are in memory.
+template <int NR>
+struct Queries {
+  uint32_t w[NR][8];
+};
+
+// The loads alone: aligned rows in whole 16-byte pieces (a.q_vec), others
+// element by element as fp32.
+template <int NR>
+__device__ __forceinline__ void load_queries(const SpanArgs& a, bool shared, int b, int kv, int R0, int rows, int tid,
+                                             Queries<NR>& x) {
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int c = 8 * (tid & 15), r = 16 * i + (tid >> 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.w[i][e] = 0u;
+    if (r >= rows || c >= a.D) continue;
+    const RowOf o = row_of(a, shared, b, kv, R0 + r);
+    const int64_t off = o.b * a.q_sb + o.h * a.q_sh + c * a.q_sd;
+    if (!a.q_vec) {
+      for (int e = 0; e < 8; ++e)
+        if (c + e < a.D) x.w[i][e] = __builtin_bit_cast(uint32_t, load_any(a.q, off + e * a.q_sd, a.q_dtype));
+    } else if (a.q_dtype == F32::kRk) {
+      load_words<4>((gptr)a.q + 4 * off, x.w[i]);
+      load_words<4>((gptr)a.q + 4 * off + 16, x.w[i] + 4);
+    } else {
+      load_words<4>((gptr)a.q + 2 * off, x.w[i]);
+    }
+  }
+}
+
+// ... and their NT terms of TT in LDS, [term][row][stride], zeros past the
+// head's channels and the unit's rows; channels up to kW.
+template <class TT, int NT, int NR, int kW>
+__device__ __forceinline__ void stage_queries(const SpanArgs& a, int tid, const Queries<NR>& x, uint16_t* dst,
+                                              int stride) {
+  const int c = 8 * (tid & 15);
+  if (c >= kW) return;
+  const int dt = a.q_vec ? a.q_dtype : F32::kRk;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t h = x.w[i][e >> 1] >> (16 * (e & 1));
+      v[e] = dt == F32::kRk ? __builtin_bit_cast(float, x.w[i][e])
+             : dt == F16::kRk ? F16::to_f32((uint16_t)h)
+                              : BF16::to_f32((uint16_t)h);
+    }
+    uint4 t[NT];
+    terms8<TT, NT>(v, t);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *(uint4*)(dst + (j * 16 * NR + 16 * i + (tid >> 4)) * stride + c) = t[j];
+  }
+}
+
+// Sixteen columns of [R_partial | delta_mu] as a matrix operand's 32 elements
+// per lane: rows 32 ks + 8 g + e of column 16 ct + n (tile 2 KV: delta_mu, in
+// column 0), raw.
+template <int KV>
+__device__ __forceinline__ void load_columns(const SpanArgs& a, int rb, int kv, int ct, int g, int n, uint32_t (&w)[32]) {
+  const bool mu = ct == 2 * KV;
+  const int dt = mu ? a.dm_dtype : a.r_dtype;
+  const int c = mu ? 0 : min(ct * 16 + n, max(a.Dk - 1, 0));
+  const int64_t head = mu ? rb * a.dm_sb + kv * a.dm_sh : rb * a.R_sb + kv * a.R_sh;
+  const int64_t sd = mu ? a.dm_sd : a.R_sd;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) w[i] = 0u;
+  if (mu ? a.dm == nullptr : a.Dk == 0) return;
+  const int el = dt == F32::kRk ? 4 : 2;
+  const char* base = (const char*)(mu ? a.dm : a.R) + head * el;
+  const uint32_t col = (uint32_t)(c * (mu ? 0 : a.R_sk)) * el, row8 = (uint32_t)(8 * g * sd) * el;
+  if (a.D & 7) {
+    for (int i = 0; i < 32; ++i) {
+      const int d = 32 * (i >> 3) + 8 * g + (i & 7);
+      if (d < a.D) w[i] = dt == F32::kRk ? *(const uint32_t*)(base + d * sd * el + col)
+                                         : *(const uint16_t*)(base + d * sd * el + col);
+    }
+    return;
+  }
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    if (32 * ks >= a.D) break;
+    const uint32_t off = col + (32 * ks + 8 * g < a.D ? row8 : 0u);
+    if (dt == F32::kRk) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[8 * ks + e] = *(const uint32_t*)(base + (32 * ks + e) * sd * 4 + off);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[8 * ks + e] = *(const uint16_t*)(base + (32 * ks + e) * sd * 2 + off);
+    }
+  }
+}
+
+// The rotated queries q R and the biases q . delta_mu of a unit on the bf16
+// matrix cores: q from its exact terms `raw` [NQ][row][136], R from at most
+// three (bf16 exact in one, fp16 two, fp32 three); q R is left as NTV terms of
+// TT in `dst`.  A wave takes tiles of 16 columns, its first one (w) loaded
+// ahead.
+template <class TT, int NQ, int NTV, int NR, int KV>
+__device__ __forceinline__ void rotate_queries(const SpanArgs& a, int rb, int kv, int wave, int lane, uint32_t (&w)[32],
+                                               const uint16_t* raw, uint16_t* dst, int stride, float* bias) {
+  constexpr int kRows = 16 * NR;
+  const int g = lane >> 4, n = lane & 15;
+  const int nq = a.q_dtype == BF16::kRk ? 1 : NQ;
+  for (int ct = wave; ct <= 2 * KV; ct += kSpanWaves) {
+    if (ct != wave) load_columns<KV>(a, rb, kv, ct, g, n, w);
+    const bool mu = ct == 2 * KV;
+    const int dt = mu ? a.dm_dtype : a.r_dtype;
+    const bool have = mu ? n == 0 : ct * 16 + n < a.Dk;
+    const int nt = dt == BF16::kRk ? 1 : dt == F32::kRk ? 3 : 2;
+    f32x4 o[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) o[nr] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (32 * ks >= a.D) break;
+      float r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = have && 32 * ks + 8 * g + e < a.D ? raw_to_f32(w[8 * ks + e], dt) : 0.f;
+      uint4 t[3];
+      terms8<BF16, 3>(r, t);
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          if (q >= nq) break;
+          const uint4 x = *(const uint4*)(raw + (q * kRows + 16 * nr + n) * 136 + 32 * ks + 8 * g);
+          o[nr] = BF16::mfma(x, t[0], o[nr]);
+          if (nt > 1) o[nr] = BF16::mfma(x, t[1], o[nr]);
+          if (nt > 2) o[nr] = BF16::mfma(x, t[2], o[nr]);
+        }
+    }
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v = o[nr][i];
+        const int row = 16 * nr + 4 * g + i;
+        if (mu) {
+          if (n == 0) bias[row] = v;
+        } else {
+#pragma unroll
+          for (int t = 0; t < NTV; ++t) {
+            const uint16_t h = TT::from_f32(v);
+            dst[(t * kRows + row) * stride + ct * 16 + n] = h;
+            v -= TT::to_f32(h);
+          }
+        }
+      }
+  }
+}
+
+// Four output channels of a row, in the output's dtype.
+__device__ __forceinline__ void store_out4(const SpanArgs& a, int64_t b, int64_t h, int c, f32x4 v) {
+  const int64_t off = b * a.o_sb + h * a.o_sh + c * a.o_sd;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (c + e >= a.D) break;
+    const int64_t at = off + e * a.o_sd;
+    if (a.o_dtype == F32::kRk)
+      ((float*)a.out)[at] = v[e];
+    else
+      ((uint16_t*)a.out)[at] = a.o_dtype == F16::kRk ? F16::from_f32(v[e]) : BF16::from_f32(v[e]);
+  }
+}
+
+// JOIN: the launch behind the split one, over the suffix rows of a shared call
+// (short ones: one workgroup per unit).  It folds the other spans' records in
+// and writes the output.
+template <class F, int KV, int KF, int NR, int NT, int NP, bool VEC, bool JOIN = false>
+__global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_kernel(const SpanArgs a) {
   using TT = typename F::TT;
   constexpr int VB = KF == 2 ? 4 : 8;
   constexpr int DV = 16 * VB;
   constexpr int NTV = NT < 2 ? 2 : NT;  // terms of a rotated query
+  constexpr int NQ = NT == 3 ? 3 : 2;   // bf16 terms of a query
   constexpr int kRows = 16 * NR;
   constexpr int kWide = 32 * (KV > KF ? KV : KF) + 8;  // +8: rows start in other banks
   constexpr int kQ = kRows * kWide * (KV > 0 ? NTV : NT);
-  constexpr int kAcc = 2 * kRows * DV;  // two waves' sums
-  __shared__ __attribute__((aligned(16))) char s_mem[kQ * 2 > kAcc * 4 ? kQ * 2 : kAcc * 4];
+  constexpr int kRaw = KV > 0 ? NQ * kRows * 136 : 0;
+  constexpr int kAccRow = DV + 4;       // floats; +4: rows start in other banks
+  constexpr int kAcc = kSpanWaves * kRows * kAccRow;
+  __shared__ __attribute__((aligned(16))) char s_mem[(kQ + kRaw) * 2 > kAcc * 4 ? (kQ + kRaw) * 2 : kAcc * 4];
   __shared__ float s_bias[kRows];
-  __shared__ float s_m[kSpanWaves][kRows], s_l[kSpanWaves][kRows];
+  __shared__ float s_m[kSpanWaves][kRows], s_top[kSpanWaves][kRows], s_l[kSpanWaves][kRows];
   uint16_t* s_q = (uint16_t*)s_mem;
+  uint16_t* s_raw = s_q + kQ;
   float* s_acc = (float*)s_mem;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int id = (int)blockIdx.x;
-  const int k = id >= a.first[2] ? kTail : id >= a.first[1] ? kFull : kRotated;
+  const int k = JOIN || id >= a.first[2] ? kTail : id >= a.first[1] ? kFull : kRotated;
   const Span& sp = a.span[k];
-  const int rel = id - a.first[k];
-  const int x = rel / a.units[k], u = rel - x * a.units[k];
+  const int rel = JOIN ? id : id - a.first[k];
+  // (quotients are formed on the vector unit: back to scalar registers, so that
+  // everything derived from them stays there)
+  const int x = __builtin_amdgcn_readfirstlane(rel / a.units[k]), u = rel - x * a.units[k];
   const bool shared = a.shared && k != kTail;
   const int blocks = a.blocks[k];
-  const int ukv = u / blocks, R0 = (u - ukv * blocks) * kRows;
-  const int b = shared ? 0 : ukv / a.H, kv = shared ? ukv : ukv - b * a.H;
+  const int ukv = __builtin_amdgcn_readfirstlane(u / blocks), R0 = (u - ukv * blocks) * kRows;
+  const int b = shared ? 0 : __builtin_amdgcn_readfirstlane(ukv / a.H), kv = shared ? ukv : ukv - b * a.H;
   const int rows = min((shared ? a.B * a.G : a.G) - R0, kRows);
-
-  SpanHead hd;
-  constexpr int kEl = F::kMx ? 1 : 2;
-  hd.k = (const char*)sp.k + kEl * (b * sp.k_sb + kv * sp.k_sh);
-  hd.v = (const char*)sp.v + kEl * (b * sp.v_sb + kv * sp.v_sh);
-  if constexpr (F::kMx) {
-    hd.ksc = sp.ksc + b * sp.ksc_sb + kv * sp.ksc_sh;
-    hd.vsc = sp.vsc + b * sp.vsc_sb + kv * sp.vsc_sh;
-  }
 
   State<NR, VB> st;
 #pragma unroll
   for (int nr = 0; nr < NR; ++nr) {
-    st.m[nr] = kNegInit;
-    st.l[nr] = 0.f;
+    st.m[nr] = 0.f;
+    st.top[nr] = -INFINITY;
+    st.seen[nr] = false;
+    st.l[nr] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < VB; ++j) st.acc[nr][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
 
+  auto head = [&](auto& hd) {
+    constexpr int kEl = F::kMx ? 1 : 2;
+    // bytes to the end of the unit's last row
+    const uint32_t kb = VEC ? sp.width : (sp.width > 0 ? (sp.width - 1) * sp.k_sd + 1 : 0);
+    const uint32_t vb = VEC ? (F::kMx ? a.v_row : a.D) : (a.D - 1) * sp.v_sd + 1;
+    hd.k = make_rsrc((const char*)sp.k + kEl * (b * sp.k_sb + kv * sp.k_sh),
+                     sp.width > 0 ? kEl * (uint32_t)(sp.S - 1) * sp.k_ss + (F::kMx ? sp.k_row : kEl * kb) : 256u);
+    hd.v = make_rsrc((const char*)sp.v + kEl * (b * sp.v_sb + kv * sp.v_sh),
+                     kEl * ((uint32_t)(sp.S - 1) * sp.v_ss + vb));
+    if constexpr (F::kMx) {
+      hd.ksc = make_rsrc(sp.ksc + b * sp.ksc_sb + kv * sp.ksc_sh,
+                         (uint32_t)(max(sp.width / 32, 1) - 1) * sp.ksc_sn + (uint32_t)sp.S);
+      hd.vsc = sp.vsc + b * sp.vsc_sb + kv * sp.vsc_sh;
+    }
+  };
+  // the small loads first: loads return in order, and nothing below then waits
+  // for the first K and V block
+  Queries<NR> qw;
+  load_queries<NR>(a, shared, b, kv, R0, rows, tid, qw);
   bool done = false;
   if constexpr (KV > 0) {
     if (k == kRotated) {
-      constexpr int W = 32 * KV;
-      for (int i = tid; i < NTV * kRows * (W / 8); i += kSpanThreads) {
-        const int c = 8 * (i % (W / 8)), r = (i / (W / 8)) % kRows, t = i / (W / 8) / kRows;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows && c < a.Dkp) {
-          const RowOf o = row_of(a, shared, b, kv, R0 + r);
-          v = *(const uint4*)(a.qr + (((int64_t)o.b * a.Hq + o.h) * NTV + t) * a.Dkp + c);
-        }
-        *(uint4*)(s_q + (t * kRows + r) * kWide + c) = v;
-      }
-      for (int r = tid; r < kRows; r += kSpanThreads) {
-        float v = 0.f;
-        if (r < rows) {
-          const RowOf o = row_of(a, shared, b, kv, R0 + r);
-          v = a.bias[(int64_t)o.b * a.Hq + o.h];
-        }
-        s_bias[r] = v;
-      }
-      __syncthreads();
-      run_span<F, KV, VB, NR, NTV, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias, st);
+      uint32_t w[32];
+      if (wave <= 2 * KV) load_columns<KV>(a, shared ? 0 : b, kv, wave, g, n, w);
+      SpanLane<KV> hd;
+      head(hd);
+      auto pre = [&]() {
+        stage_queries<BF16, NQ, NR, 128>(a, tid, qw, s_raw, 136);
+        __syncthreads();
+        rotate_queries<TT, NQ, NTV, NR, KV>(a, shared ? 0 : b, kv, wave, lane, w, s_raw, s_q, kWide, s_bias);
+        __syncthreads();
+      };
+      run_span<F, KV, VB, NR, NTV, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias, st, pre);
       done = true;
     }
   }
   if (!done) {
-    constexpr int W = 32 * KF;
-    for (int i = tid; i < kRows * (W / 8); i += kSpanThreads) {
-      const int c = 8 * (i % (W / 8)), r = i / (W / 8);
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      if (r < rows) {
-        const RowOf o = row_of(a, shared, b, kv, R0 + r);
-        const int64_t off = o.b * a.q_sb + o.h * a.q_sh;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < a.D) v[e] = load_any(a.q, off + (c + e) * a.q_sd, a.q_dtype);
-      }
-      uint4 t[NT];
-      terms8<TT, NT>(v, t);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) *(uint4*)(s_q + (j * kRows + r) * kWide + c) = t[j];
-    }
-    __syncthreads();
-    run_span<F, KF, VB, NR, NT, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, st);
+    SpanLane<KF> hd;
+    head(hd);
+    auto pre = [&]() {
+      stage_queries<TT, NT, NR, 32 * KF>(a, tid, qw, s_q, kWide);
+      __syncthreads();
+    };
+    run_span<F, KF, VB, NR, NT, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, st, pre);
   }
 
-  // join the four waves: the common maximum, then sums in pairs through LDS
-  __syncthreads();
+  // from here: the true maxima, and the sum's one value; a row without tokens
+  // has the least maximum
+  float l[NR];
 #pragma unroll
   for (int nr = 0; nr < NR; ++nr) {
-    st.l[nr] += shfl_xor(st.l[nr], 16);
-    st.l[nr] += shfl_xor(st.l[nr], 32);
-    if (g == 0) {
-      s_m[wave][16 * nr + n] = st.m[nr];
-      s_l[wave][16 * nr + n] = st.l[nr];
+    l[nr] = st.l[nr][0];
+    st.top[nr] = fmaxf(st.top[nr], shfl_xor(st.top[nr], 16));
+    st.top[nr] = fmaxf(st.top[nr], shfl_xor(st.top[nr], 32));
+    st.top[nr] = st.seen[nr] ? st.top[nr] + st.m[nr] - kLift<TT> : kNegInit;
+    st.m[nr] = st.seen[nr] ? st.m[nr] : kNegInit;
+  }
+  if constexpr (JOIN) {
+    // the records of the spans before this one, shared out over the waves
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      const int r = 16 * nr + n;
+      const RowOf o = row_of(a, shared, b, kv, R0 + min(r, rows - 1));
+      const int64_t at = ((int64_t)o.b * a.Hq + o.h) * a.np;
+      for (int p = wave; p < a.np; p += kSpanWaves) {
+        const float2 ml = *(const float2*)(a.ml + 2 * (at + p));
+        f32x4 v[4][VB / 4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < VB / 4; ++j)
+            v[i][j] = *(const f32x4*)(a.acc + (at + p) * DV + (4 * g + i) * VB + 4 * j);
+        st.top[nr] = fmaxf(st.top[nr], ml.x);
+        float m_new = fmaxf(st.m[nr], ml.x);
+        const float alpha = fast_exp2(st.m[nr] - m_new), beta = fast_exp2(ml.x - m_new + kLift<TT>);
+        st.m[nr] = m_new;
+        l[nr] = l[nr] * alpha + ml.y * beta;
+#pragma unroll
+        for (int j = 0; j < VB; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.acc[nr][j][i] = st.acc[nr][j][i] * alpha + v[i][j / 4][j % 4] * beta;
+      }
     }
   }
-  __syncthreads();
-  float M[NR], L[NR];
+
+  // join the four waves: the common maximum, every wave's sums under it through
+  // LDS, then a thread adds four channels of a row
 #pragma unroll
   for (int nr = 0; nr < NR; ++nr) {
-    const int r = 16 * nr + n;
-    M[nr] = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-    L[nr] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kSpanWaves; ++w) L[nr] += s_l[w][r] * fast_exp2(s_m[w][r] - M[nr] - kLift<TT>);
-    const float f = fast_exp2(st.m[nr] - M[nr] - kLift<TT>);
-#pragma unroll
-    for (int j = 0; j < VB; ++j) st.acc[nr][j] *= f;
+    if (g == 0) {
+      s_m[wave][16 * nr + n] = st.m[nr];
+      s_top[wave][16 * nr + n] = st.top[nr];
+      s_l[wave][16 * nr + n] = l[nr];
+    }
   }
-  // s_acc[slot][row][channel]; a lane's values of one row are VB neighbours
-  auto put = [&](int slot) {
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < VB; j += 4)
-          *(f32x4*)(s_acc + ((slot * kRows + 16 * nr + n) * DV + (4 * g + i) * VB + j)) =
-              (f32x4){st.acc[nr][j][i], st.acc[nr][j + 1][i], st.acc[nr][j + 2][i], st.acc[nr][j + 3][i]};
-  };
-  auto add = [&](int slot) {
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < VB; j += 4) {
-          const f32x4 v = *(const f32x4*)(s_acc + ((slot * kRows + 16 * nr + n) * DV + (4 * g + i) * VB + j));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) st.acc[nr][j + e][i] += v[e];
-        }
-  };
-  if (wave >= 2) put(wave - 2);
-  __syncthreads();
-  if (wave < 2) add(wave);
-  __syncthreads();
-  if (wave == 1) put(0);
-  __syncthreads();
-  if (wave != 0) return;
-  add(0);
-  const int rec = sp.np0 + x;
+  __syncthreads();  // (also: no wave reads queries any more)
 #pragma unroll
   for (int nr = 0; nr < NR; ++nr) {
     const int r = 16 * nr + n;
     if (r >= rows) continue;
-    const RowOf o = row_of(a, shared, b, kv, R0 + r);
-    const int64_t at = ((int64_t)o.b * a.Hq + o.h) * a.np + rec;
+    const float M = fmaxf(fmaxf(s_top[0][r], s_top[1][r]), fmaxf(s_top[2][r], s_top[3][r]));
+    const float f = fast_exp2(st.m[nr] - M - kLift<TT>);
+    float* dst = s_acc + (wave * kRows + r) * kAccRow + 4 * g * VB;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < VB; j += 4)
-        *(f32x4*)(a.acc + at * DV + (4 * g + i) * VB + j) =
-            (f32x4){st.acc[nr][j][i], st.acc[nr][j + 1][i], st.acc[nr][j + 2][i], st.acc[nr][j + 3][i]};
-    if (g == 0) *(float2*)(a.ml + 2 * at) = make_float2(M[nr], L[nr]);
+        *(f32x4*)(dst + i * VB + j) = (f32x4){st.acc[nr][j][i] * f, st.acc[nr][j + 1][i] * f,
+                                              st.acc[nr][j + 2][i] * f, st.acc[nr][j + 3][i] * f};
+  }
+  __syncthreads();
+  const int rec = sp.np0 + x;
+  for (int i = tid; i < rows * (DV / 4); i += kSpanThreads) {
+    const int r = i / (DV / 4), c = 4 * (i % (DV / 4));
+    f32x4 v = *(const f32x4*)(s_acc + r * kAccRow + c);
+#pragma unroll
+    for (int w = 1; w < kSpanWaves; ++w) v += *(const f32x4*)(s_acc + (w * kRows + r) * kAccRow + c);
+    const RowOf o = row_of(a, shared, b, kv, R0 + r);
+    const int64_t at = ((int64_t)o.b * a.Hq + o.h) * a.np + rec;
+    if (JOIN || c == 0) {
+      const float M = fmaxf(fmaxf(s_top[0][r], s_top[1][r]), fmaxf(s_top[2][r], s_top[3][r]));
+      float L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kSpanWaves; ++w) L += s_l[w][r] * fast_exp2(s_m[w][r] - M - kLift<TT>);
+      if constexpr (JOIN)
+        store_out4(a, o.b, o.h, c, v / (L + kDenomEps));
+      else
+        *(float2*)(a.ml + 2 * at) = make_float2(M, L);
+    }
+    if constexpr (!JOIN) *(f32x4*)(a.acc + at * DV + c) = v;
   }
 }
 
@@ -565,6 +863,16 @@ hipError_t pick_widths(int kv, int kf, const SpanArgs& a, unsigned grid, hipStre
     case 2: return launch_span<F, 2, 4, NR, NT, NP, VEC>(a, grid, s);
     default: return launch_span<F, 4, 4, NR, NT, NP, VEC>(a, grid, s);
   }
+}
+
+// The suffix rows of a shared call and the join (kf as above).
+template <class F, int NT, int NP, bool VEC>
+hipError_t pick_join(int kf, const SpanArgs& a, unsigned grid, hipStream_t s) {
+  if (kf == 2)
+    hipLaunchKernelGGL((span_kernel<F, 0, 2, 1, NT, NP, VEC, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((span_kernel<F, 0, 4, 1, NT, NP, VEC, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+  return hipGetLastError();
 }
 
 }  // namespace rk

@@ -6,7 +6,12 @@ import ctypes
 import torch
 
 from rotatek_amd import _lib
-from rotatek_amd.quantized import MXRows, _same_device, check_lens, on_device
+from rotatek_amd.quantized import MXRows, check_lens, on_device, same_device
+
+# Workspace bytes that calls on queries of a shape have needed so far: a call
+# asks for as many, and sizes itself only where they do not suffice (the entry
+# point checks).
+_need: dict = {}
 
 
 def rows_of(x):
@@ -24,39 +29,52 @@ def check_query(q: torch.Tensor) -> None:
 
 
 def launch(what, q, rotation, rows, mask, lens, num_kv_groups, out, shared):
-    """Validate, allocate ``out`` [B, H_q, D] and the workspace, and launch.
+    """Validate, allocate ``out`` and the workspace, and launch; returns ``out``
+    as [B, 1, H_q, D].
 
     ``rotation``: (R_partial, delta_mu); ``rows``: (K, V) of the full-width,
     rotated and, if ``shared``, suffix spans.  The workspace is this call's
     own, from torch's allocator: calls on two streams, and graphs captured one
     after the other, share none."""
-    _same_device(what, q.device, *rotation, *rows, mask, lens, out)
+    dev = q.get_device()
+    same_device(what, dev, *rotation, *rows, mask, lens, out)
     if lens is not None:
         check_lens(lens, q.shape[0], "lens")
     lib = _lib.load()
+    desc = _lib.desc
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dq, dR, dm, do, dk = (_lib.desc(t) for t in (q, *rotation, out, mask))
-    dr = [rows_of(x) for x in rows]
-    ref = _lib.ref
-    head = (ref(dq), ref(dR), ref(dm))
-    groups, need = int(num_kv_groups), ctypes.c_size_t(0)
+        out = torch.empty((q.shape[0], 1, *q.shape[1:]), dtype=q.dtype, device=q.device)
+        do = desc(q)    # contiguous, q's sizes
+        do.data = out.data_ptr()
+        do.stride[0], do.stride[1], do.stride[2] = q.shape[1] * q.shape[2], q.shape[2], 1
+    else:
+        do = desc(out)
+        out = out.unsqueeze(1)
+    dq, dR, dm, dk = desc(q), desc(rotation[0]), desc(rotation[1]), desc(mask)
+    r = [rows_of(x) for x in rows]
+    groups = int(num_kv_groups)
     lens_ptr = None if lens is None else lens.data_ptr()
-    r = [ref(x) for x in dr]
-    with on_device(q.device):
-        if shared:
-            args = (*head, *r)
-            st = lib.rk_shared_prefix_decode_check(*args, groups, ref(do), 0, ctypes.byref(need))
-        else:
-            st = lib.rk_quantized_decode_check(*head, r[0], r[1], ref(dk), r[2], r[3], groups, ref(do), 0,
-                                               ctypes.byref(need))
-        _lib.check(st, what)
-        ws = torch.empty(max(need.value, 256), dtype=torch.uint8, device=q.device)
-        s = _lib.stream_handle(q.device)
-        if shared:
-            st = lib.rk_shared_prefix_decode(*args, lens_ptr, groups, ref(do), ws.data_ptr(), ws.numel(), s)
-        else:
-            st = lib.rk_quantized_decode(*head, r[0], r[1], ref(dk), lens_ptr, r[2], r[3], groups, ref(do),
-                                         ws.data_ptr(), ws.numel(), s)
-        _lib.check(st, what)
-    return out.unsqueeze(1)
+    key = (dev, shared, q.shape)
+    with on_device(dev):
+        s = _lib.raw_stream(dev)
+
+        def call(ws):
+            if shared:
+                return lib.rk_shared_prefix_decode(dq, dR, dm, *r, lens_ptr, groups, do, ws.data_ptr(), ws.numel(), s)
+            return lib.rk_quantized_decode(dq, dR, dm, r[0], r[1], dk, lens_ptr, r[2], r[3], groups, do, ws.data_ptr(),
+                                           ws.numel(), s)
+
+        st = call(torch.empty(_need.get(key, 256), dtype=torch.uint8, device=q.device))
+        if st == _lib.RK_ERR_WORKSPACE:
+            need = ctypes.c_size_t(0)
+            if shared:
+                st = lib.rk_shared_prefix_decode_check(dq, dR, dm, *r, groups, do, 0, need)
+            else:
+                st = lib.rk_quantized_decode_check(dq, dR, dm, r[0], r[1], dk, r[2], r[3], groups, do, 0, need)
+            _lib.check(st, what)
+            if len(_need) > 4096:
+                _need.clear()
+            _need[key] = need.value
+            st = call(torch.empty(need.value, dtype=torch.uint8, device=q.device))
+    _lib.check(st, what)
+    return out

@@ -99,23 +99,24 @@ class MXRows:
         return f"MXRows({tuple(self.shape)}, {self.fmt!r}, device={str(self.device)!r})"
 
 
-def _same_device(what: str, device: torch.device, *tensors) -> None:
-    """All on one GPU (a tensor, MXRows or None each)."""
-    if device.type != "cuda":
+def same_device(what: str, index: int, *tensors) -> None:
+    """All on GPU ``index`` (a tensor, MXRows or None each)."""
+    if index < 0:
         raise RuntimeError(f"{what}: the kernels run only on the HIP device")
     for t in tensors:
+        if t is None:
+            continue
         if isinstance(t, MXRows):
-            if t.codes.device != device or t.scales.device != device:
-                raise ValueError(f"{what}: every tensor must be on {device}")
-        elif t is not None and t.device != device:
-            raise ValueError(f"{what}: every tensor must be on {device}")
+            ok = t.codes.get_device() == index and t.scales.get_device() == index
+        else:
+            ok = t.get_device() == index
+        if not ok:
+            raise ValueError(f"{what}: every tensor must be on cuda:{index}")
 
 
-def on_device(device: torch.device):
-    """Launches go to ``device`` whichever device is current."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def on_device(index: int):
+    """Launches go to GPU ``index`` whichever is current."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def check_lens(lens: torch.Tensor, batch: int, name: str) -> None:
@@ -129,13 +130,15 @@ def quantize_rows(x: torch.Tensor, fmt: str = "mx8", out: Optional[MXRows] = Non
     _format(fmt)
     if x.dim() != 4:
         raise ValueError(f"x needs 4 dims [B, H, S, D], got shape {tuple(x.shape)}")
-    _same_device("quantize_rows", x.device, out)
+    dev = x.get_device()
+    same_device("quantize_rows", dev, out)
     if out is None:
         out = MXRows.empty(*x.shape, fmt=fmt, device=x.device)
     elif out.fmt != fmt:
         raise ValueError(f"out holds {out.fmt} rows, not {fmt}")
-    with on_device(x.device):
-        st = _lib.load().rk_mx_write(ctypes.byref(_lib.desc(x)), ctypes.byref(out.desc()), _lib.stream_handle(x.device))
+    dx, dr = _lib.desc(x), out.desc()
+    with on_device(dev):
+        st = _lib.load().rk_mx_write(ctypes.byref(dx), ctypes.byref(dr), _lib.raw_stream(dev))
     _lib.check(st, "quantize_rows")
     return out
 
@@ -144,12 +147,13 @@ def dequantize_rows(rows: MXRows, dtype: torch.dtype = torch.bfloat16,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values [B, H, S, head_dim] that ``rows`` stand for, rounded once to
     ``dtype`` (into ``out``, of any strides and its own dtype, if given)."""
-    _same_device("dequantize_rows", rows.device, rows, out)
+    dev = rows.codes.get_device()
+    same_device("dequantize_rows", dev, rows, out)
     if out is None:
         out = torch.empty(rows.shape, dtype=dtype, device=rows.device)
-    with on_device(rows.device):
-        st = _lib.load().rk_mx_read(ctypes.byref(rows.desc()), ctypes.byref(_lib.desc(out)),
-                                    _lib.stream_handle(rows.device))
+    dr, do = rows.desc(), _lib.desc(out)
+    with on_device(dev):
+        st = _lib.load().rk_mx_read(ctypes.byref(dr), ctypes.byref(do), _lib.raw_stream(dev))
     _lib.check(st, "dequantize_rows")
     return out
 
@@ -165,13 +169,13 @@ def append_rows(k_new: torch.Tensor, v_new: Optional[torch.Tensor], k_rows: MXRo
     captured in a HIP graph and replayed."""
     if (v_new is None) != (v_rows is None):
         raise ValueError("v_new and v_rows go together")
-    _same_device("append_rows", k_new.device, v_new, k_rows, v_rows, lens)
+    dev = k_new.get_device()
+    same_device("append_rows", dev, v_new, k_rows, v_rows, lens)
     check_lens(lens, k_new.shape[0], "lens")
-    dv, rv = _lib.desc(v_new), None if v_rows is None else v_rows.desc()
-    with on_device(k_new.device):
-        st = _lib.load().rk_mx_append(ctypes.byref(_lib.desc(k_new)), _lib.ref(dv), ctypes.byref(k_rows.desc()),
-                                      _lib.ref(rv), lens.data_ptr(), int(bool(advance)),
-                                      _lib.stream_handle(k_new.device))
+    dk, dv, rk, rv = _lib.desc(k_new), _lib.desc(v_new), k_rows.desc(), None if v_rows is None else v_rows.desc()
+    with on_device(dev):
+        st = _lib.load().rk_mx_append(ctypes.byref(dk), _lib.ref(dv), ctypes.byref(rk), _lib.ref(rv), lens.data_ptr(),
+                                      int(bool(advance)), _lib.raw_stream(dev))
     _lib.check(st, "append_rows")
 
 
