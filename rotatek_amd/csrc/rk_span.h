@@ -38,21 +38,35 @@ struct SpanArgs {
   // (kv, row block over the batch's queries)
   int32_t units[kSpans], blocks[kSpans];
   int32_t first[kSpans];  // first workgroup of each span
-  const void* q;
+  const void* q;       // [B, H_q, *] in whole, 16-byte aligned pieces of eight channels
   void* out;
+  const uint16_t* qr;  // rotated queries formed ahead, [row][terms][32 KV] 16 bits, or null
+  const float* bias;   // ... and q . delta_mu
   float* acc;  // [row][np][DV] partial sums
   float* ml;   // [row][np][2] running maximum and sum
-  int64_t q_sb, q_sh, q_sd, o_sb, o_sh, o_sd;
+  int64_t q_sb, q_sh, o_sb, o_sh, o_sd;
   int32_t B, Hq, H, G, D, Dk, np, shared;
   int32_t q_dtype, o_dtype;
   int32_t v_row;  // bytes of a quantised Value row
-  int32_t q_vec;  // queries in whole, 16-byte aligned pieces of eight channels
   float scale_log2;  // log2(e) / sqrt(D)
-  // the rotation of the rotated span's queries
+  // the rotation of the rotated span's queries (qr null): in q's 16-bit type,
+  // unit column stride, aligned pieces of eight channels
   const void* R;
   const void* dm;
-  int64_t R_sb, R_sh, R_sd, R_sk, dm_sb, dm_sh, dm_sd;
-  int32_t r_dtype, dm_dtype;
+  int64_t R_sb, R_sh, R_sd, dm_sb, dm_sh;
+};
+
+// Queries that the split launch does not take as they are: a copy of q in
+// whole pieces, and q R in `terms` terms with q . delta_mu.
+struct QueryArgs {
+  const void* q;
+  const void* R;
+  const void* dm;
+  void* q_out;      // [row][Dp], or null
+  uint16_t* qr;     // [row][terms][W], or null
+  float* bias;
+  int64_t q_sb, q_sh, q_sd, R_sb, R_sh, R_sd, R_sk, dm_sb, dm_sh, dm_sd;
+  int32_t Hq, G, D, Dp, Dk, W, terms, shared, q_dtype, r_dtype, dm_dtype, f16;
 };
 
 constexpr int kSpanThreads = 256;

@@ -1,7 +1,8 @@
 // rk_span.hip -- host side of the attention over quantised and shared spans
 // (rk_quantized_decode, rk_shared_prefix_decode of rotatek_hip.h): validation,
-// the split plan, and the kernel behind the split launch
-// (rk_span_dev.h): the join of a row's partial sums after it.
+// the split plan, the split launch's kernels' companions
+// (rk_span_dev.h), and two small ones: queries that it does not take as they
+// are, and the join of a row's partial sums after it.
 #include <hip/hip_runtime.h>
 #include <string.h>
 
@@ -26,6 +27,51 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
 // ---------------------------------------------------------------- kernels
+
+// The queries of calls in other layouts and types, a row per workgroup: a
+// padded copy, and q R_partial and q . delta_mu in fp32, q R stored as a sum of
+// `terms` 16-bit values (two hold 16 or more bits of it, three an fp32's 24).
+__global__ void __launch_bounds__(128) span_queries_kernel(const rk::QueryArgs a) {
+  __shared__ float s_q[128];
+  __shared__ float s_b[2];
+  const int c = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const int64_t b = row / a.Hq, h = row - b * a.Hq, kv = h / a.G, rb = a.shared ? 0 : b;
+  const float q = c < a.D ? rk::load_any(a.q, b * a.q_sb + h * a.q_sh + c * a.q_sd, a.q_dtype) : 0.f;
+  s_q[c] = q;
+  if (a.q_out && c < a.Dp) {
+    if (a.q_dtype == RK_F32)
+      ((float*)a.q_out)[row * a.Dp + c] = q;
+    else
+      ((uint16_t*)a.q_out)[row * a.Dp + c] = a.q_dtype == RK_F16 ? rk::F16::from_f32(q) : rk::BF16::from_f32(q);
+  }
+  if (!a.qr) return;
+  __syncthreads();
+  if (c < a.W) {
+    float v = 0.f;
+    if (c < a.Dk) {
+      const int64_t off = rb * a.R_sb + kv * a.R_sh + c * a.R_sk;
+      for (int d = 0; d < a.D; d += 32) {
+        float r[32];
+        rk::load_any_rows<32>(a.R, off, a.R_sd, a.r_dtype, d, a.D, r);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (d + i < a.D) v = fmaf(s_q[d + i], r[i], v);
+      }
+    }
+    for (int t = 0; t < a.terms; ++t) {
+      const uint16_t w = a.f16 ? rk::F16::from_f32(v) : rk::BF16::from_f32(v);
+      a.qr[(row * a.terms + t) * a.W + c] = w;
+      v -= a.f16 ? rk::F16::to_f32(w) : rk::BF16::to_f32(w);
+    }
+  }
+  float p = 0.f;
+  if (a.dm && c < a.D) p = q * rk::load_any(a.dm, rb * a.dm_sb + kv * a.dm_sh + c * a.dm_sd, a.dm_dtype);
+  for (int d = 32; d; d >>= 1) p += rk::shfl_xor(p, d);
+  if ((c & 63) == 0) s_b[c >> 6] = p;
+  __syncthreads();
+  if (c == 0) a.bias[row] = s_b[0] + s_b[1];
+}
 
 // Joins a row's records: out = sum_p acc_p 2^(m_p - M) / (sum_p l_p 2^(m_p -
 // M) + 1e-6).  A wave per row: four groups of 16 lanes (DV / 16 channels a
@@ -125,8 +171,9 @@ struct Plan {
   int64_t B, Hq, H, G, D, Dk;
   int format, kv, kf, nr, terms;
   bool vec, join;  // join: the suffix rows run in the launch that joins the records
+  bool copy_q, ahead;  // queries copied into whole pieces; rotated ahead of the split launch
   int64_t S[kSpans], chunk[kSpans], wgs[kSpans], units[kSpans], blocks[kSpans], np, grid, rows;
-  size_t zero, zero_bytes, acc, ml, total;
+  size_t q, qr, bias, zero, zero_bytes, acc, ml, total;
 };
 
 bool mx(const rk_rows* r) { return r->format != RK_ROWS_PLAIN; }
@@ -189,11 +236,9 @@ int make_plan(const Call& c, int cus, Plan* out) {
     p.Dk = c.R->shape[3];
     if (p.Dk < 0 || p.Dk > p.D) return RK_ERR_KEEP_DIM;
     if (c.R->shape[0] != N || c.R->shape[1] != p.H || c.R->shape[2] != p.D) return RK_ERR_SHAPE;
-    if (p.D * c.R->stride[2] + p.Dk * c.R->stride[3] >= (INT64_C(1) << 28)) return RK_ERR_STRIDE;
     if (c.dm) {
       if ((st = check_float(c.dm, 3))) return st;
       if (c.dm->shape[0] != N || c.dm->shape[1] != p.H || c.dm->shape[2] != p.D) return RK_ERR_SHAPE;
-      if (p.D * c.dm->stride[2] >= (INT64_C(1) << 28)) return RK_ERR_STRIDE;
     }
   }
   p.vec = true;
@@ -273,6 +318,17 @@ int make_plan(const Call& c, int cus, Plan* out) {
     at += (bytes + 255) & ~size_t(255);
     return here;
   };
+  // Queries as the split launch takes them: eight channels in one aligned
+  // piece; their rotation there if everything has q's 16-bit type and lies in
+  // pieces as well, else in a launch ahead.
+  p.copy_q = !rk::vec_ok(c.q) || p.D % 8 != 0;
+  p.ahead = p.kv && (p.copy_q || c.q->dtype == RK_F32 || p.Dk == 0 || c.R->dtype != c.q->dtype ||
+                     (c.R->stride[3] != 1 && p.Dk > 1) || (p.D + 32) * c.R->stride[2] >= (INT64_C(1) << 30) ||
+                     (c.dm && (c.dm->dtype != c.q->dtype || !rk::vec_ok(c.dm))));
+  const size_t el = c.q->dtype == RK_F32 ? 4 : 2;
+  p.q = take(p.copy_q ? (size_t)p.rows * round_up(p.D, 8) * el : 0);
+  p.qr = take(p.ahead ? (size_t)p.rows * std::max(p.terms, 2) * 32 * p.kv * 2 : 0);
+  p.bias = take(p.ahead ? (size_t)p.rows * 4 : 0);
   // rotated rows without channels: one zero row and its scales
   p.zero_bytes = p.kv && p.Dk == 0 ? 256 + (size_t)round_up(p.S[kRotated], 32) : 0;
   p.zero = take(p.zero_bytes);
@@ -370,10 +426,43 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
     first += p.wgs[i] * p.units[i];
     np0 += p.wgs[i];
   }
+  const hipStream_t s = (hipStream_t)stream;
+  hipError_t e = hipSuccess;
   a.q = c.q->data;
-  a.q_sb = c.q->stride[0]; a.q_sh = c.q->stride[1]; a.q_sd = c.q->stride[2];
+  a.q_sb = c.q->stride[0]; a.q_sh = c.q->stride[1];
   a.q_dtype = c.q->dtype;
-  a.q_vec = rk::vec_ok(c.q) && p.D % 8 == 0;
+  if (p.copy_q || p.ahead) {
+    rk::QueryArgs qa;
+    memset(&qa, 0, sizeof(qa));
+    qa.q = c.q->data;
+    qa.q_sb = c.q->stride[0]; qa.q_sh = c.q->stride[1]; qa.q_sd = c.q->stride[2];
+    qa.q_dtype = c.q->dtype;
+    qa.Hq = (int32_t)p.Hq; qa.G = (int32_t)p.G; qa.D = (int32_t)p.D; qa.Dp = (int32_t)round_up(p.D, 8);
+    qa.shared = c.shared;
+    if (p.copy_q) {
+      qa.q_out = ws + p.q;
+      a.q = ws + p.q;
+      a.q_sb = p.Hq * qa.Dp; a.q_sh = qa.Dp;
+    }
+    if (p.ahead) {
+      qa.R = c.R->data;
+      qa.R_sb = c.R->stride[0]; qa.R_sh = c.R->stride[1]; qa.R_sd = c.R->stride[2]; qa.R_sk = c.R->stride[3];
+      qa.r_dtype = c.R->dtype;
+      if (c.dm) {
+        qa.dm = c.dm->data;
+        qa.dm_sb = c.dm->stride[0]; qa.dm_sh = c.dm->stride[1]; qa.dm_sd = c.dm->stride[2];
+        qa.dm_dtype = c.dm->dtype;
+      }
+      qa.Dk = (int32_t)p.Dk; qa.W = 32 * p.kv; qa.terms = std::max(p.terms, 2);
+      qa.f16 = p.format == RK_ROWS_PLAIN && c.q->dtype == RK_F16;
+      qa.qr = (uint16_t*)(ws + p.qr);
+      qa.bias = (float*)(ws + p.bias);
+      a.qr = qa.qr;
+      a.bias = qa.bias;
+    }
+    hipLaunchKernelGGL(span_queries_kernel, dim3((unsigned)p.rows), dim3(128), 0, s, qa);
+    if (hipGetLastError() != hipSuccess) return RK_ERR_HIP;
+  }
   a.out = c.out->data;
   a.o_sb = c.out->stride[0]; a.o_sh = c.out->stride[1]; a.o_sd = c.out->stride[2];
   a.o_dtype = c.out->dtype;
@@ -384,21 +473,18 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
   a.shared = c.shared;
   a.v_row = p.format == RK_ROWS_PLAIN ? 0 : (int32_t)rk::mx_row_bytes(p.D, p.format);
   a.scale_log2 = rk::kLog2e / sqrtf((float)p.D);
-  const hipStream_t s = (hipStream_t)stream;
-  hipError_t e = hipSuccess;
-  if (p.kv) {
-    if (p.zero_bytes)
-      hipLaunchKernelGGL(span_zero_kernel, dim3(64), dim3(256), 0, s, (uint32_t*)(ws + p.zero),
-                         (int64_t)(p.zero_bytes / 4));
+  if (p.zero_bytes) {
+    hipLaunchKernelGGL(span_zero_kernel, dim3(64), dim3(256), 0, s, (uint32_t*)(ws + p.zero),
+                       (int64_t)(p.zero_bytes / 4));
+    if (hipGetLastError() != hipSuccess) return RK_ERR_HIP;
+  }
+  if (p.kv && !p.ahead) {
     a.R = c.R->data;
-    a.R_sb = c.R->stride[0]; a.R_sh = c.R->stride[1]; a.R_sd = c.R->stride[2]; a.R_sk = c.R->stride[3];
-    a.r_dtype = c.R->dtype;
+    a.R_sb = c.R->stride[0]; a.R_sh = c.R->stride[1]; a.R_sd = c.R->stride[2];
     if (c.dm) {
       a.dm = c.dm->data;
-      a.dm_sb = c.dm->stride[0]; a.dm_sh = c.dm->stride[1]; a.dm_sd = c.dm->stride[2];
-      a.dm_dtype = c.dm->dtype;
+      a.dm_sb = c.dm->stride[0]; a.dm_sh = c.dm->stride[1];
     }
-    if ((e = hipGetLastError()) != hipSuccess) return RK_ERR_HIP;
   }
   if (p.grid > 0) {
     const unsigned grid = (unsigned)p.grid;

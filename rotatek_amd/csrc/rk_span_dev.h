@@ -492,156 +492,167 @@ __device__ __forceinline__ RowOf row_of(const SpanArgs& a, bool shared, int b, i
 }
 
 // A unit's queries: thread i holds the i-th eight channels of every 256 of
-// them (16 to a row), as they are in memory.
-template <int NR>
+// them (16 to a row), as they are in memory (the host sees to whole, 16-byte
+// aligned pieces).  NW: 32-bit words of eight channels.
+template <int NR, int NW>
 struct Queries {
-  uint32_t w[NR][8];
+  uint32_t w[NR][NW];
 };
 
-// The loads alone: aligned rows in whole 16-byte pieces (a.q_vec), others
-// element by element as fp32.
-template <int NR>
+template <int NR, int NW>
 __device__ __forceinline__ void load_queries(const SpanArgs& a, bool shared, int b, int kv, int R0, int rows, int tid,
-                                             Queries<NR>& x) {
+                                             Queries<NR, NW>& x) {
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const int c = 8 * (tid & 15), r = 16 * i + (tid >> 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x.w[i][e] = 0u;
-    if (r >= rows || c >= a.D) continue;
-    const RowOf o = row_of(a, shared, b, kv, R0 + r);
-    const int64_t off = o.b * a.q_sb + o.h * a.q_sh + c * a.q_sd;
-    if (!a.q_vec) {
-      for (int e = 0; e < 8; ++e)
-        if (c + e < a.D) x.w[i][e] = __builtin_bit_cast(uint32_t, load_any(a.q, off + e * a.q_sd, a.q_dtype));
-    } else if (a.q_dtype == F32::kRk) {
-      load_words<4>((gptr)a.q + 4 * off, x.w[i]);
-      load_words<4>((gptr)a.q + 4 * off + 16, x.w[i] + 4);
+    for (int e = 0; e < NW; ++e) x.w[i][e] = 0u;
+    if (r < rows && c < a.D) {
+      const RowOf o = row_of(a, shared, b, kv, R0 + r);
+      const char* p = (const char*)a.q + (NW / 2) * (o.b * a.q_sb + o.h * a.q_sh + c);
+#pragma unroll
+      for (int e = 0; e < NW; e += 4) {
+        const u32x4 v = *(const u32x4*)(p + 4 * e);
+        x.w[i][e] = v.x; x.w[i][e + 1] = v.y; x.w[i][e + 2] = v.z; x.w[i][e + 3] = v.w;
+      }
+    }
+  }
+}
+
+// Eight channels of a held row as fp32.
+template <int NR, int NW>
+__device__ __forceinline__ void query8(const Queries<NR, NW>& x, int i, bool f16, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (NW == 8) {
+      v[e] = __builtin_bit_cast(float, x.w[i][e]);
     } else {
-      load_words<4>((gptr)a.q + 2 * off, x.w[i]);
+      const uint16_t h = (uint16_t)(x.w[i][e >> 1] >> (16 * (e & 1)));
+      v[e] = f16 ? F16::to_f32(h) : BF16::to_f32(h);
     }
   }
 }
 
 // ... and their NT terms of TT in LDS, [term][row][stride], zeros past the
 // head's channels and the unit's rows; channels up to kW.
-template <class TT, int NT, int NR, int kW>
-__device__ __forceinline__ void stage_queries(const SpanArgs& a, int tid, const Queries<NR>& x, uint16_t* dst,
-                                              int stride) {
+template <class TT, int NT, int NR, int NW, int kW>
+__device__ __forceinline__ void stage_queries(int tid, const Queries<NR, NW>& x, bool f16, uint16_t* dst, int stride) {
   const int c = 8 * (tid & 15);
   if (c >= kW) return;
-  const int dt = a.q_vec ? a.q_dtype : F32::kRk;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t h = x.w[i][e >> 1] >> (16 * (e & 1));
-      v[e] = dt == F32::kRk ? __builtin_bit_cast(float, x.w[i][e])
-             : dt == F16::kRk ? F16::to_f32((uint16_t)h)
-                              : BF16::to_f32((uint16_t)h);
-    }
     uint4 t[NT];
-    terms8<TT, NT>(v, t);
+    if constexpr (NT == 1) {
+      t[0] = make_uint4(x.w[i][0], x.w[i][1], x.w[i][2], x.w[i][3]);
+    } else {
+      float v[8];
+      query8(x, i, f16, v);
+      terms8<TT, NT>(v, t);
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j) *(uint4*)(dst + (j * 16 * NR + 16 * i + (tid >> 4)) * stride + c) = t[j];
   }
 }
 
-// Sixteen columns of [R_partial | delta_mu] as a matrix operand's 32 elements
-// per lane: rows 32 ks + 8 g + e of column 16 ct + n (tile 2 KV: delta_mu, in
-// column 0), raw.
+// The rotation of a unit's queries where q, R_partial and delta_mu share one
+// 16-bit type and lie in whole 16-byte pieces; other calls find q R and the
+// biases formed ahead (span_queries_kernel).
+//
+// Loads: a wave takes tiles of 16 columns of R, as a matrix operand (rows 32
+// ks + 8 g + e of column 16 ct + n, KV > 2: two tiles); a thread the eight
+// channels of delta_mu that it holds of a query.
 template <int KV>
-__device__ __forceinline__ void load_columns(const SpanArgs& a, int rb, int kv, int ct, int g, int n, uint32_t (&w)[32]) {
-  const bool mu = ct == 2 * KV;
-  const int dt = mu ? a.dm_dtype : a.r_dtype;
-  const int c = mu ? 0 : min(ct * 16 + n, max(a.Dk - 1, 0));
-  const int64_t head = mu ? rb * a.dm_sb + kv * a.dm_sh : rb * a.R_sb + kv * a.R_sh;
-  const int64_t sd = mu ? a.dm_sd : a.R_sd;
+struct Rotation {
+  static constexpr int kTiles = KV > 2 ? 2 : 1;
+  uint16_t r[kTiles][32];
+  u32x4 mu;
+};
+
+template <int KV>
+__device__ __forceinline__ void load_rotation(const SpanArgs& a, int rb, int kv, int wave, int g, int n, int tid,
+                                              Rotation<KV>& x) {
+  const int c8 = 8 * (tid & 15);
+  x.mu = (u32x4){0u, 0u, 0u, 0u};
+  if (a.dm && c8 < a.D) x.mu = *(const u32x4*)((const uint16_t*)a.dm + rb * a.dm_sb + kv * a.dm_sh + c8);
+  const uint32_t sd = (uint32_t)a.R_sd * 2u;
+  const Rsrc r = make_rsrc((const uint16_t*)a.R + rb * a.R_sb + kv * a.R_sh, (uint32_t)(a.D - 1) * sd + 2u * a.Dk);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) w[i] = 0u;
-  if (mu ? a.dm == nullptr : a.Dk == 0) return;
-  const int el = dt == F32::kRk ? 4 : 2;
-  const char* base = (const char*)(mu ? a.dm : a.R) + head * el;
-  const uint32_t col = (uint32_t)(c * (mu ? 0 : a.R_sk)) * el, row8 = (uint32_t)(8 * g * sd) * el;
-  if (a.D & 7) {
-    for (int i = 0; i < 32; ++i) {
-      const int d = 32 * (i >> 3) + 8 * g + (i & 7);
-      if (d < a.D) w[i] = dt == F32::kRk ? *(const uint32_t*)(base + d * sd * el + col)
-                                         : *(const uint16_t*)(base + d * sd * el + col);
-    }
-    return;
-  }
+  for (int t = 0; t < Rotation<KV>::kTiles; ++t) {
+    const int ct = wave + 4 * t;
+    if (ct >= 2 * KV) break;  // KV 1: two tiles in all
+    // past R's last row or column: out of the buffer's range, or a value that
+    // meets the query's zero or forms a column that no Key has
+    const uint32_t off = (uint32_t)(8 * g) * sd + 2u * (uint32_t)(ct * 16 + n);
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    if (32 * ks >= a.D) break;
-    const uint32_t off = col + (32 * ks + 8 * g < a.D ? row8 : 0u);
-    if (dt == F32::kRk) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[8 * ks + e] = *(const uint32_t*)(base + (32 * ks + e) * sd * 4 + off);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[8 * ks + e] = *(const uint16_t*)(base + (32 * ks + e) * sd * 2 + off);
-    }
+    for (int i = 0; i < 32; ++i)
+      x.r[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, (uint32_t)(32 * (i >> 3) + (i & 7)) * sd, 0);
   }
 }
 
-// The rotated queries q R and the biases q . delta_mu of a unit on the bf16
-// matrix cores: q from its exact terms `raw` [NQ][row][136], R from at most
-// three (bf16 exact in one, fp16 two, fp32 three); q R is left as NTV terms of
-// TT in `dst`.  A wave takes tiles of 16 columns, its first one (w) loaded
-// ahead.
-template <class TT, int NQ, int NTV, int NR, int KV>
-__device__ __forceinline__ void rotate_queries(const SpanArgs& a, int rb, int kv, int wave, int lane, uint32_t (&w)[32],
-                                               const uint16_t* raw, uint16_t* dst, int stride, float* bias) {
+// raw: the queries as they are, [row][136].  q R is left as NTV terms of TT in
+// `dst`, q . delta_mu in `bias`.
+template <class TT, int NTV, int NR, int KV>
+__device__ __forceinline__ void rotate_queries(const SpanArgs& a, int wave, int lane, const Rotation<KV>& x, bool f16,
+                                               const uint16_t* raw, uint16_t* dst, int stride) {
   constexpr int kRows = 16 * NR;
   const int g = lane >> 4, n = lane & 15;
-  const int nq = a.q_dtype == BF16::kRk ? 1 : NQ;
-  for (int ct = wave; ct <= 2 * KV; ct += kSpanWaves) {
-    if (ct != wave) load_columns<KV>(a, rb, kv, ct, g, n, w);
-    const bool mu = ct == 2 * KV;
-    const int dt = mu ? a.dm_dtype : a.r_dtype;
-    const bool have = mu ? n == 0 : ct * 16 + n < a.Dk;
-    const int nt = dt == BF16::kRk ? 1 : dt == F32::kRk ? 3 : 2;
+#pragma unroll
+  for (int t = 0; t < Rotation<KV>::kTiles; ++t) {
+    const int ct = wave + 4 * t;
+    if (ct >= 2 * KV) break;
+    const bool have = ct * 16 + n < a.Dk;
     f32x4 o[NR];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) o[nr] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      if (32 * ks >= a.D) break;
-      float r[8];
+      uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = have && 32 * ks + 8 * g + e < a.D ? raw_to_f32(w[8 * ks + e], dt) : 0.f;
-      uint4 t[3];
-      terms8<BF16, 3>(r, t);
+      for (int e = 0; e < 4; ++e) {
+        // a row past the head's channels may be the next head's: zero
+        const bool ok = have && 32 * ks + 8 * g < a.D;
+        w[e] = ok ? x.r[t][8 * ks + 2 * e] | (uint32_t)x.r[t][8 * ks + 2 * e + 1] << 16 : 0u;
+      }
+      const uint4 m = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          if (q >= nq) break;
-          const uint4 x = *(const uint4*)(raw + (q * kRows + 16 * nr + n) * 136 + 32 * ks + 8 * g);
-          o[nr] = BF16::mfma(x, t[0], o[nr]);
-          if (nt > 1) o[nr] = BF16::mfma(x, t[1], o[nr]);
-          if (nt > 2) o[nr] = BF16::mfma(x, t[2], o[nr]);
-        }
+      for (int nr = 0; nr < NR; ++nr) {
+        const uint4 q = *(const uint4*)(raw + (16 * nr + n) * 136 + 32 * ks + 8 * g);
+        o[nr] = f16 ? F16::mfma(q, m, o[nr]) : BF16::mfma(q, m, o[nr]);
+      }
     }
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float v = o[nr][i];
-        const int row = 16 * nr + 4 * g + i;
-        if (mu) {
-          if (n == 0) bias[row] = v;
-        } else {
 #pragma unroll
-          for (int t = 0; t < NTV; ++t) {
-            const uint16_t h = TT::from_f32(v);
-            dst[(t * kRows + row) * stride + ct * 16 + n] = h;
-            v -= TT::to_f32(h);
-          }
+        for (int k = 0; k < NTV; ++k) {
+          const uint16_t h = TT::from_f32(v);
+          dst[(k * kRows + 16 * nr + 4 * g + i) * stride + ct * 16 + n] = h;
+          v -= TT::to_f32(h);
         }
       }
+  }
+}
+
+template <int NR, int NW>
+__device__ __forceinline__ void bias_queries(const Queries<NR, NW>& q, const u32x4& mu, bool f16, int tid, float* bias) {
+  const uint32_t w[4] = {mu.x, mu.y, mu.z, mu.w};
+  float m[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    m[e] = f16 ? F16::to_f32(h) : BF16::to_f32(h);
+  }
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    float v[8], s = 0.f;
+    query8(q, i, f16, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(v[e], m[e], s);
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) s += shfl_xor(s, d);
+    if ((tid & 15) == 0) bias[16 * i + (tid >> 4)] = s;
   }
 }
 
@@ -668,11 +679,11 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_ker
   constexpr int VB = KF == 2 ? 4 : 8;
   constexpr int DV = 16 * VB;
   constexpr int NTV = NT < 2 ? 2 : NT;  // terms of a rotated query
-  constexpr int NQ = NT == 3 ? 3 : 2;   // bf16 terms of a query
+  constexpr int NW = NT == 3 ? 8 : 4;   // words of eight channels of a query
   constexpr int kRows = 16 * NR;
   constexpr int kWide = 32 * (KV > KF ? KV : KF) + 8;  // +8: rows start in other banks
   constexpr int kQ = kRows * kWide * (KV > 0 ? NTV : NT);
-  constexpr int kRaw = KV > 0 ? NQ * kRows * 136 : 0;
+  constexpr int kRaw = KV > 0 && NT < 3 ? kRows * 136 : 0;
   constexpr int kAccRow = DV + 4;       // floats; +4: rows start in other banks
   constexpr int kAcc = kSpanWaves * kRows * kAccRow;
   __shared__ __attribute__((aligned(16))) char s_mem[(kQ + kRaw) * 2 > kAcc * 4 ? (kQ + kRaw) * 2 : kAcc * 4];
@@ -686,7 +697,7 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_ker
   const int g = lane >> 4, n = lane & 15;
   const int id = (int)blockIdx.x;
   const int k = JOIN || id >= a.first[2] ? kTail : id >= a.first[1] ? kFull : kRotated;
-  const Span& sp = a.span[k];
+  const Span sp = a.span[k];  // (copied whole: few, wide scalar loads)
   const int rel = JOIN ? id : id - a.first[k];
   // (quotients are formed on the vector unit: back to scalar registers, so that
   // everything derived from them stays there)
@@ -723,21 +734,45 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_ker
       hd.vsc = sp.vsc + b * sp.vsc_sb + kv * sp.vsc_sh;
     }
   };
-  // the small loads first: loads return in order, and nothing below then waits
-  // for the first K and V block
-  Queries<NR> qw;
-  load_queries<NR>(a, shared, b, kv, R0, rows, tid, qw);
+  // The small loads first: loads return in order, and nothing below then waits
+  // for the first K and V block.
+  const bool f16 = F::kMx ? a.q_dtype == F16::kRk : TT::kRk == F16::kRk;
+  Queries<NR, NW> qw;
   bool done = false;
   if constexpr (KV > 0) {
     if (k == kRotated) {
-      uint32_t w[32];
-      if (wave <= 2 * KV) load_columns<KV>(a, shared ? 0 : b, kv, wave, g, n, w);
       SpanLane<KV> hd;
       head(hd);
+      const bool here = NT < 3 && !a.qr;
+      Rotation<KV> rot;
+      if (here) {
+        load_queries<NR, NW>(a, shared, b, kv, R0, rows, tid, qw);
+        load_rotation<KV>(a, shared ? 0 : b, kv, wave, g, n, tid, rot);
+      }
       auto pre = [&]() {
-        stage_queries<BF16, NQ, NR, 128>(a, tid, qw, s_raw, 136);
-        __syncthreads();
-        rotate_queries<TT, NQ, NTV, NR, KV>(a, shared ? 0 : b, kv, wave, lane, w, s_raw, s_q, kWide, s_bias);
+        if (here) {
+          if constexpr (NT < 3) {
+            stage_queries<TT, 1, NR, NW, 128>(tid, qw, f16, s_raw, 136);
+            bias_queries(qw, rot.mu, f16, tid, s_bias);
+            __syncthreads();
+            rotate_queries<TT, NTV, NR, KV>(a, wave, lane, rot, f16, s_raw, s_q, kWide);
+          }
+        } else {
+          constexpr int W = 32 * KV;
+          for (int i = tid; i < NTV * kRows * (W / 8); i += kSpanThreads) {
+            const int c = 8 * (i % (W / 8)), r = (i / (W / 8)) % kRows, t = i / (W / 8) / kRows;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < rows) {
+              const RowOf o = row_of(a, shared, b, kv, R0 + r);
+              v = *(const uint4*)(a.qr + (((int64_t)o.b * a.Hq + o.h) * NTV + t) * W + c);
+            }
+            *(uint4*)(s_q + (t * kRows + r) * kWide + c) = v;
+          }
+          if (tid < kRows) {
+            const RowOf o = row_of(a, shared, b, kv, R0 + min(tid, rows - 1));
+            s_bias[tid] = a.bias[(int64_t)o.b * a.Hq + o.h];
+          }
+        }
         __syncthreads();
       };
       run_span<F, KV, VB, NR, NTV, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias, st, pre);
@@ -747,8 +782,9 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_ker
   if (!done) {
     SpanLane<KF> hd;
     head(hd);
+    load_queries<NR, NW>(a, shared, b, kv, R0, rows, tid, qw);
     auto pre = [&]() {
-      stage_queries<TT, NT, NR, 32 * KF>(a, tid, qw, s_q, kWide);
+      stage_queries<TT, NT, NR, NW, 32 * KF>(tid, qw, f16, s_q, kWide);
       __syncthreads();
     };
     run_span<F, KF, VB, NR, NT, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, st, pre);
