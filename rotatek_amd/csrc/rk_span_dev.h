@@ -127,16 +127,18 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* p, uint32_t bytes) {
                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32;
   return __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, (int)__builtin_amdgcn_readfirstlane((int)bytes), 0x00027000);
 }
-template <int N>
+// AUX 2: non-temporal, for rows that one instruction reads whole lines of and
+// that no other unit reads.
+template <int N, int AUX = 0>
 __device__ __forceinline__ void load_words(Rsrc r, uint32_t off, uint32_t base, uint32_t* w) {
   if constexpr (N == 4) {
-    const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, base, 0));
+    const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, base, AUX));
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   } else if constexpr (N == 2) {
-    const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, base, 0));
+    const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, base, AUX));
     w[0] = v.x; w[1] = v.y;
   } else {
-    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, base, 0);
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, base, AUX);
   }
 }
 
@@ -185,7 +187,7 @@ __device__ __forceinline__ int block_row(const Span& sp, int blk) {
   return min(blk * kSpanBlk, max(sp.S - kSpanBlk, 0));
 }
 
-template <class F, int KB, int VB, bool VEC>
+template <class F, int KB, int VB, bool VEC, int AUX>
 __device__ __forceinline__ void load_k(const Span& sp, const SpanLane<KB>& hd, int blk, int g, Block<F, KB, VB>& x) {
   const uint32_t t0 = block_row(sp, blk), base = t0 * sp.k_ss * (F::kMx ? 1 : 2);
 #pragma unroll
@@ -196,7 +198,7 @@ __device__ __forceinline__ void load_k(const Span& sp, const SpanLane<KB>& hd, i
         load_words<4>(hd.k, hd.ko[tt], base, x.k[tt]);
         load_words<4>(hd.k, hd.ko[tt] + 16, base, x.k[tt] + 4);
       } else {
-        load_words<kAll>(hd.k, hd.ko[tt], base, x.k[tt]);
+        load_words<kAll, KB == 1 ? AUX : 0>(hd.k, hd.ko[tt], base, x.k[tt]);
       }
       x.ks[tt] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(hd.ksc, hd.so[tt], t0, 0);
     } else if constexpr (VEC) {
@@ -222,7 +224,7 @@ __device__ __forceinline__ void load_k(const Span& sp, const SpanLane<KB>& hd, i
   }
 }
 
-template <class F, int KB, int VB, bool VEC>
+template <class F, int KB, int VB, bool VEC, int AUX>
 __device__ __forceinline__ void load_v(const Span& sp, const SpanLane<KB>& hd, int D, int blk, int n,
                                        Block<F, KB, VB>& x) {
   const uint32_t t0 = block_row(sp, blk), base = t0 * sp.v_ss * (F::kMx ? 1 : 2);
@@ -230,13 +232,13 @@ __device__ __forceinline__ void load_v(const Span& sp, const SpanLane<KB>& hd, i
   for (int r = 0; r < 8; ++r) {
     if constexpr (F::kMx) {
       if constexpr (VB == 8)
-        load_words<F::kw>(hd.v, hd.vo[r], base, x.v[r]);
+        load_words<F::kw, AUX>(hd.v, hd.vo[r], base, x.v[r]);
       else if constexpr (F::kw == 2)
-        load_words<1>(hd.v, hd.vo[r], base, x.v[r]);
+        load_words<1, AUX>(hd.v, hd.vo[r], base, x.v[r]);
       else
         x.v[r][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(hd.v, hd.vo[r], base, 0);
     } else if constexpr (VEC) {
-      load_words<VB / 2>(hd.v, hd.vo[r], base, x.v[r]);
+      load_words<VB / 2, AUX>(hd.v, hd.vo[r], base, x.v[r]);
     } else {
       const int cv = n * VB < D ? n * VB : 0;
 #pragma unroll
@@ -327,9 +329,10 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
   // past the wave's last block the ring reads that block again
   auto blk_of = [&](int i) { return blk0 + kSpanWaves * min(i, max(nw - 1, 0)); };
   lane_offsets<F, KB, VB>(sp, a.D, g, n, hd);
+  constexpr int kAux = NR == 1 ? 2 : 0;
   Block<F, KB, VB> buf;
-  load_k<F, KB, VB, VEC>(sp, hd, blk_of(0), g, buf);
-  load_v<F, KB, VB, VEC>(sp, hd, a.D, blk_of(0), n, buf);
+  load_k<F, KB, VB, VEC, kAux>(sp, hd, blk_of(0), g, buf);
+  load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, blk_of(0), n, buf);
   pre();
   constexpr bool kRegQ = NR * NT * KB <= (NR == 1 ? 12 : 8);  // queries held in registers
   uint4 qreg[kRegQ ? NR : 1][kRegQ ? NT : 1][kRegQ ? KB : 1];
@@ -376,7 +379,7 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
               s[tt][nr] = TT::mfma(kop, qload(nr, t, j), s[tt][nr]);
           }
       }
-    load_k<F, KB, VB, VEC>(sp, hd, next, g, x);
+    load_k<F, KB, VB, VEC, kAux>(sp, hd, next, g, x);
     // which of the lane's eight tokens count
     const int t0 = block_row(sp, blk) + 8 * g;
     uint32_t on = 0xffu;
@@ -388,6 +391,15 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
         bool ok = t0 + r >= blk * kSpanBlk && t0 + r < lim;
         if (sp.mask && ok) ok = sp.mask[b * sp.m_sb + (t0 + r) * sp.m_ss] != 0;
         on |= (uint32_t)ok << r;
+        // a row that does not count holds anything: 0 x NaN must not reach the
+        // sum.  (Here, under the branch: as selects at V^T they would run in
+        // every block, 64 of 233 vector instructions.)
+        if constexpr (F::kMx) {
+          uint32_t& vs = r < 4 ? x.vs.x : x.vs.y;
+          vs = ok ? vs : vs & ~(0xffu << (8 * (r & 3)));
+        }
+#pragma unroll
+        for (int w = 0; w < Block<F, KB, VB>::kvw; ++w) x.v[r][w] = ok ? x.v[r][w] : 0u;
       }
     }
     // V^T of channel slots 2 w and 2 w + 1: eight tokens of each
@@ -404,8 +416,6 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
         } else {
           y[r] = x.v[r][w];
         }
-        // rows that do not count hold anything: 0 x NaN must not reach the sum
-        if (!whole) y[r] = (on >> r) & 1u ? y[r] : 0u;
       }
       lo = make_uint4(pack_lo(y[0], y[1]), pack_lo(y[2], y[3]), pack_lo(y[4], y[5]), pack_lo(y[6], y[7]));
       hi = make_uint4(pack_hi(y[0], y[1]), pack_hi(y[2], y[3]), pack_hi(y[4], y[5]), pack_hi(y[6], y[7]));
@@ -415,7 +425,7 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
     if constexpr (NR > 1) {
 #pragma unroll
       for (int w = 0; w < VB / 2; ++w) turn(w, av[2 * w], av[2 * w + 1]);
-      load_v<F, KB, VB, VEC>(sp, hd, a.D, next, n, x);
+      load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, next, n, x);
     }
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -472,7 +482,7 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
             st.acc[nr][2 * w + 1] = TT::mfma(hi, p[t], st.acc[nr][2 * w + 1]);
           }
         }
-        load_v<F, KB, VB, VEC>(sp, hd, a.D, next, n, x);
+        load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, next, n, x);
       }
     }
   };
@@ -670,9 +680,43 @@ __device__ __forceinline__ void store_out4(const SpanArgs& a, int64_t b, int64_t
   }
 }
 
+// Four channels of a row's suffix sums (M, L, v) joined with the records of the
+// spans before it, eight records' loads in flight, and written out.
+template <int DV>
+__device__ __forceinline__ void join_records(const SpanArgs& a, const RowOf& o, int c, float M, float L, f32x4 v) {
+  constexpr int NB = 8;
+  const int64_t at = ((int64_t)o.b * a.Hq + o.h) * a.np;
+  const float2* ml = (const float2*)a.ml + at;
+  const float* acc = a.acc + at * DV + c;
+  for (int p = 0; p < a.np; p += NB) {
+    float2 r[NB];
+    f32x4 x[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int q = min(p + i, a.np - 1);  // past the last: it again, with weight 0
+      r[i] = ml[q];
+      x[i] = *(const f32x4*)(acc + (int64_t)q * DV);
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) top = fmaxf(top, r[i].x);
+    const float f = fast_exp2(M - top);
+    M = top;
+    L *= f;
+    v *= f;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const float w = p + i < a.np ? fast_exp2(r[i].x - M) : 0.f;
+      L = fmaf(r[i].y, w, L);
+      v += x[i] * w;
+    }
+  }
+  store_out4(a, o.b, o.h, c, v / (L + kDenomEps));
+}
+
 // JOIN: the launch behind the split one, over the suffix rows of a shared call
-// (short ones: one workgroup per unit).  It folds the other spans' records in
-// and writes the output.
+// (short ones: one workgroup per unit).  It joins the other spans' records to
+// its sums and writes the output.
 template <class F, int KV, int KF, int NR, int NT, int NP, bool VEC, bool JOIN = false>
 __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_kernel(const SpanArgs a) {
   using TT = typename F::TT;
@@ -801,34 +845,6 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_ker
     st.top[nr] = st.seen[nr] ? st.top[nr] + st.m[nr] - kLift<TT> : kNegInit;
     st.m[nr] = st.seen[nr] ? st.m[nr] : kNegInit;
   }
-  if constexpr (JOIN) {
-    // the records of the spans before this one, shared out over the waves
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      const int r = 16 * nr + n;
-      const RowOf o = row_of(a, shared, b, kv, R0 + min(r, rows - 1));
-      const int64_t at = ((int64_t)o.b * a.Hq + o.h) * a.np;
-      for (int p = wave; p < a.np; p += kSpanWaves) {
-        const float2 ml = *(const float2*)(a.ml + 2 * (at + p));
-        f32x4 v[4][VB / 4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < VB / 4; ++j)
-            v[i][j] = *(const f32x4*)(a.acc + (at + p) * DV + (4 * g + i) * VB + 4 * j);
-        st.top[nr] = fmaxf(st.top[nr], ml.x);
-        float m_new = fmaxf(st.m[nr], ml.x);
-        const float alpha = fast_exp2(st.m[nr] - m_new), beta = fast_exp2(ml.x - m_new + kLift<TT>);
-        st.m[nr] = m_new;
-        l[nr] = l[nr] * alpha + ml.y * beta;
-#pragma unroll
-        for (int j = 0; j < VB; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) st.acc[nr][j][i] = st.acc[nr][j][i] * alpha + v[i][j / 4][j % 4] * beta;
-      }
-    }
-  }
-
   // join the four waves: the common maximum, every wave's sums under it through
   // LDS, then a thread adds four channels of a row
 #pragma unroll
@@ -869,7 +885,7 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_ker
 #pragma unroll
       for (int w = 0; w < kSpanWaves; ++w) L += s_l[w][r] * fast_exp2(s_m[w][r] - M - kLift<TT>);
       if constexpr (JOIN)
-        store_out4(a, o.b, o.h, c, v / (L + kDenomEps));
+        join_records<DV>(a, o, c, M, L, v);
       else
         *(float2*)(a.ml + 2 * at) = make_float2(M, L);
     }
