@@ -36,7 +36,7 @@ struct SpanArgs {
   Span span[kSpans];
   // units: (b, kv, row block) or, where the batch shares the span's rows,
   // (kv, row block over the batch's queries)
-  int32_t units[kSpans], blocks[kSpans];
+  int32_t heads[kSpans], blocks[kSpans];  // heads: (b, kv) or kv; blocks: row blocks of each
   int32_t first[kSpans];  // first workgroup of each span
   const void* q;       // [B, H_q, *] in whole, 16-byte aligned pieces of eight channels
   void* out;

@@ -309,7 +309,7 @@ int make_plan(const Call& c, int cus, Plan* out) {
     p.chunk[kTail] = round_up(p.S[kTail], align);
     p.wgs[kTail] = 1;
   }
-  if (p.grid >= (INT64_C(1) << 31) || p.rows >= (INT64_C(1) << 31) || p.rows * p.np >= (INT64_C(1) << 40))
+  if (p.grid + 24 * p.units[0] + 24 * p.units[1] + 24 * p.units[2] >= (INT64_C(1) << 31) || p.rows >= (INT64_C(1) << 31) || p.rows * p.np >= (INT64_C(1) << 40))
     return RK_ERR_SHAPE;
   const int64_t dv = p.kf == 2 ? 64 : 128;
   size_t at = 0;
@@ -391,6 +391,11 @@ Span make_span(const Call& c, const Plan& p, int i, char* ws) {
   return s;
 }
 
+// Workgroup ids of a span: eight (chunk, head) pairs' row blocks at a time.
+int64_t launched(const Plan& p, int i) {
+  return p.S[i] == 0 ? 0 : 8 * p.blocks[i] * cdiv(p.wgs[i] * (p.units[i] / p.blocks[i]), 8);
+}
+
 int resolve_cus(int num_cus, int* st) {
   *st = RK_OK;
   if (num_cus > 0) return num_cus;
@@ -417,13 +422,13 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
   int64_t first = 0, np0 = 0;
   for (int i = 0; i < kSpans; ++i) {
     a.first[i] = (int32_t)first;
-    a.units[i] = (int32_t)std::max<int64_t>(p.units[i], 1);
-    a.blocks[i] = (int32_t)p.blocks[i];
+    a.heads[i] = (int32_t)std::max<int64_t>(p.units[i] / std::max<int64_t>(p.blocks[i], 1), 1);
+    a.blocks[i] = (int32_t)std::max<int64_t>(p.blocks[i], 1);
     if (p.S[i] == 0) continue;
     a.span[i] = make_span(c, p, i, ws);
     a.span[i].np0 = (int32_t)np0;
     if (p.join && i == kTail) break;
-    first += p.wgs[i] * p.units[i];
+    first += launched(p, i);
     np0 += p.wgs[i];
   }
   const hipStream_t s = (hipStream_t)stream;
@@ -486,8 +491,8 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
       a.dm_sb = c.dm->stride[0]; a.dm_sh = c.dm->stride[1];
     }
   }
-  if (p.grid > 0) {
-    const unsigned grid = (unsigned)p.grid;
+  if (first > 0) {
+    const unsigned grid = (unsigned)first;
     if (p.format == RK_ROWS_MX8)
       e = rk::span_launch_mx8(p.kv, p.kf, p.nr, p.terms, a, grid, s);
     else if (p.format == RK_ROWS_MX4)
@@ -499,7 +504,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
     if (e != hipSuccess) return RK_ERR_HIP;
   }
   if (p.join) {
-    const unsigned grid = (unsigned)p.units[kTail];
+    const unsigned grid = (unsigned)launched(p, kTail);
     if (p.format == RK_ROWS_MX8)
       e = rk::span_join_mx8(p.kf, p.terms, a, grid, s);
     else if (p.format == RK_ROWS_MX4)

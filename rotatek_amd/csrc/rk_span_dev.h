@@ -19,8 +19,8 @@
 //                 any order of channels will do as long as Q has the same;
 //   O^T += V^T P^T  A = V^T: a lane holds eight tokens of VB channels as it
 //                 loads them and transposes them in registers.  P^T is the
-//                 lane's own eight scores: A's rows are dealt so that the
-//                 lane (g, n) gets tokens 8g .. 8g + 7 of query n.
+//                 lane's own eight scores: lane (g, n) gets tokens 4g .. 4g + 3
+//                 and 16 + 4g .. 16 + 4g + 3 of query n.
 // Quantised rows are widened to bf16, which holds code 2^e exactly, by the
 // conversion that applies the block's scale; queries then enter as one, two
 // or three bf16 terms, in which bf16, fp16 and fp32 are exact.
@@ -106,7 +106,10 @@ __device__ __forceinline__ void load_words(gptr p, uint32_t* w) {
 }
 
 // A block of 32 tokens as one wave holds it.  k[tt]: the lane's 8 KB channels
-// of token 8 (n / 4) + 4 tt + n % 4; v[r]: its VB channels of token 8 g + r.
+// of token 16 tt + n; v[r]: its VB channels of token token_of(g, r).  (A tile's
+// 16 rows are neighbours: the 16 lanes that load one piece of them touch the
+// fewest cache lines.)
+__device__ __forceinline__ int token_of(int g, int r) { return 16 * (r >> 2) + 4 * g + (r & 3); }
 template <class F, int KB, int VB>
 struct Block {
   static constexpr int kvw = VB == 8 ? F::kw : (F::kw + 1) / 2;
@@ -156,7 +159,7 @@ __device__ __forceinline__ void lane_offsets(const Span& sp, int D, int g, int n
   const int cv = n * VB < D ? n * VB : 0;    // lanes past the head's channels: any will do
 #pragma unroll
   for (int tt = 0; tt < 2; ++tt) {
-    const uint32_t t = min((uint32_t)(8 * (n >> 2) + 4 * tt + (n & 3)), last);
+    const uint32_t t = min((uint32_t)(16 * tt + n), last);
     if constexpr (F::kMx) {
       // eight KB channels in one piece; past the row's width the first ones
       // stand in (the query is zero there)
@@ -173,13 +176,13 @@ __device__ __forceinline__ void lane_offsets(const Span& sp, int D, int g, int n
   }
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
-    const uint32_t t = min((uint32_t)(8 * g + r), last);
+    const uint32_t t = min((uint32_t)token_of(g, r), last);
     if constexpr (F::kMx)
       x.vo[r] = t * sp.v_ss + (F::kw == 2 ? cv : cv >> 1);
     else
       x.vo[r] = 2 * (t * sp.v_ss + (uint32_t)cv);
   }
-  if constexpr (F::kMx) x.vso = (cv >> 5) * sp.vsc_sn + 8 * g;
+  if constexpr (F::kMx) x.vso = (cv >> 5) * sp.vsc_sn + 4 * g;
 }
 
 // First row of a block: the span's last block ends with the span.
@@ -255,7 +258,16 @@ __device__ __forceinline__ void load_v(const Span& sp, const SpanLane<KB>& hd, i
     }
   }
   // eight tokens' scales of the lane's block column, at any byte address
-  if constexpr (F::kMx) __builtin_memcpy(&x.vs, hd.vsc + t0 + hd.vso, 8);
+  if constexpr (F::kMx) {
+    __builtin_memcpy(&x.vs.x, hd.vsc + t0 + hd.vso, 4);
+    __builtin_memcpy(&x.vs.y, hd.vsc + t0 + hd.vso + 16, 4);
+  }
+}
+
+// Blocks of a wave in flight.
+template <class F, int NR, int NT>
+constexpr int blocks_ahead() {
+  return F::kMx && NR == 1 ? 1 : 1;
 }
 
 // Values as the products take them: x as the sum of NT 16-bit terms.
@@ -329,12 +341,17 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
   // past the wave's last block the ring reads that block again
   auto blk_of = [&](int i) { return blk0 + kSpanWaves * min(i, max(nw - 1, 0)); };
   lane_offsets<F, KB, VB>(sp, a.D, g, n, hd);
-  constexpr int kAux = NR == 1 ? 2 : 0;
-  Block<F, KB, VB> buf;
-  load_k<F, KB, VB, VEC, kAux>(sp, hd, blk_of(0), g, buf);
-  load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, blk_of(0), n, buf);
+  // rows of whole lines: 16 lanes' Value channels, four rows of 32 Key channels
+  constexpr int kAux = NR == 1 && Block<F, KB, VB>::kvw * 64 >= 128 ? 2 : 0;
+  constexpr int NBUF = blocks_ahead<F, NR, NT>();
+  Block<F, KB, VB> buf[NBUF];
+#pragma unroll
+  for (int i = 0; i < NBUF; ++i) {
+    load_k<F, KB, VB, VEC, kAux>(sp, hd, blk_of(i), g, buf[i]);
+    load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, blk_of(i), n, buf[i]);
+  }
   pre();
-  constexpr bool kRegQ = NR * NT * KB <= (NR == 1 ? 12 : 8);  // queries held in registers
+  constexpr bool kRegQ = NR * NT * KB <= (NR == 1 ? (F::kMx ? 4 : 8) : 8);  // queries held in registers
   uint4 qreg[kRegQ ? NR : 1][kRegQ ? NT : 1][kRegQ ? KB : 1];
   auto qload = [&](int nr, int t, int j) {
     const int c = F::kMx ? 8 * KB * g + 8 * j : 32 * j + 8 * g;
@@ -381,15 +398,16 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
       }
     load_k<F, KB, VB, VEC, kAux>(sp, hd, next, g, x);
     // which of the lane's eight tokens count
-    const int t0 = block_row(sp, blk) + 8 * g;
+    const int t0 = block_row(sp, blk);
     uint32_t on = 0xffu;
     const bool whole = (blk + 1) * kSpanBlk <= lim && !sp.mask;
     if (!whole) {
       on = 0;
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        bool ok = t0 + r >= blk * kSpanBlk && t0 + r < lim;
-        if (sp.mask && ok) ok = sp.mask[b * sp.m_sb + (t0 + r) * sp.m_ss] != 0;
+        const int t = t0 + token_of(g, r);
+        bool ok = t >= blk * kSpanBlk && t < lim;
+        if (sp.mask && ok) ok = sp.mask[b * sp.m_sb + t * sp.m_ss] != 0;
         on |= (uint32_t)ok << r;
         // a row that does not count holds anything: 0 x NaN must not reach the
         // sum.  (Here, under the branch: as selects at V^T they would run in
@@ -487,7 +505,11 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
     }
   };
 
-  for (int i = 0; i < nw; ++i) compute(buf, blk_of(i), blk_of(i + 1));
+  for (int i = 0; i < nw; i += NBUF) {
+#pragma unroll
+    for (int j = 0; j < NBUF; ++j)
+      if (j == 0 || i + j < nw) compute(buf[j], blk_of(i + j), blk_of(i + j + NBUF));
+  }
 }
 
 // Query row R of a unit: its batch row and head.
@@ -718,7 +740,7 @@ __device__ __forceinline__ void join_records(const SpanArgs& a, const RowOf& o, 
 // (short ones: one workgroup per unit).  It joins the other spans' records to
 // its sums and writes the output.
 template <class F, int KV, int KF, int NR, int NT, int NP, bool VEC, bool JOIN = false>
-__global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_kernel(const SpanArgs a) {
+__global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3) : 2) span_kernel(const SpanArgs a) {
   using TT = typename F::TT;
   constexpr int VB = KF == 2 ? 4 : 8;
   constexpr int DV = 16 * VB;
@@ -743,12 +765,17 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? 3 : 2) span_ker
   const int k = JOIN || id >= a.first[2] ? kTail : id >= a.first[1] ? kFull : kRotated;
   const Span sp = a.span[k];  // (copied whole: few, wide scalar loads)
   const int rel = JOIN ? id : id - a.first[k];
-  // (quotients are formed on the vector unit: back to scalar registers, so that
-  // everything derived from them stays there)
-  const int x = __builtin_amdgcn_readfirstlane(rel / a.units[k]), u = rel - x * a.units[k];
+  // Workgroups go to the 8 XCDs, each with an L2 of its own, in turn: the row
+  // blocks that read the same rows are 8 ids apart, on one XCD (32 requests of
+  // 4 heads behind 16001 tokens: TTT us).  The last of the ids may have none.
+  // (Quotients are formed on the vector unit: back to scalar registers, so that
+  // everything derived from them stays there.)
   const bool shared = a.shared && k != kTail;
-  const int blocks = a.blocks[k];
-  const int ukv = __builtin_amdgcn_readfirstlane(u / blocks), R0 = (u - ukv * blocks) * kRows;
+  const int blocks = a.blocks[k], heads = a.heads[k];
+  const int q8 = __builtin_amdgcn_readfirstlane((rel >> 3) / blocks);
+  const int t = 8 * q8 + (rel & 7), R0 = ((rel >> 3) - q8 * blocks) * kRows;
+  const int x = __builtin_amdgcn_readfirstlane(t / heads), ukv = t - x * heads;
+  if (x >= sp.wgs) return;
   const int b = shared ? 0 : __builtin_amdgcn_readfirstlane(ukv / a.H), kv = shared ? ukv : ukv - b * a.H;
   const int rows = min((shared ? a.B * a.G : a.G) - R0, kRows);
 
