@@ -88,4 +88,11 @@ hipError_t span_join_bf16(int kf, bool vec, const SpanArgs& a, unsigned grid, hi
 hipError_t span_join_mx8(int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
 hipError_t span_join_mx4(int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
 
+// The split launch over rows that more than 32 queries share, 64 of them a
+// workgroup (rk_tile_dev.h).
+hipError_t tile_launch_f16(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t tile_launch_bf16(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t tile_launch_mx8(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t tile_launch_mx4(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
+
 }  // namespace rk

@@ -154,6 +154,8 @@ __global__ void __launch_bounds__(256) span_zero_kernel(uint32_t* p, int64_t n) 
 // Suffix rows up to this many are attended in the joining launch, one
 // workgroup per request and KV head; more are split like the other spans.
 constexpr int64_t kJoinTokens = 1024;
+// Queries on the same rows past which the waves take queries instead of tokens.
+constexpr int64_t kTileRows = 32;
 // Bytes a workgroup streams at most.
 constexpr int64_t kMaxShare = INT64_C(512) << 10;
 
@@ -171,6 +173,7 @@ struct Plan {
   int64_t B, Hq, H, G, D, Dk;
   int format, kv, kf, nr, terms;
   bool vec, join;  // join: the suffix rows run in the launch that joins the records
+  bool tile;           // rk_tile_dev.h over the shared spans, 64 queries a workgroup
   bool copy_q, ahead;  // queries copied into whole pieces; rotated ahead of the split launch
   int64_t S[kSpans], chunk[kSpans], wgs[kSpans], units[kSpans], blocks[kSpans], np, grid, rows;
   size_t q, qr, bias, zero, zero_bytes, acc, ml, total;
@@ -272,13 +275,15 @@ int make_plan(const Call& c, int cus, Plan* out) {
   // K and V (element loads and fp32 queries stay at 16)
   const int64_t rows = c.shared ? p.B * p.G : p.G;
   p.nr = rows <= 16 || !p.vec || p.terms == 3 ? 1 : 2;
+  // more than 32: the waves of a workgroup take queries, not tokens
+  p.tile = c.shared && rows > kTileRows && p.vec && p.terms < 3;
   p.rows = p.B * p.Hq;
-  const int64_t unit_rows = 16 * p.nr;
   p.join = c.shared && p.S[kTail] > 0 && p.S[kTail] <= kJoinTokens;
   int64_t cost[kSpans], total = 0;  // bytes of a token; of all units
   for (int i = 0; i < kSpans; ++i) {
     const bool per_request = !c.shared || i == kTail;
-    const int64_t r = p.join && i == kTail ? 16 : unit_rows;
+    const bool tiles = p.tile && i != kTail;
+    const int64_t r = tiles ? 64 : p.join && i == kTail ? 16 : 16 * p.nr;
     p.blocks[i] = cdiv(per_request ? p.G : p.B * p.G, r);
     p.units[i] = p.H * p.blocks[i] * (per_request ? p.B : 1);
     const int64_t kd = i == kRotated ? p.Dk : p.D;
@@ -288,25 +293,33 @@ int make_plan(const Call& c, int cus, Plan* out) {
   // Equal shares of the bytes for every workgroup, of whole rounds of the
   // workgroups that are resident at a time: the fewest rounds that keep a
   // share at kMaxShare, and within them the largest grid that fits.
-  const int64_t slots = (int64_t)cus * (p.nr == 1 ? 3 : 2);
-  const int64_t rounds = std::max<int64_t>(cdiv(total, slots * kMaxShare), 1);
-  const int64_t align = rk::kSpanWaves * rk::kSpanBlk;
-  for (int64_t share = std::max<int64_t>(cdiv(total, slots * rounds), 1);; share += cdiv(share, 32)) {
-    p.np = p.grid = 0;
-    bool least = true;  // one workgroup per unit and span
-    for (int i = 0; i < kSpans; ++i) {
-      p.wgs[i] = p.chunk[i] = 0;
-      if (p.S[i] == 0 || (p.join && i == kTail)) continue;
-      p.chunk[i] = std::min(round_up(cdiv(share, cost[i]), align), round_up(p.S[i], align));
-      p.wgs[i] = cdiv(p.S[i], p.chunk[i]);
-      least = least && p.wgs[i] == 1;
-      p.np += p.wgs[i];
-      p.grid += p.wgs[i] * p.units[i];
+  auto split = [&](int64_t slots) {
+    const int64_t rounds = std::max<int64_t>(cdiv(total, slots * kMaxShare), 1);
+    const int64_t align = rk::kSpanWaves * rk::kSpanBlk;
+    for (int64_t share = std::max<int64_t>(cdiv(total, slots * rounds), 1);; share += cdiv(share, 32)) {
+      p.np = p.grid = 0;
+      bool least = true;  // one workgroup per unit and span
+      for (int i = 0; i < kSpans; ++i) {
+        p.wgs[i] = p.chunk[i] = 0;
+        if (p.S[i] == 0 || (p.join && i == kTail)) continue;
+        p.chunk[i] = std::min(round_up(cdiv(share, cost[i]), align), round_up(p.S[i], align));
+        p.wgs[i] = cdiv(p.S[i], p.chunk[i]);
+        least = least && p.wgs[i] == 1;
+        p.np += p.wgs[i];
+        p.grid += p.wgs[i] * p.units[i];
+      }
+      if (least || p.grid <= slots * rounds) break;
     }
-    if (least || p.grid <= slots * rounds) break;
-  }
+  };
+  // Three workgroups are resident on a CU (two of 32 queries).  Over 64 queries
+  // a workgroup's records weigh as much as 64 tokens' rows and the join reads
+  // them again: two there where three would leave it less than 768 tokens
+  // (32 requests of 4 heads behind 16001: 35 us at two, 512 tokens, 38 at three;
+  // 64 of 7 heads behind 32768: 90 at two, 77 at three).
+  split((int64_t)cus * (p.tile || p.nr == 1 ? 3 : 2));
+  if (p.tile && std::max(p.chunk[kRotated], p.chunk[kFull]) < 768) split((int64_t)cus * 2);
   if (p.join) {
-    p.chunk[kTail] = round_up(p.S[kTail], align);
+    p.chunk[kTail] = round_up(p.S[kTail], rk::kSpanWaves * rk::kSpanBlk);
     p.wgs[kTail] = 1;
   }
   if (p.grid + 24 * p.units[0] + 24 * p.units[1] + 24 * p.units[2] >= (INT64_C(1) << 31) || p.rows >= (INT64_C(1) << 31) || p.rows * p.np >= (INT64_C(1) << 40))
@@ -322,9 +335,8 @@ int make_plan(const Call& c, int cus, Plan* out) {
   // piece; their rotation there if everything has q's 16-bit type and lies in
   // pieces as well, else in a launch ahead.
   p.copy_q = !rk::vec_ok(c.q) || p.D % 8 != 0;
-  p.ahead = p.kv && (p.copy_q || c.q->dtype == RK_F32 || p.Dk == 0 || c.R->dtype != c.q->dtype ||
-                     (c.R->stride[3] != 1 && p.Dk > 1) || (p.D + 32) * c.R->stride[2] >= (INT64_C(1) << 30) ||
-                     (c.dm && (c.dm->dtype != c.q->dtype || !rk::vec_ok(c.dm))));
+  p.ahead = p.kv && (p.copy_q || c.q->dtype == RK_F32 || p.Dk == 0 || p.Dk % 8 != 0 || c.R->dtype != c.q->dtype ||
+                     !rk::vec_ok(c.R) || (c.dm && (c.dm->dtype != c.q->dtype || !rk::vec_ok(c.dm))));
   const size_t el = c.q->dtype == RK_F32 ? 4 : 2;
   p.q = take(p.copy_q ? (size_t)p.rows * round_up(p.D, 8) * el : 0);
   p.qr = take(p.ahead ? (size_t)p.rows * std::max(p.terms, 2) * 32 * p.kv * 2 : 0);
@@ -491,17 +503,28 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
       a.dm_sb = c.dm->stride[0]; a.dm_sh = c.dm->stride[1];
     }
   }
-  if (first > 0) {
-    const unsigned grid = (unsigned)first;
-    if (p.format == RK_ROWS_MX8)
-      e = rk::span_launch_mx8(p.kv, p.kf, p.nr, p.terms, a, grid, s);
-    else if (p.format == RK_ROWS_MX4)
-      e = rk::span_launch_mx4(p.kv, p.kf, p.nr, p.terms, a, grid, s);
-    else if (c.q->dtype == RK_F16)
-      e = rk::span_launch_f16(p.kv, p.kf, p.nr, p.vec, a, grid, s);
-    else
-      e = rk::span_launch_bf16(p.kv, p.kf, p.nr, p.vec, a, grid, s);
-    if (e != hipSuccess) return RK_ERR_HIP;
+  auto split = [&](const SpanArgs& b, int kv, unsigned grid) {
+    if (p.format == RK_ROWS_MX8) return rk::span_launch_mx8(kv, p.kf, p.nr, p.terms, b, grid, s);
+    if (p.format == RK_ROWS_MX4) return rk::span_launch_mx4(kv, p.kf, p.nr, p.terms, b, grid, s);
+    if (c.q->dtype == RK_F16) return rk::span_launch_f16(kv, p.kf, p.nr, p.vec, b, grid, s);
+    return rk::span_launch_bf16(kv, p.kf, p.nr, p.vec, b, grid, s);
+  };
+  auto tiles = [&](unsigned grid) {
+    if (p.format == RK_ROWS_MX8) return rk::tile_launch_mx8(p.kv, p.kf, a, grid, s);
+    if (p.format == RK_ROWS_MX4) return rk::tile_launch_mx4(p.kv, p.kf, a, grid, s);
+    if (c.q->dtype == RK_F16) return rk::tile_launch_f16(p.kv, p.kf, a, grid, s);
+    return rk::tile_launch_bf16(p.kv, p.kf, a, grid, s);
+  };
+  if (!p.tile) {
+    if (first > 0 && split(a, p.kv, (unsigned)first) != hipSuccess) return RK_ERR_HIP;
+  } else {
+    const int64_t shared = a.first[kTail];  // ids of the shared spans
+    if (shared > 0 && tiles((unsigned)shared) != hipSuccess) return RK_ERR_HIP;
+    if (first > shared) {  // a long suffix: its rows have few queries each
+      SpanArgs b = a;
+      b.first[kRotated] = b.first[kFull] = b.first[kTail] = 0;
+      if (split(b, 0, (unsigned)(first - shared)) != hipSuccess) return RK_ERR_HIP;
+    }
   }
   if (p.join) {
     const unsigned grid = (unsigned)launched(p, kTail);

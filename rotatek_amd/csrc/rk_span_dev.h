@@ -121,8 +121,8 @@ struct Block {
 
 // A unit's rows of one tensor as a buffer: a load is descriptor + scalar
 // offset of the block + fixed 32-bit offset of the lane (an address needs two
-// registers and a 64-bit vector addition per load), and nothing past `bytes`
-// is read.
+// registers and a 64-bit vector addition per load).  The hardware checks the
+// lane's offset alone, so the kernels clamp rows and columns themselves.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 __device__ __forceinline__ Rsrc make_rsrc(const void* p, uint32_t bytes) {
   const uint64_t v = (uint64_t)p;
@@ -324,6 +324,80 @@ __device__ __forceinline__ uint4 ones() {
   return make_uint4(w, w, w, w);
 }
 
+// Scores to sums for one block of 32 tokens: softmax of s (raw products; off:
+// the addend of a score, moved with the maximum) and O^T += V^T P^T.  on: which
+// of the lane's eight tokens count, unless the block is whole.  turn(w, lo, hi)
+// gives V^T of channel slots 2 w and 2 w + 1, all of them ahead of the softmax or
+// each as it is needed; used() is called once V is.
+template <class TT, int VB, int NR, int NP, bool AHEAD, class Turn, class Used>
+__device__ __forceinline__ void weigh_block(const f32x4 (&s)[2][NR], float scale, float (&off)[NR], bool whole,
+                                            uint32_t on, State<NR, VB>& st, const Turn& turn, const Used& used) {
+  uint4 av[AHEAD ? VB : 1];
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int w = 0; w < VB / 2; ++w) turn(w, av[2 * w], av[2 * w + 1]);
+    used();
+  }
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr) {
+    float sc[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) sc[r] = fmaf(s[r >> 2][nr][r & 3], scale, off[nr]);
+    if (!whole) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) sc[r] = (on >> r) & 1u ? sc[r] : -INFINITY;
+    }
+    float mx = max3(sc[0], sc[1], sc[2]);
+    mx = max3(mx, sc[3], sc[4]);
+    mx = max3(mx, sc[5], sc[6]);
+    mx = max3(mx, sc[7], sc[7]);
+    st.top[nr] = max3(st.top[nr], mx, mx);
+    if (!st.seen[nr] || __any(mx > kSlack<TT> + kLift<TT>)) {
+      mx = fmaxf(mx, shfl_xor(mx, 16));
+      mx = fmaxf(mx, shfl_xor(mx, 32));
+      // how far the maximum rises; the first tokens set it
+      float up = mx - kLift<TT>;
+      if (st.seen[nr]) up = fmaxf(up, 0.f);
+      st.seen[nr] = st.seen[nr] || __any(mx > -INFINITY);
+      up = up > -INFINITY ? up : 0.f;
+      const float alpha = fast_exp2(-up);
+#pragma unroll
+      for (int j = 0; j < VB; ++j) st.acc[nr][j] *= alpha;
+      st.l[nr] *= alpha;
+      st.m[nr] += up;
+      st.top[nr] -= up;
+      off[nr] -= up;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) sc[r] -= up;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) sc[r] = fast_exp2(sc[r]);
+    uint4 p[NP];
+    terms8<TT, NP>(sc, p);
+#pragma unroll
+    for (int t = 0; t < NP; ++t) st.l[nr] = TT::mfma(ones<TT>(), p[t], st.l[nr]);
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int t = 0; t < NP; ++t)
+#pragma unroll
+        for (int j = 0; j < VB; ++j) st.acc[nr][j] = TT::mfma(av[j], p[t], st.acc[nr][j]);
+    } else {
+#pragma unroll
+      for (int w = 0; w < VB / 2; ++w) {
+        uint4 lo, hi;
+        __builtin_amdgcn_sched_barrier(0);  // one pair's registers at a time
+        turn(w, lo, hi);
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+          st.acc[nr][2 * w] = TT::mfma(lo, p[t], st.acc[nr][2 * w]);
+          st.acc[nr][2 * w + 1] = TT::mfma(hi, p[t], st.acc[nr][2 * w + 1]);
+        }
+      }
+      used();
+    }
+  }
+}
+
 // One chunk of one span: adds the wave's blocks to `st`.  pre(): stages the
 // unit's queries in LDS, sq [term][row][stride] 16-bit in the lane's channel
 // order, while the first blocks are on their way.
@@ -439,70 +513,8 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
       hi = make_uint4(pack_hi(y[0], y[1]), pack_hi(y[2], y[3]), pack_hi(y[4], y[5]), pack_hi(y[6], y[7]));
     };
     // several row blocks share V^T; one forms it as it goes
-    uint4 av[NR > 1 ? VB : 1];
-    if constexpr (NR > 1) {
-#pragma unroll
-      for (int w = 0; w < VB / 2; ++w) turn(w, av[2 * w], av[2 * w + 1]);
-      load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, next, n, x);
-    }
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      float sc[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) sc[r] = fmaf(s[r >> 2][nr][r & 3], a.scale_log2, off[nr]);
-      if (!whole) {
-#pragma unroll
-        for (int r = 0; r < 8; ++r) sc[r] = (on >> r) & 1u ? sc[r] : -INFINITY;
-      }
-      float mx = max3(sc[0], sc[1], sc[2]);
-      mx = max3(mx, sc[3], sc[4]);
-      mx = max3(mx, sc[5], sc[6]);
-      mx = max3(mx, sc[7], sc[7]);
-      st.top[nr] = max3(st.top[nr], mx, mx);
-      if (!st.seen[nr] || __any(mx > kSlack<TT> + kLift<TT>)) {
-        mx = fmaxf(mx, shfl_xor(mx, 16));
-        mx = fmaxf(mx, shfl_xor(mx, 32));
-        // how far the maximum rises; the first tokens set it
-        float up = mx - kLift<TT>;
-        if (st.seen[nr]) up = fmaxf(up, 0.f);
-        st.seen[nr] = st.seen[nr] || __any(mx > -INFINITY);
-        up = up > -INFINITY ? up : 0.f;
-        const float alpha = fast_exp2(-up);
-#pragma unroll
-        for (int j = 0; j < VB; ++j) st.acc[nr][j] *= alpha;
-        st.l[nr] *= alpha;
-        st.m[nr] += up;
-        st.top[nr] -= up;
-        off[nr] -= up;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) sc[r] -= up;
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) sc[r] = fast_exp2(sc[r]);
-      uint4 p[NP];
-      terms8<TT, NP>(sc, p);
-#pragma unroll
-      for (int t = 0; t < NP; ++t) st.l[nr] = TT::mfma(ones<TT>(), p[t], st.l[nr]);
-      if constexpr (NR > 1) {
-#pragma unroll
-        for (int t = 0; t < NP; ++t)
-#pragma unroll
-          for (int j = 0; j < VB; ++j) st.acc[nr][j] = TT::mfma(av[j], p[t], st.acc[nr][j]);
-      } else {
-#pragma unroll
-        for (int w = 0; w < VB / 2; ++w) {
-          uint4 lo, hi;
-          __builtin_amdgcn_sched_barrier(0);  // one pair's registers at a time
-          turn(w, lo, hi);
-#pragma unroll
-          for (int t = 0; t < NP; ++t) {
-            st.acc[nr][2 * w] = TT::mfma(lo, p[t], st.acc[nr][2 * w]);
-            st.acc[nr][2 * w + 1] = TT::mfma(hi, p[t], st.acc[nr][2 * w + 1]);
-          }
-        }
-        load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, next, n, x);
-      }
-    }
+    weigh_block<TT, VB, NR, NP, (NR > 1)>(s, a.scale_log2, off, whole, on, st, turn,
+                                [&]() { load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, next, n, x); });
   };
 
   for (int i = 0; i < nw; i += NBUF) {
@@ -590,65 +602,86 @@ __device__ __forceinline__ void stage_queries(int tid, const Queries<NR, NW>& x,
 // 16-bit type and lie in whole 16-byte pieces; other calls find q R and the
 // biases formed ahead (span_queries_kernel).
 //
-// Loads: a wave takes tiles of 16 columns of R, as a matrix operand (rows 32
-// ks + 8 g + e of column 16 ct + n, KV > 2: two tiles); a thread the eight
-// channels of delta_mu that it holds of a query.
+// Each thread's pieces of R, and of delta_mu.
 template <int KV>
 struct Rotation {
-  static constexpr int kTiles = KV > 2 ? 2 : 1;
-  uint16_t r[kTiles][32];
-  u32x4 mu;
+  u32x4 r[2 * KV], mu;
 };
 
 template <int KV>
-__device__ __forceinline__ void load_rotation(const SpanArgs& a, int rb, int kv, int wave, int g, int n, int tid,
-                                              Rotation<KV>& x) {
-  const int c8 = 8 * (tid & 15);
-  x.mu = (u32x4){0u, 0u, 0u, 0u};
-  if (a.dm && c8 < a.D) x.mu = *(const u32x4*)((const uint16_t*)a.dm + rb * a.dm_sb + kv * a.dm_sh + c8);
-  const uint32_t sd = (uint32_t)a.R_sd * 2u;
-  const Rsrc r = make_rsrc((const uint16_t*)a.R + rb * a.R_sb + kv * a.R_sh, (uint32_t)(a.D - 1) * sd + 2u * a.Dk);
+__device__ __forceinline__ void load_rotation(const SpanArgs& a, int rb, int kv, int tid, Rotation<KV>& x) {
+  const uint16_t* R = (const uint16_t*)a.R + rb * a.R_sb + kv * a.R_sh;
 #pragma unroll
-  for (int t = 0; t < Rotation<KV>::kTiles; ++t) {
-    const int ct = wave + 4 * t;
-    if (ct >= 2 * KV) break;  // KV 1: two tiles in all
-    // past R's last row or column: out of the buffer's range, or a value that
-    // meets the query's zero or forms a column that no Key has
-    const uint32_t off = (uint32_t)(8 * g) * sd + 2u * (uint32_t)(ct * 16 + n);
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      x.r[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, (uint32_t)(32 * (i >> 3) + (i & 7)) * sd, 0);
+  for (int i = 0; i < 2 * KV; ++i) {
+    const int id = i * kSpanThreads + tid, d = id / (4 * KV), c = 8 * (id % (4 * KV));
+    x.r[i] = (u32x4){0u, 0u, 0u, 0u};
+    if (d < a.D && c < a.Dk) x.r[i] = *(const u32x4*)(R + d * a.R_sd + c);
   }
+  x.mu = (u32x4){0u, 0u, 0u, 0u};
+  if (a.dm && 8 * tid < a.D) x.mu = *(const u32x4*)((const uint16_t*)a.dm + rb * a.dm_sb + kv * a.dm_sh + 8 * tid);
 }
 
-// raw: the queries as they are, [row][136].  q R is left as NTV terms of TT in
-// `dst`, q . delta_mu in `bias`.
+// Where piece p of row r lies for a transposing read, which takes 32
+// neighbouring bytes of 16 rows: rows of P pieces (4, 8, 16), eight rows' 32
+// bytes fill the banks once.
+template <int P>
+__device__ __forceinline__ int swizzle_v(int p, int r) {
+  return p ^ (2 * ((r / (16 / P)) & (P / 2 - 1)));
+}
+
+// Columns 16 j .. 16 j + 15 of the rows r0 + 4 g .. + 3 and r0 + 16 + 4 g .. + 3
+// of a matrix in LDS (rows of P swizzled pieces), a column a lane: lane 4 t + q of
+// 16 names row t, columns 4 q .. 4 q + 3, and receives its column of all four.
+template <int P>
+__device__ __forceinline__ uint4 read_columns(const void* m, int r0, int j, int g, int n) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4* lptr;
+  uint2 x[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + 16 * i + 4 * g + (n >> 2), p = 2 * j + ((n >> 1) & 1);
+    const char* at = (const char*)m + 16 * (r * P + swizzle_v<P>(p, r)) + 8 * (n & 1);
+    x[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)at));
+  }
+  return make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+}
+
+template <int KV>
+__device__ __forceinline__ void stage_rotation(int tid, const Rotation<KV>& x, uint4* r, uint4* mu) {
+#pragma unroll
+  for (int i = 0; i < 2 * KV; ++i) {
+    const int id = i * kSpanThreads + tid, d = id / (4 * KV), p = id % (4 * KV);
+    r[d * (4 * KV) + swizzle_v<4 * KV>(p, d)] = make_uint4(x.r[i].x, x.r[i].y, x.r[i].z, x.r[i].w);
+  }
+  if (tid < 16) mu[tid] = make_uint4(x.mu.x, x.mu.y, x.mu.z, x.mu.w);
+}
+
+// raw: the queries as they are, [row][136]; r, mu: the staged rotation.  q R is
+// left as NTV terms of TT in `dst`, q . delta_mu in `bias`.  A wave takes tiles of
+// 16 columns; one more has delta_mu in every column.  (Channel order within 32:
+// as read_columns gives them.)
 template <class TT, int NTV, int NR, int KV>
-__device__ __forceinline__ void rotate_queries(const SpanArgs& a, int wave, int lane, const Rotation<KV>& x, bool f16,
-                                               const uint16_t* raw, uint16_t* dst, int stride) {
+__device__ __forceinline__ void rotate_queries(const SpanArgs& a, int wave, int lane, bool f16, const uint16_t* raw,
+                                               const uint4* r, const uint4* mu, uint16_t* dst, int stride, float* bias) {
   constexpr int kRows = 16 * NR;
   const int g = lane >> 4, n = lane & 15;
-#pragma unroll
-  for (int t = 0; t < Rotation<KV>::kTiles; ++t) {
-    const int ct = wave + 4 * t;
-    if (ct >= 2 * KV) break;
-    const bool have = ct * 16 + n < a.Dk;
+  for (int ct = wave; ct <= 2 * KV; ct += kSpanWaves) {
     f32x4 o[NR];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) o[nr] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // a row past the head's channels may be the next head's: zero
-        const bool ok = have && 32 * ks + 8 * g < a.D;
-        w[e] = ok ? x.r[t][8 * ks + 2 * e] | (uint32_t)x.r[t][8 * ks + 2 * e + 1] << 16 : 0u;
+      uint4 m;
+      if (ct < 2 * KV) {
+        m = read_columns<4 * KV>(r, 32 * ks, ct, g, n);
+      } else {
+        const uint2 lo = ((const uint2*)mu)[8 * ks + g], hi = ((const uint2*)mu)[8 * ks + 4 + g];
+        m = make_uint4(lo.x, lo.y, hi.x, hi.y);
       }
-      const uint4 m = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr) {
-        const uint4 q = *(const uint4*)(raw + (16 * nr + n) * 136 + 32 * ks + 8 * g);
+        const uint2* p = (const uint2*)(raw + (16 * nr + n) * 136 + 32 * ks);
+        const uint4 q = make_uint4(p[g].x, p[g].y, p[4 + g].x, p[4 + g].y);
         o[nr] = f16 ? F16::mfma(q, m, o[nr]) : BF16::mfma(q, m, o[nr]);
       }
     }
@@ -657,34 +690,18 @@ __device__ __forceinline__ void rotate_queries(const SpanArgs& a, int wave, int 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float v = o[nr][i];
+        const int row = 16 * nr + 4 * g + i;
+        if (ct == 2 * KV) {
+          if (n == 0) bias[row] = v;
+        } else {
 #pragma unroll
-        for (int k = 0; k < NTV; ++k) {
-          const uint16_t h = TT::from_f32(v);
-          dst[(k * kRows + 16 * nr + 4 * g + i) * stride + ct * 16 + n] = h;
-          v -= TT::to_f32(h);
+          for (int k = 0; k < NTV; ++k) {
+            const uint16_t h = TT::from_f32(v);
+            dst[(k * kRows + row) * stride + ct * 16 + n] = h;
+            v -= TT::to_f32(h);
+          }
         }
       }
-  }
-}
-
-template <int NR, int NW>
-__device__ __forceinline__ void bias_queries(const Queries<NR, NW>& q, const u32x4& mu, bool f16, int tid, float* bias) {
-  const uint32_t w[4] = {mu.x, mu.y, mu.z, mu.w};
-  float m[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-    m[e] = f16 ? F16::to_f32(h) : BF16::to_f32(h);
-  }
-#pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    float v[8], s = 0.f;
-    query8(q, i, f16, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(v[e], m[e], s);
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) s += shfl_xor(s, d);
-    if ((tid & 15) == 0) bias[16 * i + (tid >> 4)] = s;
   }
 }
 
@@ -749,7 +766,7 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3
   constexpr int kRows = 16 * NR;
   constexpr int kWide = 32 * (KV > KF ? KV : KF) + 8;  // +8: rows start in other banks
   constexpr int kQ = kRows * kWide * (KV > 0 ? NTV : NT);
-  constexpr int kRaw = KV > 0 && NT < 3 ? kRows * 136 : 0;
+  constexpr int kRaw = KV > 0 && NT < 3 ? kRows * 136 + 128 * 32 * KV + 128 : 0;
   constexpr int kAccRow = DV + 4;       // floats; +4: rows start in other banks
   constexpr int kAcc = kSpanWaves * kRows * kAccRow;
   __shared__ __attribute__((aligned(16))) char s_mem[(kQ + kRaw) * 2 > kAcc * 4 ? (kQ + kRaw) * 2 : kAcc * 4];
@@ -818,15 +835,17 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3
       Rotation<KV> rot;
       if (here) {
         load_queries<NR, NW>(a, shared, b, kv, R0, rows, tid, qw);
-        load_rotation<KV>(a, shared ? 0 : b, kv, wave, g, n, tid, rot);
+        load_rotation<KV>(a, shared ? 0 : b, kv, tid, rot);
       }
       auto pre = [&]() {
         if (here) {
           if constexpr (NT < 3) {
+            uint4* s_r = (uint4*)(s_raw + kRows * 136);
+            uint4* s_mu = s_r + 128 * 4 * KV;
             stage_queries<TT, 1, NR, NW, 128>(tid, qw, f16, s_raw, 136);
-            bias_queries(qw, rot.mu, f16, tid, s_bias);
+            stage_rotation<KV>(tid, rot, s_r, s_mu);
             __syncthreads();
-            rotate_queries<TT, NTV, NR, KV>(a, wave, lane, rot, f16, s_raw, s_q, kWide);
+            rotate_queries<TT, NTV, NR, KV>(a, wave, lane, f16, s_raw, s_r, s_mu, s_q, kWide, s_bias);
           }
         } else {
           constexpr int W = 32 * KV;

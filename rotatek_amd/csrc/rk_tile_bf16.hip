@@ -1,0 +1,11 @@
+// rk_tile_bf16.hip -- attention over shared rows of this format (kernels in
+// rk_tile_dev.h): terms of a query, and of a probability, as in rk_span_bf16.hip.
+#include "rk_tile_dev.h"
+
+namespace rk {
+
+hipError_t tile_launch_bf16(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s) {
+  return pick_tiles<PlainFmt<BF16>, 1, 2>(kv, kf, a, grid, s);
+}
+
+}  // namespace rk
