@@ -79,7 +79,7 @@ class RkDecodePlan(ctypes.Structure):
 
 
 _P = ctypes.POINTER(RkTensor)
-_W = ctypes.POINTER(RkRows)
+_V = ctypes.c_void_p
 _SIGNATURES = {
     "rk_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "rk_abi_version": (ctypes.c_int, []),
@@ -142,17 +142,18 @@ _SIGNATURES = {
     "rk_spark_recover_check": (ctypes.c_int, [_P, _P, _P, _P, _P, _P]),
     "rk_spark_recover": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, ctypes.c_void_p]),
     "rk_channel_selection": (ctypes.c_int, [_P, _P, ctypes.c_void_p]),
-    "rk_mx_write": (ctypes.c_int, [_P, _W, ctypes.c_void_p]),
-    "rk_mx_read": (ctypes.c_int, [_W, _P, ctypes.c_void_p]),
-    "rk_mx_append": (ctypes.c_int, [_P, _P, _W, _W, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]),
-    "rk_quantized_decode_check": (ctypes.c_int, [_P, _P, _P, _W, _W, _P, _W, _W, ctypes.c_int64, _P, ctypes.c_int32,
+    # (descriptors as void*: bytes or byref)
+    "rk_mx_write": (ctypes.c_int, [_V, _V, _V]),
+    "rk_mx_read": (ctypes.c_int, [_V, _V, _V]),
+    "rk_mx_append": (ctypes.c_int, [_V, _V, _V, _V, _V, ctypes.c_int32, _V]),
+    "rk_quantized_decode_check": (ctypes.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_int64, _V, ctypes.c_int32,
                                                  ctypes.POINTER(ctypes.c_size_t)]),
-    "rk_quantized_decode": (ctypes.c_int, [_P, _P, _P, _W, _W, _P, ctypes.c_void_p, _W, _W, ctypes.c_int64, _P,
-                                           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
-    "rk_shared_prefix_decode_check": (ctypes.c_int, [_P, _P, _P, _W, _W, _W, _W, _W, _W, ctypes.c_int64, _P,
+    "rk_quantized_decode": (ctypes.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_int64, _V, _V,
+                                           ctypes.c_size_t, _V]),
+    "rk_shared_prefix_decode_check": (ctypes.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_int64, _V,
                                                      ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
-    "rk_shared_prefix_decode": (ctypes.c_int, [_P, _P, _P, _W, _W, _W, _W, _W, _W, ctypes.c_void_p, ctypes.c_int64,
-                                               _P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "rk_shared_prefix_decode": (ctypes.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_int64, _V, _V,
+                                               ctypes.c_size_t, _V]),
 }
 
 _lib = None
@@ -226,23 +227,46 @@ def desc(t: torch.Tensor | None):
 
 # rk_rows: two rk_tensors, head_dim, format
 _RK_ROWS = struct.Struct("=Qii8qQii8qqii")
+_PLAIN_ROWS = (0,) * 11
+
+
+def pack(t: torch.Tensor | None) -> bytes | None:
+    """desc() as bytes, which a ``void*`` argument takes as they are (a ctypes
+    structure costs 0.4 us more)."""
+    if t is None:
+        return None
+    shape = t.shape
+    nd = len(shape)
+    code = _DTYPES.get(t.dtype)
+    if nd > 4 or code is None:
+        raise ValueError(f"tensors of rank > 4 or dtype {t.dtype} are not supported")
+    pad = _PAD[4 - nd]
+    return _RK_TENSOR.pack(t.data_ptr(), code, nd, *shape, *pad, *t.stride(), *pad)
+
+
+def pack_contiguous(ptr: int, dtype: torch.dtype, shape) -> bytes:
+    """pack() of a contiguous [a, b, c] tensor at ``ptr``."""
+    a, b, c = shape
+    return _RK_TENSOR.pack(ptr, _DTYPES[dtype], 3, a, b, c, 0, b * c, c, 1, 0)
+
+
+def pack_rows(data: torch.Tensor, scales: torch.Tensor | None, head_dim: int, fmt: int) -> bytes:
+    """rk_rows of quantised rows, or of plain ones (``scales`` None), as bytes."""
+    code, shape = _DTYPES.get(data.dtype), data.shape
+    if len(shape) != 4 or code is None:
+        raise ValueError(f"rows need 4 dims [B, H, S, D] of a known dtype, got {tuple(shape)} {data.dtype}")
+    if scales is None:
+        return _RK_ROWS.pack(data.data_ptr(), code, 4, *shape, *data.stride(), *_PLAIN_ROWS, head_dim, fmt, 0)
+    sc, sshape = _DTYPES.get(scales.dtype), scales.shape
+    if len(sshape) != 4 or sc is None:
+        raise ValueError(f"scales need 4 dims of a known dtype, got {tuple(sshape)} {scales.dtype}")
+    return _RK_ROWS.pack(data.data_ptr(), code, 4, *shape, *data.stride(), scales.data_ptr(), sc, 4, *sshape,
+                         *scales.stride(), head_dim, fmt, 0)
 
 
 def rows_desc(data: torch.Tensor, scales: torch.Tensor | None, head_dim: int, fmt: int) -> RkRows:
-    """rk_rows descriptor of quantised rows, or of plain ones (``scales``
-    None), packed in one step (a call has up to six)."""
-    code = _DTYPES.get(data.dtype)
-    if data.dim() != 4 or code is None:
-        raise ValueError(f"rows need 4 dims [B, H, S, D] of a known dtype, got {tuple(data.shape)} {data.dtype}")
-    if scales is None:
-        tail = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    else:
-        sc = _DTYPES.get(scales.dtype)
-        if scales.dim() != 4 or sc is None:
-            raise ValueError(f"scales need 4 dims of a known dtype, got {tuple(scales.shape)} {scales.dtype}")
-        tail = (scales.data_ptr(), sc, 4, *scales.shape, *scales.stride())
-    return RkRows.from_buffer_copy(_RK_ROWS.pack(data.data_ptr(), code, 4, *data.shape, *data.stride(), *tail,
-                                                 head_dim, fmt, 0))
+    """pack_rows as a structure."""
+    return RkRows.from_buffer_copy(pack_rows(data, scales, head_dim, fmt))
 
 
 def ref(d):

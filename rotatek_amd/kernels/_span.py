@@ -23,6 +23,15 @@ def rows_of(x):
     return _lib.rows_desc(x, None, x.shape[-1] if x.dim() else 0, _lib.RK_ROWS_PLAIN)
 
 
+def _pack(x):
+    """rows_of as bytes."""
+    if x is None:
+        return None
+    if isinstance(x, MXRows):
+        return x.pack()
+    return _lib.pack_rows(x, None, x.shape[-1] if x.dim() else 0, _lib.RK_ROWS_PLAIN)
+
+
 def check_query(q: torch.Tensor) -> None:
     if q.dim() != 3:
         raise ValueError(f"q needs 3 dims [B, H_q, D], got shape {tuple(q.shape)}")
@@ -41,30 +50,31 @@ def launch(what, q, rotation, rows, mask, lens, num_kv_groups, out, shared):
     if lens is not None:
         check_lens(lens, q.shape[0], "lens")
     lib = _lib.load()
-    desc = _lib.desc
+    pack = _lib.pack
+    dq = pack(q)
+    shape = q.shape
     if out is None:
-        out = torch.empty((q.shape[0], 1, *q.shape[1:]), dtype=q.dtype, device=q.device)
-        do = desc(q)    # contiguous, q's sizes
-        do.data = out.data_ptr()
-        do.stride[0], do.stride[1], do.stride[2] = q.shape[1] * q.shape[2], q.shape[2], 1
+        out = torch.empty((shape[0], 1, *shape[1:]), dtype=q.dtype, device=q.device)
+        do = _lib.pack_contiguous(out.data_ptr(), q.dtype, shape)
     else:
-        do = desc(out)
+        do = pack(out)
         out = out.unsqueeze(1)
-    dq, dR, dm, dk = desc(q), desc(rotation[0]), desc(rotation[1]), desc(mask)
-    r = [rows_of(x) for x in rows]
+    dR, dm, dk = pack(rotation[0]), pack(rotation[1]), pack(mask)
+    r = [_pack(x) for x in rows]
     groups = int(num_kv_groups)
     lens_ptr = None if lens is None else lens.data_ptr()
-    key = (dev, shared, q.shape)
+    key = (dev, shared, shape)
     with on_device(dev):
         s = _lib.raw_stream(dev)
 
-        def call(ws):
+        def call(nbytes):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             if shared:
-                return lib.rk_shared_prefix_decode(dq, dR, dm, *r, lens_ptr, groups, do, ws.data_ptr(), ws.numel(), s)
+                return lib.rk_shared_prefix_decode(dq, dR, dm, *r, lens_ptr, groups, do, ws.data_ptr(), nbytes, s)
             return lib.rk_quantized_decode(dq, dR, dm, r[0], r[1], dk, lens_ptr, r[2], r[3], groups, do, ws.data_ptr(),
-                                           ws.numel(), s)
+                                           nbytes, s)
 
-        st = call(torch.empty(_need.get(key, 256), dtype=torch.uint8, device=q.device))
+        st = call(_need.get(key, 256))
         if st == _lib.RK_ERR_WORKSPACE:
             need = ctypes.c_size_t(0)
             if shared:
@@ -75,6 +85,6 @@ def launch(what, q, rotation, rows, mask, lens, num_kv_groups, out, shared):
             if len(_need) > 4096:
                 _need.clear()
             _need[key] = need.value
-            st = call(torch.empty(need.value, dtype=torch.uint8, device=q.device))
+            st = call(need.value)
     _lib.check(st, what)
     return out

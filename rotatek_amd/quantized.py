@@ -20,7 +20,6 @@ nothing.
 from __future__ import annotations
 
 import contextlib
-import ctypes
 from typing import Optional
 
 import torch
@@ -93,7 +92,12 @@ class MXRows:
         return MXRows(self.codes.narrow(0, start, count), self.scales.narrow(0, start, count), self.head_dim, self.fmt)
 
     def desc(self):
+        """rk_rows of these rows."""
         return _lib.rows_desc(self.codes, self.scales, self.head_dim, FORMATS[self.fmt])
+
+    def pack(self) -> bytes:
+        """desc() as bytes."""
+        return _lib.pack_rows(self.codes, self.scales, self.head_dim, FORMATS[self.fmt])
 
     def __repr__(self) -> str:
         return f"MXRows({tuple(self.shape)}, {self.fmt!r}, device={str(self.device)!r})"
@@ -114,9 +118,12 @@ def same_device(what: str, index: int, *tensors) -> None:
             raise ValueError(f"{what}: every tensor must be on cuda:{index}")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(index: int):
     """Launches go to GPU ``index`` whichever is current."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def check_lens(lens: torch.Tensor, batch: int, name: str) -> None:
@@ -136,9 +143,9 @@ def quantize_rows(x: torch.Tensor, fmt: str = "mx8", out: Optional[MXRows] = Non
         out = MXRows.empty(*x.shape, fmt=fmt, device=x.device)
     elif out.fmt != fmt:
         raise ValueError(f"out holds {out.fmt} rows, not {fmt}")
-    dx, dr = _lib.desc(x), out.desc()
+    dx, dr = _lib.pack(x), out.pack()
     with on_device(dev):
-        st = _lib.load().rk_mx_write(ctypes.byref(dx), ctypes.byref(dr), _lib.raw_stream(dev))
+        st = _lib.load().rk_mx_write(dx, dr, _lib.raw_stream(dev))
     _lib.check(st, "quantize_rows")
     return out
 
@@ -151,9 +158,9 @@ def dequantize_rows(rows: MXRows, dtype: torch.dtype = torch.bfloat16,
     same_device("dequantize_rows", dev, rows, out)
     if out is None:
         out = torch.empty(rows.shape, dtype=dtype, device=rows.device)
-    dr, do = rows.desc(), _lib.desc(out)
+    dr, do = rows.pack(), _lib.pack(out)
     with on_device(dev):
-        st = _lib.load().rk_mx_read(ctypes.byref(dr), ctypes.byref(do), _lib.raw_stream(dev))
+        st = _lib.load().rk_mx_read(dr, do, _lib.raw_stream(dev))
     _lib.check(st, "dequantize_rows")
     return out
 
@@ -172,10 +179,9 @@ def append_rows(k_new: torch.Tensor, v_new: Optional[torch.Tensor], k_rows: MXRo
     dev = k_new.get_device()
     same_device("append_rows", dev, v_new, k_rows, v_rows, lens)
     check_lens(lens, k_new.shape[0], "lens")
-    dk, dv, rk, rv = _lib.desc(k_new), _lib.desc(v_new), k_rows.desc(), None if v_rows is None else v_rows.desc()
+    dk, dv, rk, rv = _lib.pack(k_new), _lib.pack(v_new), k_rows.pack(), None if v_rows is None else v_rows.pack()
     with on_device(dev):
-        st = _lib.load().rk_mx_append(ctypes.byref(dk), _lib.ref(dv), ctypes.byref(rk), _lib.ref(rv), lens.data_ptr(),
-                                      int(bool(advance)), _lib.raw_stream(dev))
+        st = _lib.load().rk_mx_append(dk, dv, rk, rv, lens.data_ptr(), int(bool(advance)), _lib.raw_stream(dev))
     _lib.check(st, "append_rows")
 
 
