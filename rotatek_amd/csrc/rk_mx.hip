@@ -9,7 +9,9 @@
 //
 // A lane holds eight channels; the four lanes of a block share its maximum by
 // two lane exchanges inside the quad.  Both kernels move bytes and little
-// else: bound by HBM on long spans, by launch latency on short ones.
+// else: 98 MB of bf16 to 51 MB of 8-bit rows takes 31 us (4.8 TB/s, the rate
+// of a large copy), back 23 us (6.4 TB/s); spans of a few MB are bound by the
+// launch (4 us).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -21,8 +23,8 @@ namespace {
 
 using rk::kMxBlock;
 
-constexpr int kTile = 64;  // tokens of one (batch row, head) per workgroup
 constexpr int kThreads = 256;
+constexpr int kTile = 64;  // tokens of one (batch row, head) per workgroup: a pass of 256 lanes per block of a row
 
 struct MxArgs {
   const void* x;  // read: the output
@@ -36,21 +38,40 @@ struct MxArgs {
   int32_t H, D, tiles;
 };
 
+// Values pass through once, so they are loaded and stored as non-temporal and
+// leave the caches to the codes, which the next kernel reads: a span of 8 x 4
+// heads x 12001 tokens of 128 channels written and read back takes 54.3 us,
+// 58.5 without; 32 x 8 heads x 256 tokens read back, K and V, 14.1 and 20.0.
+template <class V>
+__device__ __forceinline__ V load_once(const void* p) {
+  return __builtin_nontemporal_load((const V*)p);
+}
+template <class V>
+__device__ __forceinline__ void store_once(void* p, V v) {
+  __builtin_nontemporal_store(v, (V*)p);
+}
+
 // Eight elements at p (stride sd), channels past nv zero.
 template <class DT, bool VEC>
 __device__ __forceinline__ void load_x8(const void* base, int64_t off, int64_t sd, int nv, float (&x)[8]) {
   if constexpr (DT::kBytes == 4) {
     const float* p = (const float*)base + off;
     if constexpr (VEC) {
-      const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+      const rk::f32x4 a = load_once<rk::f32x4>(p), b = load_once<rk::f32x4>(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = i < nv ? p[i * sd] : 0.f;
     }
   } else {
-    const uint4 w = rk::load8<VEC>((const uint16_t*)base + off, sd, nv);
+    uint4 w;
+    if constexpr (VEC) {
+      const rk::u32x4 v = load_once<rk::u32x4>((const uint16_t*)base + off);
+      w = make_uint4(v[0], v[1], v[2], v[3]);
+    } else {
+      w = rk::load8<false>((const uint16_t*)base + off, sd, nv);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = DT::to_f32((uint16_t)(rk::word(w, i >> 1) >> (16 * (i & 1))));
   }
@@ -149,14 +170,15 @@ __global__ void __launch_bounds__(kThreads) mx_write_kernel(const MxArgs a) {
   write_tile<DT, FMT, NB, VEC>(a, s_sc);
 }
 
-// K and V of an append in one launch (blockIdx.y).
-template <class DT, int FMT, int NBK, int NBV, bool VEC>
+// K and V of an append in one launch (blockIdx.y) where their rows hold as
+// many blocks; others take a launch each.
+template <class DT, int FMT, int NB, bool VEC>
 __global__ void __launch_bounds__(kThreads) mx_append_kernel(const MxArgs k, const MxArgs v) {
-  __shared__ uint8_t s_sc[4 * kTile];
+  __shared__ uint8_t s_sc[NB * kTile];
   if (blockIdx.y == 0)
-    write_tile<DT, FMT, NBK, VEC>(k, s_sc);
+    write_tile<DT, FMT, NB, VEC>(k, s_sc);
   else
-    write_tile<DT, FMT, NBV, VEC>(v, s_sc);
+    write_tile<DT, FMT, NB, VEC>(v, s_sc);
 }
 
 // Lengths after an append, in a launch of its own: every workgroup of the
@@ -226,16 +248,16 @@ __global__ void __launch_bounds__(kThreads) mx_read_kernel(const MxArgs a) {
     if constexpr (DT::kBytes == 4) {
       float* p = (float*)a.x + off;
       if constexpr (VEC) {
-        ((float4*)p)[0] = make_float4(y[0], y[1], y[2], y[3]);
-        ((float4*)p)[1] = make_float4(y[4], y[5], y[6], y[7]);
+        store_once(p, rk::f32x4{y[0], y[1], y[2], y[3]});
+        store_once(p + 4, rk::f32x4{y[4], y[5], y[6], y[7]});
       } else {
         for (int k = 0; k < nv; ++k) p[k * a.x_sd] = y[k];
       }
     } else {
       uint16_t* p = (uint16_t*)a.x + off;
       if constexpr (VEC) {
-        *(uint4*)p = make_uint4(DT::pack2(y[0], y[1]), DT::pack2(y[2], y[3]), DT::pack2(y[4], y[5]),
-                                DT::pack2(y[6], y[7]));
+        store_once(p, rk::u32x4{DT::pack2(y[0], y[1]), DT::pack2(y[2], y[3]), DT::pack2(y[4], y[5]),
+                                 DT::pack2(y[6], y[7])});
       } else {
         for (int k = 0; k < nv; ++k) p[k * a.x_sd] = DT::from_f32(y[k]);
       }
@@ -302,10 +324,12 @@ int by_type(int dtype, int format, int64_t nb, bool vec, F f) {
       default: return RK_ERR_HEAD_DIM;
     }
   };
-  auto vecs = [&](auto dt, auto fmt) { return vec ? blocks(dt, fmt, std::true_type{}) : blocks(dt, fmt, std::false_type{}); };
+  auto vecs = [&](auto dt, auto fmt) {
+    return vec ? blocks(dt, fmt, std::true_type{}) : blocks(dt, fmt, std::false_type{});
+  };
   auto formats = [&](auto dt) {
     return format == RK_ROWS_MX8 ? vecs(dt, std::integral_constant<int, RK_ROWS_MX8>{})
-                            : vecs(dt, std::integral_constant<int, RK_ROWS_MX4>{});
+                                 : vecs(dt, std::integral_constant<int, RK_ROWS_MX4>{});
   };
   switch (dtype) {
     case RK_F16: return formats(rk::F16{});
@@ -319,7 +343,16 @@ int done(int st) {
   return hipGetLastError() == hipSuccess ? RK_OK : RK_ERR_HIP;
 }
 
-bool grid_ok(const MxArgs& a, int64_t B) { return a.S <= (INT64_C(1) << 31) && B * a.H * a.tiles < (INT64_C(1) << 31); }
+bool grid_ok(const MxArgs& a, int64_t B) {
+  return a.S <= (INT64_C(1) << 31) && B * a.H * a.tiles < (INT64_C(1) << 31);
+}
+
+// Two rows at one address would be written by two workgroups at once.
+bool distinct(const rk_tensor& t) {
+  for (int i = 0; i < t.ndim; ++i)
+    if (t.shape[i] > 1 && t.stride[i] == 0) return false;
+  return true;
+}
 
 }  // namespace
 
@@ -329,6 +362,7 @@ extern "C" int rk_mx_write(const rk_tensor* x, const rk_rows* rows, void* stream
   if (rk::numel(x) == 0) return RK_OK;
   const MxArgs a = make_args(x, rows);
   if (!grid_ok(a, x->shape[0])) return RK_ERR_SHAPE;
+  if (!distinct(rows->data) || !distinct(rows->scales)) return RK_ERR_STRIDE;
   const dim3 grid((unsigned)(x->shape[0] * a.H * a.tiles));
   st = by_type(x->dtype, rows->format, cdiv(a.D, kMxBlock), vec8_ok(x), [&](auto dt, auto fmt, auto nb, auto vec) {
     hipLaunchKernelGGL((mx_write_kernel<decltype(dt), decltype(fmt)::value, decltype(nb)::value, decltype(vec)::value>),
@@ -343,6 +377,7 @@ extern "C" int rk_mx_read(const rk_rows* rows, const rk_tensor* out, void* strea
   if (rk::numel(out) == 0) return RK_OK;
   const MxArgs a = make_args(out, rows);
   if (!grid_ok(a, out->shape[0])) return RK_ERR_SHAPE;
+  if (!distinct(*out)) return RK_ERR_STRIDE;
   const dim3 grid((unsigned)(out->shape[0] * a.H * a.tiles));
   st = by_type(out->dtype, rows->format, cdiv(a.D, kMxBlock), vec8_ok(out), [&](auto dt, auto fmt, auto nb, auto vec) {
     hipLaunchKernelGGL((mx_read_kernel<decltype(dt), decltype(fmt)::value, decltype(nb)::value, decltype(vec)::value>),
@@ -370,6 +405,8 @@ extern "C" int rk_mx_append(const rk_tensor* k_new, const rk_tensor* v_new, cons
   if (cap >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
   MxArgs k = make_args(k_new, k_rows), v = v_new ? make_args(v_new, v_rows) : k;
   if (!grid_ok(k, B)) return RK_ERR_SHAPE;
+  for (const rk_rows* r : {k_rows, v_rows})
+    if (r && (!distinct(r->data) || !distinct(r->scales))) return RK_ERR_STRIDE;
   k.pos = v.pos = lens;
   const hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(B * k.H * k.tiles));
@@ -379,15 +416,16 @@ extern "C" int rk_mx_append(const rk_tensor* k_new, const rk_tensor* v_new, cons
     if (v_new && nbk == nbv) {
       st = by_type(k_new->dtype, k_rows->format, nbk, vec, [&](auto dt, auto fmt, auto nb, auto vc) {
         constexpr int NB = decltype(nb)::value;
-        hipLaunchKernelGGL((mx_append_kernel<decltype(dt), decltype(fmt)::value, NB, NB, decltype(vc)::value>),
+        hipLaunchKernelGGL((mx_append_kernel<decltype(dt), decltype(fmt)::value, NB, decltype(vc)::value>),
                            dim3(grid.x, 2), dim3(kThreads), 0, s, k, v);
       });
     } else {
       for (int i = 0; i < (v_new ? 2 : 1) && !st; ++i) {
         const MxArgs a = i ? v : k;
         st = by_type(k_new->dtype, k_rows->format, i ? nbv : nbk, vec, [&](auto dt, auto fmt, auto nb, auto vc) {
-          hipLaunchKernelGGL((mx_write_kernel<decltype(dt), decltype(fmt)::value, decltype(nb)::value, decltype(vc)::value>),
-                             grid, dim3(kThreads), 0, s, a);
+          constexpr int NB = decltype(nb)::value;
+          hipLaunchKernelGGL((mx_write_kernel<decltype(dt), decltype(fmt)::value, NB, decltype(vc)::value>), grid,
+                             dim3(kThreads), 0, s, a);
         });
       }
     }

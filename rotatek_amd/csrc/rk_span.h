@@ -26,7 +26,6 @@ struct Span {
   int32_t wgs;       // workgroups of a unit
   int32_t np0;       // record number of the unit's first workgroup
   int32_t width;     // stored channels of a score row (a multiple of 32, or D)
-  int32_t k_row;     // bytes of a quantised score row
 };
 
 // Spans by what their rows score with.
@@ -47,7 +46,6 @@ struct SpanArgs {
   int64_t q_sb, q_sh, o_sb, o_sh, o_sd;
   int32_t B, Hq, H, G, D, Dk, np, shared;
   int32_t q_dtype, o_dtype;
-  int32_t v_row;  // bytes of a quantised Value row
   float scale_log2;  // log2(e) / sqrt(D)
   // the rotation of the rotated span's queries (qr null): in q's 16-bit type,
   // unit column stride, aligned pieces of eight channels
@@ -74,25 +72,24 @@ constexpr int kSpanWaves = 4;
 constexpr int kSpanBlk = 32;  // tokens of a wave's step
 
 // The split launch: kv = score blocks of 32 channels of the rotated span (0:
-// none, 1, 2 or 4), kf the full-width spans' (2: D <= 64, or 4), nr = blocks
-// of 16 queries per unit, terms = 16-bit terms that a query is exact in.
-hipError_t span_launch_f16(int kv, int kf, int nr, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
-hipError_t span_launch_bf16(int kv, int kf, int nr, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
-hipError_t span_launch_mx8(int kv, int kf, int nr, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
-hipError_t span_launch_mx4(int kv, int kf, int nr, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
+// none, 1, 2 or 4), kf the full-width spans' (2: D <= 64, or 4), terms = 16-bit
+// terms that a query is exact in.
+hipError_t span_launch_f16(int kv, int kf, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_launch_bf16(int kv, int kf, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_launch_mx8(int kv, int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_launch_mx4(int kv, int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
 
-// The launch behind it where a shared call's suffix is short: the suffix rows
-// and the join of all records.
-hipError_t span_join_f16(int kf, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
-hipError_t span_join_bf16(int kf, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s);
-hipError_t span_join_mx8(int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
-hipError_t span_join_mx4(int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s);
-
-// The split launch over rows that more than 32 queries share, 64 of them a
-// workgroup (rk_tile_dev.h).
+// The split launch over rows that many queries share, 64 of them a workgroup
+// (rk_tile_dev.h; 16-bit queries, whole pieces).
 hipError_t tile_launch_f16(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
 hipError_t tile_launch_bf16(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
 hipError_t tile_launch_mx8(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
 hipError_t tile_launch_mx4(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
+
+// The launch behind that one: the suffix rows and the join of all records.
+hipError_t span_join_f16(int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_join_bf16(int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_join_mx8(int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
+hipError_t span_join_mx4(int kf, const SpanArgs& a, unsigned grid, hipStream_t s);
 
 }  // namespace rk

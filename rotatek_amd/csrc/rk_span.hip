@@ -1,8 +1,8 @@
 // rk_span.hip -- host side of the attention over quantised and shared spans
 // (rk_quantized_decode, rk_shared_prefix_decode of rotatek_hip.h): validation,
-// the split plan, the split launch's kernels' companions
-// (rk_span_dev.h), and two small ones: queries that it does not take as they
-// are, and the join of a row's partial sums after it.
+// the split plan and the launches, and the small kernels beside the split one
+// (rk_span_dev.h, rk_tile_dev.h): queries that it does not take as they are,
+// and the join of a row's partial sums.
 #include <hip/hip_runtime.h>
 #include <string.h>
 
@@ -151,11 +151,19 @@ __global__ void __launch_bounds__(256) span_zero_kernel(uint32_t* p, int64_t n) 
 
 // ------------------------------------------------------------------- host
 
-// Suffix rows up to this many are attended in the joining launch, one
-// workgroup per request and KV head; more are split like the other spans.
-constexpr int64_t kJoinTokens = 1024;
-// Queries on the same rows past which the waves take queries instead of tokens.
-constexpr int64_t kTileRows = 32;
+// Rows that many queries share: past this many bytes of a token's K and V, times
+// blocks of 16 queries, the waves of a workgroup take queries (tile_kernel), up to
+// it tokens, and the row blocks read the rows from one L2 (span_kernel).  Below,
+// tiles and tokens: 96 queries of 264-byte tokens 27.1 and 22.7 us, 98 of 85
+// bytes 30.0 and 22.7, 49 of 320 bytes 24.2 and 22.0; above: 64 of 512 bytes 46.7
+// and 51, 128 of 512 bytes 33.6 and 58, 448 of 165 bytes 64 and 73.
+constexpr int64_t kTileBytes = 2048;
+// Suffix rows up to this many are attended in the launch that joins the tiles'
+// records, one workgroup per request and KV head, for a launch less: 64 requests
+// of 4 KV heads with 2000 tokens 84 us, with a launch each 122; 48 of 2 heads,
+// too few to fill the chip, 43.8 and 42.3.  (Without tiles the suffix is split
+// with the other spans: 2 requests of 4 heads 11.3 us, joined 12.9.)
+constexpr int64_t kJoinTokens = 4096;
 // Bytes a workgroup streams at most.
 constexpr int64_t kMaxShare = INT64_C(512) << 10;
 
@@ -171,9 +179,9 @@ struct Call {
 
 struct Plan {
   int64_t B, Hq, H, G, D, Dk;
-  int format, kv, kf, nr, terms;
-  bool vec, join;  // join: the suffix rows run in the launch that joins the records
-  bool tile;           // rk_tile_dev.h over the shared spans, 64 queries a workgroup
+  int format, kv, kf, terms;
+  bool vec, join;  // join: the suffix rows run in the launch that joins the tiles' records
+  bool tile;       // rk_tile_dev.h over the shared spans, 64 queries a workgroup
   bool copy_q, ahead;  // queries copied into whole pieces; rotated ahead of the split launch
   int64_t S[kSpans], chunk[kSpans], wgs[kSpans], units[kSpans], blocks[kSpans], np, grid, rows;
   size_t q, qr, bias, zero, zero_bytes, acc, ml, total;
@@ -194,11 +202,11 @@ int check_rows(const rk_rows* r, int format, int dtype, int64_t N, int64_t H, in
     if (st) return st;
     if (r->data.dtype != dtype) return RK_ERR_DTYPE;
     if (r->data.shape[3] != dim || r->head_dim != dim) return RK_ERR_SHAPE;
-    // 32-bit offsets inside a head
+    // 32-bit byte offsets inside a head
     if ((S + 64) * r->data.stride[2] + dim * r->data.stride[3] >= (INT64_C(1) << 31)) return RK_ERR_STRIDE;
   }
   if (r->data.shape[0] != N || r->data.shape[1] != H || r->data.shape[2] != S) return RK_ERR_SHAPE;
-  return RK_OK;
+  return S < (INT64_C(1) << 30) ? RK_OK : RK_ERR_SHAPE;  // (rows that repeat by stride 0 can be any number)
 }
 
 int check_float(const rk_tensor* t, int ndim) {
@@ -264,65 +272,75 @@ int make_plan(const Call& c, int cus, Plan* out) {
   if (c.out) {
     if ((st = rk::check_desc(c.out, 3))) return st;
     if (c.out->dtype != c.q->dtype) return RK_ERR_DTYPE;
-    for (int i = 0; i < 3; ++i)
+    for (int i = 0; i < 3; ++i) {
       if (c.out->shape[i] != c.q->shape[i]) return RK_ERR_SHAPE;
+      if (c.out->shape[i] > 1 && c.out->stride[i] == 0) return RK_ERR_STRIDE;  // two rows at one address
+    }
   }
 
   p.kf = p.D <= 64 ? 2 : 4;
   p.kv = p.S[kRotated] == 0 ? 0 : p.Dk <= 32 ? 1 : p.Dk <= 64 ? 2 : 4;
   p.terms = quantised ? (c.q->dtype == RK_F32 ? 3 : 2) : 1;
-  // more than 16 queries on the same rows: 32 to a unit, for one read of
-  // K and V (element loads and fp32 queries stay at 16)
-  const int64_t rows = c.shared ? p.B * p.G : p.G;
-  p.nr = rows <= 16 || !p.vec || p.terms == 3 ? 1 : 2;
-  // more than 32: the waves of a workgroup take queries, not tokens
-  p.tile = c.shared && rows > kTileRows && p.vec && p.terms < 3;
+  if (p.B >= (INT64_C(1) << 31) / p.Hq) return RK_ERR_SHAPE;
   p.rows = p.B * p.Hq;
-  p.join = c.shared && p.S[kTail] > 0 && p.S[kTail] <= kJoinTokens;
-  int64_t cost[kSpans], total = 0;  // bytes of a token; of all units
+  int64_t cost[kSpans], shared_bytes = 0, shared_tokens = 0;  // cost: bytes of a token
   for (int i = 0; i < kSpans; ++i) {
-    const bool per_request = !c.shared || i == kTail;
-    const bool tiles = p.tile && i != kTail;
-    const int64_t r = tiles ? 64 : p.join && i == kTail ? 16 : 16 * p.nr;
-    p.blocks[i] = cdiv(per_request ? p.G : p.B * p.G, r);
-    p.units[i] = p.H * p.blocks[i] * (per_request ? p.B : 1);
     const int64_t kd = i == kRotated ? p.Dk : p.D;
     cost[i] = quantised ? rk::mx_row_bytes(kd, p.format) + rk::mx_row_bytes(p.D, p.format) : 2 * (kd + p.D);
-    if (!(p.join && i == kTail)) total += p.units[i] * p.S[i] * cost[i];
+    if (i == kTail) continue;
+    shared_bytes += p.S[i] * cost[i];
+    shared_tokens += p.S[i];
+  }
+  p.tile = c.shared && p.vec && p.terms < 3 && cdiv(p.B * p.G, 16) * shared_bytes > kTileBytes * shared_tokens;
+  p.join = p.tile && p.S[kTail] > 0 && p.S[kTail] <= kJoinTokens;
+  int64_t total = 0;
+  for (int i = 0; i < kSpans; ++i) {
+    const bool per_request = !c.shared || i == kTail;
+    p.blocks[i] = cdiv(per_request ? p.G : p.B * p.G, p.tile && i != kTail ? 64 : 16);
+    p.units[i] = p.H * p.blocks[i] * (per_request ? p.B : 1);
+    if (p.units[i] * p.S[i] >= (INT64_C(1) << 50)) return RK_ERR_SHAPE;
+    if (!(p.tile && i == kTail)) total += p.units[i] * p.S[i] * cost[i];
   }
   // Equal shares of the bytes for every workgroup, of whole rounds of the
   // workgroups that are resident at a time: the fewest rounds that keep a
-  // share at kMaxShare, and within them the largest grid that fits.
+  // share at kMaxShare, and within them the largest grid that fits.  Spans that
+  // are not split fill slots by their bytes, short ones many to a slot (as many
+  // slots as workgroups would leave the others too few: 16 requests of 8 heads
+  // with 264 tokens behind 8192, 34.0 us and 30.6); tiles fill one each.
   auto split = [&](int64_t slots) {
     const int64_t rounds = std::max<int64_t>(cdiv(total, slots * kMaxShare), 1);
     const int64_t align = rk::kSpanWaves * rk::kSpanBlk;
     for (int64_t share = std::max<int64_t>(cdiv(total, slots * rounds), 1);; share += cdiv(share, 32)) {
       p.np = p.grid = 0;
+      int64_t used = 0;
       bool least = true;  // one workgroup per unit and span
       for (int i = 0; i < kSpans; ++i) {
         p.wgs[i] = p.chunk[i] = 0;
         if (p.S[i] == 0 || (p.join && i == kTail)) continue;
         p.chunk[i] = std::min(round_up(cdiv(share, cost[i]), align), round_up(p.S[i], align));
         p.wgs[i] = cdiv(p.S[i], p.chunk[i]);
-        least = least && p.wgs[i] == 1;
         p.np += p.wgs[i];
         p.grid += p.wgs[i] * p.units[i];
+        if (p.tile && i == kTail) continue;  // a launch of its own
+        least = least && p.wgs[i] == 1;
+        used += p.wgs[i] > 1 || p.tile ? p.wgs[i] * p.units[i] : cdiv(p.units[i] * p.S[i] * cost[i], share);
       }
-      if (least || p.grid <= slots * rounds) break;
+      if (least || used <= slots * rounds) break;
     }
   };
-  // Three workgroups are resident on a CU (two of 32 queries).  Over 64 queries
-  // a workgroup's records weigh as much as 64 tokens' rows and the join reads
-  // them again: two there where three would leave it less than 768 tokens
-  // (32 requests of 4 heads behind 16001: 35 us at two, 512 tokens, 38 at three;
-  // 64 of 7 heads behind 32768: 90 at two, 77 at three).
-  split((int64_t)cus * (p.tile || p.nr == 1 ? 3 : 2));
+  // Three workgroups are resident on a CU.  Over 64 queries a workgroup's
+  // records weigh as much as 64 tokens' rows and the join reads them again: two
+  // there where three would leave it less than 768 tokens (32 requests of 4 heads
+  // behind 16001: 35 us at two, 512 tokens, 38 at three; 64 of 7 heads behind
+  // 32768: 90 at two, 77 at three).
+  split((int64_t)cus * 3);
   if (p.tile && std::max(p.chunk[kRotated], p.chunk[kFull]) < 768) split((int64_t)cus * 2);
   if (p.join) {
     p.chunk[kTail] = round_up(p.S[kTail], rk::kSpanWaves * rk::kSpanBlk);
     p.wgs[kTail] = 1;
   }
-  if (p.grid + 24 * p.units[0] + 24 * p.units[1] + 24 * p.units[2] >= (INT64_C(1) << 31) || p.rows >= (INT64_C(1) << 31) || p.rows * p.np >= (INT64_C(1) << 40))
+  // (24: the ids that launched() adds)
+  if (p.grid + 24 * (p.units[0] + p.units[1] + p.units[2]) >= (INT64_C(1) << 31) || p.rows * p.np >= (INT64_C(1) << 40))
     return RK_ERR_SHAPE;
   const int64_t dv = p.kf == 2 ? 64 : 128;
   size_t at = 0;
@@ -383,7 +401,6 @@ Span make_span(const Call& c, const Plan& p, int i, char* ws) {
     s.k_ss = (uint32_t)k->data.stride[2]; s.k_sd = (uint32_t)k->data.stride[3];
     s.width = (int32_t)(quantised ? rk::mx_width(k->head_dim) : k->head_dim);
     if (quantised) {
-      s.k_row = (int32_t)rk::mx_row_bytes(k->head_dim, p.format);
       s.ksc = (const uint8_t*)k->scales.data;
       s.ksc_sb = k->scales.stride[0]; s.ksc_sh = k->scales.stride[1]; s.ksc_sn = (uint32_t)k->scales.stride[2];
     }
@@ -439,7 +456,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
     if (p.S[i] == 0) continue;
     a.span[i] = make_span(c, p, i, ws);
     a.span[i].np0 = (int32_t)np0;
-    if (p.join && i == kTail) break;
+    if (p.join && i == kTail) continue;
     first += launched(p, i);
     np0 += p.wgs[i];
   }
@@ -488,7 +505,6 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
   a.B = (int32_t)p.B; a.Hq = (int32_t)p.Hq; a.H = (int32_t)p.H; a.G = (int32_t)p.G;
   a.D = (int32_t)p.D; a.Dk = (int32_t)p.Dk; a.np = (int32_t)p.np;
   a.shared = c.shared;
-  a.v_row = p.format == RK_ROWS_PLAIN ? 0 : (int32_t)rk::mx_row_bytes(p.D, p.format);
   a.scale_log2 = rk::kLog2e / sqrtf((float)p.D);
   if (p.zero_bytes) {
     hipLaunchKernelGGL(span_zero_kernel, dim3(64), dim3(256), 0, s, (uint32_t*)(ws + p.zero),
@@ -503,39 +519,42 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
       a.dm_sb = c.dm->stride[0]; a.dm_sh = c.dm->stride[1];
     }
   }
-  auto split = [&](const SpanArgs& b, int kv, unsigned grid) {
-    if (p.format == RK_ROWS_MX8) return rk::span_launch_mx8(kv, p.kf, p.nr, p.terms, b, grid, s);
-    if (p.format == RK_ROWS_MX4) return rk::span_launch_mx4(kv, p.kf, p.nr, p.terms, b, grid, s);
-    if (c.q->dtype == RK_F16) return rk::span_launch_f16(kv, p.kf, p.nr, p.vec, b, grid, s);
-    return rk::span_launch_bf16(kv, p.kf, p.nr, p.vec, b, grid, s);
-  };
-  auto tiles = [&](unsigned grid) {
-    if (p.format == RK_ROWS_MX8) return rk::tile_launch_mx8(p.kv, p.kf, a, grid, s);
-    if (p.format == RK_ROWS_MX4) return rk::tile_launch_mx4(p.kv, p.kf, a, grid, s);
-    if (c.q->dtype == RK_F16) return rk::tile_launch_f16(p.kv, p.kf, a, grid, s);
-    return rk::tile_launch_bf16(p.kv, p.kf, a, grid, s);
+  auto split = [&](const SpanArgs& b, int kv, int64_t grid) {
+    if (p.format == RK_ROWS_MX8) return rk::span_launch_mx8(kv, p.kf, p.terms, b, (unsigned)grid, s);
+    if (p.format == RK_ROWS_MX4) return rk::span_launch_mx4(kv, p.kf, p.terms, b, (unsigned)grid, s);
+    if (c.q->dtype == RK_F16) return rk::span_launch_f16(kv, p.kf, p.vec, b, (unsigned)grid, s);
+    return rk::span_launch_bf16(kv, p.kf, p.vec, b, (unsigned)grid, s);
   };
   if (!p.tile) {
-    if (first > 0 && split(a, p.kv, (unsigned)first) != hipSuccess) return RK_ERR_HIP;
+    if (first > 0 && split(a, p.kv, first) != hipSuccess) return RK_ERR_HIP;
   } else {
-    const int64_t shared = a.first[kTail];  // ids of the shared spans
-    if (shared > 0 && tiles((unsigned)shared) != hipSuccess) return RK_ERR_HIP;
-    if (first > shared) {  // a long suffix: its rows have few queries each
-      SpanArgs b = a;
-      b.first[kRotated] = b.first[kFull] = b.first[kTail] = 0;
-      if (split(b, 0, (unsigned)(first - shared)) != hipSuccess) return RK_ERR_HIP;
+    const int64_t shared = a.first[kTail];
+    if (first > shared) {  // a suffix that is split: a launch of its own
+      SpanArgs tail = a;
+      tail.first[kRotated] = tail.first[kFull] = tail.first[kTail] = 0;
+      if (split(tail, 0, first - shared) != hipSuccess) return RK_ERR_HIP;
     }
+    const unsigned grid = (unsigned)shared;
+    if (p.format == RK_ROWS_MX8)
+      e = rk::tile_launch_mx8(p.kv, p.kf, a, grid, s);
+    else if (p.format == RK_ROWS_MX4)
+      e = rk::tile_launch_mx4(p.kv, p.kf, a, grid, s);
+    else if (c.q->dtype == RK_F16)
+      e = rk::tile_launch_f16(p.kv, p.kf, a, grid, s);
+    else
+      e = rk::tile_launch_bf16(p.kv, p.kf, a, grid, s);
+    if (e != hipSuccess) return RK_ERR_HIP;
   }
   if (p.join) {
     const unsigned grid = (unsigned)launched(p, kTail);
     if (p.format == RK_ROWS_MX8)
-      e = rk::span_join_mx8(p.kf, p.terms, a, grid, s);
+      e = rk::span_join_mx8(p.kf, a, grid, s);
     else if (p.format == RK_ROWS_MX4)
-      e = rk::span_join_mx4(p.kf, p.terms, a, grid, s);
+      e = rk::span_join_mx4(p.kf, a, grid, s);
     else if (c.q->dtype == RK_F16)
-      e = rk::span_join_f16(p.kf, p.vec, a, grid, s);
+      e = rk::span_join_f16(p.kf, a, grid, s);
     else
-      e = rk::span_join_bf16(p.kf, p.vec, a, grid, s);
+      e = rk::span_join_bf16(p.kf, a, grid, s);
     return e == hipSuccess ? RK_OK : RK_ERR_HIP;
   }
   const dim3 mg((unsigned)cdiv(p.rows, 4));

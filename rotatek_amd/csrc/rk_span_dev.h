@@ -7,9 +7,12 @@
 // a workgroup covers one chunk of one span for one unit of query rows and
 // leaves (m, l, o) for each row; merge_rows joins a row's records.
 //
-// Units.  A unit is up to 16 NR query rows that read the same K and V: the
-// heads of a KV group, or, over a span that the batch shares, all the batch's
-// queries on a KV head.  Each K/V byte is then read once per 16 NR rows.
+// Units.  A unit is up to 16 query rows that read the same K and V: of the heads
+// of a KV group, or, over a span that the batch shares, of all the batch's
+// queries on a KV head.  Units of the same rows run on one XCD, whose L2 serves
+// all but the first.  (32 rows to a unit need more registers than leave three
+// workgroups on a CU: 17 to 32 queries on the same rows took 14.1 .. 56 us in
+// ten shapes, two units of 16 take 13.1 .. 32 us.)
 //
 // A workgroup is four waves that take interleaved blocks of 32 tokens.  Rows
 // come straight from memory into registers in the matrix core's layout, so a
@@ -88,23 +91,6 @@ __device__ __forceinline__ uint4 widen8(const uint32_t* w, float sc) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-typedef const __attribute__((address_space(1))) char* gptr;  // global memory
-#define RK_GLOBAL(T) const __attribute__((address_space(1))) T*
-
-template <int N>
-__device__ __forceinline__ void load_words(gptr p, uint32_t* w) {
-  if constexpr (N == 4) {
-    const u32x4 v = *(RK_GLOBAL(u32x4))p;
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (N == 2) {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    const u32x2 v = *(RK_GLOBAL(u32x2))p;
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = *(RK_GLOBAL(uint32_t))p;
-  }
-}
-
 // A block of 32 tokens as one wave holds it.  k[tt]: the lane's 8 KB channels
 // of token 16 tt + n; v[r]: its VB channels of token token_of(g, r).  (A tile's
 // 16 rows are neighbours: the 16 lanes that load one piece of them touch the
@@ -121,14 +107,14 @@ struct Block {
 
 // A unit's rows of one tensor as a buffer: a load is descriptor + scalar
 // offset of the block + fixed 32-bit offset of the lane (an address needs two
-// registers and a 64-bit vector addition per load).  The hardware checks the
-// lane's offset alone, so the kernels clamp rows and columns themselves.
+// registers and a 64-bit vector addition per load).  The hardware would check
+// the lane's offset alone, so the kernels clamp rows and columns themselves.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
-__device__ __forceinline__ Rsrc make_rsrc(const void* p, uint32_t bytes) {
+__device__ __forceinline__ Rsrc make_rsrc(const void* p) {
   const uint64_t v = (uint64_t)p;
   const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) |
                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32;
-  return __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, (int)__builtin_amdgcn_readfirstlane((int)bytes), 0x00027000);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, -1, 0x00027000);  // 2^32 - 1 bytes
 }
 // AUX 2: non-temporal, for rows that one instruction reads whole lines of and
 // that no other unit reads.
@@ -264,12 +250,6 @@ __device__ __forceinline__ void load_v(const Span& sp, const SpanLane<KB>& hd, i
   }
 }
 
-// Blocks of a wave in flight.
-template <class F, int NR, int NT>
-constexpr int blocks_ahead() {
-  return F::kMx && NR == 1 ? 1 : 1;
-}
-
 // Values as the products take them: x as the sum of NT 16-bit terms.
 template <class TT, int NT>
 __device__ __forceinline__ void terms8(const float (&x)[8], uint4 (&o)[NT]) {
@@ -301,16 +281,23 @@ constexpr float kLift = TT::kRk == 0 ? 10.f : 0.f;
 template <class TT>
 constexpr float kSlack = TT::kRk == 0 ? 5.f : 8.f;
 
-// The running state of one wave: NR blocks of 16 query rows.  m: the maximum
-// that the sums are relative to (0 until a token was `seen`, which all rows of
-// a block do together); top: the lane's largest score so far, relative to m
-// and lifted.  l: the sum of the probabilities, formed with the others as the
-// product of P with ones: every register of it is the sum.
-template <int NR, int VB>
+// The running state of one wave's 16 query rows, a row a lane (n).  m: the
+// maximum that the sums are relative to (0 until the row's first score above
+// -infinity); high: the score, relative to m and lifted, that raises it; top:
+// the lane's largest score so far, likewise.  l: the sum of the probabilities,
+// formed with the others as the product of P with ones: every register of it is
+// the sum.
+template <int VB>
 struct State {
-  float m[NR], top[NR];
-  bool seen[NR];
-  f32x4 l[NR], acc[NR][VB];
+  float m, high, top;
+  f32x4 l, acc[VB];
+  __device__ __forceinline__ void clear() {
+    m = 0.f;
+    high = top = -INFINITY;
+    l = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < VB; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
 };
 // One instruction: fmaxf quiets each operand with another.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -327,73 +314,70 @@ __device__ __forceinline__ uint4 ones() {
 // Scores to sums for one block of 32 tokens: softmax of s (raw products; off:
 // the addend of a score, moved with the maximum) and O^T += V^T P^T.  on: which
 // of the lane's eight tokens count, unless the block is whole.  turn(w, lo, hi)
-// gives V^T of channel slots 2 w and 2 w + 1, all of them ahead of the softmax or
-// each as it is needed; used() is called once V is.
-template <class TT, int VB, int NR, int NP, bool AHEAD, class Turn, class Used>
-__device__ __forceinline__ void weigh_block(const f32x4 (&s)[2][NR], float scale, float (&off)[NR], bool whole,
-                                            uint32_t on, State<NR, VB>& st, const Turn& turn, const Used& used) {
+// gives V^T of channel slots 2 w and 2 w + 1: AHEAD, all of them before the
+// softmax (reads of LDS, which it hides), or each as it is needed.
+template <class TT, int VB, int NP, bool AHEAD, class Turn>
+__device__ __forceinline__ void weigh_block(const f32x4 (&s)[2], float scale, float& off, bool whole, uint32_t on,
+                                            State<VB>& st, const Turn& turn) {
   uint4 av[AHEAD ? VB : 1];
   if constexpr (AHEAD) {
 #pragma unroll
     for (int w = 0; w < VB / 2; ++w) turn(w, av[2 * w], av[2 * w + 1]);
-    used();
+  }
+  float sc[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) sc[r] = fmaf(s[r >> 2][r & 3], scale, off);
+  if (!whole) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) sc[r] = (on >> r) & 1u ? sc[r] : -INFINITY;
+  }
+  float mx = max3(sc[0], sc[1], sc[2]);
+  mx = max3(mx, sc[3], sc[4]);
+  mx = max3(mx, sc[5], sc[6]);
+  mx = max3(mx, sc[7], sc[7]);
+  st.top = max3(st.top, mx, mx);
+  if (__any(mx > st.high)) {
+    mx = fmaxf(mx, shfl_xor(mx, 16));
+    mx = fmaxf(mx, shfl_xor(mx, 32));
+    // how far the maximum rises; the first tokens set it
+    float up = mx - kLift<TT>;
+    if (st.high > -INFINITY) up = fmaxf(up, 0.f);
+    if (up > -INFINITY)
+      st.high = kSlack<TT> + kLift<TT>;
+    else
+      up = 0.f;
+    const float alpha = fast_exp2(-up);
+#pragma unroll
+    for (int j = 0; j < VB; ++j) st.acc[j] *= alpha;
+    st.l *= alpha;
+    st.m += up;
+    st.top -= up;
+    off -= up;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) sc[r] -= up;
   }
 #pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-    float sc[8];
+  for (int r = 0; r < 8; ++r) sc[r] = fast_exp2(sc[r]);
+  uint4 p[NP];
+  terms8<TT, NP>(sc, p);
 #pragma unroll
-    for (int r = 0; r < 8; ++r) sc[r] = fmaf(s[r >> 2][nr][r & 3], scale, off[nr]);
-    if (!whole) {
+  for (int t = 0; t < NP; ++t) st.l = TT::mfma(ones<TT>(), p[t], st.l);
+  if constexpr (AHEAD) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) sc[r] = (on >> r) & 1u ? sc[r] : -INFINITY;
-    }
-    float mx = max3(sc[0], sc[1], sc[2]);
-    mx = max3(mx, sc[3], sc[4]);
-    mx = max3(mx, sc[5], sc[6]);
-    mx = max3(mx, sc[7], sc[7]);
-    st.top[nr] = max3(st.top[nr], mx, mx);
-    if (!st.seen[nr] || __any(mx > kSlack<TT> + kLift<TT>)) {
-      mx = fmaxf(mx, shfl_xor(mx, 16));
-      mx = fmaxf(mx, shfl_xor(mx, 32));
-      // how far the maximum rises; the first tokens set it
-      float up = mx - kLift<TT>;
-      if (st.seen[nr]) up = fmaxf(up, 0.f);
-      st.seen[nr] = st.seen[nr] || __any(mx > -INFINITY);
-      up = up > -INFINITY ? up : 0.f;
-      const float alpha = fast_exp2(-up);
+    for (int t = 0; t < NP; ++t)
 #pragma unroll
-      for (int j = 0; j < VB; ++j) st.acc[nr][j] *= alpha;
-      st.l[nr] *= alpha;
-      st.m[nr] += up;
-      st.top[nr] -= up;
-      off[nr] -= up;
+      for (int j = 0; j < VB; ++j) st.acc[j] = TT::mfma(av[j], p[t], st.acc[j]);
+  } else {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) sc[r] -= up;
-    }
+    for (int w = 0; w < VB / 2; ++w) {
+      uint4 lo, hi;
+      __builtin_amdgcn_sched_barrier(0);  // one pair's registers at a time
+      turn(w, lo, hi);
 #pragma unroll
-    for (int r = 0; r < 8; ++r) sc[r] = fast_exp2(sc[r]);
-    uint4 p[NP];
-    terms8<TT, NP>(sc, p);
-#pragma unroll
-    for (int t = 0; t < NP; ++t) st.l[nr] = TT::mfma(ones<TT>(), p[t], st.l[nr]);
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int t = 0; t < NP; ++t)
-#pragma unroll
-        for (int j = 0; j < VB; ++j) st.acc[nr][j] = TT::mfma(av[j], p[t], st.acc[nr][j]);
-    } else {
-#pragma unroll
-      for (int w = 0; w < VB / 2; ++w) {
-        uint4 lo, hi;
-        __builtin_amdgcn_sched_barrier(0);  // one pair's registers at a time
-        turn(w, lo, hi);
-#pragma unroll
-        for (int t = 0; t < NP; ++t) {
-          st.acc[nr][2 * w] = TT::mfma(lo, p[t], st.acc[nr][2 * w]);
-          st.acc[nr][2 * w + 1] = TT::mfma(hi, p[t], st.acc[nr][2 * w + 1]);
-        }
+      for (int t = 0; t < NP; ++t) {
+        st.acc[2 * w] = TT::mfma(lo, p[t], st.acc[2 * w]);
+        st.acc[2 * w + 1] = TT::mfma(hi, p[t], st.acc[2 * w + 1]);
       }
-      used();
     }
   }
 }
@@ -401,10 +385,10 @@ __device__ __forceinline__ void weigh_block(const f32x4 (&s)[2][NR], float scale
 // One chunk of one span: adds the wave's blocks to `st`.  pre(): stages the
 // unit's queries in LDS, sq [term][row][stride] 16-bit in the lane's channel
 // order, while the first blocks are on their way.
-template <class F, int KB, int VB, int NR, int NT, int NP, bool VEC, class Pre>
+template <class F, int KB, int VB, int NT, int NP, bool VEC, class Pre>
 __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, SpanLane<KB>& hd, int b, int chunk, int wave,
                                          int lane, const uint16_t* sq, int qstride, const float* sbias,
-                                         State<NR, VB>& st, const Pre& pre) {
+                                         State<VB>& st, const Pre& pre) {
   using TT = typename F::TT;
   const int g = lane >> 4, n = lane & 15;
   int lim = min(chunk * sp.chunk + sp.chunk, sp.S);
@@ -412,45 +396,34 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
   lim = __builtin_amdgcn_readfirstlane(lim);  // (a loaded length sits in a vector register)
   const int blk0 = chunk * sp.chunk / kSpanBlk + wave, nblk = (lim + kSpanBlk - 1) / kSpanBlk;
   const int nw = nblk > blk0 ? (nblk - blk0 - 1) / kSpanWaves + 1 : 0;
-  // past the wave's last block the ring reads that block again
+  // past the wave's last block the loads ahead take that block again
   auto blk_of = [&](int i) { return blk0 + kSpanWaves * min(i, max(nw - 1, 0)); };
   lane_offsets<F, KB, VB>(sp, a.D, g, n, hd);
   // rows of whole lines: 16 lanes' Value channels, four rows of 32 Key channels
-  constexpr int kAux = NR == 1 && Block<F, KB, VB>::kvw * 64 >= 128 ? 2 : 0;
-  constexpr int NBUF = blocks_ahead<F, NR, NT>();
-  Block<F, KB, VB> buf[NBUF];
-#pragma unroll
-  for (int i = 0; i < NBUF; ++i) {
-    load_k<F, KB, VB, VEC, kAux>(sp, hd, blk_of(i), g, buf[i]);
-    load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, blk_of(i), n, buf[i]);
-  }
+  constexpr int kAux = Block<F, KB, VB>::kvw * 64 >= 128 ? 2 : 0;
+  Block<F, KB, VB> x;
+  load_k<F, KB, VB, VEC, kAux>(sp, hd, blk_of(0), g, x);
+  load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, blk_of(0), n, x);
   pre();
-  constexpr bool kRegQ = NR * NT * KB <= (NR == 1 ? (F::kMx ? 4 : 8) : 8);  // queries held in registers
-  uint4 qreg[kRegQ ? NR : 1][kRegQ ? NT : 1][kRegQ ? KB : 1];
-  auto qload = [&](int nr, int t, int j) {
+  // queries held in registers where that leaves room for the blocks
+  constexpr bool kRegQ = NT * KB <= (F::kMx ? 4 : 8);
+  uint4 qreg[kRegQ ? NT : 1][kRegQ ? KB : 1];
+  auto qload = [&](int t, int j) {
     const int c = F::kMx ? 8 * KB * g + 8 * j : 32 * j + 8 * g;
-    return *(const uint4*)(sq + ((t * NR + nr) * 16 + n) * qstride + c);
+    return *(const uint4*)(sq + (t * 16 + n) * qstride + c);
   };
   if constexpr (kRegQ) {
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int j = 0; j < KB; ++j) qreg[nr][t][j] = qload(nr, t, j);
+      for (int j = 0; j < KB; ++j) qreg[t][j] = qload(t, j);
   }
   // a score is one fused multiply-add: the bias, the maximum and the lift in
   // its addend
-  float off[NR];
-#pragma unroll
-  for (int nr = 0; nr < NR; ++nr) off[nr] = (sbias ? sbias[nr * 16 + n] * a.scale_log2 : 0.f) + kLift<TT>;
+  float off = (sbias ? sbias[n] * a.scale_log2 : 0.f) + kLift<TT>;
 
-  auto compute = [&](Block<F, KB, VB>& x, int blk, int next) {
-    f32x4 s[2][NR];
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-      for (int nr = 0; nr < NR; ++nr) s[tt][nr] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  auto compute = [&](int blk, int next) {
+    f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int j = 0; j < KB; ++j)
 #pragma unroll
@@ -461,14 +434,12 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
         if constexpr (!F::kMx && VEC)
           if (sp.width < 32 * KB && 32 * j + 8 * g >= sp.width) kop = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if constexpr (kRegQ)
-              s[tt][nr] = TT::mfma(kop, qreg[nr][t][j], s[tt][nr]);
-            else
-              s[tt][nr] = TT::mfma(kop, qload(nr, t, j), s[tt][nr]);
-          }
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (kRegQ)
+            s[tt] = TT::mfma(kop, qreg[t][j], s[tt]);
+          else
+            s[tt] = TT::mfma(kop, qload(t, j), s[tt]);
+        }
       }
     load_k<F, KB, VB, VEC, kAux>(sp, hd, next, g, x);
     // which of the lane's eight tokens count
@@ -512,16 +483,11 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
       lo = make_uint4(pack_lo(y[0], y[1]), pack_lo(y[2], y[3]), pack_lo(y[4], y[5]), pack_lo(y[6], y[7]));
       hi = make_uint4(pack_hi(y[0], y[1]), pack_hi(y[2], y[3]), pack_hi(y[4], y[5]), pack_hi(y[6], y[7]));
     };
-    // several row blocks share V^T; one forms it as it goes
-    weigh_block<TT, VB, NR, NP, (NR > 1)>(s, a.scale_log2, off, whole, on, st, turn,
-                                [&]() { load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, next, n, x); });
+    weigh_block<TT, VB, NP, false>(s, a.scale_log2, off, whole, on, st, turn);
+    load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, next, n, x);
   };
 
-  for (int i = 0; i < nw; i += NBUF) {
-#pragma unroll
-    for (int j = 0; j < NBUF; ++j)
-      if (j == 0 || i + j < nw) compute(buf[j], blk_of(i + j), blk_of(i + j + NBUF));
-  }
+  for (int i = 0; i < nw; ++i) compute(blk_of(i), blk_of(i + 1));
 }
 
 // Query row R of a unit: its batch row and head.
@@ -753,17 +719,20 @@ __device__ __forceinline__ void join_records(const SpanArgs& a, const RowOf& o, 
   store_out4(a, o.b, o.h, c, v / (L + kDenomEps));
 }
 
-// JOIN: the launch behind the split one, over the suffix rows of a shared call
-// (short ones: one workgroup per unit).  It joins the other spans' records to
-// its sums and writes the output.
-template <class F, int KV, int KF, int NR, int NT, int NP, bool VEC, bool JOIN = false>
-__global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3) : 2) span_kernel(const SpanArgs a) {
+// JOIN: the launch behind tile_kernel's, over the suffix rows of a shared call
+// (one workgroup per unit).  It joins the other spans' records to its sums and
+// writes the output.
+//
+// A workgroup of MX rows has room for four on a CU in its 128 registers a lane,
+// of plain ones for three; element loads (VEC false) keep more addresses.
+template <class F, int KV, int KF, int NT, int NP, bool VEC, bool JOIN = false>
+__global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span_kernel(const SpanArgs a) {
   using TT = typename F::TT;
   constexpr int VB = KF == 2 ? 4 : 8;
   constexpr int DV = 16 * VB;
   constexpr int NTV = NT < 2 ? 2 : NT;  // terms of a rotated query
   constexpr int NW = NT == 3 ? 8 : 4;   // words of eight channels of a query
-  constexpr int kRows = 16 * NR;
+  constexpr int kRows = 16;
   constexpr int kWide = 32 * (KV > KF ? KV : KF) + 8;  // +8: rows start in other banks
   constexpr int kQ = kRows * kWide * (KV > 0 ? NTV : NT);
   constexpr int kRaw = KV > 0 && NT < 3 ? kRows * 136 + 128 * 32 * KV + 128 : 0;
@@ -779,12 +748,12 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int id = (int)blockIdx.x;
-  const int k = JOIN || id >= a.first[2] ? kTail : id >= a.first[1] ? kFull : kRotated;
+  const int k = JOIN || id >= a.first[kTail] ? kTail : id >= a.first[kFull] ? kFull : kRotated;
   const Span sp = a.span[k];  // (copied whole: few, wide scalar loads)
   const int rel = JOIN ? id : id - a.first[k];
   // Workgroups go to the 8 XCDs, each with an L2 of its own, in turn: the row
-  // blocks that read the same rows are 8 ids apart, on one XCD (32 requests of
-  // 4 heads behind 16001 tokens: TTT us).  The last of the ids may have none.
+  // blocks that read the same rows are 8 ids apart, on one XCD.  The last of the
+  // ids may have none.
   // (Quotients are formed on the vector unit: back to scalar registers, so that
   // everything derived from them stays there.)
   const bool shared = a.shared && k != kTail;
@@ -796,36 +765,22 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3
   const int b = shared ? 0 : __builtin_amdgcn_readfirstlane(ukv / a.H), kv = shared ? ukv : ukv - b * a.H;
   const int rows = min((shared ? a.B * a.G : a.G) - R0, kRows);
 
-  State<NR, VB> st;
-#pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-    st.m[nr] = 0.f;
-    st.top[nr] = -INFINITY;
-    st.seen[nr] = false;
-    st.l[nr] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < VB; ++j) st.acc[nr][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  }
+  State<VB> st;
+  st.clear();
 
   auto head = [&](auto& hd) {
     constexpr int kEl = F::kMx ? 1 : 2;
-    // bytes to the end of the unit's last row
-    const uint32_t kb = VEC ? sp.width : (sp.width > 0 ? (sp.width - 1) * sp.k_sd + 1 : 0);
-    const uint32_t vb = VEC ? (F::kMx ? a.v_row : a.D) : (a.D - 1) * sp.v_sd + 1;
-    hd.k = make_rsrc((const char*)sp.k + kEl * (b * sp.k_sb + kv * sp.k_sh),
-                     sp.width > 0 ? kEl * (uint32_t)(sp.S - 1) * sp.k_ss + (F::kMx ? sp.k_row : kEl * kb) : 256u);
-    hd.v = make_rsrc((const char*)sp.v + kEl * (b * sp.v_sb + kv * sp.v_sh),
-                     kEl * ((uint32_t)(sp.S - 1) * sp.v_ss + vb));
+    hd.k = make_rsrc((const char*)sp.k + kEl * (b * sp.k_sb + kv * sp.k_sh));
+    hd.v = make_rsrc((const char*)sp.v + kEl * (b * sp.v_sb + kv * sp.v_sh));
     if constexpr (F::kMx) {
-      hd.ksc = make_rsrc(sp.ksc + b * sp.ksc_sb + kv * sp.ksc_sh,
-                         (uint32_t)(max(sp.width / 32, 1) - 1) * sp.ksc_sn + (uint32_t)sp.S);
+      hd.ksc = make_rsrc(sp.ksc + b * sp.ksc_sb + kv * sp.ksc_sh);
       hd.vsc = sp.vsc + b * sp.vsc_sb + kv * sp.vsc_sh;
     }
   };
   // The small loads first: loads return in order, and nothing below then waits
   // for the first K and V block.
   const bool f16 = F::kMx ? a.q_dtype == F16::kRk : TT::kRk == F16::kRk;
-  Queries<NR, NW> qw;
+  Queries<1, NW> qw;
   bool done = false;
   if constexpr (KV > 0) {
     if (k == kRotated) {
@@ -834,7 +789,7 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3
       const bool here = NT < 3 && !a.qr;
       Rotation<KV> rot;
       if (here) {
-        load_queries<NR, NW>(a, shared, b, kv, R0, rows, tid, qw);
+        load_queries<1, NW>(a, shared, b, kv, R0, rows, tid, qw);
         load_rotation<KV>(a, shared ? 0 : b, kv, tid, rot);
       }
       auto pre = [&]() {
@@ -842,10 +797,10 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3
           if constexpr (NT < 3) {
             uint4* s_r = (uint4*)(s_raw + kRows * 136);
             uint4* s_mu = s_r + 128 * 4 * KV;
-            stage_queries<TT, 1, NR, NW, 128>(tid, qw, f16, s_raw, 136);
+            stage_queries<TT, 1, 1, NW, 128>(tid, qw, f16, s_raw, 136);
             stage_rotation<KV>(tid, rot, s_r, s_mu);
             __syncthreads();
-            rotate_queries<TT, NTV, NR, KV>(a, wave, lane, f16, s_raw, s_r, s_mu, s_q, kWide, s_bias);
+            rotate_queries<TT, NTV, 1, KV>(a, wave, lane, f16, s_raw, s_r, s_mu, s_q, kWide, s_bias);
           }
         } else {
           constexpr int W = 32 * KV;
@@ -865,56 +820,45 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3
         }
         __syncthreads();
       };
-      run_span<F, KV, VB, NR, NTV, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias, st, pre);
+      run_span<F, KV, VB, NTV, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias, st, pre);
       done = true;
     }
   }
   if (!done) {
     SpanLane<KF> hd;
     head(hd);
-    load_queries<NR, NW>(a, shared, b, kv, R0, rows, tid, qw);
+    load_queries<1, NW>(a, shared, b, kv, R0, rows, tid, qw);
     auto pre = [&]() {
-      stage_queries<TT, NT, NR, NW, 32 * KF>(tid, qw, f16, s_q, kWide);
+      stage_queries<TT, NT, 1, NW, 32 * KF>(tid, qw, f16, s_q, kWide);
       __syncthreads();
     };
-    run_span<F, KF, VB, NR, NT, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, st, pre);
+    run_span<F, KF, VB, NT, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, st, pre);
   }
 
-  // from here: the true maxima, and the sum's one value; a row without tokens
-  // has the least maximum
-  float l[NR];
-#pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-    l[nr] = st.l[nr][0];
-    st.top[nr] = fmaxf(st.top[nr], shfl_xor(st.top[nr], 16));
-    st.top[nr] = fmaxf(st.top[nr], shfl_xor(st.top[nr], 32));
-    st.top[nr] = st.seen[nr] ? st.top[nr] + st.m[nr] - kLift<TT> : kNegInit;
-    st.m[nr] = st.seen[nr] ? st.m[nr] : kNegInit;
-  }
+  // The row's true maximum; a row without tokens has the least one.
+  float top = fmaxf(st.top, shfl_xor(st.top, 16));
+  top = fmaxf(top, shfl_xor(top, 32));
+  const bool seen = st.high > -INFINITY;
+  top = seen ? top + st.m - kLift<TT> : kNegInit;
+  const float m = seen ? st.m : kNegInit;
   // join the four waves: the common maximum, every wave's sums under it through
   // LDS, then a thread adds four channels of a row
-#pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-    if (g == 0) {
-      s_m[wave][16 * nr + n] = st.m[nr];
-      s_top[wave][16 * nr + n] = st.top[nr];
-      s_l[wave][16 * nr + n] = l[nr];
-    }
+  if (g == 0) {
+    s_m[wave][n] = m;
+    s_top[wave][n] = top;
+    s_l[wave][n] = st.l[0];
   }
   __syncthreads();  // (also: no wave reads queries any more)
-#pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-    const int r = 16 * nr + n;
-    if (r >= rows) continue;
-    const float M = fmaxf(fmaxf(s_top[0][r], s_top[1][r]), fmaxf(s_top[2][r], s_top[3][r]));
-    const float f = fast_exp2(st.m[nr] - M - kLift<TT>);
-    float* dst = s_acc + (wave * kRows + r) * kAccRow + 4 * g * VB;
+  if (n < rows) {
+    const float M = fmaxf(fmaxf(s_top[0][n], s_top[1][n]), fmaxf(s_top[2][n], s_top[3][n]));
+    const float f = fast_exp2(m - M - kLift<TT>);
+    float* dst = s_acc + (wave * kRows + n) * kAccRow + 4 * g * VB;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < VB; j += 4)
-        *(f32x4*)(dst + i * VB + j) = (f32x4){st.acc[nr][j][i] * f, st.acc[nr][j + 1][i] * f,
-                                              st.acc[nr][j + 2][i] * f, st.acc[nr][j + 3][i] * f};
+        *(f32x4*)(dst + i * VB + j) = (f32x4){st.acc[j][i] * f, st.acc[j + 1][i] * f, st.acc[j + 2][i] * f,
+                                              st.acc[j + 3][i] * f};
   }
   __syncthreads();
   const int rec = sp.np0 + x;
@@ -939,37 +883,37 @@ __global__ void __launch_bounds__(kSpanThreads, NR == 1 && VEC ? (F::kMx ? 4 : 3
   }
 }
 
-template <class F, int KV, int KF, int NR, int NT, int NP, bool VEC>
+template <class F, int KV, int KF, int NT, int NP, bool VEC>
 hipError_t launch_span(const SpanArgs& a, unsigned grid, hipStream_t s) {
-  hipLaunchKernelGGL((span_kernel<F, KV, KF, NR, NT, NP, VEC>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+  hipLaunchKernelGGL((span_kernel<F, KV, KF, NT, NP, VEC>), dim3(grid), dim3(kSpanThreads), 0, s, a);
   return hipGetLastError();
 }
 
-// The instantiation for a call's widths and row blocks.
-template <class F, int NT, int NP, bool VEC, int NR>
+// The instantiation for a call's widths.
+template <class F, int NT, int NP, bool VEC>
 hipError_t pick_widths(int kv, int kf, const SpanArgs& a, unsigned grid, hipStream_t s) {
   if (kf == 2) {
     switch (kv) {
-      case 0: return launch_span<F, 0, 2, NR, NT, NP, VEC>(a, grid, s);
-      case 1: return launch_span<F, 1, 2, NR, NT, NP, VEC>(a, grid, s);
-      default: return launch_span<F, 2, 2, NR, NT, NP, VEC>(a, grid, s);
+      case 0: return launch_span<F, 0, 2, NT, NP, VEC>(a, grid, s);
+      case 1: return launch_span<F, 1, 2, NT, NP, VEC>(a, grid, s);
+      default: return launch_span<F, 2, 2, NT, NP, VEC>(a, grid, s);
     }
   }
   switch (kv) {
-    case 0: return launch_span<F, 0, 4, NR, NT, NP, VEC>(a, grid, s);
-    case 1: return launch_span<F, 1, 4, NR, NT, NP, VEC>(a, grid, s);
-    case 2: return launch_span<F, 2, 4, NR, NT, NP, VEC>(a, grid, s);
-    default: return launch_span<F, 4, 4, NR, NT, NP, VEC>(a, grid, s);
+    case 0: return launch_span<F, 0, 4, NT, NP, VEC>(a, grid, s);
+    case 1: return launch_span<F, 1, 4, NT, NP, VEC>(a, grid, s);
+    case 2: return launch_span<F, 2, 4, NT, NP, VEC>(a, grid, s);
+    default: return launch_span<F, 4, 4, NT, NP, VEC>(a, grid, s);
   }
 }
 
 // The suffix rows of a shared call and the join (kf as above).
-template <class F, int NT, int NP, bool VEC>
+template <class F, int NT, int NP>
 hipError_t pick_join(int kf, const SpanArgs& a, unsigned grid, hipStream_t s) {
   if (kf == 2)
-    hipLaunchKernelGGL((span_kernel<F, 0, 2, 1, NT, NP, VEC, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+    hipLaunchKernelGGL((span_kernel<F, 0, 2, NT, NP, true, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((span_kernel<F, 0, 4, 1, NT, NP, VEC, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+    hipLaunchKernelGGL((span_kernel<F, 0, 4, NT, NP, true, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
   return hipGetLastError();
 }
 

@@ -6,14 +6,12 @@ namespace rk {
 
 using F = PlainFmt<F16>;
 
-hipError_t span_launch_f16(int kv, int kf, int nr, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s) {
-  if (!vec) return pick_widths<F, 1, 2, false, 1>(kv, kf, a, grid, s);
-  return nr == 1 ? pick_widths<F, 1, 2, true, 1>(kv, kf, a, grid, s)
-                 : pick_widths<F, 1, 2, true, 2>(kv, kf, a, grid, s);
+hipError_t span_launch_f16(int kv, int kf, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s) {
+  return vec ? pick_widths<F, 1, 2, true>(kv, kf, a, grid, s) : pick_widths<F, 1, 2, false>(kv, kf, a, grid, s);
 }
 
-hipError_t span_join_f16(int kf, bool vec, const SpanArgs& a, unsigned grid, hipStream_t s) {
-  return vec ? pick_join<F, 1, 2, true>(kf, a, grid, s) : pick_join<F, 1, 2, false>(kf, a, grid, s);
+hipError_t span_join_f16(int kf, const SpanArgs& a, unsigned grid, hipStream_t s) {
+  return pick_join<F, 1, 2>(kf, a, grid, s);
 }
 
 }  // namespace rk

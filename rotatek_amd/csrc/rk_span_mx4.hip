@@ -8,14 +8,12 @@ using F = Mx4Fmt;
 
 // terms 2: bf16 and fp16 queries, exact in two bf16 terms, probabilities in
 // two; 3: fp32 ones, exact in three, probabilities in three.
-hipError_t span_launch_mx4(int kv, int kf, int nr, int terms, const SpanArgs& a, unsigned grid, hipStream_t s) {
-  if (terms == 3) return pick_widths<F, 3, 3, true, 1>(kv, kf, a, grid, s);
-  return nr == 1 ? pick_widths<F, 2, 2, true, 1>(kv, kf, a, grid, s)
-                 : pick_widths<F, 2, 2, true, 2>(kv, kf, a, grid, s);
+hipError_t span_launch_mx4(int kv, int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s) {
+  return terms == 3 ? pick_widths<F, 3, 3, true>(kv, kf, a, grid, s) : pick_widths<F, 2, 2, true>(kv, kf, a, grid, s);
 }
 
-hipError_t span_join_mx4(int kf, int terms, const SpanArgs& a, unsigned grid, hipStream_t s) {
-  return terms == 3 ? pick_join<F, 3, 3, true>(kf, a, grid, s) : pick_join<F, 2, 2, true>(kf, a, grid, s);
+hipError_t span_join_mx4(int kf, const SpanArgs& a, unsigned grid, hipStream_t s) {
+  return pick_join<F, 2, 2>(kf, a, grid, s);
 }
 
 }  // namespace rk

@@ -2,7 +2,7 @@
 // gfx950), included by the per-format units rk_tile_*.hip.
 //
 // The mathematics and the products are rk_span_dev.h's; the split is another.
-// There a workgroup's four waves take different tokens for the same 16 NR
+// There a workgroup's four waves take different tokens for the same 16
 // queries, which suits rows that few queries read.  Where a batch shares its
 // prefix, one KV head's rows meet all the batch's queries: here the four waves
 // take different queries, 16 each, and the same 64 tokens at a time, staged in
@@ -91,7 +91,7 @@ __device__ __forceinline__ void store_tile(const Span& sp, int D, int t0, int ti
 // One chunk of a span for the wave's 16 queries, which pre() leaves in q and off.
 template <class F, int KB, int VB, int NT, int NP, class Pre>
 __device__ __forceinline__ void run_tiles(const SpanArgs& a, const Span& sp, const SpanLane<1>& hd, Rsrc vsc, int chunk,
-                                          int tid, char* mem, State<1, VB>& st, const Pre& pre) {
+                                          int tid, char* mem, State<VB>& st, const Pre& pre) {
   using TT = typename F::TT;
   const int lane = tid & 63, g = lane >> 4, n = lane & 15;
   const int first = chunk * sp.chunk, lim = min(first + sp.chunk, sp.S);
@@ -99,8 +99,8 @@ __device__ __forceinline__ void run_tiles(const SpanArgs& a, const Span& sp, con
   TilePart<F, KB, VB> part;
   load_tile<F, KB, VB>(sp, hd, vsc, a.D, first, tid, part);
   uint4 q[NT][KB];
-  float off[1];
-  pre(q, off[0]);
+  float off;
+  pre(q, off);
   __syncthreads();  // (the queries' LDS is the tiles')
   store_tile<F, KB, VB>(sp, a.D, first, tid, part, (uint4*)mem, (uint4*)(mem + kKBytes));
   __syncthreads();
@@ -113,7 +113,7 @@ __device__ __forceinline__ void run_tiles(const SpanArgs& a, const Span& sp, con
     for (int h = 0; h < 2; ++h) {
       const int tb = t0 + 32 * h;
       if (tb >= lim) break;
-      f32x4 s[2][1] = {{{0.f, 0.f, 0.f, 0.f}}, {{0.f, 0.f, 0.f, 0.f}}};
+      f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int j = 0; j < KB; ++j)
 #pragma unroll
@@ -121,7 +121,7 @@ __device__ __forceinline__ void run_tiles(const SpanArgs& a, const Span& sp, con
           const int r = 32 * h + 16 * tt + n;
           const uint4 kop = ks[r * (4 * KB) + swizzle<4 * KB>(4 * j + g, r)];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) s[tt][0] = TT::mfma(kop, q[t][j], s[tt][0]);
+          for (int t = 0; t < NT; ++t) s[tt] = TT::mfma(kop, q[t][j], s[tt]);
         }
       const bool whole = tb + 32 <= lim;
       uint32_t on = 0xffu;
@@ -135,7 +135,7 @@ __device__ __forceinline__ void run_tiles(const SpanArgs& a, const Span& sp, con
         lo = read_columns<2 * VB>(vs, 32 * h, 2 * w, g, n);
         hi = read_columns<2 * VB>(vs, 32 * h, 2 * w + 1, g, n);
       };
-      weigh_block<TT, VB, 1, NP, true>(s, a.scale_log2, off, whole, on, st, turn, [] {});
+      weigh_block<TT, VB, NP, true>(s, a.scale_log2, off, whole, on, st, turn);
     }
     __syncthreads();
     if (more)
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kSpanThreads, 3) tile_kernel(const SpanArgs a)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int id = (int)blockIdx.x;
-  const int k = id >= a.first[1] ? kFull : kRotated;
+  const int k = id >= a.first[kFull] ? kFull : kRotated;
   const Span sp = a.span[k];
   const int rel = id - a.first[k];
   // row blocks of the same rows on one XCD, as in span_kernel
@@ -177,23 +177,18 @@ __global__ void __launch_bounds__(kSpanThreads, 3) tile_kernel(const SpanArgs a)
   const RowOf o = row_of(a, true, 0, kv, R0 + min(r, rows - 1));
   const int64_t row = (int64_t)o.b * a.Hq + o.h;
 
-  State<1, VB> st;
-  st.m[0] = 0.f;
-  st.top[0] = -INFINITY;
-  st.seen[0] = false;
-  st.l[0] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < VB; ++j) st.acc[0][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  State<VB> st;
+  st.clear();
 
   // (every row and piece is clamped into the span: the buffers' bounds do not
   // count the scalar offset)
   SpanLane<1> hd;
   Rsrc vsc;
-  hd.k = make_rsrc((const char*)sp.k + (F::kMx ? 1 : 2) * (kv * sp.k_sh), 0xffffffffu);
-  hd.v = make_rsrc((const char*)sp.v + (F::kMx ? 1 : 2) * (kv * sp.v_sh), 0xffffffffu);
+  hd.k = make_rsrc((const char*)sp.k + (F::kMx ? 1 : 2) * (kv * sp.k_sh));
+  hd.v = make_rsrc((const char*)sp.v + (F::kMx ? 1 : 2) * (kv * sp.v_sh));
   if constexpr (F::kMx) {
-    hd.ksc = make_rsrc(sp.ksc + kv * sp.ksc_sh, 0xffffffffu);
-    vsc = make_rsrc(sp.vsc + kv * sp.vsc_sh, 0xffffffffu);
+    hd.ksc = make_rsrc(sp.ksc + kv * sp.ksc_sh);
+    vsc = make_rsrc(sp.vsc + kv * sp.vsc_sh);
   }
   const bool f16 = F::kMx ? a.q_dtype == F16::kRk : TT::kRk == F16::kRk;
 
@@ -256,15 +251,16 @@ __global__ void __launch_bounds__(kSpanThreads, 3) tile_kernel(const SpanArgs a)
   }
 
   // the record, straight from the registers
-  float top = fmaxf(st.top[0], shfl_xor(st.top[0], 16));
+  float top = fmaxf(st.top, shfl_xor(st.top, 16));
   top = fmaxf(top, shfl_xor(top, 32));
-  const float M = st.seen[0] ? top + st.m[0] - kLift<TT> : kNegInit;
-  const float f = st.seen[0] ? fast_exp2(st.m[0] - M - kLift<TT>) : 0.f;
+  const bool seen = st.high > -INFINITY;
+  const float M = seen ? top + st.m - kLift<TT> : kNegInit;
+  const float f = seen ? fast_exp2(st.m - M - kLift<TT>) : 0.f;
   if (r >= rows) return;
   const int64_t at = row * a.np + sp.np0 + x;
 #pragma unroll
-  for (int j = 0; j < VB; ++j) *(f32x4*)(a.acc + at * DV + 16 * j + 4 * g) = st.acc[0][j] * f;
-  if (g == 0) *(float2*)(a.ml + 2 * at) = make_float2(M, st.l[0][0] * f);
+  for (int j = 0; j < VB; ++j) *(f32x4*)(a.acc + at * DV + 16 * j + 4 * g) = st.acc[j] * f;
+  if (g == 0) *(float2*)(a.ml + 2 * at) = make_float2(M, st.l[0] * f);
 }
 
 // Widths as in pick_widths.
