@@ -283,17 +283,16 @@ constexpr float kSlack = TT::kRk == 0 ? 5.f : 8.f;
 
 // The running state of one wave's 16 query rows, a row a lane (n).  m: the
 // maximum that the sums are relative to (0 until the row's first score above
-// -infinity); high: the score, relative to m and lifted, that raises it; top:
-// the lane's largest score so far, likewise.  l: the sum of the probabilities,
-// formed with the others as the product of P with ones: every register of it is
-// the sum.
+// -infinity); top: the lane's largest score so far, relative to m and lifted.
+// l: the sum of the probabilities, formed with the others as the product of P
+// with ones: every register of it is the sum.
 template <int VB>
 struct State {
-  float m, high, top;
+  float m, top;
   f32x4 l, acc[VB];
   __device__ __forceinline__ void clear() {
     m = 0.f;
-    high = top = -INFINITY;
+    top = -INFINITY;
     l = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < VB; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -304,6 +303,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
+}
+// The largest of a row's four lanes.
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, shfl_xor(x, 16));
+  return fmaxf(x, shfl_xor(x, 32));
 }
 template <class TT>
 __device__ __forceinline__ uint4 ones() {
@@ -335,17 +339,16 @@ __device__ __forceinline__ void weigh_block(const f32x4 (&s)[2], float scale, fl
   mx = max3(mx, sc[3], sc[4]);
   mx = max3(mx, sc[5], sc[6]);
   mx = max3(mx, sc[7], sc[7]);
+  // (a lane whose first score this is asks as well)
+  const bool raise = mx > (st.top > -INFINITY ? kSlack<TT> + kLift<TT> : -INFINITY);
+  const float was = st.top;
   st.top = max3(st.top, mx, mx);
-  if (__any(mx > st.high)) {
-    mx = fmaxf(mx, shfl_xor(mx, 16));
-    mx = fmaxf(mx, shfl_xor(mx, 32));
-    // how far the maximum rises; the first tokens set it
+  if (__any(raise)) {
+    mx = row_max(mx);
+    // how far the maximum rises; the row's first scores set it
     float up = mx - kLift<TT>;
-    if (st.high > -INFINITY) up = fmaxf(up, 0.f);
-    if (up > -INFINITY)
-      st.high = kSlack<TT> + kLift<TT>;
-    else
-      up = 0.f;
+    if (row_max(was) > -INFINITY) up = fmaxf(up, 0.f);
+    if (!(up > -INFINITY)) up = 0.f;
     const float alpha = fast_exp2(-up);
 #pragma unroll
     for (int j = 0; j < VB; ++j) st.acc[j] *= alpha;
@@ -836,9 +839,8 @@ __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span
   }
 
   // The row's true maximum; a row without tokens has the least one.
-  float top = fmaxf(st.top, shfl_xor(st.top, 16));
-  top = fmaxf(top, shfl_xor(top, 32));
-  const bool seen = st.high > -INFINITY;
+  float top = row_max(st.top);
+  const bool seen = top > -INFINITY;
   top = seen ? top + st.m - kLift<TT> : kNegInit;
   const float m = seen ? st.m : kNegInit;
   // join the four waves: the common maximum, every wave's sums under it through

@@ -251,9 +251,8 @@ __global__ void __launch_bounds__(kSpanThreads, 3) tile_kernel(const SpanArgs a)
   }
 
   // the record, straight from the registers
-  float top = fmaxf(st.top, shfl_xor(st.top, 16));
-  top = fmaxf(top, shfl_xor(top, 32));
-  const bool seen = st.high > -INFINITY;
+  const float top = row_max(st.top);
+  const bool seen = top > -INFINITY;
   const float M = seen ? top + st.m - kLift<TT> : kNegInit;
   const float f = seen ? fast_exp2(st.m - M - kLift<TT>) : 0.f;
   if (r >= rows) return;
