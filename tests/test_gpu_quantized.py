@@ -156,3 +156,50 @@ def test_lengths_below_zero_and_past_the_capacity():
     assert (k.codes[0, 0, :2] != 0).all() and (k.codes[0, 0, 2:] == 0).all()
     assert (k.codes[1] == 0).all()
     assert (k.codes[2, 0, 9] != 0).all() and (k.codes[2, 0, :9] == 0).all()
+
+
+@pytest.mark.parametrize("fmt", ["mx8", "mx4"])
+def test_requests_far_apart(fmt):
+    """Offsets between requests past 32 bits: write, append, read, attend."""
+    from rotatek_amd.kernels import full_channel_decode_quantized
+    from rotatek_amd.quantized import MXRows, append_rows, dequantize_rows, quantize_rows
+    _say(f"far apart {fmt}")
+    B, S, D, far = 3, 40, 128, 2200 * 2 ** 20
+    near = MXRows.empty(B, 1, S, D, fmt)
+    buf = torch.zeros(2 * far + 2 ** 14, dtype=torch.uint8, device="cuda")
+    codes = buf.as_strided(near.codes.shape, (far, 0, near.codes.shape[3], 1))
+    scales = buf.as_strided(near.scales.shape, (far, 0, 64, 1), 2 ** 13)
+    rows = MXRows(codes, scales, D, fmt)
+    x = _x(41, B, 1, S, D, dtype=torch.bfloat16).cuda()
+    quantize_rows(x, fmt, out=near)
+    assert quantize_rows(x, fmt, out=rows) is rows
+    new = _x(42, B, 1, 3, D, dtype=torch.bfloat16).cuda()
+    lens = torch.tensor([5, 0, 39], dtype=torch.int32, device="cuda")
+    for r in (near, rows):
+        append_rows(new, new, r, MXRows.empty(B, 1, S, D, fmt), lens, advance=False)
+    assert torch.equal(rows.codes, near.codes) and torch.equal(rows.scales[..., :S], near.scales[..., :S])
+    assert torch.equal(dequantize_rows(rows), dequantize_rows(near))
+    q = torch.randn(B, 4, D, device="cuda").half()
+    assert torch.equal(full_channel_decode_quantized(q, rows, rows, 4), full_channel_decode_quantized(q, near, near, 4))
+
+
+def test_one_address_for_two_rows_is_refused():
+    from rotatek_amd.kernels import full_channel_decode_quantized
+    from rotatek_amd.quantized import MXRows, append_rows, dequantize_rows, quantize_rows
+    _say("overlap")
+    x = torch.randn(2, 1, 8, 32, device="cuda")
+    one = MXRows.empty(1, 1, 8, 32)
+    both = MXRows(one.codes.expand(2, 1, 8, 32), one.scales.expand(2, 1, 1, 32), 32)
+    with pytest.raises(ValueError):
+        quantize_rows(x, out=both)
+    with pytest.raises(ValueError):
+        append_rows(x, x, both, both, torch.zeros(2, dtype=torch.int32, device="cuda"))
+    quantize_rows(x[:1], out=one)
+    with pytest.raises(ValueError):
+        dequantize_rows(both, out=torch.empty(1, 1, 8, 32, device="cuda").expand(2, 1, 8, 32))
+    assert torch.equal(dequantize_rows(both)[0], dequantize_rows(one)[0])      # read, they may repeat
+    q = torch.randn(2, 1, 32, device="cuda")
+    with pytest.raises(ValueError):
+        full_channel_decode_quantized(q, both, both, 1, out=torch.empty(1, 1, 32, device="cuda").expand(2, 1, 32))
+    a, b = full_channel_decode_quantized(q, both, both, 1), full_channel_decode_quantized(q[1:], one, one, 1)
+    assert torch.equal(a[1:], b)

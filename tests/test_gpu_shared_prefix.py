@@ -162,3 +162,143 @@ def test_same_as_the_expanded_batch():
                                     x(kw["v_sparse"]), c["groups"])
     # two roundings to fp16 of values within 4 of zero
     assert (got.float() - want.float()).abs().max() <= 2 * 2.0 ** -11 * want.float().abs().max() + 1e-4
+
+
+# As many queries on the same rows as make the waves take queries (past 2048
+# bytes of a token times blocks of 16 queries), in every format.
+MANY = [
+    (61, 8, 2, 128, 100, 0, 0, 20, [20, 0, 3]),        # 244 rows: 4 blocks of 64, the last of 52
+    (101, 4, 1, 128, 33, 32, 517, 9, [9, 0, 1, 4]),
+    (101, 4, 1, 128, 1, 64, 70, 5, None),
+    (65, 4, 1, 128, 0, 128, 130, None, None),          # no prompt, no text, all channels kept
+    (150, 4, 1, 64, 150, 16, 70, 31, [31, 0]),
+    (130, 4, 1, 96, 257, 40, 64, 0, None),             # a suffix of no rows
+    (160, 2, 1, 80, 1, 8, 1, 1, None),                 # single tokens
+]
+
+
+@pytest.mark.parametrize("fmt,dtype", [("plain", torch.bfloat16), ("plain", torch.float16), ("mx8", torch.bfloat16),
+                                       ("mx8", torch.float16), ("mx4", torch.bfloat16), ("mx4", torch.float32)])
+@pytest.mark.parametrize("case", MANY)
+def test_many_requests(case, fmt, dtype):
+    _say(f"{case} {fmt} {dtype}")
+    _check(_case(*case[:8], dtype, fmt, seed=sum(case[:7]), lens=case[8]))
+
+
+@pytest.mark.parametrize("rows", [63, 64, 65, 79, 81, 127, 128, 129])
+def test_either_side_of_a_block_of_queries(rows):
+    _say(f"{rows} rows")
+    _check(_case(rows, 1, 1, 128, 130, 0, 0, 3, torch.bfloat16, "plain", seed=rows, lens=[3, 0]))
+    _check(_case(rows, 1, 1, 128, 66, 32, 130, 3, torch.float16, "plain", seed=rows, lens=[2, 1]))
+
+
+@pytest.mark.parametrize("B,S_s,lens", [(40, 4200, [4200, 0, 4097, 31]), (40, 4096, [4096, 1]), (3, 4200, [4200, 129])])
+def test_long_texts(B, S_s, lens):
+    _say(f"long texts {B} {S_s}")
+    _check(_case(B, 2, 1, 128, 200, 0, 0, S_s, torch.bfloat16, "plain", seed=S_s, lens=lens))
+
+
+@pytest.mark.parametrize("B", [3, 70])
+@pytest.mark.parametrize("fmt,dtype", [("plain", torch.bfloat16), ("mx8", torch.float16)])
+def test_other_layouts_of_the_queries_and_the_rotation(B, fmt, dtype):
+    """Queries and rotations that are not in whole aligned pieces of one type."""
+    from rotatek_amd.kernels import shared_prefix_decode
+    _say(f"layouts {B} {fmt}")
+    c = _case(B, 4, 1, 128, 40, 32, 150, 7, dtype, fmt, seed=21, lens=[7, 0])
+    kw = dict(c["kw"])
+    wide = torch.zeros(B, 4, 260, dtype=dtype, device="cuda")
+    wide[..., 1::2] = torch.cat([c["q"].cuda(), torch.zeros(B, 4, 2, dtype=dtype, device="cuda")], -1)
+    q = wide[..., 1:257:2]
+    assert torch.equal(q, c["q"].cuda())
+    call = lambda q, **k: shared_prefix_decode(q, c["k"], c["v"], c["k2"], c["v2"], 4, **{**kw, **k})  # noqa: E731
+    sp.check(call(q), c["q"], 4, c["spans"], fmt, dtype)
+    sp.check(call(c["q"].cuda(), R_partial=kw["R_partial"].float()), c["q"], 4, c["spans"], fmt, dtype)
+    sp.check(call(c["q"].cuda(), R_partial=kw["R_partial"].transpose(2, 3).contiguous().transpose(2, 3)), c["q"], 4,
+             c["spans"], fmt, dtype)
+    sp.check(call(c["q"].cuda(), delta_mu=kw["delta_mu"].float()), c["q"], 4, c["spans"], fmt, dtype)
+    out = torch.full((B, 8, 128), 7.0, dtype=dtype, device="cuda")
+    sp.check(call(q, out=out[:, ::2]), c["q"], 4, c["spans"], fmt, dtype)
+    assert (out[:, 1::2] == 7).all()
+
+
+@pytest.mark.parametrize("B", [3, 70])
+@pytest.mark.parametrize("fmt", ["plain", "mx8"])
+def test_rotation_that_keeps_no_channel(B, fmt):
+    """Scores of the image are q . delta_mu alone."""
+    _say(f"no channel kept {B} {fmt}")
+    dtype = torch.bfloat16
+    c = _case(B, 4, 1, 128, 40, 0, 150, 7, dtype, fmt, seed=22, lens=[7, 0])
+    _check(c)
+
+
+@pytest.mark.parametrize("B", [4, 70])
+def test_scores_of_minus_infinity(B):
+    """Products past the range of fp32: weight zero, also where a row's first
+    tokens are all such and its neighbours' are not."""
+    from rotatek_amd.kernels import shared_prefix_decode
+    _say(f"scores past the range {B}")
+    c = _case(B, 2, 1, 128, 300, 0, 0, 33, torch.bfloat16, "plain", seed=23)
+    q, k = c["q"].clone(), c["k"].clone()
+    # channel 0 is the odd heads' alone: 2^126 there, Keys of -2^10 in 0 .. 259,
+    # of 0 behind and in the text
+    q[:, 0, 0], q[:, 1, 0] = 0, 2.0 ** 126
+    k[..., 0] = 0
+    k[:, :, :260, 0] = -2.0 ** 10
+    c["k2"][..., 0] = 0
+    got = shared_prefix_decode(q.cuda(), k, c["v"], c["k2"], c["v2"], 2)
+    even, odd = [dict(s) for s in c["spans"]], [dict(s) for s in c["spans"]]
+    even[0]["k"] = odd[0]["k"] = sp.np64(k)
+    even[1]["k"] = odd[1]["k"] = sp.np64(c["k2"])
+    odd[0]["valid"] = np.broadcast_to(np.arange(300) >= 260, (B, 300))
+    for h, spans in ((0, even), (1, odd)):
+        qh = q[:, h:h + 1].clone()
+        qh[..., 0] = 0
+        sp.check(got[:, :, h:h + 1], qh, 1, spans, "plain", torch.bfloat16)
+    # nothing else to attend: zeros
+    alone = shared_prefix_decode(q.cuda(), k[:, :, :260], c["v"][:, :, :260], None, None, 2)
+    assert (alone[:, 0, 1] == 0).all() and torch.isfinite(alone).all()
+
+
+def test_heads_far_apart():
+    """Offsets between heads and requests past 32 bits."""
+    from rotatek_amd.kernels import shared_prefix_decode
+    _say("far apart")
+    c = _case(3, 4, 2, 128, 70, 0, 0, 20, torch.bfloat16, "plain", seed=24, lens=[20, 0, 5])
+    want = _run(c)
+    far = 1100 * 2 ** 20        # elements: 2.2 GB
+    buf = torch.zeros(2 * far + 2 ** 16, dtype=torch.bfloat16, device="cuda")
+    at = 0
+
+    def apart(t, sb, sh):
+        nonlocal at
+        w = buf.as_strided(t.shape, (sb, sh, 128, 1), at)
+        w.copy_(t)
+        at += t.shape[2] * 128
+        return w
+
+    k, v = apart(c["k"], 0, far), apart(c["v"], 0, far)
+    k2, v2 = (apart(t, far, 40 * 128) for t in (c["k2"], c["v2"]))
+    got = shared_prefix_decode(c["q"].cuda(), k, v, k2, v2, 2, **c["kw"])
+    assert torch.equal(got, want)
+
+
+def test_captured_with_tiles():
+    """Replays as the text grows, with eager work between."""
+    from rotatek_amd.kernels import shared_prefix_decode
+    _say("captured")
+    c = _case(70, 4, 1, 128, 90, 32, 300, 40, torch.bfloat16, "plain", seed=25, lens=[1])
+    q, kw = c["q"].cuda(), c["kw"]
+    call = lambda: shared_prefix_decode(q, c["k"], c["v"], c["k2"], c["v2"], 4, **kw)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for step in range(5):
+        kw["len_suffix"].fill_(1 + 9 * step)
+        q.mul_(-0.9)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        torch.randn(500, 500, device="cuda").sum()
