@@ -74,26 +74,29 @@ __global__ void __launch_bounds__(128) span_queries_kernel(const rk::QueryArgs a
 }
 
 // Joins a row's records: out = sum_p acc_p 2^(m_p - M) / (sum_p l_p 2^(m_p -
-// M) + 1e-6).  A wave per row: four groups of 16 lanes (DV / 16 channels a
-// lane) fold every fourth record, four records' loads in flight, and are
-// combined by lane exchange.
-template <int DV>
+// M) + 1e-6).  W waves to a row: each has four groups of 16 lanes (DV / 16
+// channels a lane), and a group folds every 4 W-th record, four records' loads
+// in flight; groups are combined by lane exchange, waves through LDS.
+// Bound by the latency of its rounds, 16 W records each: a call with 28 rows of
+// 190 records takes 15.5 us with four waves to a row, 23.7 with one.
+template <int DV, int W>
 __global__ void __launch_bounds__(256) span_merge_kernel(const SpanArgs a) {
-  constexpr int C = DV / 16, NB = 4;
-  const int lane = threadIdx.x & 63, s = lane >> 4, n = lane & 15;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.B * a.Hq) return;
+  constexpr int C = DV / 16, NB = 4, kStep = 4 * W;
+  __shared__ float s_part[W][16][C + 2];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, s = lane >> 4, n = lane & 15;
+  const int64_t row = (int64_t)blockIdx.x * (4 / W) + wave / W;
+  if (row >= (int64_t)a.B * a.Hq) return;  // (W 4: the whole workgroup)
   const float* acc = a.acc + row * a.np * DV + n * C;
   const float2* ml = (const float2*)a.ml + row * a.np;
   float M = rk::kNegInit, L = 0.f, A[C];
 #pragma unroll
   for (int e = 0; e < C; ++e) A[e] = 0.f;
-  for (int p = s; p < a.np; p += 4 * NB) {
+  for (int p = s + 4 * (wave % W); p < a.np; p += kStep * NB) {
     float2 r[NB];
     float4 v[NB][C / 4];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int q = p + 4 * i < a.np ? p + 4 * i : p;  // past the last: a record again, with weight 0
+      const int q = p + kStep * i < a.np ? p + kStep * i : p;  // past the last: a record again, with weight 0
       r[i] = ml[q];
 #pragma unroll
       for (int e = 0; e < C / 4; ++e) v[i][e] = *(const float4*)(acc + (int64_t)q * DV + 4 * e);
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(256) span_merge_kernel(const SpanArgs a) {
     for (int e = 0; e < C; ++e) A[e] *= f;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      if (p + 4 * i >= a.np) break;
+      if (p + kStep * i >= a.np) break;
       const float w = rk::fast_exp2(r[i].x - M);
       L += r[i].y * w;
 #pragma unroll
@@ -126,6 +129,25 @@ __global__ void __launch_bounds__(256) span_merge_kernel(const SpanArgs a) {
 #pragma unroll
     for (int e = 0; e < C; ++e) A[e] = A[e] * f + rk::shfl_xor(A[e], d) * fo;
     M = top;
+  }
+  if constexpr (W > 1) {
+    if (s == 0) {
+      s_part[wave][n][C] = M;
+      s_part[wave][n][C + 1] = L;
+#pragma unroll
+      for (int e = 0; e < C; ++e) s_part[wave][n][e] = A[e];
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const float* o = s_part[w][n];
+      const float top = fmaxf(M, o[C]), f = rk::fast_exp2(M - top), fo = rk::fast_exp2(o[C] - top);
+      L = L * f + o[C + 1] * fo;
+#pragma unroll
+      for (int e = 0; e < C; ++e) A[e] = A[e] * f + o[e] * fo;
+      M = top;
+    }
   }
   if (s != 0) return;
   const int64_t b = row / a.Hq, h = row - b * a.Hq;
@@ -164,6 +186,9 @@ constexpr int64_t kTileBytes = 2048;
 // too few to fill the chip, 43.8 and 42.3.  (Without tiles the suffix is split
 // with the other spans: 2 requests of 4 heads 11.3 us, joined 12.9.)
 constexpr int64_t kJoinTokens = 4096;
+// Records that one wave joins; four take more.  (A call of 32 rows of 19 records:
+// 14.7 us with one wave to a row, 13.7 with four; 1024 rows of 5: equal.)
+constexpr int64_t kMergeWave = 8;
 // Bytes a workgroup streams at most.
 constexpr int64_t kMaxShare = INT64_C(512) << 10;
 
@@ -328,7 +353,9 @@ int make_plan(const Call& c, int cus, Plan* out) {
       if (least || used <= slots * rounds) break;
     }
   };
-  // Three workgroups are resident on a CU.  Over 64 queries a workgroup's
+  // Three workgroups a CU (16 requests of 7 heads on a KV head over 32768 4-bit
+  // rows: 46.2 us, 48.3 with four, 49.9 with two; 32 requests of one head to 16000
+  // 8-bit rows: 436, 431, 436).  Over 64 queries a workgroup's
   // records weigh as much as 64 tokens' rows and the join reads them again: two
   // there where three would leave it less than 768 tokens (32 requests of 4 heads
   // behind 16001: 35 us at two, 512 tokens, 38 at three; 64 of 7 heads behind
@@ -557,11 +584,16 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
       e = rk::span_join_bf16(p.kf, a, grid, s);
     return e == hipSuccess ? RK_OK : RK_ERR_HIP;
   }
-  const dim3 mg((unsigned)cdiv(p.rows, 4));
-  if (p.kf == 2)
-    hipLaunchKernelGGL(span_merge_kernel<64>, mg, dim3(256), 0, s, a);
+  const int w = p.np > kMergeWave ? 4 : 1;
+  const dim3 mg((unsigned)cdiv(p.rows, 4 / w));
+  if (p.kf == 2 && w == 1)
+    hipLaunchKernelGGL((span_merge_kernel<64, 1>), mg, dim3(256), 0, s, a);
+  else if (p.kf == 2)
+    hipLaunchKernelGGL((span_merge_kernel<64, 4>), mg, dim3(256), 0, s, a);
+  else if (w == 1)
+    hipLaunchKernelGGL((span_merge_kernel<128, 1>), mg, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL(span_merge_kernel<128>, mg, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((span_merge_kernel<128, 4>), mg, dim3(256), 0, s, a);
   return hipGetLastError() == hipSuccess ? RK_OK : RK_ERR_HIP;
 }
 
