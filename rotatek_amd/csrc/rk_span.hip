@@ -359,7 +359,7 @@ int make_plan(const Call& c, int cus, Plan* out) {
   // records weigh as much as 64 tokens' rows and the join reads them again: two
   // there where three would leave it less than 768 tokens (32 requests of 4 heads
   // behind 16001: 35 us at two, 512 tokens, 38 at three; 64 of 7 heads behind
-  // 32768: 90 at two, 77 at three).
+  // 32768: 81 at two, 73 at three).
   split((int64_t)cus * 3);
   if (p.tile && std::max(p.chunk[kRotated], p.chunk[kFull]) < 768) split((int64_t)cus * 2);
   if (p.join) {

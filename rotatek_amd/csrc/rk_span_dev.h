@@ -30,9 +30,16 @@
 //
 // Loads run ahead of the products: the K registers are reloaded with the
 // wave's next block as soon as the scores are formed, the V registers as soon
-// as V^T is.  All offsets of a lane are fixed; a block moves
-// the wave-uniform base alone.  The last block of a span starts 32 rows before
-// its end, its rows of the block before it left out.
+// as V^T is.  (Two blocks ahead: 47.9 us where one takes 45.4, 4-bit rows; 452
+// and 435, 8-bit ones.)  All offsets of a lane are fixed; a block moves the
+// wave-uniform base alone.  The last block of a span starts 32 rows before its
+// end, its rows of the block before it left out.
+//
+// What bounds it.  8-bit rows of one head each, 2.9 GB: 435 us, 6.7 TB/s, HBM.
+// 4-bit rows of seven heads, 186 MB: 42 us, 4.4 TB/s; per 32 rows a wave issues
+// about 90 vector and 22 matrix instructions, which 12 waves on a CU fit into
+// 60 % of the time; the rest waits for rows.  One request over 13 MB: 10 us, of
+// them 4 to launch, rotate the queries and fetch the first rows.
 #pragma once
 
 #include <math.h>
@@ -116,8 +123,9 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* p) {
                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32;
   return __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, -1, 0x00027000);  // 2^32 - 1 bytes
 }
-// AUX 2: non-temporal, for rows that one instruction reads whole lines of and
-// that no other unit reads.
+// AUX 2: non-temporal, for rows that one instruction reads whole lines of (447
+// against 451 us over 2.9 GB of 8-bit rows; the half lines of 4-bit rows came from
+// memory twice, so those go through the caches).
 template <int N, int AUX = 0>
 __device__ __forceinline__ void load_words(Rsrc r, uint32_t off, uint32_t base, uint32_t* w) {
   if constexpr (N == 4) {
@@ -273,7 +281,8 @@ __device__ __forceinline__ void terms8(const float (&x)[8], uint4 (&o)[NT]) {
 
 // The running maximum is raised (and the sums rescaled) only when a score
 // passes it by kSlack, in log2 units: a probability is then at most 2^kSlack,
-// and most blocks need no exchange between lanes.  fp16 probabilities are
+// and most blocks need no exchange between lanes.  The sums are fp32, which
+// scales by powers of two without loss: the slack costs no accuracy.  fp16 probabilities are
 // formed as 2^kLift p (at most 2^15): those below 2^-24, not 2^-14, fall into
 // fp16's subnormals.  A workgroup's record is free of both.
 template <class TT>
@@ -389,8 +398,8 @@ __device__ __forceinline__ void weigh_block(const f32x4 (&s)[2], float scale, fl
 // unit's queries in LDS, sq [term][row][stride] 16-bit in the lane's channel
 // order, while the first blocks are on their way.
 template <class F, int KB, int VB, int NT, int NP, bool VEC, class Pre>
-__device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, SpanLane<KB>& hd, int b, int chunk, int wave,
-                                         int lane, const uint16_t* sq, int qstride, const float* sbias,
+__device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, SpanLane<KB>& hd, int b, int chunk,
+                                         int wave, int lane, const uint16_t* sq, int qstride, const float* sbias,
                                          State<VB>& st, const Pre& pre) {
   using TT = typename F::TT;
   const int g = lane >> 4, n = lane & 15;
@@ -631,7 +640,8 @@ __device__ __forceinline__ void stage_rotation(int tid, const Rotation<KV>& x, u
 // as read_columns gives them.)
 template <class TT, int NTV, int NR, int KV>
 __device__ __forceinline__ void rotate_queries(const SpanArgs& a, int wave, int lane, bool f16, const uint16_t* raw,
-                                               const uint4* r, const uint4* mu, uint16_t* dst, int stride, float* bias) {
+                                               const uint4* r, const uint4* mu, uint16_t* dst, int stride,
+                                               float* bias) {
   constexpr int kRows = 16 * NR;
   const int g = lane >> 4, n = lane & 15;
   for (int ct = wave; ct <= 2 * KV; ct += kSpanWaves) {
@@ -726,8 +736,10 @@ __device__ __forceinline__ void join_records(const SpanArgs& a, const RowOf& o, 
 // (one workgroup per unit).  It joins the other spans' records to its sums and
 // writes the output.
 //
-// A workgroup of MX rows has room for four on a CU in its 128 registers a lane,
-// of plain ones for three; element loads (VEC false) keep more addresses.
+// Registers: 128 a lane for quantised rows (four workgroups on a CU, of which the
+// plan fills three and the fourth takes a late one), 168 for plain ones, whose
+// blocks are twice as wide, 256 for element loads (VEC false), which keep an
+// address per element.
 template <class F, int KV, int KF, int NT, int NP, bool VEC, bool JOIN = false>
 __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span_kernel(const SpanArgs a) {
   using TT = typename F::TT;

@@ -15,10 +15,16 @@
 // at another place of their row for each row, so that the rows that one read
 // takes the same piece of lie in different banks.
 //
-// One tile buffer and 16 queries a wave leave registers and LDS for three
-// workgroups on a CU, which hide each other's barriers and latencies: 32 queries
-// a wave (two workgroups) and two buffers were slower (64 requests of 7 heads
-// behind 32768 tokens: 77 us, 82 and 90).
+// One tile buffer, one tile ahead and 16 queries a wave leave registers and LDS
+// for three workgroups on a CU, which hide each other's barriers and latencies:
+// 32 queries a wave, two buffers, or two tiles ahead (two workgroups each) took 6,
+// 17 and 16 % longer, both halves of a tile in one softmax (spills) 2 to 14 %.
+//
+// What bounds it: issue.  64 requests of 7 heads behind 32768 tokens, 64 channels
+// kept: 71 us with the join (11), 324 TFLOP/s of the formula; a wave issues 26
+// matrix and 90 other vector instructions for 32 tokens, the matrix pipes are busy
+// for 47 % of the loop, and waves wait for their turn for 42 % of their time.  32
+// requests of 4 heads behind 16001: 34 us with the join (8.6), 2.2 TB/s.
 #pragma once
 
 #include "rk_span_dev.h"
