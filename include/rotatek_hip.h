@@ -532,7 +532,9 @@ typedef struct rk_rows {
   int32_t format;   /* rk_rows_format */
 } rk_rows;
 
-/* rows[b,h,t] = quantised x[b,h,t]; x [B,H,S,D] F16/BF16/F32, any strides. */
+/* rows[b,h,t] = quantised x[b,h,t]; x [B,H,S,D] F16/BF16/F32, any strides.
+ * What a call of this header's rk_mx_* and decode entries writes must not
+ * repeat by a stride of 0 (RK_ERR_STRIDE); what it reads may. */
 int rk_mx_write(const rk_tensor* x, const rk_rows* rows, void* stream);
 
 /* The inverse: out [B,H,S,D] F16/BF16/F32 (any strides), each value code 2^e
@@ -582,9 +584,10 @@ int rk_quantized_decode(const rk_tensor* q, const rk_tensor* R_partial, const rk
  *   k_suffix, v_suffix [B,H_kv,S_s,D]   each request's own rows (both NULL:
  *                                       none), t < len_suffix[b] (device int32
  *                                       [B] or NULL) attended.
- * The shared rows are read once for all the batch's queries (once per 64 on a
- * KV head).  All rows are of one format: plain in q's dtype (F16, BF16; any
- * strides), or quantised (q F16/BF16/F32).  Workspace and capture as above. */
+ * The shared rows are read from memory once for all the batch's queries.  All
+ * rows are of one format: plain in q's dtype (F16, BF16; any strides), or
+ * quantised (q F16/BF16/F32).  R_partial and delta_mu are not looked at without
+ * a rotated span.  Workspace and capture as above. */
 int rk_shared_prefix_decode_check(const rk_tensor* q, const rk_tensor* R_partial, const rk_tensor* delta_mu,
                                   const rk_rows* k_prefix, const rk_rows* v_prefix, const rk_rows* k_sparse,
                                   const rk_rows* v_sparse, const rk_rows* k_suffix, const rk_rows* v_suffix,

@@ -343,8 +343,10 @@ int done(int st) {
   return hipGetLastError() == hipSuccess ? RK_OK : RK_ERR_HIP;
 }
 
+// A launch has less than 2^32 threads (an append twice as many).
 bool grid_ok(const MxArgs& a, int64_t B) {
-  return a.S <= (INT64_C(1) << 31) && B * a.H * a.tiles < (INT64_C(1) << 31);
+  return a.S < (INT64_C(1) << 30) && B < (INT64_C(1) << 23) && B * a.H < (INT64_C(1) << 23) &&
+         B * a.H * a.tiles < (INT64_C(1) << 23);
 }
 
 // Two rows at one address would be written by two workgroups at once.

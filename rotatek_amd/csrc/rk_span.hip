@@ -192,6 +192,9 @@ constexpr int64_t kMergeWave = 8;
 // Bytes a workgroup streams at most.
 constexpr int64_t kMaxShare = INT64_C(512) << 10;
 
+// A launch has less than 2^32 threads.
+constexpr int64_t kMaxGrid = INT64_C(1) << 24;
+
 // One call as the entry points give it; pairs may be null.
 struct Call {
   const rk_tensor *q, *R, *dm, *mask, *out;
@@ -208,9 +211,14 @@ struct Plan {
   bool vec, join;  // join: the suffix rows run in the launch that joins the tiles' records
   bool tile;       // rk_tile_dev.h over the shared spans, 64 queries a workgroup
   bool copy_q, ahead;  // queries copied into whole pieces; rotated ahead of the split launch
-  int64_t S[kSpans], chunk[kSpans], wgs[kSpans], units[kSpans], blocks[kSpans], np, grid, rows;
+  int64_t S[kSpans], chunk[kSpans], wgs[kSpans], units[kSpans], blocks[kSpans], np, rows;
   size_t q, qr, bias, zero, zero_bytes, acc, ml, total;
 };
+
+// Workgroup ids of a span: eight (chunk, head) pairs' row blocks at a time.
+int64_t launched(const Plan& p, int i) {
+  return p.S[i] == 0 ? 0 : 8 * p.blocks[i] * cdiv(p.wgs[i] * (p.units[i] / p.blocks[i]), 8);
+}
 
 bool mx(const rk_rows* r) { return r->format != RK_ROWS_PLAIN; }
 
@@ -306,7 +314,7 @@ int make_plan(const Call& c, int cus, Plan* out) {
   p.kf = p.D <= 64 ? 2 : 4;
   p.kv = p.S[kRotated] == 0 ? 0 : p.Dk <= 32 ? 1 : p.Dk <= 64 ? 2 : 4;
   p.terms = quantised ? (c.q->dtype == RK_F32 ? 3 : 2) : 1;
-  if (p.B >= (INT64_C(1) << 31) / p.Hq) return RK_ERR_SHAPE;
+  if (p.B >= kMaxGrid / p.Hq) return RK_ERR_SHAPE;
   p.rows = p.B * p.Hq;
   int64_t cost[kSpans], shared_bytes = 0, shared_tokens = 0;  // cost: bytes of a token
   for (int i = 0; i < kSpans; ++i) {
@@ -336,7 +344,7 @@ int make_plan(const Call& c, int cus, Plan* out) {
     const int64_t rounds = std::max<int64_t>(cdiv(total, slots * kMaxShare), 1);
     const int64_t align = rk::kSpanWaves * rk::kSpanBlk;
     for (int64_t share = std::max<int64_t>(cdiv(total, slots * rounds), 1);; share += cdiv(share, 32)) {
-      p.np = p.grid = 0;
+      p.np = 0;
       int64_t used = 0;
       bool least = true;  // one workgroup per unit and span
       for (int i = 0; i < kSpans; ++i) {
@@ -345,7 +353,6 @@ int make_plan(const Call& c, int cus, Plan* out) {
         p.chunk[i] = std::min(round_up(cdiv(share, cost[i]), align), round_up(p.S[i], align));
         p.wgs[i] = cdiv(p.S[i], p.chunk[i]);
         p.np += p.wgs[i];
-        p.grid += p.wgs[i] * p.units[i];
         if (p.tile && i == kTail) continue;  // a launch of its own
         least = least && p.wgs[i] == 1;
         used += p.wgs[i] > 1 || p.tile ? p.wgs[i] * p.units[i] : cdiv(p.units[i] * p.S[i] * cost[i], share);
@@ -366,9 +373,9 @@ int make_plan(const Call& c, int cus, Plan* out) {
     p.chunk[kTail] = round_up(p.S[kTail], rk::kSpanWaves * rk::kSpanBlk);
     p.wgs[kTail] = 1;
   }
-  // (24: the ids that launched() adds)
-  if (p.grid + 24 * (p.units[0] + p.units[1] + p.units[2]) >= (INT64_C(1) << 31) || p.rows * p.np >= (INT64_C(1) << 40))
-    return RK_ERR_SHAPE;
+  int64_t ids = 0;
+  for (int i = 0; i < kSpans; ++i) ids += launched(p, i);
+  if (ids >= kMaxGrid || p.rows * p.np >= (INT64_C(1) << 40)) return RK_ERR_SHAPE;
   const int64_t dv = p.kf == 2 ? 64 : 128;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -445,11 +452,6 @@ Span make_span(const Call& c, const Plan& p, int i, char* ws) {
   s.chunk = (int32_t)p.chunk[i];
   s.wgs = (int32_t)p.wgs[i];
   return s;
-}
-
-// Workgroup ids of a span: eight (chunk, head) pairs' row blocks at a time.
-int64_t launched(const Plan& p, int i) {
-  return p.S[i] == 0 ? 0 : 8 * p.blocks[i] * cdiv(p.wgs[i] * (p.units[i] / p.blocks[i]), 8);
 }
 
 int resolve_cus(int num_cus, int* st) {

@@ -2,8 +2,8 @@
 
 Many questions about one image (or behind one system prompt) attend over the
 same Keys and Values.  ``rotatek_decode`` on an expanded batch reads them once
-per request; here all the batch's queries on a KV head form one unit of work,
-so the shared rows are read once for every 64 of them, and a request's own
+per request; here all the batch's queries on a KV head work on the same rows at
+the same time, so the shared rows come from memory once, and a request's own
 text is joined to the result in the same step.  No counterpart in the
 reference.
 """
@@ -41,8 +41,10 @@ def shared_prefix_decode(q: torch.Tensor, k_prefix: Rows, v_prefix: Rows, k_suff
     check_query(q)
     if (k_sparse is None) != (v_sparse is None) or (k_sparse is None) != (R_partial is None):
         raise ValueError("k_sparse, v_sparse and R_partial go together")
-    if (k_suffix is None) != (v_suffix is None):
-        raise ValueError("k_suffix and v_suffix go together")
+    if delta_mu is not None and R_partial is None:
+        raise ValueError("delta_mu goes with R_partial")
+    if (k_suffix is None) != (v_suffix is None) or (k_suffix is None and len_suffix is not None):
+        raise ValueError("k_suffix and v_suffix go together, len_suffix with them")
     return launch("shared_prefix_decode", q, (R_partial, delta_mu),
                   (k_prefix, v_prefix, k_sparse, v_sparse, k_suffix, v_suffix), None, len_suffix, num_kv_groups, out,
                   True)

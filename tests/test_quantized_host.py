@@ -235,3 +235,74 @@ def test_python_refusals():
         shared_prefix_decode(q, x, x, None, None, 1, k_sparse=x)
     with pytest.raises(RuntimeError):
         shared_prefix_decode(q, x, x, None, None, 1)
+    with pytest.raises(ValueError):
+        shared_prefix_decode(q, x, x, None, None, 1, delta_mu=torch.zeros(1, 2, 128))
+    with pytest.raises(ValueError):
+        shared_prefix_decode(q, x, x, None, None, 1, len_suffix=torch.zeros(1, dtype=torch.int32))
+
+
+def test_outputs_that_repeat_are_refused():
+    x = _aligned((2, 2, 64, 128), torch.bfloat16)
+    q, r = torch.zeros(2, 4, 128, dtype=torch.bfloat16), _rows()
+    assert _decode(q, out=q)[0] == 0
+    assert _decode(q, out=q[:1].expand(2, 4, 128))[0] == _lib.RK_ERR_STRIDE
+    assert _decode(q, out=q[:, :1].expand(2, 4, 128))[0] == _lib.RK_ERR_STRIDE
+    once = MXRows(r.codes[:1].expand(2, 2, 64, 128), r.scales[:1].expand(2, 2, 4, 64), 128)
+    assert _decode(q, kf=once, vf=once)[0] == 0         # read, rows may repeat
+    dx, dr = _lib.desc(x), once.desc()
+    lens = torch.zeros(2, dtype=torch.int32)
+    lib = _lib.load()
+    assert lib.rk_mx_write(ref(dx), ref(dr), None) == _lib.RK_ERR_STRIDE
+    assert lib.rk_mx_append(ref(dx), None, ref(dr), None, lens.data_ptr(), 1, None) == _lib.RK_ERR_STRIDE
+    dx, dr = _lib.desc(x[:1].expand(2, 2, 64, 128)), r.desc()
+    assert lib.rk_mx_read(ref(dr), ref(dx), None) == _lib.RK_ERR_STRIDE
+
+
+def test_sizes_past_a_launch_are_refused():
+    bf = torch.bfloat16
+    lib, n = _lib.load(), ctypes.c_size_t(0)
+    # rows that repeat by stride 0 can be any number
+    p = torch.zeros(1, 1, 1, 128, dtype=bf).expand(1, 2, 1 << 31, 128)
+    q = torch.zeros(3, 4, 128, dtype=bf)
+    assert _shared(q, p, p)[0] == _lib.RK_ERR_SHAPE
+    assert _shared(q, p[:, :, :1 << 20], p[:, :, :1 << 20])[0] == 0
+    p = torch.zeros(1, 2, 8, 128, dtype=bf)
+    many = torch.zeros(1, 4, 128, dtype=bf).expand(1 << 24, 4, 128)
+    assert _shared(many, p, p)[0] == _lib.RK_ERR_SHAPE
+    st, size = _shared(many[:1 << 20], p, p)
+    assert st == 0 and size < 1 << 34
+    r = _rows(B=1)
+    wide = MXRows(r.codes.expand(1 << 24, 2, 64, 128), r.scales.expand(1 << 24, 2, 4, 64), 128)
+    assert _decode(many, kf=wide, vf=wide)[0] == _lib.RK_ERR_SHAPE
+    x = torch.zeros(1, 1, 1, 128).expand(1 << 23, 2, 64, 128)
+    part = MXRows(wide.codes[:1 << 23], wide.scales[:1 << 23], 128)
+    dx, dr = _lib.desc(x), part.desc()
+    assert lib.rk_mx_write(ref(dx), ref(dr), None) == _lib.RK_ERR_SHAPE
+    assert lib.rk_mx_read(ref(dr), ref(dx), None) == _lib.RK_ERR_SHAPE
+
+
+@pytest.mark.parametrize("cus", [1, 64, 256, 304])
+def test_every_plan_is_bounded(cus):
+    """Workspace over sizes, batch and formats: never more than a record for 512
+    KB of rows, 32 per CU and one a unit and span."""
+    for dtype, fmt in ((torch.bfloat16, "plain"), (torch.float16, "mx8"), (torch.float32, "mx4")):
+        for B in (1, 3, 64, 1000):
+            for S in (0, 1, 31, 33, 4096, 100000):
+                for S_s in (None, 1, 300, 9000):
+                    q = torch.zeros(1, 8, 128, dtype=dtype).expand(B, 8, 128)
+                    if fmt == "plain":
+                        p = torch.zeros(1, 1, 1, 128, dtype=dtype).expand(1, 2, S, 128)
+                        t = None if S_s is None else p.new_zeros(1, 1, 1, 128).expand(B, 2, S_s, 128)
+                    else:
+                        p = _rows(B=1, S=S, fmt=fmt)
+                        t = None
+                        if S_s is not None:
+                            t = _rows(B=1, S=S_s, fmt=fmt)
+                            t = MXRows(t.codes.expand(B, *t.codes.shape[1:]), t.scales.expand(B, *t.scales.shape[1:]), 128,
+                                       fmt)
+                    st, size = _shared(q, p, p, k2=t, v2=t, G=4, cus=cus)
+                    assert st == 0
+                    units = 2 * (B + -(-4 * B // 16))
+                    rows_bytes = 512 * (S * 2 * -(-4 * B // 16) + (S_s or 0) * 2 * B)
+                    records = 64 * (2 * units + 32 * cus + rows_bytes // (1 << 18))
+                    assert size <= records * (128 * 4 + 8) + 4096 + B * 8 * 128 * 8, (B, S, S_s, size)
