@@ -173,12 +173,13 @@ __global__ void __launch_bounds__(256) span_zero_kernel(uint32_t* p, int64_t n) 
 
 // ------------------------------------------------------------------- host
 
-// Rows that many queries share: past this many bytes of a token's K and V, times
-// blocks of 16 queries, the waves of a workgroup take queries (tile_kernel), up to
-// it tokens, and the row blocks read the rows from one L2 (span_kernel).  Below,
-// tiles and tokens: 96 queries of 264-byte tokens 27.1 and 22.7 us, 98 of 85
-// bytes 30.0 and 22.7, 49 of 320 bytes 24.2 and 22.0; above: 64 of 512 bytes 46.7
-// and 51, 128 of 512 bytes 33.6 and 58, 448 of 165 bytes 64 and 73.
+// Rows that many queries share: from this many bytes of a token's K and V, times
+// blocks of 16 queries, the waves of a workgroup take queries (tile_kernel), below
+// it tokens, and the row blocks read the rows from one L2 (span_kernel).  Tiles and
+// tokens behind 16384 rows, us: 64 queries of 512 bytes 31.1 and 36.4, 128 34.8 and
+// 57.6; of 256 bytes 96 39.0 and 34.7, 128 39.7 and 41.1, 256 60.2 and 65.1; of 128
+// bytes 192 47.5 and 39.8, 256 51.6 and 48.8.  448 of 160 bytes behind 32768: 64 and
+// 73.
 constexpr int64_t kTileBytes = 2048;
 // Suffix rows up to this many are attended in the launch that joins the tiles'
 // records, one workgroup per request and KV head, for a launch less: 64 requests
@@ -324,7 +325,8 @@ int make_plan(const Call& c, int cus, Plan* out) {
     shared_bytes += p.S[i] * cost[i];
     shared_tokens += p.S[i];
   }
-  p.tile = c.shared && p.vec && p.terms < 3 && cdiv(p.B * p.G, 16) * shared_bytes > kTileBytes * shared_tokens;
+  p.tile = c.shared && p.vec && p.terms < 3 && shared_tokens > 0 &&
+           cdiv(p.B * p.G, 16) * shared_bytes >= kTileBytes * shared_tokens;
   p.join = p.tile && p.S[kTail] > 0 && p.S[kTail] <= kJoinTokens;
   int64_t total = 0;
   for (int i = 0; i < kSpans; ++i) {

@@ -18,12 +18,14 @@
 // One tile buffer, one tile ahead and 16 queries a wave leave registers and LDS
 // for three workgroups on a CU, which hide each other's barriers and latencies:
 // 32 queries a wave, two buffers, or two tiles ahead (two workgroups each) took 6,
-// 17 and 16 % longer, both halves of a tile in one softmax (spills) 2 to 14 %.
+// 17 and 16 % longer, both halves of a tile in one softmax (spills) 2 to 14 %,
+// eight waves that take half a tile each 10 %.
 //
 // What bounds it: issue.  64 requests of 7 heads behind 32768 tokens, 64 channels
 // kept: 71 us with the join (11), 324 TFLOP/s of the formula; a wave issues 26
-// matrix and 90 other vector instructions for 32 tokens, the matrix pipes are busy
-// for 47 % of the loop, and waves wait for their turn for 42 % of their time.  32
+// matrix and 90 other vector instructions for 32 tokens and reads 24 KB of a tile's
+// LDS for 64; the matrix pipes are busy for 47 % of the loop, LDS for about as much,
+// and waves wait for their turn for 42 % of their time.  32
 // requests of 4 heads behind 16001: 34 us with the join (8.6), 2.2 TB/s.
 #pragma once
 

@@ -164,7 +164,7 @@ def test_same_as_the_expanded_batch():
     assert (got.float() - want.float()).abs().max() <= 2 * 2.0 ** -11 * want.float().abs().max() + 1e-4
 
 
-# As many queries on the same rows as make the waves take queries (past 2048
+# As many queries on the same rows as make the waves take queries (from 2048
 # bytes of a token times blocks of 16 queries), in every format.
 MANY = [
     (61, 8, 2, 128, 100, 0, 0, 20, [20, 0, 3]),        # 244 rows: 4 blocks of 64, the last of 52
