@@ -190,6 +190,27 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     return _lib
 
 
+_bind = None
+_BOUND = ("rk_mx_write", "rk_mx_read", "rk_mx_append", "rk_quantized_decode_check", "rk_quantized_decode",
+          "rk_shared_prefix_decode_check", "rk_shared_prefix_decode")
+
+
+def bind():
+    """The C++ host path of the quantised and shared-prefix calls (``_bind``,
+    csrc/rk_bind.cpp), over the library that ``load`` gave."""
+    global _bind
+    if _bind is None:
+        lib = load()
+        try:
+            from rotatek_amd import _bind as module
+        except ImportError as e:
+            raise HipLibraryMissing(f"rotatek_amd/_bind.so is not built or does not load ({e}); run "
+                                    "`python -m rotatek_amd.build`") from e
+        module.init(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _BOUND))
+        _bind = module
+    return _bind
+
+
 def strerror(status: int) -> str:
     return load().rk_strerror(status).decode()
 
@@ -225,48 +246,13 @@ def desc(t: torch.Tensor | None):
                                                      *t.shape, *pad, *t.stride(), *pad))
 
 
-# rk_rows: two rk_tensors, head_dim, format
-_RK_ROWS = struct.Struct("=Qii8qQii8qqii")
-_PLAIN_ROWS = (0,) * 11
-
-
-def pack(t: torch.Tensor | None) -> bytes | None:
-    """desc() as bytes, which a ``void*`` argument takes as they are (a ctypes
-    structure costs 0.4 us more)."""
-    if t is None:
-        return None
-    shape = t.shape
-    nd = len(shape)
-    code = _DTYPES.get(t.dtype)
-    if nd > 4 or code is None:
-        raise ValueError(f"tensors of rank > 4 or dtype {t.dtype} are not supported")
-    pad = _PAD[4 - nd]
-    return _RK_TENSOR.pack(t.data_ptr(), code, nd, *shape, *pad, *t.stride(), *pad)
-
-
-def pack_contiguous(ptr: int, dtype: torch.dtype, shape) -> bytes:
-    """pack() of a contiguous [a, b, c] tensor at ``ptr``."""
-    a, b, c = shape
-    return _RK_TENSOR.pack(ptr, _DTYPES[dtype], 3, a, b, c, 0, b * c, c, 1, 0)
-
-
-def pack_rows(data: torch.Tensor, scales: torch.Tensor | None, head_dim: int, fmt: int) -> bytes:
-    """rk_rows of quantised rows, or of plain ones (``scales`` None), as bytes."""
-    code, shape = _DTYPES.get(data.dtype), data.shape
-    if len(shape) != 4 or code is None:
-        raise ValueError(f"rows need 4 dims [B, H, S, D] of a known dtype, got {tuple(shape)} {data.dtype}")
-    if scales is None:
-        return _RK_ROWS.pack(data.data_ptr(), code, 4, *shape, *data.stride(), *_PLAIN_ROWS, head_dim, fmt, 0)
-    sc, sshape = _DTYPES.get(scales.dtype), scales.shape
-    if len(sshape) != 4 or sc is None:
-        raise ValueError(f"scales need 4 dims of a known dtype, got {tuple(sshape)} {scales.dtype}")
-    return _RK_ROWS.pack(data.data_ptr(), code, 4, *shape, *data.stride(), scales.data_ptr(), sc, 4, *sshape,
-                         *scales.stride(), head_dim, fmt, 0)
-
-
 def rows_desc(data: torch.Tensor, scales: torch.Tensor | None, head_dim: int, fmt: int) -> RkRows:
-    """pack_rows as a structure."""
-    return RkRows.from_buffer_copy(pack_rows(data, scales, head_dim, fmt))
+    """rk_rows of quantised rows, or of plain ones (``scales`` None)."""
+    r = RkRows(head_dim=head_dim, format=fmt)
+    r.data = desc(data)
+    if scales is not None:
+        r.scales = desc(scales)
+    return r
 
 
 def ref(d):

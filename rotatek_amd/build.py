@@ -3,7 +3,9 @@
 ``python -m rotatek_amd.build`` (or ``__graft_entry__.build()``) compiles
 every ``csrc/*.hip`` translation unit in parallel and links them into
 ``rotatek_amd/librotatek_hip.so``.  All HIP code is compiled with packed
-fp32 instructions disabled (``-target-feature -packed-fp32-ops``).
+fp32 instructions disabled (``-target-feature -packed-fp32-ops``).  Beside
+it ``rotatek_amd/_bind.so``, host code alone: ``csrc/rk_bind.cpp`` against
+torch's headers.
 """
 from __future__ import annotations
 
@@ -13,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -20,6 +23,7 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "librotatek_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
+BIND_PATH = os.path.join(HERE, "_bind.so")
 ARCH = os.environ.get("ROTATEK_OFFLOAD_ARCH", "gfx950")
 
 COMMON_FLAGS = [
@@ -45,6 +49,25 @@ def _compile(hipcc: str, src: str, obj: str, verbose: bool) -> None:
         raise RuntimeError(f"hipcc failed on {os.path.basename(src)}:\n{res.stderr[-4000:]}")
 
 
+def _build_bind(hipcc: str, verbose: bool) -> None:
+    """The Python module of host code (torch only when it is built)."""
+    import torch
+    cxx = shutil.which("g++") or shutil.which("c++") or hipcc
+    inc, lib = (os.path.join(os.path.dirname(torch.__file__), d) for d in ("include", "lib"))
+    tmp = BIND_PATH + ".tmp"
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", inc,
+           "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+           os.path.join(CSRC, "rk_bind.cpp"), "-o", tmp, f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{os.path.basename(cxx)} failed on rk_bind.cpp:\n{res.stderr[-4000:]}")
+    os.replace(tmp, BIND_PATH)
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> str:
     """Compile and link the library; returns its path."""
     hipcc = _hipcc()
@@ -54,7 +77,8 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
     objs = [os.path.join(objdir, os.path.basename(s)[:-4] + ".o") for s in srcs]
     jobs = jobs or min(len(srcs), max(1, (os.cpu_count() or 4)))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        futs = [ex.submit(_compile, hipcc, s, o, verbose) for s, o in zip(srcs, objs)]
+        futs = [ex.submit(_build_bind, hipcc, verbose)]
+        futs += [ex.submit(_compile, hipcc, s, o, verbose) for s, o in zip(srcs, objs)]
         for f in futs:
             f.result()
     tmp = LIB_PATH + ".tmp"

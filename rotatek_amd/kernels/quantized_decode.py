@@ -39,7 +39,7 @@ def rotatek_decode_quantized(q_full: torch.Tensor, R_partial: torch.Tensor, delt
     to attend gets zeros."""
     check_query(q_full)
     _check_rows(k_full=k_full, v_full=v_full, k_sparse=k_sparse, v_sparse=v_sparse)
-    o = launch("rotatek_decode_quantized", q_full, (R_partial, delta_mu), (k_full, v_full, k_sparse, v_sparse),
+    o = launch("rotatek_decode_quantized", q_full, (R_partial, delta_mu), (k_full, v_full, k_sparse, v_sparse, None, None),
                mask_full, len_full, num_kv_groups, out, False)
     return o, None, None
 
@@ -52,8 +52,8 @@ def full_channel_decode_quantized(q: torch.Tensor, k: MXRows, v: MXRows, num_kv_
     bool and ``lens`` device int32 [B] as above.  Returns [B, 1, H_q, D]."""
     check_query(q)
     _check_rows(k=k, v=v)
-    return launch("full_channel_decode_quantized", q, (None, None), (k, v, None, None), mask, lens, num_kv_groups, out,
-                  False)
+    return launch("full_channel_decode_quantized", q, (None, None), (k, v, None, None, None, None), mask, lens,
+                  num_kv_groups, out, False)
 
 
 __all__ = ["full_channel_decode_quantized", "rotatek_decode_quantized"]

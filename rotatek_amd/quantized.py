@@ -19,7 +19,6 @@ nothing.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Optional
 
 import torch
@@ -95,10 +94,6 @@ class MXRows:
         """rk_rows of these rows."""
         return _lib.rows_desc(self.codes, self.scales, self.head_dim, FORMATS[self.fmt])
 
-    def pack(self) -> bytes:
-        """desc() as bytes."""
-        return _lib.pack_rows(self.codes, self.scales, self.head_dim, FORMATS[self.fmt])
-
     def __repr__(self) -> str:
         return f"MXRows({tuple(self.shape)}, {self.fmt!r}, device={str(self.device)!r})"
 
@@ -118,12 +113,11 @@ def same_device(what: str, index: int, *tensors) -> None:
             raise ValueError(f"{what}: every tensor must be on cuda:{index}")
 
 
-_HERE = contextlib.nullcontext()
-
-
-def on_device(index: int):
-    """Launches go to GPU ``index`` whichever is current."""
-    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+def refused(what: str, status: int, index: int, *tensors) -> None:
+    """Raise for a call that the host path answered with ``status``."""
+    if status == _lib.bind().OTHER_DEVICE:
+        same_device(what, index, *tensors)
+    _lib.check(status, what)
 
 
 def check_lens(lens: torch.Tensor, batch: int, name: str) -> None:
@@ -137,16 +131,14 @@ def quantize_rows(x: torch.Tensor, fmt: str = "mx8", out: Optional[MXRows] = Non
     _format(fmt)
     if x.dim() != 4:
         raise ValueError(f"x needs 4 dims [B, H, S, D], got shape {tuple(x.shape)}")
-    dev = x.get_device()
-    same_device("quantize_rows", dev, out)
-    if out is None:
-        out = MXRows.empty(*x.shape, fmt=fmt, device=x.device)
-    elif out.fmt != fmt:
+    if out is not None and out.fmt != fmt:
         raise ValueError(f"out holds {out.fmt} rows, not {fmt}")
-    dx, dr = _lib.pack(x), out.pack()
-    with on_device(dev):
-        st = _lib.load().rk_mx_write(dx, dr, _lib.raw_stream(dev))
-    _lib.check(st, "quantize_rows")
+    dev = x.get_device()
+    r = _lib.bind().write(x, out, fmt, _lib.raw_stream(dev))
+    if r.__class__ is tuple:
+        return MXRows(*r, x.shape[3], fmt)
+    if r:
+        refused("quantize_rows", r, dev, x, out)
     return out
 
 
@@ -155,13 +147,11 @@ def dequantize_rows(rows: MXRows, dtype: torch.dtype = torch.bfloat16,
     """The values [B, H, S, head_dim] that ``rows`` stand for, rounded once to
     ``dtype`` (into ``out``, of any strides and its own dtype, if given)."""
     dev = rows.codes.get_device()
-    same_device("dequantize_rows", dev, rows, out)
-    if out is None:
-        out = torch.empty(rows.shape, dtype=dtype, device=rows.device)
-    dr, do = rows.pack(), _lib.pack(out)
-    with on_device(dev):
-        st = _lib.load().rk_mx_read(dr, do, _lib.raw_stream(dev))
-    _lib.check(st, "dequantize_rows")
+    r = _lib.bind().read(rows, out, dtype, _lib.raw_stream(dev))
+    if r.__class__ is not int:
+        return r
+    if r:
+        refused("dequantize_rows", r, dev, rows, out)
     return out
 
 
@@ -177,12 +167,10 @@ def append_rows(k_new: torch.Tensor, v_new: Optional[torch.Tensor], k_rows: MXRo
     if (v_new is None) != (v_rows is None):
         raise ValueError("v_new and v_rows go together")
     dev = k_new.get_device()
-    same_device("append_rows", dev, v_new, k_rows, v_rows, lens)
-    check_lens(lens, k_new.shape[0], "lens")
-    dk, dv, rk, rv = _lib.pack(k_new), _lib.pack(v_new), k_rows.pack(), None if v_rows is None else v_rows.pack()
-    with on_device(dev):
-        st = _lib.load().rk_mx_append(dk, dv, rk, rv, lens.data_ptr(), int(bool(advance)), _lib.raw_stream(dev))
-    _lib.check(st, "append_rows")
+    st = _lib.bind().append(k_new, v_new, k_rows, v_rows, lens, advance, _lib.raw_stream(dev))
+    if st:
+        check_lens(lens, k_new.shape[0], "lens")
+        refused("append_rows", st, dev, k_new, v_new, k_rows, v_rows, lens)
 
 
 __all__ = ["MXRows", "append_rows", "dequantize_rows", "quantize_rows"]

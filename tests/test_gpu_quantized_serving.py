@@ -187,3 +187,73 @@ def test_store_and_growth_refusals():
     assert c.spans(0)[0].shape[2] >= 1005
     assert torch.equal(c.spans(0)[0].codes[:, :, :5], before[:, :, :5])
     assert c.nbytes > 0 and len(c) == 1
+
+
+def test_threads_issue_at_once():
+    """Calls of several threads, a stream each, on shared rows."""
+    from concurrent.futures import ThreadPoolExecutor
+    from rotatek_amd.kernels import full_channel_decode_quantized, shared_prefix_decode
+    from rotatek_amd.quantized import dequantize_rows, quantize_rows
+    _say("threads")
+    g = torch.Generator().manual_seed(6)
+    x = sp.randn(g, 2, 4, 700, 128, dtype=torch.bfloat16).cuda()
+    rows = quantize_rows(x, "mx8")
+    back = dequantize_rows(rows)
+    qs = [sp.randn(g, 2, 8, 128, dtype=torch.bfloat16).cuda() for _ in range(6)]
+    want = [full_channel_decode_quantized(q, rows, rows, 2) for q in qs]
+    both = [shared_prefix_decode(q, x[:1], x[:1], x, x, 2) for q in qs]
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                a = full_channel_decode_quantized(qs[i], rows, rows, 2)
+                b = shared_prefix_decode(qs[i], x[:1], x[:1], x, x, 2)
+                c = dequantize_rows(quantize_rows(x, "mx8"))
+        stream.synchronize()
+        return torch.equal(a, want[i]) and torch.equal(b, both[i]) and torch.equal(c, back)
+
+    with ThreadPoolExecutor(6) as pool:
+        assert all(pool.map(work, range(6)))
+
+
+def test_tensors_elsewhere_and_other_objects_are_refused():
+    from rotatek_amd.kernels import full_channel_decode_quantized, rotatek_decode_quantized, shared_prefix_decode
+    from rotatek_amd.quantized import MXRows, append_rows, dequantize_rows, quantize_rows
+    _say("elsewhere")
+    x = torch.randn(1, 2, 40, 128, device="cuda")
+    r, q = quantize_rows(x), torch.randn(1, 4, 128, device="cuda")
+    away = MXRows(r.codes.cpu(), r.scales, 128)
+    lens = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for call in (lambda: full_channel_decode_quantized(q, r, away, 2),
+                 lambda: full_channel_decode_quantized(q, r, r, 2, lens=lens.cpu()),
+                 lambda: full_channel_decode_quantized(q, r, r, 2, lens=lens.long()),
+                 lambda: full_channel_decode_quantized(q, r, r, 2, lens=torch.zeros(2, dtype=torch.int32, device="cuda")),
+                 lambda: full_channel_decode_quantized(q, r, r, 2, mask=torch.ones(1, 40, dtype=torch.bool)),
+                 lambda: full_channel_decode_quantized(q, r, r, 2, out=torch.empty(1, 4, 128)),
+                 lambda: full_channel_decode_quantized(q, r, r, 2, out=torch.empty(1, 4, 128, device="cuda").half()),
+                 lambda: full_channel_decode_quantized(q, r, r, 3),
+                 lambda: full_channel_decode_quantized(q, r, r, 0),
+                 lambda: full_channel_decode_quantized(q, r, quantize_rows(x, "mx4"), 2),
+                 lambda: full_channel_decode_quantized(q, MXRows(None, r.scales, 128), r, 2),
+                 lambda: rotatek_decode_quantized(q, x[..., :32], None, r, r, None, None, None, 2),
+                 lambda: shared_prefix_decode(q, x, x, None, None, 2),      # plain fp32 rows
+                 lambda: quantize_rows(x, out=away),
+                 lambda: quantize_rows(x.double()),
+                 lambda: quantize_rows(torch.zeros(1, 1, 4, 129, device="cuda")),
+                 lambda: dequantize_rows(r, torch.int32),
+                 lambda: dequantize_rows(r, out=torch.empty(1, 2, 40, 128)),
+                 lambda: append_rows(x[:, :, :1], None, r, None, lens.cpu()),
+                 lambda: append_rows(x[:, :, :1], None, r, None, lens.long()),
+                 lambda: append_rows(x[:, :, :1], None, away, None, lens)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(AttributeError):
+        shared_prefix_decode(q, [x], [x], None, None, 2)
+    with pytest.raises(ValueError):     # int("two")
+        full_channel_decode_quantized(q, r, r, "two")
+    with pytest.raises(RuntimeError):
+        full_channel_decode_quantized(q.cpu(), r, r, 2)
+    # after all that a call as it should be
+    assert torch.isfinite(full_channel_decode_quantized(q, r, r, 2)).all()
