@@ -394,10 +394,14 @@ __device__ __forceinline__ void weigh_block(const f32x4 (&s)[2], float scale, fl
   }
 }
 
-// One chunk of one span: adds the wave's blocks to `st`.  pre(): stages the
+// One chunk of one span: adds the wave's blocks to `st`.  MASK: a mask of
+// neighbouring bytes over at least a block, a lane's eight asked for ahead of the
+// block's scores.  (8 requests of 64 heads to 8000 masked tokens: 56.5 us, 68 with a
+// load and a wait per token, as other masks have; in kernels that calls without a
+// mask share, the registers spill and those take 3 to 30 % longer.)  pre(): stages the
 // unit's queries in LDS, sq [term][row][stride] 16-bit in the lane's channel
 // order, while the first blocks are on their way.
-template <class F, int KB, int VB, int NT, int NP, bool VEC, class Pre>
+template <class F, int KB, int VB, int NT, int NP, bool VEC, bool MASK, class Pre>
 __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, SpanLane<KB>& hd, int b, int chunk,
                                          int wave, int lane, const uint16_t* sq, int qstride, const float* sbias,
                                          State<VB>& st, const Pre& pre) {
@@ -435,6 +439,12 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
   float off = (sbias ? sbias[n] * a.scale_log2 : 0.f) + kLift<TT>;
 
   auto compute = [&](int blk, int next) {
+    uint2 mask;
+    if constexpr (MASK) {
+      const uint8_t* p = sp.mask + b * sp.m_sb + block_row(sp, blk) + 4 * g;
+      __builtin_memcpy(&mask.x, p, 4);
+      __builtin_memcpy(&mask.y, p + 16, 4);
+    }
     f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int j = 0; j < KB; ++j)
@@ -464,7 +474,10 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
       for (int r = 0; r < 8; ++r) {
         const int t = t0 + token_of(g, r);
         bool ok = t >= blk * kSpanBlk && t < lim;
-        if (sp.mask && ok) ok = sp.mask[b * sp.m_sb + t * sp.m_ss] != 0;
+        if constexpr (MASK)
+          ok = ok && ((r < 4 ? mask.x : mask.y) >> (8 * (r & 3)) & 0xffu) != 0;
+        else if (sp.mask && ok)
+          ok = sp.mask[b * sp.m_sb + t * sp.m_ss] != 0;
         on |= (uint32_t)ok << r;
         // a row that does not count holds anything: 0 x NaN must not reach the
         // sum.  (Here, under the branch: as selects at V^T they would run in
@@ -740,7 +753,7 @@ __device__ __forceinline__ void join_records(const SpanArgs& a, const RowOf& o, 
 // plan fills three and the fourth takes a late one), 168 for plain ones, whose
 // blocks are twice as wide, 256 for element loads (VEC false), which keep an
 // address per element.
-template <class F, int KV, int KF, int NT, int NP, bool VEC, bool JOIN = false>
+template <class F, int KV, int KF, int NT, int NP, bool VEC, bool MASK, bool JOIN>
 __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span_kernel(const SpanArgs a) {
   using TT = typename F::TT;
   constexpr int VB = KF == 2 ? 4 : 8;
@@ -835,7 +848,7 @@ __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span
         }
         __syncthreads();
       };
-      run_span<F, KV, VB, NTV, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias, st, pre);
+      run_span<F, KV, VB, NTV, NP, VEC, false>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias, st, pre);
       done = true;
     }
   }
@@ -847,7 +860,7 @@ __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span
       stage_queries<TT, NT, 1, NW, 32 * KF>(tid, qw, f16, s_q, kWide);
       __syncthreads();
     };
-    run_span<F, KF, VB, NT, NP, VEC>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, st, pre);
+    run_span<F, KF, VB, NT, NP, VEC, MASK>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, st, pre);
   }
 
   // The row's true maximum; a row without tokens has the least one.
@@ -899,7 +912,14 @@ __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span
 
 template <class F, int KV, int KF, int NT, int NP, bool VEC>
 hipError_t launch_span(const SpanArgs& a, unsigned grid, hipStream_t s) {
-  hipLaunchKernelGGL((span_kernel<F, KV, KF, NT, NP, VEC>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+  if constexpr (F::kMx) {  // (plain rows are a shared call's, which has no mask)
+    const Span& sp = a.span[kFull];
+    if (sp.mask && sp.m_ss == 1 && sp.S >= kSpanBlk) {
+      hipLaunchKernelGGL((span_kernel<F, KV, KF, NT, NP, VEC, true, false>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+      return hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((span_kernel<F, KV, KF, NT, NP, VEC, false, false>), dim3(grid), dim3(kSpanThreads), 0, s, a);
   return hipGetLastError();
 }
 
@@ -925,9 +945,9 @@ hipError_t pick_widths(int kv, int kf, const SpanArgs& a, unsigned grid, hipStre
 template <class F, int NT, int NP>
 hipError_t pick_join(int kf, const SpanArgs& a, unsigned grid, hipStream_t s) {
   if (kf == 2)
-    hipLaunchKernelGGL((span_kernel<F, 0, 2, NT, NP, true, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+    hipLaunchKernelGGL((span_kernel<F, 0, 2, NT, NP, true, false, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((span_kernel<F, 0, 4, NT, NP, true, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
+    hipLaunchKernelGGL((span_kernel<F, 0, 4, NT, NP, true, false, true>), dim3(grid), dim3(kSpanThreads), 0, s, a);
   return hipGetLastError();
 }
 

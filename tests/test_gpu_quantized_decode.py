@@ -181,3 +181,29 @@ def test_strided_queries_rows_masks_and_outputs():
         view.scales.copy_(r.scales)
         views.append(view)
     assert torch.equal(full_channel_decode_quantized(c["q"].cuda(), *views, 2), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("S_f", [1, 2, 31, 32, 33, 100, 700])
+def test_masks_in_every_layout(S_f, dtype):
+    """Neighbouring bytes at any address, every third byte, one row for all."""
+    from rotatek_amd.kernels import full_channel_decode_quantized, rotatek_decode_quantized
+    _say(f"mask layouts {S_f} {dtype}")
+    for Dk, S_v in ((0, 0), (32, 70)):
+        c = _case(3, 8, 2, 128, Dk, S_v, S_f, dtype, "mx8", seed=31 + S_f, mask=True)
+        m = c["mask"]
+        flat = torch.full((3 * S_f + 1,), 255, dtype=torch.uint8, device="cuda")
+        flat[1:] = m.reshape(-1)
+        wide = torch.full((3, S_f, 3), 255, dtype=torch.uint8, device="cuda")
+        wide[..., 1] = m
+        for mask in (m, m.bool(), flat[1:].view(3, S_f), wide[..., 1], m * 128):
+            if S_v:
+                out = rotatek_decode_quantized(c["q"].cuda(), c["R"], c["dm"], c["k_full"], c["v_full"], mask, c["k_sparse"],
+                                               c["v_sparse"], c["groups"])[0]
+            else:
+                out = full_channel_decode_quantized(c["q"].cuda(), c["k_full"], c["v_full"], c["groups"], mask=mask)
+            sp.check(out, c["q"], c["groups"], c["spans"], "mx8", dtype)
+        one = m[1:2].expand(3, S_f)
+        same = full_channel_decode_quantized(c["q"].cuda(), c["k_full"], c["v_full"], c["groups"], mask=one)
+        want = full_channel_decode_quantized(c["q"].cuda(), c["k_full"], c["v_full"], c["groups"], mask=one.contiguous())
+        assert torch.equal(same, want)
