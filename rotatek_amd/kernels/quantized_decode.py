@@ -39,8 +39,8 @@ def rotatek_decode_quantized(q_full: torch.Tensor, R_partial: torch.Tensor, delt
     to attend gets zeros."""
     check_query(q_full)
     _check_rows(k_full=k_full, v_full=v_full, k_sparse=k_sparse, v_sparse=v_sparse)
-    o = launch("rotatek_decode_quantized", q_full, (R_partial, delta_mu), (k_full, v_full, k_sparse, v_sparse, None, None),
-               mask_full, len_full, num_kv_groups, out, False)
+    o = launch("rotatek_decode_quantized", q_full, (R_partial, delta_mu),
+               (k_full, v_full, k_sparse, v_sparse, None, None), mask_full, len_full, num_kv_groups, out, False)
     return o, None, None
 
 
