@@ -358,7 +358,8 @@ __device__ __forceinline__ void weigh_block(const f32x4 (&s)[2], float scale, fl
     float up = mx - kLift<TT>;
     if (row_max(was) > -INFINITY) up = fmaxf(up, 0.f);
     if (!(up > -INFINITY)) up = 0.f;
-    const float alpha = fast_exp2(-up);
+    // (first scores far below zero: the sums are zero, and 2^-up is infinite)
+    const float alpha = fast_exp2(-fmaxf(up, 0.f));
 #pragma unroll
     for (int j = 0; j < VB; ++j) st.acc[j] *= alpha;
     st.l *= alpha;
