@@ -4,6 +4,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 namespace rk {
@@ -52,6 +53,7 @@ struct SpanArgs {
   const void* R;
   const void* dm;
   int64_t R_sb, R_sh, R_sd, dm_sb, dm_sh;
+  const float* qtop;  // with qr of fp16 terms: a row's largest |q R|
 };
 
 // Queries that the split launch does not take as they are: a copy of q in
@@ -63,6 +65,7 @@ struct QueryArgs {
   void* q_out;      // [row][Dp], or null
   uint16_t* qr;     // [row][terms][W], or null
   float* bias;
+  float* qtop;      // [row], fp16 terms' alone
   int64_t q_sb, q_sh, q_sd, R_sb, R_sh, R_sd, R_sk, dm_sb, dm_sh, dm_sd;
   int32_t Hq, G, D, Dp, Dk, W, terms, shared, q_dtype, r_dtype, dm_dtype, f16;
 };
@@ -70,6 +73,15 @@ struct QueryArgs {
 constexpr int kSpanThreads = 256;
 constexpr int kSpanWaves = 4;
 constexpr int kSpanBlk = 32;  // tokens of a wave's step
+
+// fp16 terms of q R.  fp16 ends at 65504, and queries of order 10^4 take q R past
+// it: a row whose largest entry `top` is 2^15 or more is split as q R 2^-shift,
+// below 2^15, and its scores take 2^shift back in their factor.  Both are exact.
+// (Each row by itself: a large query leaves its neighbours' terms alone.)
+constexpr float kSplitTop = 32768.f;
+__device__ __forceinline__ int split_shift(float top) {
+  return top >= kSplitTop && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+}
 
 // The split launch: kv = score blocks of 32 channels of the rotated span (0:
 // none, 1, 2 or 4), kf the full-width spans' (2: D <= 64, or 4), terms = 16-bit

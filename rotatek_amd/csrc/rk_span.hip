@@ -33,7 +33,7 @@ int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 // `terms` 16-bit values (two hold 16 or more bits of it, three an fp32's 24).
 __global__ void __launch_bounds__(128) span_queries_kernel(const rk::QueryArgs a) {
   __shared__ float s_q[128];
-  __shared__ float s_b[2];
+  __shared__ float s_b[2], s_t[2];
   const int c = threadIdx.x;
   const int64_t row = blockIdx.x;
   const int64_t b = row / a.Hq, h = row - b * a.Hq, kv = h / a.G, rb = a.shared ? 0 : b;
@@ -47,18 +47,27 @@ __global__ void __launch_bounds__(128) span_queries_kernel(const rk::QueryArgs a
   }
   if (!a.qr) return;
   __syncthreads();
-  if (c < a.W) {
-    float v = 0.f;
-    if (c < a.Dk) {
-      const int64_t off = rb * a.R_sb + kv * a.R_sh + c * a.R_sk;
-      for (int d = 0; d < a.D; d += 32) {
-        float r[32];
-        rk::load_any_rows<32>(a.R, off, a.R_sd, a.r_dtype, d, a.D, r);
+  float v = 0.f;
+  if (c < a.Dk) {
+    const int64_t off = rb * a.R_sb + kv * a.R_sh + c * a.R_sk;
+    for (int d = 0; d < a.D; d += 32) {
+      float r[32];
+      rk::load_any_rows<32>(a.R, off, a.R_sd, a.r_dtype, d, a.D, r);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (d + i < a.D) v = fmaf(s_q[d + i], r[i], v);
-      }
+      for (int i = 0; i < 32; ++i)
+        if (d + i < a.D) v = fmaf(s_q[d + i], r[i], v);
     }
+  }
+  if (a.f16) {
+    float top = fabsf(v);
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, rk::shfl_xor(top, d));
+    if ((c & 63) == 0) s_t[c >> 6] = top;
+    __syncthreads();
+    top = fmaxf(s_t[0], s_t[1]);
+    if (c == 0) a.qtop[row] = top;
+    v = ldexpf(v, -rk::split_shift(top));
+  }
+  if (c < a.W) {
     for (int t = 0; t < a.terms; ++t) {
       const uint16_t w = a.f16 ? rk::F16::from_f32(v) : rk::BF16::from_f32(v);
       a.qr[(row * a.terms + t) * a.W + c] = w;
@@ -213,7 +222,7 @@ struct Plan {
   bool tile;       // rk_tile_dev.h over the shared spans, 64 queries a workgroup
   bool copy_q, ahead;  // queries copied into whole pieces; rotated ahead of the split launch
   int64_t S[kSpans], chunk[kSpans], wgs[kSpans], units[kSpans], blocks[kSpans], np, rows;
-  size_t q, qr, bias, zero, zero_bytes, acc, ml, total;
+  size_t q, qr, bias, qtop, zero, zero_bytes, acc, ml, total;
 };
 
 // Workgroup ids of a span: eight (chunk, head) pairs' row blocks at a time.
@@ -395,6 +404,7 @@ int make_plan(const Call& c, int cus, Plan* out) {
   p.q = take(p.copy_q ? (size_t)p.rows * round_up(p.D, 8) * el : 0);
   p.qr = take(p.ahead ? (size_t)p.rows * std::max(p.terms, 2) * 32 * p.kv * 2 : 0);
   p.bias = take(p.ahead ? (size_t)p.rows * 4 : 0);
+  p.qtop = take(p.ahead && !quantised && c.q->dtype == RK_F16 ? (size_t)p.rows * 4 : 0);
   // rotated rows without channels: one zero row and its scales
   p.zero_bytes = p.kv && p.Dk == 0 ? 256 + (size_t)round_up(p.S[kRotated], 32) : 0;
   p.zero = take(p.zero_bytes);
@@ -524,6 +534,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
       qa.bias = (float*)(ws + p.bias);
       a.qr = qa.qr;
       a.bias = qa.bias;
+      if (qa.f16) a.qtop = qa.qtop = (float*)(ws + p.qtop);
     }
     hipLaunchKernelGGL(span_queries_kernel, dim3((unsigned)p.rows), dim3(128), 0, s, qa);
     if (hipGetLastError() != hipSuccess) return RK_ERR_HIP;

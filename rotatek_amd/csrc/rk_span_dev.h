@@ -401,11 +401,12 @@ __device__ __forceinline__ void weigh_block(const f32x4 (&s)[2], float scale, fl
 // load and a wait per token, as other masks have; in kernels that calls without a
 // mask share, the registers spill and those take 3 to 30 % longer.)  pre(): stages the
 // unit's queries in LDS, sq [term][row][stride] 16-bit in the lane's channel
-// order, while the first blocks are on their way.
+// order, while the first blocks are on their way; it leaves the rows' biases in sbias
+// and, of fp16 terms, their largest |q R| in stop (null: none).
 template <class F, int KB, int VB, int NT, int NP, bool VEC, bool MASK, class Pre>
 __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, SpanLane<KB>& hd, int b, int chunk,
                                          int wave, int lane, const uint16_t* sq, int qstride, const float* sbias,
-                                         State<VB>& st, const Pre& pre) {
+                                         const uint32_t* stop, State<VB>& st, const Pre& pre) {
   using TT = typename F::TT;
   const int g = lane >> 4, n = lane & 15;
   int lim = min(chunk * sp.chunk + sp.chunk, sp.S);
@@ -438,6 +439,9 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
   // a score is one fused multiply-add: the bias, the maximum and the lift in
   // its addend
   float off = (sbias ? sbias[n] * a.scale_log2 : 0.f) + kLift<TT>;
+  float scale = a.scale_log2;
+  if constexpr (TT::kRk == F16::kRk)
+    if (stop) scale = ldexpf(scale, split_shift(__builtin_bit_cast(float, stop[n])));
 
   auto compute = [&](int blk, int next) {
     uint2 mask;
@@ -509,7 +513,7 @@ __device__ __forceinline__ void run_span(const SpanArgs& a, const Span& sp, Span
       lo = make_uint4(pack_lo(y[0], y[1]), pack_lo(y[2], y[3]), pack_lo(y[4], y[5]), pack_lo(y[6], y[7]));
       hi = make_uint4(pack_hi(y[0], y[1]), pack_hi(y[2], y[3]), pack_hi(y[4], y[5]), pack_hi(y[6], y[7]));
     };
-    weigh_block<TT, VB, NP, false>(s, a.scale_log2, off, whole, on, st, turn);
+    weigh_block<TT, VB, NP, false>(s, scale, off, whole, on, st, turn);
     load_v<F, KB, VB, VEC, kAux>(sp, hd, a.D, next, n, x);
   };
 
@@ -649,52 +653,66 @@ __device__ __forceinline__ void stage_rotation(int tid, const Rotation<KV>& x, u
 }
 
 // raw: the queries as they are, [row][136]; r, mu: the staged rotation.  q R is
-// left as NTV terms of TT in `dst`, q . delta_mu in `bias`.  A wave takes tiles of
-// 16 columns; one more has delta_mu in every column.  (Channel order within 32:
-// as read_columns gives them.)
+// left as NTV terms of TT in `dst`, q . delta_mu in `bias`, behind a barrier.  A wave
+// takes tiles of 16 columns; one more has delta_mu in every column.  (Channel order
+// within 32: as read_columns gives them.)  fp16 terms: `top`, zero before, gets the
+// largest |q R| of the rows that pass kSplitTop; if one does, all form their terms
+// again, those rows scaled.
 template <class TT, int NTV, int NR, int KV>
 __device__ __forceinline__ void rotate_queries(const SpanArgs& a, int wave, int lane, bool f16, const uint16_t* raw,
                                                const uint4* r, const uint4* mu, uint16_t* dst, int stride,
-                                               float* bias) {
+                                               float* bias, uint32_t* top) {
   constexpr int kRows = 16 * NR;
+  constexpr bool kScaled = TT::kRk == F16::kRk;
   const int g = lane >> 4, n = lane & 15;
-  for (int ct = wave; ct <= 2 * KV; ct += kSpanWaves) {
-    f32x4 o[NR];
+  for (bool again = false;; again = true) {
+    for (int ct = wave; ct <= 2 * KV; ct += kSpanWaves) {
+      f32x4 o[NR];
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr) o[nr] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int nr = 0; nr < NR; ++nr) o[nr] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint4 m;
-      if (ct < 2 * KV) {
-        m = read_columns<4 * KV>(r, 32 * ks, ct, g, n);
-      } else {
-        const uint2 lo = ((const uint2*)mu)[8 * ks + g], hi = ((const uint2*)mu)[8 * ks + 4 + g];
-        m = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      }
-#pragma unroll
-      for (int nr = 0; nr < NR; ++nr) {
-        const uint2* p = (const uint2*)(raw + (16 * nr + n) * 136 + 32 * ks);
-        const uint4 q = make_uint4(p[g].x, p[g].y, p[4 + g].x, p[4 + g].y);
-        o[nr] = f16 ? F16::mfma(q, m, o[nr]) : BF16::mfma(q, m, o[nr]);
-      }
-    }
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float v = o[nr][i];
-        const int row = 16 * nr + 4 * g + i;
-        if (ct == 2 * KV) {
-          if (n == 0) bias[row] = v;
+      for (int ks = 0; ks < 4; ++ks) {
+        uint4 m;
+        if (ct < 2 * KV) {
+          m = read_columns<4 * KV>(r, 32 * ks, ct, g, n);
         } else {
+          const uint2 lo = ((const uint2*)mu)[8 * ks + g], hi = ((const uint2*)mu)[8 * ks + 4 + g];
+          m = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
 #pragma unroll
-          for (int k = 0; k < NTV; ++k) {
-            const uint16_t h = TT::from_f32(v);
-            dst[(k * kRows + row) * stride + ct * 16 + n] = h;
-            v -= TT::to_f32(h);
-          }
+        for (int nr = 0; nr < NR; ++nr) {
+          const uint2* p = (const uint2*)(raw + (16 * nr + n) * 136 + 32 * ks);
+          const uint4 q = make_uint4(p[g].x, p[g].y, p[4 + g].x, p[4 + g].y);
+          o[nr] = f16 ? F16::mfma(q, m, o[nr]) : BF16::mfma(q, m, o[nr]);
         }
       }
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = o[nr][i];
+          const int row = 16 * nr + 4 * g + i;
+          if (ct == 2 * KV) {
+            if (n == 0) bias[row] = v;
+          } else {
+            if constexpr (kScaled) {
+              if (again)
+                v = ldexpf(v, -split_shift(__builtin_bit_cast(float, top[row])));
+              else if (fabsf(v) >= kSplitTop)
+                atomicMax(top + row, __builtin_bit_cast(uint32_t, fabsf(v)));
+            }
+#pragma unroll
+            for (int k = 0; k < NTV; ++k) {
+              const uint16_t h = TT::from_f32(v);
+              dst[(k * kRows + row) * stride + ct * 16 + n] = h;
+              v -= TT::to_f32(h);
+            }
+          }
+        }
+    }
+    __syncthreads();
+    // (the same in every wave: nothing writes `top` any more)
+    if (!kScaled || again || !__any(top[lane & (kRows - 1)] != 0u)) break;
   }
 }
 
@@ -769,6 +787,8 @@ __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span
   constexpr int kAcc = kSpanWaves * kRows * kAccRow;
   __shared__ __attribute__((aligned(16))) char s_mem[(kQ + kRaw) * 2 > kAcc * 4 ? (kQ + kRaw) * 2 : kAcc * 4];
   __shared__ float s_bias[kRows];
+  constexpr bool kScaled = KV > 0 && TT::kRk == F16::kRk;
+  __shared__ uint32_t s_qtop[kScaled ? kRows : 1];
   __shared__ float s_m[kSpanWaves][kRows], s_top[kSpanWaves][kRows], s_l[kSpanWaves][kRows];
   uint16_t* s_q = (uint16_t*)s_mem;
   uint16_t* s_raw = s_q + kQ;
@@ -828,8 +848,10 @@ __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span
             uint4* s_mu = s_r + 128 * 4 * KV;
             stage_queries<TT, 1, 1, NW, 128>(tid, qw, f16, s_raw, 136);
             stage_rotation<KV>(tid, rot, s_r, s_mu);
+            if constexpr (kScaled)
+              if (tid < kRows) s_qtop[tid] = 0u;
             __syncthreads();
-            rotate_queries<TT, NTV, 1, KV>(a, wave, lane, f16, s_raw, s_r, s_mu, s_q, kWide, s_bias);
+            rotate_queries<TT, NTV, 1, KV>(a, wave, lane, f16, s_raw, s_r, s_mu, s_q, kWide, s_bias, s_qtop);
           }
         } else {
           constexpr int W = 32 * KV;
@@ -845,11 +867,13 @@ __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span
           if (tid < kRows) {
             const RowOf o = row_of(a, shared, b, kv, R0 + min(tid, rows - 1));
             s_bias[tid] = a.bias[(int64_t)o.b * a.Hq + o.h];
+            if constexpr (kScaled) s_qtop[tid] = __builtin_bit_cast(uint32_t, a.qtop[(int64_t)o.b * a.Hq + o.h]);
           }
+          __syncthreads();
         }
-        __syncthreads();
       };
-      run_span<F, KV, VB, NTV, NP, VEC, false>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias, st, pre);
+      run_span<F, KV, VB, NTV, NP, VEC, false>(a, sp, hd, b, x, wave, lane, s_q, kWide, s_bias,
+                                               kScaled ? s_qtop : nullptr, st, pre);
       done = true;
     }
   }
@@ -861,7 +885,7 @@ __global__ void __launch_bounds__(kSpanThreads, VEC ? (F::kMx ? 4 : 3) : 2) span
       stage_queries<TT, NT, 1, NW, 32 * KF>(tid, qw, f16, s_q, kWide);
       __syncthreads();
     };
-    run_span<F, KF, VB, NT, NP, VEC, MASK>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, st, pre);
+    run_span<F, KF, VB, NT, NP, VEC, MASK>(a, sp, hd, b, x, wave, lane, s_q, kWide, nullptr, nullptr, st, pre);
   }
 
   // The row's true maximum; a row without tokens has the least one.

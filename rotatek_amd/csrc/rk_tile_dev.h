@@ -96,7 +96,8 @@ __device__ __forceinline__ void store_tile(const Span& sp, int D, int t0, int ti
   }
 }
 
-// One chunk of a span for the wave's 16 queries, which pre() leaves in q and off.
+// One chunk of a span for the wave's 16 queries, which pre() leaves in q, off and,
+// where it is not the call's, scale.
 template <class F, int KB, int VB, int NT, int NP, class Pre>
 __device__ __forceinline__ void run_tiles(const SpanArgs& a, const Span& sp, const SpanLane<1>& hd, Rsrc vsc, int chunk,
                                           int tid, char* mem, State<VB>& st, const Pre& pre) {
@@ -107,8 +108,8 @@ __device__ __forceinline__ void run_tiles(const SpanArgs& a, const Span& sp, con
   TilePart<F, KB, VB> part;
   load_tile<F, KB, VB>(sp, hd, vsc, a.D, first, tid, part);
   uint4 q[NT][KB];
-  float off;
-  pre(q, off);
+  float off, scale = a.scale_log2;
+  pre(q, off, scale);
   __syncthreads();  // (the queries' LDS is the tiles')
   store_tile<F, KB, VB>(sp, a.D, first, tid, part, (uint4*)mem, (uint4*)(mem + kKBytes));
   __syncthreads();
@@ -143,7 +144,7 @@ __device__ __forceinline__ void run_tiles(const SpanArgs& a, const Span& sp, con
         lo = read_columns<2 * VB>(vs, 32 * h, 2 * w, g, n);
         hi = read_columns<2 * VB>(vs, 32 * h, 2 * w + 1, g, n);
       };
-      weigh_block<TT, VB, NP, true>(s, a.scale_log2, off, whole, on, st, turn);
+      weigh_block<TT, VB, NP, true>(s, scale, off, whole, on, st, turn);
     }
     __syncthreads();
     if (more)
@@ -165,6 +166,8 @@ __global__ void __launch_bounds__(kSpanThreads, 3) tile_kernel(const SpanArgs a)
   constexpr int kQ = KV > 0 ? 2 * (NTV * kRows * kWide + kRows * 136 + 128 * 32 * KV + 128) : 0;
   __shared__ __attribute__((aligned(16))) char s_mem[kTiles > kQ ? kTiles : kQ];
   __shared__ float s_bias[KV > 0 ? kRows : 1];
+  constexpr bool kScaled = KV > 0 && TT::kRk == F16::kRk;
+  __shared__ uint32_t s_qtop[kScaled ? kRows : 1];
   uint16_t* s_q = (uint16_t*)s_mem;
   uint16_t* s_raw = s_q + NTV * kRows * kWide;
 
@@ -209,15 +212,16 @@ __global__ void __launch_bounds__(kSpanThreads, 3) tile_kernel(const SpanArgs a)
         load_queries<4, 4>(a, true, 0, kv, R0, rows, tid, qw);
         load_rotation<KV>(a, 0, kv, tid, rot);
       }
-      auto pre = [&](uint4(&q)[NTV][KV], float& off) {
+      auto pre = [&](uint4(&q)[NTV][KV], float& off, float& scale) {
         if (!a.qr) {
           uint4* s_r = (uint4*)(s_raw + kRows * 136);
           uint4* s_mu = s_r + 128 * 4 * KV;
           stage_queries<TT, 1, 4, 4, 128>(tid, qw, f16, s_raw, 136);
           stage_rotation<KV>(tid, rot, s_r, s_mu);
+          if constexpr (kScaled)
+            if (tid < kRows) s_qtop[tid] = 0u;
           __syncthreads();
-          rotate_queries<TT, NTV, 4, KV>(a, wave, lane, f16, s_raw, s_r, s_mu, s_q, kWide, s_bias);
-          __syncthreads();
+          rotate_queries<TT, NTV, 4, KV>(a, wave, lane, f16, s_raw, s_r, s_mu, s_q, kWide, s_bias, s_qtop);
         }
 #pragma unroll
         for (int t = 0; t < NTV; ++t)
@@ -226,13 +230,15 @@ __global__ void __launch_bounds__(kSpanThreads, 3) tile_kernel(const SpanArgs a)
             q[t][j] = a.qr ? *(const uint4*)(a.qr + (row * NTV + t) * (32 * KV) + 32 * j + 8 * g)
                            : *(const uint4*)(s_q + (t * kRows + r) * kWide + 32 * j + 8 * g);
         off = (a.qr ? a.bias[row] : s_bias[r]) * a.scale_log2 + kLift<TT>;
+        if constexpr (kScaled)
+          scale = ldexpf(scale, split_shift(a.qr ? a.qtop[row] : __builtin_bit_cast(float, s_qtop[r])));
       };
       run_tiles<F, KV, VB, NTV, NP>(a, sp, hd, vsc, x, tid, s_mem, st, pre);
       done = true;
     }
   }
   if (!done) {
-    auto pre = [&](uint4(&q)[NT][KF], float& off) {
+    auto pre = [&](uint4(&q)[NT][KF], float& off, float&) {
       off = kLift<TT>;
       const uint16_t* src = (const uint16_t*)a.q + o.b * a.q_sb + o.h * a.q_sh;
 #pragma unroll
