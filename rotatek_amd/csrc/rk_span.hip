@@ -225,9 +225,10 @@ struct Plan {
   size_t q, qr, bias, qtop, zero, zero_bytes, acc, ml, total;
 };
 
-// Workgroup ids of a span: eight (chunk, head) pairs' row blocks at a time.
+// Workgroup ids of a span: eight (chunk, head) pairs' row blocks at a time.  (A
+// batch of none has no row blocks over shared rows.)
 int64_t launched(const Plan& p, int i) {
-  return p.S[i] == 0 ? 0 : 8 * p.blocks[i] * cdiv(p.wgs[i] * (p.units[i] / p.blocks[i]), 8);
+  return p.S[i] == 0 || p.units[i] == 0 ? 0 : 8 * p.blocks[i] * cdiv(p.wgs[i] * (p.units[i] / p.blocks[i]), 8);
 }
 
 bool mx(const rk_rows* r) { return r->format != RK_ROWS_PLAIN; }
