@@ -29,9 +29,10 @@ from rotatek_amd.quantized import BLOCK, MXRows, _format, append_rows, quantize_
 class _Layer:
     """One layer's rows: ``k`` / ``v`` prompt | text | free, ``ks`` / ``vs``
     visual.  ``lens[b]`` (device int32) counts prompt and text tokens, ``n`` is
-    the host's count of ``update``'s."""
+    the host's count of ``update``'s, ``ahead`` whether ``append_`` has moved the
+    lengths past it."""
 
-    __slots__ = ("k", "v", "ks", "vs", "lens", "s_prompt", "s_vision", "n")
+    __slots__ = ("k", "v", "ks", "vs", "lens", "s_prompt", "s_vision", "n", "ahead")
 
 
 class QuantizedCache(Cache):
@@ -66,7 +67,7 @@ class QuantizedCache(Cache):
             raise ValueError("value_states must hold the prompt, visual and text tokens")
         B, H, _, D = key_states_prompt.shape
         x = _Layer()
-        x.s_prompt, x.s_vision, x.n = s_p, s_v, s_t
+        x.s_prompt, x.s_vision, x.n, x.ahead = s_p, s_v, s_t, False
         dev, cap = key_states_prompt.device, s_p + s_t + self.reserve_tokens
         x.k, x.v = (MXRows.empty(B, H, cap, D, self.fmt, dev) for _ in range(2))
         x.lens = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -77,29 +78,34 @@ class QuantizedCache(Cache):
         self._layers.append(x)
 
     def _grow(self, x: _Layer, need: int) -> None:
-        rows = x.s_prompt + x.n
-        cap = x.s_prompt + max(2 * (x.k.shape[2] - x.s_prompt), need)
-        pad = -(-rows // BLOCK) * BLOCK
+        """Reallocate one layer at >= twice its text capacity.  Every row moves:
+        the device's lengths may be ahead of the host's count."""
+        rows = x.k.shape[2]
+        cap = x.s_prompt + max(2 * (rows - x.s_prompt), need)
         for name in ("k", "v"):
             old = getattr(x, name)
             new = MXRows.empty(*old.shape[:2], cap, old.head_dim, self.fmt, old.device)
-            new.codes[:, :, :rows].copy_(old.codes[:, :, :rows])
-            new.scales[..., :pad].copy_(old.scales[..., :pad])
+            new.codes[:, :, :rows].copy_(old.codes)
+            new.scales[..., :old.scales.shape[3]].copy_(old.scales)
             setattr(x, name, new)
 
     def reserve(self, tokens: int) -> None:
-        """Room for ``tokens`` more in every layer (before graph capture: the
-        rows may move)."""
+        """Room for ``tokens`` more in every layer, behind what ``append_`` and
+        replays have added (synchronises; before graph capture: the rows may
+        move)."""
+        self.sync_lengths()
         for x in self._layers:
             if x.s_prompt + x.n + tokens > x.k.shape[2]:
                 self._grow(x, x.n + tokens)
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
         """Append decode tokens [B, H_kv, T, D] to a layer, with room made for
-        them (the host counts along; after replays of ``append_`` call
-        ``sync_lengths`` first)."""
+        them (the host counts along; the first after an ``append_`` asks the
+        device; after replays of one call ``sync_lengths`` first)."""
         x = self._layers[layer_idx]
         steps = key_states.shape[-2]
+        if x.ahead:
+            self._sync(x)
         if x.s_prompt + x.n + steps > x.k.shape[2]:
             self._grow(x, x.n + steps)
         append_rows(key_states, value_states, x.k, x.v, x.lens)
@@ -109,13 +115,18 @@ class QuantizedCache(Cache):
         """Append on the device alone, at each request's own length; a full
         request drops the tokens."""
         x = self._layers[layer_idx]
+        x.ahead = True
         append_rows(key_states, value_states, x.k, x.v, x.lens)
 
+    def _sync(self, x: _Layer) -> None:
+        x.n = int(x.lens.max()) - x.s_prompt if x.lens.numel() else x.n
+        x.ahead = False
+
     def sync_lengths(self) -> None:
-        """The host's counts from the device's (one synchronisation); the
-        largest where requests differ."""
+        """The host's counts from the device's (synchronises); the largest where
+        requests differ."""
         for x in self._layers:
-            x.n = int(x.lens.max()) - x.s_prompt if x.lens.numel() else x.n
+            self._sync(x)
 
     def lengths(self, layer_idx: int) -> torch.Tensor:
         """Device int32 [B]: prompt + text tokens per request."""

@@ -1,0 +1,72 @@
+"""Rows of the quantised cache that move as it grows, with tokens that only the
+device has counted."""
+import numpy as np
+import pytest
+import torch
+
+import spans as sp
+from test_gpu_quantized_serving import _cache, _prefill, _q
+
+pytestmark = pytest.mark.gpu
+
+
+def _say(msg):
+    print(f"[case] {msg}", flush=True)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("mx8", torch.bfloat16), ("mx4", torch.float16)])
+@pytest.mark.parametrize("how", ["reserve", "update", "replays"])
+def test_growth_after_appends_of_the_device(fmt, dtype, how):
+    """Tokens of ``append_`` (eager, or replayed) that the host has not counted are
+    neither lost when the rows move nor in the way of those that follow."""
+    _say(f"{how} {fmt} {dtype}")
+    g = torch.Generator().manual_seed(41)
+    B, H, G, D, s_p, s_v, s_t = 2, 2, 4, 128, 21, 70, 5
+    x = _prefill(g, B, H, D, 32, s_p, s_v, s_t, dtype)
+    cache = _cache(x, fmt, 7)
+    k = np.concatenate([_q(x["prompt"], fmt), _q(x["text"], fmt)], 2)
+    v = np.concatenate([_q(x["V"][:, :, :s_p], fmt), _q(x["V"][:, :, s_p + s_v:], fmt)], 2)
+    vis = dict(k=_q(x["kp"], fmt), v=_q(x["V"][:, :, s_p:s_p + s_v], fmt), R=sp.np64(x["R"]), dm=sp.np64(x["dm"]))
+    new = lambda T: [sp.randn(g, B, H, T, D, dtype=dtype).cuda() for _ in range(2)]  # noqa: E731
+
+    def add(call, T=1):
+        nonlocal k, v
+        kn, vn = new(T)
+        call(kn, vn)
+        k, v = np.concatenate([k, _q(kn, fmt)], 2), np.concatenate([v, _q(vn, fmt)], 2)
+
+    def check():
+        q = sp.randn(g, B, H * G, D, dtype=dtype)
+        sp.check(cache.decode_rotatek(q.cuda(), 0, G)[0], q, G, [vis, dict(k=k, v=v)], fmt, dtype)
+        assert cache.lengths(0).tolist() == [k.shape[2]] * B
+
+    if how == "replays":
+        ks, vs = new(1)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            cache.append_(0, ks, vs)
+
+        def step(kn, vn):
+            ks.copy_(kn)
+            vs.copy_(vn)
+            graph.replay()
+    else:
+        step = lambda kn, vn: cache.append_(0, kn, vn)  # noqa: E731
+    for _ in range(6):      # 6 of the 7 free rows
+        add(step)
+    check()
+    if how == "replays":    # counted from the device, without growth
+        cache.reserve(1)
+        assert cache.get_seq_length() == s_v + k.shape[2]
+        add(lambda kn, vn: cache.update(kn, vn, 0))
+    elif how == "reserve":
+        cache.reserve(30)
+        check()
+        for _ in range(30):
+            add(step)
+    else:
+        add(lambda kn, vn: cache.update(kn, vn, 0), 9)
+        add(lambda kn, vn: cache.update(kn, vn, 0))
+        assert cache.get_seq_length() == s_v + k.shape[2]
+    check()
