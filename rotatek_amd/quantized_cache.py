@@ -13,7 +13,8 @@ and a decode step reads as much less.  No counterpart in the reference.
 
 ``append_`` and ``decode_rotatek`` work on the device alone (lengths are device
 tensors, shapes are fixed by the capacity), so a step may be captured in a HIP
-graph and replayed while the text grows; call ``reserve`` first.
+graph and replayed while the text grows; call ``reserve`` first (rows that a graph
+holds do not move, ``release_graphs``).
 """
 from __future__ import annotations
 
@@ -30,9 +31,9 @@ class _Layer:
     """One layer's rows: ``k`` / ``v`` prompt | text | free, ``ks`` / ``vs``
     visual.  ``lens[b]`` (device int32) counts prompt and text tokens, ``n`` is
     the host's count of ``update``'s, ``ahead`` whether ``append_`` has moved the
-    lengths past it."""
+    lengths past it, ``captured`` whether a graph holds the rows."""
 
-    __slots__ = ("k", "v", "ks", "vs", "lens", "s_prompt", "s_vision", "n", "ahead")
+    __slots__ = ("k", "v", "ks", "vs", "lens", "s_prompt", "s_vision", "n", "ahead", "captured")
 
 
 class QuantizedCache(Cache):
@@ -67,7 +68,7 @@ class QuantizedCache(Cache):
             raise ValueError("value_states must hold the prompt, visual and text tokens")
         B, H, _, D = key_states_prompt.shape
         x = _Layer()
-        x.s_prompt, x.s_vision, x.n, x.ahead = s_p, s_v, s_t, False
+        x.s_prompt, x.s_vision, x.n, x.ahead, x.captured = s_p, s_v, s_t, False, False
         dev, cap = key_states_prompt.device, s_p + s_t + self.reserve_tokens
         x.k, x.v = (MXRows.empty(B, H, cap, D, self.fmt, dev) for _ in range(2))
         x.lens = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -79,7 +80,12 @@ class QuantizedCache(Cache):
 
     def _grow(self, x: _Layer, need: int) -> None:
         """Reallocate one layer at >= twice its text capacity.  Every row moves:
-        the device's lengths may be ahead of the host's count."""
+        the device's lengths may be ahead of the host's count.  Refused while a
+        captured graph holds the rows: its replays would write to memory that is
+        free and count tokens that the new rows lack."""
+        if x.captured:
+            raise RuntimeError(f"{need} text rows are needed, but a captured graph holds the layer's rows; reserve() "
+                               "enough tokens before the capture, or release_graphs() when the graphs are gone")
         rows = x.k.shape[2]
         cap = x.s_prompt + max(2 * (rows - x.s_prompt), need)
         for name in ("k", "v"):
@@ -98,13 +104,26 @@ class QuantizedCache(Cache):
             if x.s_prompt + x.n + tokens > x.k.shape[2]:
                 self._grow(x, x.n + tokens)
 
+    def release_graphs(self) -> None:
+        """The graphs that were captured over this cache are gone, or will not be
+        replayed again: the rows may move."""
+        for x in self._layers:
+            x.captured = False
+
+    @staticmethod
+    def _held(x: _Layer) -> bool:
+        """Whether this call is being captured; the graph then holds the rows."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        x.captured |= capturing
+        return capturing
+
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
         """Append decode tokens [B, H_kv, T, D] to a layer, with room made for
-        them (the host counts along; the first after an ``append_`` asks the
-        device; after replays of one call ``sync_lengths`` first)."""
+        them.  The host counts along; the first after an ``append_``, and every one
+        while a captured graph holds the rows, asks the device."""
         x = self._layers[layer_idx]
         steps = key_states.shape[-2]
-        if x.ahead:
+        if not self._held(x) and (x.ahead or x.captured):
             self._sync(x)
         if x.s_prompt + x.n + steps > x.k.shape[2]:
             self._grow(x, x.n + steps)
@@ -115,8 +134,9 @@ class QuantizedCache(Cache):
         """Append on the device alone, at each request's own length; a full
         request drops the tokens."""
         x = self._layers[layer_idx]
-        x.ahead = True
         append_rows(key_states, value_states, x.k, x.v, x.lens)
+        x.ahead = True
+        self._held(x)
 
     def _sync(self, x: _Layer) -> None:
         x.n = int(x.lens.max()) - x.s_prompt if x.lens.numel() else x.n
@@ -152,6 +172,7 @@ class QuantizedCache(Cache):
         """RotateK decode over a layer's rows, ``(out [B, 1, H_q, D], None,
         None)`` like ``rotatek_decode``."""
         x = self._layers[layer_idx]
+        self._held(x)
         return rotatek_decode_quantized(q_full, self.rotatek_rotations[layer_idx], self.rotatek_means[layer_idx], x.k,
                                         x.v, None, x.ks, x.vs, num_kv_groups, len_full=x.lens, out=out)
 

@@ -70,3 +70,54 @@ def test_growth_after_appends_of_the_device(fmt, dtype, how):
         add(lambda kn, vn: cache.update(kn, vn, 0))
         assert cache.get_seq_length() == s_v + k.shape[2]
     check()
+
+
+@pytest.mark.parametrize("what", ["append", "decode"])
+def test_rows_that_a_graph_holds_stay_where_they_are(what):
+    """Growth under a captured graph is refused, nothing changed; with the graph
+    released the rows move and a new capture works on them."""
+    _say(f"held {what}")
+    g = torch.Generator().manual_seed(42)
+    B, H, G, D, dtype = 2, 2, 2, 128, torch.bfloat16
+    x = _prefill(g, B, H, D, 32, 9, 40, 3, dtype)
+    a, b = _cache(x, "mx8", 4), _cache(x, "mx8", 64)
+    q, kn, vn = (sp.randn(g, *s, dtype=dtype).cuda() for s in ((B, H * G, D), (B, H, 1, D), (B, H, 1, D)))
+
+    def capture():
+        a.decode_rotatek(q, 0, G)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            if what == "append":
+                a.append_(0, kn, vn)
+            out = a.decode_rotatek(q, 0, G)[0]
+        return graph, out
+
+    def step(graph, out):
+        kn.copy_(sp.randn(g, *kn.shape, dtype=dtype))
+        vn.copy_(sp.randn(g, *vn.shape, dtype=dtype))
+        if what == "decode":
+            a.append_(0, kn, vn)
+        graph.replay()
+        b.update(kn, vn, 0)
+        assert torch.equal(out, b.decode_rotatek(q, 0, G)[0])
+        assert torch.equal(a.lengths(0), b.lengths(0))
+
+    graph, out = capture()
+    for _ in range(3):
+        step(graph, out)
+    codes = a.spans(0)[0].codes
+    with pytest.raises(RuntimeError, match="graph"):
+        a.reserve(2)
+    with pytest.raises(RuntimeError, match="graph"):
+        a.update(kn.expand(B, H, 2, D), vn.expand(B, H, 2, D), 0)
+    assert a.spans(0)[0].codes.data_ptr() == codes.data_ptr()
+    assert torch.equal(a.lengths(0), b.lengths(0))
+    a.reserve(1)            # one row is free
+    step(graph, out)
+    del graph
+    a.release_graphs()
+    a.reserve(20)
+    graph, out = capture()
+    for _ in range(20):
+        step(graph, out)
