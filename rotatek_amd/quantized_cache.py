@@ -161,11 +161,23 @@ class QuantizedCache(Cache):
         return x.s_prompt + x.s_vision + x.n
 
     def spans(self, layer_idx: int):
-        """A layer's rows ``(k_full, v_full, k_sparse, v_sparse)``: of a batch of
-        one, what ``shared_prefix_decode`` takes as its shared spans (cut the
-        full ones to the length that is filled)."""
+        """A layer's rows ``(k_full, v_full, k_sparse, v_sparse)`` as they lie in
+        memory: the full ones to their capacity, undefined past ``lengths``."""
         x = self._layers[layer_idx]
         return x.k, x.v, x.ks, x.vs
+
+    def prefix(self, layer_idx: int):
+        """What ``shared_prefix_decode`` takes as its shared spans ``(k_prefix,
+        v_prefix, k_sparse, v_sparse)``: a batch of one's rows, the full ones cut
+        to the prompt and text they hold now (asks the device where the host has
+        not counted along).  Views: good until the rows move."""
+        x = self._layers[layer_idx]
+        if x.k.shape[0] != 1:
+            raise ValueError(f"a shared prefix is one request's, this layer holds {x.k.shape[0]}")
+        if not self._held(x) and (x.ahead or x.captured):
+            self._sync(x)
+        filled = x.s_prompt + x.n
+        return x.k.narrow(0, filled), x.v.narrow(0, filled), x.ks, x.vs
 
     def decode_rotatek(self, q_full: torch.Tensor, layer_idx: int, num_kv_groups: int,
                        out: Optional[torch.Tensor] = None):

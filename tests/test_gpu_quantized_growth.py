@@ -121,3 +121,36 @@ def test_rows_that_a_graph_holds_stay_where_they_are(what):
     graph, out = capture()
     for _ in range(20):
         step(graph, out)
+
+
+@pytest.mark.parametrize("fmt", ["mx8", "mx4"])
+def test_prefix_of_a_cache_with_room(fmt):
+    """The shared spans of a cache that has free rows, NaN codes in them: prompt
+    and text alone, as they grow."""
+    from rotatek_amd.kernels import shared_prefix_decode
+    _say(f"prefix {fmt}")
+    g = torch.Generator().manual_seed(43)
+    B, H, G, D, s_p, s_v, dtype = 6, 2, 4, 128, 30, 70, torch.bfloat16
+    x = _prefill(g, 1, H, D, 32, s_p, s_v, 3, dtype)
+    cache = _cache(x, fmt, 256)
+    for rows in cache.spans(0)[:2]:
+        rows.codes[:, :, s_p + 3:] = 0x7f
+        rows.scales[..., s_p + 3:] = 255
+    k = np.concatenate([_q(x["prompt"], fmt), _q(x["text"], fmt)], 2)
+    v = np.concatenate([_q(x["V"][:, :, :s_p], fmt), _q(x["V"][:, :, s_p + s_v:], fmt)], 2)
+    vis = dict(k=_q(x["kp"], fmt), v=_q(x["V"][:, :, s_p:s_p + s_v], fmt), R=sp.np64(x["R"]), dm=sp.np64(x["dm"]))
+    q = sp.randn(g, B, H * G, D, dtype=dtype)
+    for call in (None, lambda kn, vn: cache.update(kn, vn, 0), lambda kn, vn: cache.append_(0, kn, vn)):
+        if call is not None:
+            kn, vn = (sp.randn(g, 1, H, 5, D, dtype=dtype).cuda() for _ in range(2))
+            call(kn, vn)
+            k, v = np.concatenate([k, _q(kn, fmt)], 2), np.concatenate([v, _q(vn, fmt)], 2)
+        kp, vp, ks, vs = cache.prefix(0)
+        assert kp.shape == vp.shape == (1, H, k.shape[2], D)
+        out = shared_prefix_decode(q.cuda(), kp, vp, None, None, G, R_partial=x["R"], delta_mu=x["dm"], k_sparse=ks,
+                                   v_sparse=vs)
+        sp.check(out, q, G, [vis, dict(k=k, v=v)], fmt, dtype)
+    with pytest.raises(ValueError):
+        _cache(_prefill(g, 2, H, D, 32, s_p, s_v, 3, dtype), fmt, 0).prefix(0)
+    with pytest.raises(IndexError):
+        cache.prefix(1)
