@@ -50,14 +50,18 @@ int32_t dtype_code(at::ScalarType t) {
   }
 }
 
-int describe(const at::Tensor& t, int64_t device, rk_tensor* d) {
+// What a call writes is asked for as mutable: a tensor that shares its memory
+// until it is written (copy-on-write) gets its own then.
+enum Use { kRead, kWrite };
+
+int describe(const at::Tensor& t, int64_t device, rk_tensor* d, Use use) {
   if (!t.device().is_cuda() || t.get_device() != device) return kOtherDevice;
   const int64_t nd = t.dim();
   const int32_t code = dtype_code(t.scalar_type());
   if (nd > 4) return RK_ERR_RANK;
   if (code < 0) return RK_ERR_DTYPE;
   memset(d, 0, sizeof(*d));
-  d->data = t.numel() > 0 ? const_cast<void*>(t.const_data_ptr()) : nullptr;
+  d->data = t.numel() == 0 ? nullptr : use == kWrite ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
   d->dtype = code;
   d->ndim = (int32_t)nd;
   for (int64_t i = 0; i < nd; ++i) {
@@ -71,11 +75,11 @@ int describe(const at::Tensor& t, int64_t device, rk_tensor* d) {
 struct Arg {
   rk_tensor d;
   const rk_tensor* p = nullptr;
-  int set(PyObject* o, int64_t device) {
+  int set(PyObject* o, int64_t device, Use use = kRead) {
     if (o == Py_None) return RK_OK;
     if (!THPVariable_Check(o)) return RK_ERR_ARG;
     p = &d;
-    return describe(THPVariable_Unpack(o), device, &d);
+    return describe(THPVariable_Unpack(o), device, &d, use);
   }
 };
 
@@ -91,7 +95,7 @@ struct RowsArg {
   rk_rows d;
   const rk_rows* p = nullptr;
   // a Python error is left where MXRows' attributes are not what they should be
-  int set(PyObject* o, int64_t device) {
+  int set(PyObject* o, int64_t device, Use use = kRead) {
     if (o == Py_None) return RK_OK;
     p = &d;
     memset(&d, 0, sizeof(d));
@@ -99,7 +103,7 @@ struct RowsArg {
       const at::Tensor& t = THPVariable_Unpack(o);
       d.head_dim = t.dim() > 0 ? t.size(-1) : 0;
       d.format = RK_ROWS_PLAIN;
-      return describe(t, device, &d.data);
+      return describe(t, device, &d.data, use);
     }
     int st = RK_ERR_ARG;
     PyObject* codes = PyObject_GetAttr(o, g_codes);
@@ -109,14 +113,22 @@ struct RowsArg {
     if (fmt && THPVariable_Check(codes) && THPVariable_Check(scales) && PyUnicode_Check(fmt)) {
       d.head_dim = PyLong_AsLongLong(dim);
       d.format = format_of(fmt);
-      st = d.format < 0 ? RK_ERR_ARG : describe(THPVariable_Unpack(codes), device, &d.data);
-      if (st == RK_OK) st = describe(THPVariable_Unpack(scales), device, &d.scales);
+      st = d.format < 0 ? RK_ERR_ARG : describe(THPVariable_Unpack(codes), device, &d.data, use);
+      if (st == RK_OK) st = describe(THPVariable_Unpack(scales), device, &d.scales, use);
     }
     Py_XDECREF(codes);
     Py_XDECREF(scales);
     Py_XDECREF(dim);
     Py_XDECREF(fmt);
     return st;
+  }
+};
+
+// The call's GPU as the current one (a tensor elsewhere is refused later).
+struct OnDevice {
+  c10::OptionalDeviceGuard guard;
+  explicit OnDevice(const at::Tensor& t) {
+    if (t.device().is_cuda()) guard.reset_device(t.device());
   }
 };
 
@@ -148,11 +160,11 @@ PyObject* py_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t dev = t.get_device();
   Arg x;
   RowsArg r;
+  const OnDevice guard(t);
   int st = x.set(a[0], dev);
-  if (!st) st = r.set(a[1], dev);
+  if (!st) st = r.set(a[1], dev, kWrite);
   void* stream = stream_of(a[3]);
   if (st || PyErr_Occurred()) return status(st);
-  const c10::DeviceGuard guard(t.device());
   at::Tensor new_codes, new_scales;
   if (!r.p) {
     if (t.dim() != 4) return status(RK_ERR_RANK);
@@ -164,8 +176,8 @@ PyObject* py_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (D > 128) return status(RK_ERR_HEAD_DIM);
     new_codes = at::empty({t.size(0), t.size(1), S, (r.d.format == RK_ROWS_MX8 ? 32 : 16) * blocks}, on(t, at::kByte));
     new_scales = at::empty({t.size(0), t.size(1), blocks, (S + 31) / 32 * 32}, on(t, at::kByte));
-    st = describe(new_codes, dev, &r.d.data);
-    if (!st) st = describe(new_scales, dev, &r.d.scales);
+    st = describe(new_codes, dev, &r.d.data, kWrite);
+    if (!st) st = describe(new_scales, dev, &r.d.scales, kWrite);
     if (st) return status(st);
   }
   {
@@ -196,11 +208,11 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t dev = t.get_device();
   RowsArg r;
   Arg x;
+  const OnDevice guard(t);
   int st = r.set(a[0], dev);
-  if (!st) st = x.set(a[1], dev);
+  if (!st) st = x.set(a[1], dev, kWrite);
   void* stream = stream_of(a[3]);
   if (st || PyErr_Occurred()) return status(st);
-  const c10::DeviceGuard guard(t.device());
   at::Tensor out;
   if (!x.p) {
     if (!THPDtype_Check(a[2])) return status(RK_ERR_DTYPE);
@@ -208,7 +220,7 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (r.d.head_dim < 0) return status(RK_ERR_HEAD_DIM);
     out = at::empty({t.size(0), t.size(1), t.size(2), r.d.head_dim},
                     on(t, reinterpret_cast<THPDtype*>(a[2])->scalar_type));
-    st = describe(out, dev, &x.d);
+    st = describe(out, dev, &x.d, kWrite);
     if (st) return status(st);
   }
   {
@@ -221,7 +233,7 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // A contiguous int32 [B] on the device, or null for None.
-int lengths(PyObject* o, int64_t device, int64_t batch, const int32_t** p) {
+int lengths(PyObject* o, int64_t device, int64_t batch, const int32_t** p, Use use = kRead) {
   *p = nullptr;
   if (o == Py_None) return RK_OK;
   if (!THPVariable_Check(o)) return RK_ERR_ARG;
@@ -229,7 +241,7 @@ int lengths(PyObject* o, int64_t device, int64_t batch, const int32_t** p) {
   if (!t.device().is_cuda() || t.get_device() != device) return kOtherDevice;
   if (t.scalar_type() != at::kInt) return RK_ERR_DTYPE;
   if (t.dim() != 1 || t.size(0) != batch || !t.is_contiguous()) return RK_ERR_SHAPE;
-  *p = static_cast<const int32_t*>(t.const_data_ptr());
+  *p = static_cast<const int32_t*>(use == kWrite ? t.mutable_data_ptr() : t.const_data_ptr());
   return RK_OK;
 }
 
@@ -243,16 +255,16 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Arg k, v;
   RowsArg kr, vr;
   const int32_t* lens = nullptr;
-  int st = k.set(a[0], dev);
-  if (!st) st = v.set(a[1], dev);
-  if (!st) st = kr.set(a[2], dev);
-  if (!st) st = vr.set(a[3], dev);
-  if (!st) st = lengths(a[4], dev, t.dim() > 0 ? t.size(0) : 0, &lens);
-  if (st) return status(st);
   const int advance = PyObject_IsTrue(a[5]);
   if (advance < 0) return nullptr;
+  const OnDevice guard(t);
+  int st = k.set(a[0], dev);
+  if (!st) st = v.set(a[1], dev);
+  if (!st) st = kr.set(a[2], dev, kWrite);
+  if (!st) st = vr.set(a[3], dev, kWrite);
+  if (!st) st = lengths(a[4], dev, t.dim() > 0 ? t.size(0) : 0, &lens, advance ? kWrite : kRead);
+  if (st) return status(st);
   void* stream = stream_of(a[6]);
-  const c10::DeviceGuard guard(t.device());
   {
     const Unlocked unlocked;
     st = g_entry.append(k.p, v.p, kr.p, vr.p, const_cast<int32_t*>(lens), advance, stream);
@@ -273,6 +285,7 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Arg dq, dR, dmu, dmask, dout;
   RowsArg r[6];
   const int32_t* lens = nullptr;
+  const OnDevice guard(q);
   int st = dq.set(a[1], dev);
   if (!st) st = dR.set(a[2], dev);
   if (!st) st = dmu.set(a[3], dev);
@@ -284,12 +297,11 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t groups = PyLong_AsLongLong(a[12]);
   void* stream = stream_of(a[14]);
   if (PyErr_Occurred()) return nullptr;
-  const c10::DeviceGuard guard(q.device());
   at::Tensor out;
   if (a[13] == Py_None) {
     out = at::empty({q.size(0), 1, q.size(1), q.size(2)}, on(q, q.scalar_type()));
     dout.p = &dout.d;
-    st = describe(out, dev, &dout.d);
+    st = describe(out, dev, &dout.d, kWrite);
     dout.d.ndim = 3;
     for (int i = 1; i < 3; ++i) {
       dout.d.shape[i] = out.size(i + 1);
@@ -297,7 +309,7 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     dout.d.shape[3] = dout.d.stride[3] = 0;
   } else {
-    st = dout.set(a[13], dev);
+    st = dout.set(a[13], dev, kWrite);
     if (!st) out = THPVariable_Unpack(a[13]).unsqueeze(1);
   }
   if (st) return status(st);
