@@ -377,8 +377,9 @@ int make_plan(const Call& c, int cus, Plan* out) {
   // 8-bit rows: 436, 431, 436).  Over 64 queries a workgroup's
   // records weigh as much as 64 tokens' rows and the join reads them again: two
   // there where three would leave it less than 768 tokens (32 requests of 4 heads
-  // behind 16001: 35 us at two, 512 tokens, 38 at three; 64 of 7 heads behind
-  // 32768: 81 at two, 73 at three).
+  // behind 16001: 35 us at two, chunks of 512 tokens, 38 at three, of 384; 64 of 7
+  // heads behind 32768: 81 at two, 73 at three, of 1200; between them nothing was
+  // measured).
   split((int64_t)cus * 3);
   if (p.tile && std::max(p.chunk[kRotated], p.chunk[kFull]) < 768) split((int64_t)cus * 2);
   if (p.join) {

@@ -5,7 +5,8 @@
 //   s_rt = (k_t . q_r + bias_r) log2(e) / sqrt(D),  o_r = sum_t 2^s_rt v_t,
 //   l_r = sum_t 2^s_rt,  all under a running maximum m_r;
 // a workgroup covers one chunk of one span for one unit of query rows and
-// leaves (m, l, o) for each row; merge_rows joins a row's records.
+// leaves (m, l, o) for each row: a record.  span_merge_kernel joins a row's records,
+// or, behind tiles, the launch that attends the suffix.
 //
 // Units.  A unit is up to 16 query rows that read the same K and V: of the heads
 // of a KV group, or, over a span that the batch shares, of all the batch's
@@ -24,9 +25,10 @@
 //                 loads them and transposes them in registers.  P^T is the
 //                 lane's own eight scores: lane (g, n) gets tokens 4g .. 4g + 3
 //                 and 16 + 4g .. 16 + 4g + 3 of query n.
-// Quantised rows are widened to bf16, which holds code 2^e exactly, by the
-// conversion that applies the block's scale; queries then enter as one, two
-// or three bf16 terms, in which bf16, fp16 and fp32 are exact.
+// Quantised rows are widened to bf16 by the conversion that applies the block's
+// scale; queries then enter as one, two or three bf16 terms, in which bf16, fp16
+// and fp32 are exact.  bf16 holds code 2^e exactly, but for 8-bit blocks whose
+// largest value is below 2^-116: their smallest codes lie under bf16's least step.
 //
 // Loads run ahead of the products: the K registers are reloaded with the
 // wave's next block as soon as the scores are formed, the V registers as soon
@@ -50,8 +52,7 @@
 namespace rk {
 
 // ------------------------------------------------------------ row formats
-// kw: 32-bit words of eight channels.  piece(g, j): first channel of the
-// lane's j-th eight of a score row of KB blocks.
+// kw: 32-bit words of eight channels.
 template <class TT_>
 struct PlainFmt {
   using TT = TT_;
@@ -125,7 +126,11 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* p) {
 }
 // AUX 2: non-temporal, for rows that one instruction reads whole lines of (447
 // against 451 us over 2.9 GB of 8-bit rows; the half lines of 4-bit rows came from
-// memory twice, so those go through the caches).
+// memory twice, so those go through the caches).  The rule is the format's alone.
+// Where several row blocks read the same rows it goes either way; us, with and
+// without: bf16, one block, 8 heads behind 32768 rows 29.8 and 35.5; two blocks 38.1
+// and 40.7, of 4 heads behind 16384 17.9 and 16.6; 8-bit, four blocks, 8 heads behind
+// 65536 71.8 and 68.5.
 template <int N, int AUX = 0>
 __device__ __forceinline__ void load_words(Rsrc r, uint32_t off, uint32_t base, uint32_t* w) {
   if constexpr (N == 4) {

@@ -19,10 +19,13 @@
 // for three workgroups on a CU, which hide each other's barriers and latencies:
 // 32 queries a wave, two buffers, or two tiles ahead (two workgroups each) took 6,
 // 17 and 16 % longer, both halves of a tile in one softmax (spills) 2 to 14 %,
-// eight waves that take half a tile each 10 %.
+// eight waves that take half a tile each 10 %.  With more than 64 kept channels the
+// rotation's staging (85 KB) leaves one workgroup on a CU, for the full-width span
+// as well: 64 fp16 requests of 7 heads behind 32768 tokens take 74 us with 64
+// channels kept, 154 with 128, and 82 without a rotation.
 //
 // What bounds it: issue.  64 requests of 7 heads behind 32768 tokens, 64 channels
-// kept: 71 us with the join (11), 324 TFLOP/s of the formula; a wave issues 26
+// kept: 70 to 74 us with the join (11), 320 TFLOP/s of the formula; a wave issues 26
 // matrix and 90 other vector instructions for 32 tokens and reads 24 KB of a tile's
 // LDS for 64; the matrix pipes are busy for 47 % of the loop, LDS for about as much,
 // and waves wait for their turn for 42 % of their time.  32

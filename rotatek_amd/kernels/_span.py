@@ -8,7 +8,8 @@ from rotatek_amd.quantized import MXRows, check_lens, refused
 
 
 def rows_of(x):
-    """rk_rows descriptor of MXRows or of a plain [B, H, S, D] tensor."""
+    """rk_rows descriptor of MXRows or of a plain [B, H, S, D] tensor, for callers of
+    the C entries (``launch`` forms its own in C++)."""
     if x is None:
         return None
     if isinstance(x, MXRows):

@@ -3,9 +3,11 @@
 The attention of ``rotatek_decode`` and ``full_channel_decode`` straight from
 8- or 4-bit rows: nothing is widened in memory.  No counterpart in the
 reference.  Queries enter the products exactly (as two bf16 terms, three for
-fp32), code times scale is exact in bf16, and sums are fp32, so the result
-differs from the same attention over the dequantised rows only by fp32
-summation and the output's rounding.
+fp32; a rotated query is q R rounded to as many), code times scale is exact in
+bf16 (8-bit blocks below 2^-116 excepted), weights are two or three bf16
+terms, and sums are fp32, so the result differs from the same attention over
+the dequantised rows by those roundings, at most 2^-16 of a weight, and the
+output's.
 """
 from __future__ import annotations
 

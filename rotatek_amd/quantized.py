@@ -91,7 +91,7 @@ class MXRows:
         return MXRows(self.codes.narrow(0, start, count), self.scales.narrow(0, start, count), self.head_dim, self.fmt)
 
     def desc(self):
-        """rk_rows of these rows."""
+        """rk_rows of these rows, for callers of the C entries."""
         return _lib.rows_desc(self.codes, self.scales, self.head_dim, FORMATS[self.fmt])
 
     def __repr__(self) -> str:
