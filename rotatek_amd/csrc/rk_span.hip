@@ -272,7 +272,7 @@ int make_plan(const Call& c, int cus, Plan* out) {
   if (c.groups <= 0) return RK_ERR_ARG;
   p.G = c.groups;
   p.H = c.k[kFull]->data.ndim == 4 ? c.k[kFull]->data.shape[1] : 0;
-  if (p.H <= 0 || p.Hq != p.H * p.G) return RK_ERR_HEADS;
+  if (p.H <= 0 || p.G > p.Hq || p.Hq % p.G != 0 || p.H != p.Hq / p.G) return RK_ERR_HEADS;
   p.format = c.k[kFull]->format;
   if (p.format != RK_ROWS_PLAIN && p.format != RK_ROWS_MX8 && p.format != RK_ROWS_MX4) return RK_ERR_ARG;
   const bool quantised = p.format != RK_ROWS_PLAIN;
