@@ -121,7 +121,8 @@ def refused(what: str, status: int, index: int, *tensors) -> None:
 
 
 def check_lens(lens: torch.Tensor, batch: int, name: str) -> None:
-    if not isinstance(lens, torch.Tensor) or lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != batch or not lens.is_contiguous():
+    if (not isinstance(lens, torch.Tensor) or lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != batch
+            or not lens.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 tensor [B]")
 
 
