@@ -599,6 +599,74 @@ int rk_shared_prefix_decode(const rk_tensor* q, const rk_tensor* R_partial, cons
                             const int32_t* len_suffix, int64_t num_kv_groups, const rk_tensor* out,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- a paged KV cache (no counterpart in the reference, whose caches are one
+ * tensor a layer).
+ *
+ * Rotation by position, of up to four axes (time, height, width): pair i of a
+ * head is its channels i and i + P, P entries of inv_freq F32 [P] (2 P <= D),
+ *   a = position[axis(i)] inv_freq[i]
+ *   out_i = x_i cos a - x_(i+P) sin a,  out_(i+P) = x_(i+P) cos a + x_i sin a
+ * (inverse = 1: by -a, which is also the gradient's way); channels from 2 P on
+ * are copied.  sections[axes] counts the pairs of each axis, in all P: one axis
+ * after the other, or with interleaved = 1 dealt in turn to the axes that have
+ * pairs left.  Angles are formed in 64 bits, values rounded once.
+ * q [B,Hq,T,D], k [B,Hkv,T,D] (or NULL), positions [axes,B,T]; or q [N,Hq,D],
+ * k [N,Hkv,D], positions [axes,N].  F16, BF16 or F32 alike; positions I32 or
+ * I64; any strides, and an output may be its input itself (not a view of it
+ * that lies otherwise). */
+int rk_rotary(const rk_tensor* q, const rk_tensor* k, const rk_tensor* positions, const rk_tensor* inv_freq,
+              const int32_t* sections, int32_t axes, int32_t interleaved, int32_t inverse, const rk_tensor* q_out,
+              const rk_tensor* k_out, void* stream);
+
+/* Pages.  Token t of request b is row t % page of page table[b][t / page];
+ * page a power of two from 8 on.  lens[b] counts the request's tokens, new ones
+ * among them (as far as the table reaches; none below zero).  A page number
+ * outside the pool is no page: what would go there is dropped, and its tokens
+ * count for nothing.  Entries past a request's last token are not read. */
+typedef struct rk_pages {
+  rk_tensor k, v;      /* [pages,H_kv,page,D] */
+  rk_tensor table;     /* I32 [B,per], unit last stride */
+  const int32_t* lens; /* device [B] */
+} rk_pages;
+
+/* Append: new Keys are rotated (positions NULL: copied) into the pages, Values
+ * copied, and q (or NULL) rotated into q_out in the same launch.
+ * k_new, v_new [N,H_kv,D], q [N,Hq,D], positions [axes,N]: request b's new
+ * tokens are starts[b] .. starts[b+1] - 1 (device int32 [B+1], ascending), or
+ * with starts NULL token b (N = B); or k_new, v_new [B,H_kv,T,D] and so on, T
+ * new tokens each, starts NULL.  Request b's i-th of n goes to position
+ * lens[b] - n + i; positions below zero or past the table are dropped, and no
+ * other row changes.  Pages in the tensors' type, any strides. */
+int rk_paged_append(const rk_tensor* k_new, const rk_tensor* v_new, const rk_pages* pages, const int32_t* starts,
+                    const rk_tensor* q, const rk_tensor* q_out, const rk_tensor* positions,
+                    const rk_tensor* inv_freq, const int32_t* sections, int32_t axes, int32_t interleaved,
+                    void* stream);
+
+/* Attention of new tokens over pages.  Request b's i-th new token of n stands
+ * at position p = lens[b] - n + i and sees the tokens j <= p with j > p - window
+ * (window 0: all of them) or j < sinks:
+ *   out = sum w v / sum w,  w = exp(q . k / sqrt(D) - max),  0 where it sees none
+ * q, out [B,Hq,D] with starts NULL (one new token each: decode), or [N,Hq,D]
+ * with starts as above (rows that no request has stay as they are).  F16 or
+ * BF16 alike; D a multiple of 8, up to 128; pages with unit last stride, other
+ * strides multiples of 8 and a 16-byte aligned base (RK_ERR_STRIDE); q and out
+ * any strides.  Workspace and capture as for the quantised decode. */
+int rk_paged_attention_check(const rk_tensor* q, const int32_t* starts, const rk_pages* pages,
+                             int64_t num_kv_groups, int64_t window, int64_t sinks, const rk_tensor* out,
+                             int32_t num_cus, size_t* workspace_bytes);
+int rk_paged_attention(const rk_tensor* q, const int32_t* starts, const rk_pages* pages, int64_t num_kv_groups,
+                       int64_t window, int64_t sinks, const rk_tensor* out, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* The same over plain rows k, v [B,H_kv,S,D] of which the first lens[b] (device
+ * int32 [B] or NULL: all) are there; q, out [B,Hq,T,D], the last T of them. */
+int rk_window_attention_check(const rk_tensor* q, const rk_tensor* k, const rk_tensor* v, const int32_t* lens,
+                              int64_t num_kv_groups, int64_t window, int64_t sinks, const rk_tensor* out,
+                              int32_t num_cus, size_t* workspace_bytes);
+int rk_window_attention(const rk_tensor* q, const rk_tensor* k, const rk_tensor* v, const int32_t* lens,
+                        int64_t num_kv_groups, int64_t window, int64_t sinks, const rk_tensor* out,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

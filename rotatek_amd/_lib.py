@@ -60,6 +60,15 @@ class RkRows(ctypes.Structure):
     ]
 
 
+class RkPages(ctypes.Structure):
+    _fields_ = [
+        ("k", RkTensor),
+        ("v", RkTensor),
+        ("table", RkTensor),
+        ("lens", ctypes.c_void_p),
+    ]
+
+
 class RkDecodePlan(ctypes.Structure):
     _fields_ = [
         ("units", ctypes.c_int64),
@@ -154,6 +163,16 @@ _SIGNATURES = {
                                                      ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
     "rk_shared_prefix_decode": (ctypes.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_int64, _V, _V,
                                                ctypes.c_size_t, _V]),
+    "rk_rotary": (ctypes.c_int, [_V, _V, _V, _V, _V, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _V, _V, _V]),
+    "rk_paged_append": (ctypes.c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_int32, ctypes.c_int32, _V]),
+    "rk_paged_attention_check": (ctypes.c_int, [_V, _V, _V, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _V,
+                                                ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
+    "rk_paged_attention": (ctypes.c_int, [_V, _V, _V, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _V, _V,
+                                          ctypes.c_size_t, _V]),
+    "rk_window_attention_check": (ctypes.c_int, [_V, _V, _V, _V, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _V,
+                                                 ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
+    "rk_window_attention": (ctypes.c_int, [_V, _V, _V, _V, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _V, _V,
+                                           ctypes.c_size_t, _V]),
 }
 
 _lib = None
@@ -192,11 +211,12 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 _bind = None
 _BOUND = ("rk_mx_write", "rk_mx_read", "rk_mx_append", "rk_quantized_decode_check", "rk_quantized_decode",
-          "rk_shared_prefix_decode_check", "rk_shared_prefix_decode")
+          "rk_shared_prefix_decode_check", "rk_shared_prefix_decode", "rk_rotary", "rk_paged_append",
+          "rk_paged_attention_check", "rk_paged_attention", "rk_window_attention_check", "rk_window_attention")
 
 
 def bind():
-    """The C++ host path of the quantised and shared-prefix calls (``_bind``,
+    """The C++ host path of the quantised, shared-prefix and paged calls (``_bind``,
     csrc/rk_bind.cpp), over the library that ``load`` gave."""
     global _bind
     if _bind is None:

@@ -1,4 +1,4 @@
-// rk_bind.cpp -- host path of the quantised and shared-prefix calls: torch
+// rk_bind.cpp -- host path of the quantised, shared-prefix and paged calls: torch
 // tensors to rk_tensor descriptors, output and workspace from torch's allocator,
 // and the library's entry point, in one C++ call from Python.
 //
@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -23,6 +24,7 @@
 namespace {
 
 constexpr int kOtherDevice = -1000;  // a tensor is not on the call's GPU: the caller words the error
+constexpr int kNeedsGrad = -1001;    // a gradient is asked of a call that has none
 
 struct Entries {
   decltype(&rk_mx_write) write;
@@ -32,6 +34,12 @@ struct Entries {
   decltype(&rk_quantized_decode) decode;
   decltype(&rk_shared_prefix_decode_check) shared_check;
   decltype(&rk_shared_prefix_decode) shared;
+  decltype(&rk_rotary) rotary;
+  decltype(&rk_paged_append) paged_append;
+  decltype(&rk_paged_attention_check) paged_check;
+  decltype(&rk_paged_attention) paged;
+  decltype(&rk_window_attention_check) window_check;
+  decltype(&rk_window_attention) window;
 } g_entry;
 
 PyObject *g_codes, *g_scales, *g_head_dim, *g_fmt;  // attribute names of MXRows
@@ -333,11 +341,231 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// init(write, read, append, decode_check, decode, shared_check, shared): addresses
+// ---- paged cache
+
+// Whether autograd would record one of these.
+template <class... T>
+bool needs_grad(T... o) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (PyObject* x : {o...})
+    if (THPVariable_Check(x) && THPVariable_Unpack(x).requires_grad()) return true;
+  return false;
+}
+
+// A new tensor like t, and its descriptor.
+int make_like(const at::Tensor& t, int64_t device, at::Tensor* out, Arg* d) {
+  *out = at::empty(t.sizes(), on(t, t.scalar_type()));
+  d->p = &d->d;
+  return describe(*out, device, &d->d, kWrite);
+}
+
+// Pairs of each axis, a sequence of integers, or None: one axis of them all.
+struct Sections {
+  int32_t n[4];
+  int32_t axes = 0;
+  int set(PyObject* o, int64_t pairs) {
+    if (o == Py_None) {
+      axes = 1;
+      n[0] = (int32_t)(pairs < 0 || pairs > 1024 ? 0 : pairs);
+      return RK_OK;
+    }
+    PyObject* seq = PySequence_Fast(o, "sections must be a sequence of integers");
+    if (!seq) return RK_ERR_ARG;
+    const Py_ssize_t size = PySequence_Fast_GET_SIZE(seq);
+    int st = size < 1 || size > 4 ? RK_ERR_ARG : RK_OK;
+    for (Py_ssize_t i = 0; i < size && !st; ++i) {
+      const long long x = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq, i));
+      if (x < 0 || x > 1024) st = RK_ERR_ARG;
+      n[i] = (int32_t)x;
+    }
+    axes = (int32_t)size;
+    Py_DECREF(seq);
+    return st;
+  }
+};
+
+// rotary(q, k, positions, inv_freq, sections, interleaved, inverse, q_out,
+// k_out, stream): (q_out, k_out), or a status
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!counts("rotary", n, 10)) return nullptr;
+  if (!THPVariable_Check(a[0])) return status(RK_ERR_ARG);
+  if (needs_grad(a[0], a[1], a[3])) return status(kNeedsGrad);
+  const at::Tensor& t = THPVariable_Unpack(a[0]);
+  const int64_t dev = t.get_device();
+  Arg q, k, pos, freq, qo, ko;
+  Sections sections;
+  const int interleaved = PyObject_IsTrue(a[5]), inverse = PyObject_IsTrue(a[6]);
+  if (interleaved < 0 || inverse < 0) return nullptr;
+  const OnDevice guard(t);
+  int st = q.set(a[0], dev);
+  if (!st) st = k.set(a[1], dev);
+  if (!st) st = pos.set(a[2], dev);
+  if (!st) st = freq.set(a[3], dev);
+  if (!st) st = sections.set(a[4], freq.p && freq.d.ndim == 1 ? freq.d.shape[0] : 0);
+  if (!st) st = qo.set(a[7], dev, kWrite);
+  if (!st) st = ko.set(a[8], dev, kWrite);
+  void* stream = stream_of(a[9]);
+  if (st || PyErr_Occurred()) return status(st);
+  at::Tensor new_q, new_k;
+  if (!qo.p) st = make_like(t, dev, &new_q, &qo);
+  if (!st && k.p && !ko.p) st = make_like(THPVariable_Unpack(a[1]), dev, &new_k, &ko);
+  if (st) return status(st);
+  {
+    const Unlocked unlocked;
+    st = g_entry.rotary(q.p, k.p, pos.p, freq.p, sections.n, sections.axes, interleaved, inverse, qo.p, ko.p, stream);
+  }
+  if (st) return status(st);
+  PyObject* x = new_q.defined() ? THPVariable_Wrap(new_q) : Py_NewRef(a[7]);
+  PyObject* y = !x ? nullptr : new_k.defined() ? THPVariable_Wrap(new_k) : Py_NewRef(a[8]);
+  PyObject* pair = y ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+// Pages, their table and lengths, of the call's device.
+struct PagesArg {
+  rk_pages d;
+  int64_t requests = 0;
+  int set(PyObject* k, PyObject* v, PyObject* table, PyObject* lens, int64_t device, Use use = kRead) {
+    memset(&d, 0, sizeof(d));
+    if (!THPVariable_Check(k) || !THPVariable_Check(v) || !THPVariable_Check(table) || !THPVariable_Check(lens))
+      return RK_ERR_ARG;
+    const at::Tensor& t = THPVariable_Unpack(table);
+    int st = describe(THPVariable_Unpack(k), device, &d.k, use);
+    if (!st) st = describe(THPVariable_Unpack(v), device, &d.v, use);
+    if (!st) st = describe(t, device, &d.table, kRead);
+    requests = t.dim() > 0 ? t.size(0) : 0;
+    return st ? st : lengths(lens, device, requests, &d.lens);
+  }
+};
+
+// paged_append(k_new, v_new, k_pages, v_pages, table, lens, starts, q, q_out,
+// positions, inv_freq, sections, interleaved, stream): q_out or None, or a status
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!counts("paged_append", n, 14)) return nullptr;
+  if (!THPVariable_Check(a[0])) return status(RK_ERR_ARG);
+  if (needs_grad(a[0], a[1], a[2], a[3], a[7], a[10])) return status(kNeedsGrad);
+  const at::Tensor& t = THPVariable_Unpack(a[0]);
+  const int64_t dev = t.get_device();
+  Arg k, v, q, qo, pos, freq;
+  PagesArg pages;
+  Sections sections;
+  const int32_t* starts = nullptr;
+  const int interleaved = PyObject_IsTrue(a[12]);
+  if (interleaved < 0) return nullptr;
+  const OnDevice guard(t);
+  int st = k.set(a[0], dev);
+  if (!st) st = v.set(a[1], dev);
+  if (!st) st = pages.set(a[2], a[3], a[4], a[5], dev, kWrite);
+  if (!st) st = lengths(a[6], dev, pages.requests + 1, &starts);
+  if (!st) st = q.set(a[7], dev);
+  if (!st) st = qo.set(a[8], dev, kWrite);
+  if (!st) st = pos.set(a[9], dev);
+  if (!st) st = freq.set(a[10], dev);
+  if (!st && pos.p) st = sections.set(a[11], freq.p && freq.d.ndim == 1 ? freq.d.shape[0] : 0);
+  void* stream = stream_of(a[13]);
+  if (st || PyErr_Occurred()) return status(st);
+  at::Tensor new_q;
+  if (q.p && !qo.p) st = make_like(THPVariable_Unpack(a[7]), dev, &new_q, &qo);
+  if (st) return status(st);
+  {
+    const Unlocked unlocked;
+    st = g_entry.paged_append(k.p, v.p, &pages.d, starts, q.p, qo.p, pos.p, freq.p, sections.n, sections.axes,
+                              interleaved, stream);
+  }
+  if (st) return status(st);
+  return new_q.defined() ? THPVariable_Wrap(new_q) : Py_NewRef(a[8]);
+  END_HANDLE_TH_ERRORS
+}
+
+// Output, workspace and launch of an attention call: `out` or a status.
+template <class Check, class Launch>
+PyObject* attend(PyObject* out_arg, const at::Tensor& q, int64_t dev, Check check, Launch launch) {
+  Arg out;
+  at::Tensor made;
+  int st = out.set(out_arg, dev, kWrite);
+  if (!st && !out.p) st = make_like(q, dev, &made, &out);
+  if (st) return status(st);
+  size_t bytes = 0;
+  if ((st = check(out.p, &bytes))) return status(st);
+  // the call's own: torch's allocator hands it on in the stream's order
+  const at::Tensor ws = at::empty({(int64_t)(bytes > 0 ? bytes : 256)}, on(q, at::kByte));
+  {
+    const Unlocked unlocked;
+    st = launch(out.p, ws.data_ptr(), (size_t)ws.numel());
+  }
+  if (st) return status(st);
+  return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(out_arg);
+}
+
+// paged_attention(q, starts, k_pages, v_pages, table, lens, groups, window,
+// sinks, out, stream): out, or a status
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!counts("paged_attention", n, 11)) return nullptr;
+  if (!THPVariable_Check(a[0])) return status(RK_ERR_ARG);
+  if (needs_grad(a[0], a[2], a[3])) return status(kNeedsGrad);
+  const at::Tensor& t = THPVariable_Unpack(a[0]);
+  const int64_t dev = t.get_device();
+  Arg q;
+  PagesArg pages;
+  const int32_t* starts = nullptr;
+  const OnDevice guard(t);
+  int st = q.set(a[0], dev);
+  if (!st) st = pages.set(a[2], a[3], a[4], a[5], dev);
+  if (!st) st = lengths(a[1], dev, pages.requests + 1, &starts);
+  const int64_t groups = PyLong_AsLongLong(a[6]), window = PyLong_AsLongLong(a[7]), sinks = PyLong_AsLongLong(a[8]);
+  void* stream = stream_of(a[10]);
+  if (st || PyErr_Occurred()) return status(st);
+  return attend(
+      a[9], t, dev,
+      [&](const rk_tensor* out, size_t* bytes) {
+        return g_entry.paged_check(q.p, starts, &pages.d, groups, window, sinks, out, 0, bytes);
+      },
+      [&](const rk_tensor* out, void* ws, size_t bytes) {
+        return g_entry.paged(q.p, starts, &pages.d, groups, window, sinks, out, ws, bytes, stream);
+      });
+  END_HANDLE_TH_ERRORS
+}
+
+// window_attention(q, k, v, lens, groups, window, sinks, out, stream): out, or a status
+PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!counts("window_attention", n, 9)) return nullptr;
+  if (!THPVariable_Check(a[0])) return status(RK_ERR_ARG);
+  if (needs_grad(a[0], a[1], a[2])) return status(kNeedsGrad);
+  const at::Tensor& t = THPVariable_Unpack(a[0]);
+  const int64_t dev = t.get_device();
+  Arg q, k, v;
+  const int32_t* lens = nullptr;
+  const OnDevice guard(t);
+  int st = q.set(a[0], dev);
+  if (!st) st = k.set(a[1], dev);
+  if (!st) st = v.set(a[2], dev);
+  if (!st) st = lengths(a[3], dev, t.dim() > 0 ? t.size(0) : 0, &lens);
+  const int64_t groups = PyLong_AsLongLong(a[4]), window = PyLong_AsLongLong(a[5]), sinks = PyLong_AsLongLong(a[6]);
+  void* stream = stream_of(a[8]);
+  if (st || PyErr_Occurred()) return status(st);
+  return attend(
+      a[7], t, dev,
+      [&](const rk_tensor* out, size_t* bytes) {
+        return g_entry.window_check(q.p, k.p, v.p, lens, groups, window, sinks, out, 0, bytes);
+      },
+      [&](const rk_tensor* out, void* ws, size_t bytes) {
+        return g_entry.window(q.p, k.p, v.p, lens, groups, window, sinks, out, ws, bytes, stream);
+      });
+  END_HANDLE_TH_ERRORS
+}
+
+// init(the entries of `Entries` in its order): addresses
 PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!counts("init", n, 7)) return nullptr;
-  void* p[7];
-  for (int i = 0; i < 7; ++i) {
+  if (!counts("init", n, 13)) return nullptr;
+  void* p[13];
+  for (int i = 0; i < 13; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
   }
@@ -348,13 +576,21 @@ PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_entry.decode = reinterpret_cast<decltype(g_entry.decode)>(p[4]);
   g_entry.shared_check = reinterpret_cast<decltype(g_entry.shared_check)>(p[5]);
   g_entry.shared = reinterpret_cast<decltype(g_entry.shared)>(p[6]);
+  g_entry.rotary = reinterpret_cast<decltype(g_entry.rotary)>(p[7]);
+  g_entry.paged_append = reinterpret_cast<decltype(g_entry.paged_append)>(p[8]);
+  g_entry.paged_check = reinterpret_cast<decltype(g_entry.paged_check)>(p[9]);
+  g_entry.paged = reinterpret_cast<decltype(g_entry.paged)>(p[10]);
+  g_entry.window_check = reinterpret_cast<decltype(g_entry.window_check)>(p[11]);
+  g_entry.window = reinterpret_cast<decltype(g_entry.window)>(p[12]);
   Py_RETURN_NONE;
 }
 
 #define RK_METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {RK_METHOD(init),   RK_METHOD(write),  RK_METHOD(read),
-                           RK_METHOD(append), RK_METHOD(decode), {nullptr, nullptr, 0, nullptr}};
+                           RK_METHOD(append), RK_METHOD(decode), RK_METHOD(rotary),
+                           RK_METHOD(paged_append), RK_METHOD(paged_attention), RK_METHOD(window_attention),
+                           {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -366,7 +602,8 @@ PyMODINIT_FUNC PyInit__bind(void) {
   g_head_dim = PyUnicode_InternFromString("head_dim");
   g_fmt = PyUnicode_InternFromString("fmt");
   PyObject* m = PyModule_Create(&g_module);
-  if (m && PyModule_AddIntConstant(m, "OTHER_DEVICE", kOtherDevice) < 0) {
+  if (m && (PyModule_AddIntConstant(m, "OTHER_DEVICE", kOtherDevice) < 0 ||
+            PyModule_AddIntConstant(m, "NEEDS_GRAD", kNeedsGrad) < 0)) {
     Py_DECREF(m);
     return nullptr;
   }

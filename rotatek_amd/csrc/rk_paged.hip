@@ -1,0 +1,523 @@
+// rk_paged.hip -- attention of new tokens over a paged KV cache or plain rows
+// on MI355X (gfx950): the host code of rk_paged_attention and
+// rk_window_attention, and the kernels of one new token a request.
+//
+// One token.  A request's Keys and Values are read once and little is computed
+// on them, so the bytes bound it.  Requests differ in length, so the work is
+// cut by tokens and not by requests: the blocks of 128 tokens that the queries
+// see, of all requests and KV heads laid end to end, are shared out evenly to
+// as many workgroups as the card holds.  A workgroup's share covers parts of a
+// few (request, KV head) units; a unit that lies in one share goes straight to
+// the output, the others leave a record (running maximum, sum and sum of
+// Values) of each part, and a second launch joins them.  Each workgroup finds
+// its share from the lengths in device memory, so a captured launch follows
+// them.
+//
+// A wave takes 32 tokens a step.  S^T = K q^T (16 tokens by 16 query heads a
+// product) leaves four tokens of one query in each lane, which is how
+// O^T = V^T P^T wants them: no weight moves between lanes.  Keys and Values
+// come straight from memory in 16-byte pieces; a lane's eight Value rows by
+// eight channels are turned by v_perm.  Weights enter the products as two
+// 16-bit terms (2^-16 of a weight in all).
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "rk_paged_dev.h"
+
+namespace {
+
+using rk::base_of;
+using rk::f32x4;
+using rk::kNone;
+using rk::kPagedThreads;
+using rk::kPagedWaves;
+using rk::PagedArgs;
+
+constexpr int kStep = 32;                     // tokens of a wave's step
+constexpr int kBlock = kStep * kPagedWaves;  // tokens of a piece of work
+constexpr int kRows = 16;                     // queries of a unit
+
+// Pieces of one request and KV head.
+__device__ __forceinline__ int pieces_of(const PagedArgs& a, int b) {
+  const int p = rk::len_of(a.map, b) - 1;
+  const rk::Seen<kStep> s(max(p, 0), p, a.window, a.sinks);
+  return (s.blocks + kPagedWaves - 1) / kPagedWaves;
+}
+
+// Shares: workers that get any work, and where share w begins.
+struct Shares {
+  int64_t pieces;
+  int workers;
+  __device__ __forceinline__ int64_t begin(int w) const { return w * pieces / workers; }
+  __device__ __forceinline__ int of(int64_t piece) const { return (int)(((piece + 1) * workers - 1) / pieces); }
+};
+__device__ __forceinline__ Shares shares_of(const PagedArgs& a, int per_request, int units) {
+  Shares s;
+  s.pieces = (int64_t)per_request * units;
+  s.workers = (int)min((int64_t)a.workers, s.pieces);
+  return s;
+}
+
+// KF: blocks of 32 channels (2 or 4).
+template <class DT, int KF>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_split_kernel(const PagedArgs a) {
+  constexpr int KD = 32 * KF;      // channels, stored ones up to D
+  constexpr int VC = KD / 16;      // channels of a Value piece: 4 or 8
+  constexpr int AccPitch = KD + 4;
+  __shared__ int s_wave[kPagedWaves], s_found[2];
+  __shared__ float s_acc[kPagedWaves][kRows][AccPitch];
+  __shared__ float s_ml[kPagedWaves][kRows][2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, n = lane & 15;
+  const int blocks = (a.G + kRows - 1) / kRows;
+  const int units = a.H * blocks;  // of a request
+  auto count = [&](int b) { return pieces_of(a, b); };
+  const Shares sh = shares_of(a, rk::pieces_of_all(a.map.B, count, s_wave), units);
+  const int w = blockIdx.x;
+  if (w >= sh.workers) return;
+  int64_t at = sh.begin(w);
+  const int64_t end = sh.begin(w + 1);
+  const rk::Found found = rk::request_at(a.map.B, count, (int)(at / units), s_wave, s_found);
+  int b = found.b;
+  int64_t first = (int64_t)found.before * units;  // first piece of request b
+  while (at < end) {
+    const int pieces = pieces_of(a, b);
+    if (at >= first + (int64_t)pieces * units) {
+      first += (int64_t)pieces * units;
+      ++b;
+      continue;
+    }
+    const int unit = (int)((at - first) / pieces);
+    const int off = (int)(at - first) - unit * pieces;
+    const int take = (int)min((int64_t)(pieces - off), end - at);
+    at += take;
+    // ---- one part of a unit
+    const int h = unit / blocks, row0 = (unit - h * blocks) * kRows;
+    const int rows = min(a.G - row0, kRows);
+    const int len = rk::len_of(a.map, b), p = len - 1;
+    const rk::Seen<kStep> seen(p, p, a.window, a.sinks);
+    uint4 q[KF];
+    {
+      const int64_t qo = b * a.q_sb + (int64_t)(h * a.G + row0 + n) * a.q_sh;
+#pragma unroll
+      for (int c = 0; c < KF; ++c) {
+        const int ch = 32 * c + 8 * g;
+        q[c] = make_uint4(0, 0, 0, 0);
+        if (n < rows && ch < a.D) {
+          const uint16_t* src = (const uint16_t*)a.q + qo + ch * a.q_sd;
+          q[c] = a.q_vec ? rk::load8<true>(src, 1, 8) : rk::load8<false>(src, a.q_sd, 8);
+        }
+      }
+    }
+    const uint16_t* kb = (const uint16_t*)a.k + h * a.k_sh;
+    const uint16_t* vb = (const uint16_t*)a.v + h * a.v_sh;
+    float m = kNone, l = 0.f;
+    f32x4 acc[VC];
+#pragma unroll
+    for (int j = 0; j < VC; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int last = min(kPagedWaves * (off + take), seen.blocks);
+    for (int i = kPagedWaves * off + wave; i < last; i += kPagedWaves) {
+      const int t0 = seen.token(i);
+      // Keys: token t0 + n (+ 16); Values: tokens t0 + 4 g + 0..3 (+ 16)
+      uint4 k[2][KF];
+      uint32_t there = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int j = t0 + 16 * s + n;
+        uint32_t page = 0;
+        bool ok = rk::sees(p, j, a.window, a.sinks);
+        if (ok) {
+          page = rk::page_of(a.map, b, j);
+          ok = page < (uint32_t)a.map.pages;
+        }
+        there |= (uint32_t)(__ballot(ok) & 0xffff) << (16 * s);
+        const uint16_t* row = kb + (int64_t)page * a.k_sp + (int64_t)(j & ((1u << a.map.shift) - 1)) * a.k_ss;
+#pragma unroll
+        for (int c = 0; c < KF; ++c)
+          k[s][c] = ok && 32 * c + 8 * g < a.D ? *(const uint4*)(row + 32 * c + 8 * g) : make_uint4(0, 0, 0, 0);
+      }
+      uint32_t v[8][VC / 2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int j = t0 + 16 * s + 4 * g;
+        uint32_t page = 0;
+        const uint32_t mine = (there >> (16 * s + 4 * g)) & 15;
+        if (mine) page = rk::page_of(a.map, b, j);
+        const uint16_t* row = vb + (int64_t)page * a.v_sp + (int64_t)(j & ((1u << a.map.shift) - 1)) * a.v_ss + VC * n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool ok = (mine >> e & 1) && VC * n < a.D;
+          if constexpr (VC == 8) {
+            const uint4 x = ok ? *(const uint4*)(row + e * a.v_ss) : make_uint4(0, 0, 0, 0);
+            v[4 * s + e][0] = x.x; v[4 * s + e][1] = x.y; v[4 * s + e][2] = x.z; v[4 * s + e][3] = x.w;
+          } else {
+            const uint2 x = ok ? *(const uint2*)(row + e * a.v_ss) : make_uint2(0, 0);
+            v[4 * s + e][0] = x.x; v[4 * s + e][1] = x.y;
+          }
+        }
+      }
+      f32x4 sc[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KF; ++c) sc[s] = DT::mfma(k[s][c], q[c], sc[s]);
+      }
+      float x[8];
+      float top = kNone;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int bit = 16 * (e >> 2) + 4 * g + (e & 3);
+        x[e] = there >> bit & 1 ? sc[e >> 2][e & 3] * a.scale_log2 : kNone;
+        top = fmaxf(top, x[e]);
+      }
+      top = fmaxf(top, rk::shfl_xor(top, 16));
+      top = fmaxf(top, rk::shfl_xor(top, 32));
+      const float m_new = fmaxf(m, top), base = base_of(m_new);
+      const float keep = rk::fast_exp2(m - base);
+      m = m_new;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = rk::fast_exp2(x[e] - base);
+        l += x[e];
+      }
+      uint4 hi, lo;
+      DT::split8(x, hi, lo);
+#pragma unroll
+      for (int j = 0; j < VC; ++j) {
+        uint32_t t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          t[e] = j & 1 ? rk::pack_hi(v[2 * e][j >> 1], v[2 * e + 1][j >> 1])
+                       : rk::pack_lo(v[2 * e][j >> 1], v[2 * e + 1][j >> 1]);
+        const uint4 vt = make_uint4(t[0], t[1], t[2], t[3]);
+        acc[j] *= keep;
+        acc[j] = DT::mfma(vt, hi, acc[j]);
+        acc[j] = DT::mfma(vt, lo, acc[j]);
+      }
+    }
+    l += rk::shfl_xor(l, 16);
+    l += rk::shfl_xor(l, 32);
+    // ---- the waves' parts: lane (g, n) holds channels VC (4 g + i) + j of query n
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < VC; ++j) s_acc[wave][n][VC * (4 * g + i) + j] = acc[j][i];
+    if (g == 0) {
+      s_ml[wave][n][0] = m;
+      s_ml[wave][n][1] = l;
+    }
+    __syncthreads();
+    const int r = threadIdx.x >> 4, c0 = VC * n;
+    if (r < rows) {
+      float top = kNone;
+#pragma unroll
+      for (int v = 0; v < kPagedWaves; ++v) top = fmaxf(top, s_ml[v][r][0]);
+      float sum = 0.f, o[VC];
+#pragma unroll
+      for (int e = 0; e < VC; ++e) o[e] = 0.f;
+#pragma unroll
+      for (int v = 0; v < kPagedWaves; ++v) {
+        const float f = rk::fast_exp2(s_ml[v][r][0] - base_of(top));
+        sum += f * s_ml[v][r][1];
+#pragma unroll
+        for (int e = 0; e < VC; ++e) o[e] += f * s_acc[v][r][c0 + e];
+      }
+      if (take == pieces) {
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        uint16_t* dst = (uint16_t*)a.out + b * a.o_sb + (int64_t)(h * a.G + row0 + r) * a.o_sh;
+#pragma unroll
+        for (int e = 0; e < VC; ++e)
+          if (c0 + e < a.D) dst[(c0 + e) * a.o_sd] = DT::from_f32(o[e] * inv);
+      } else {
+        const int64_t rec = ((int64_t)w * 2 + (off > 0 ? 0 : 1)) * kRows + r;
+        float* dst = a.acc + rec * KD + c0;
+#pragma unroll
+        for (int e = 0; e < VC; e += 4) *(float4*)(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        if (n == 0) *(float2*)(a.ml + 2 * rec) = make_float2(top, sum);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the records of one query, or clears it where it sees nothing.
+template <class DT, int KF>
+__global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedArgs a) {
+  constexpr int KD = 32 * KF;
+  constexpr int VC = KD / 16;
+  __shared__ int s_wave[kPagedWaves];
+  __shared__ float s_acc[16][KD + 4], s_ml[16][2];
+  const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq;
+  const int h = hq / a.G, r = hq - h * a.G;
+  const int blocks = (a.G + kRows - 1) / kRows;
+  const int units = a.H * blocks;
+  const int pieces = pieces_of(a, b);
+  uint16_t* dst = (uint16_t*)a.out + b * a.o_sb + (int64_t)hq * a.o_sh;
+  if (pieces == 0) {
+    for (int c = threadIdx.x; c < a.D; c += kPagedThreads) dst[c * a.o_sd] = 0;
+    return;
+  }
+  auto count = [&](int i) { return pieces_of(a, i); };
+  auto count_before = [&](int i) { return i < b ? pieces_of(a, i) : 0; };
+  const Shares sh = shares_of(a, rk::pieces_of_all(a.map.B, count, s_wave), units);
+  const int before = rk::pieces_of_all(a.map.B, count_before, s_wave);
+  const int64_t first = (int64_t)before * units + (int64_t)(h * blocks + r / kRows) * pieces;
+  const int w0 = sh.of(first), w1 = sh.of(first + pieces - 1);
+  if (w0 == w1) return;  // the split launch wrote it
+  const int grp = threadIdx.x >> 4, c0 = VC * (threadIdx.x & 15);
+  float m = kNone, l = 0.f, o[VC];
+#pragma unroll
+  for (int e = 0; e < VC; ++e) o[e] = 0.f;
+  for (int w = w0 + grp; w <= w1; w += 16) {
+    const int64_t rec = ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * kRows + (r & (kRows - 1));
+    const float2 ml = *(const float2*)(a.ml + 2 * rec);
+    float x[VC];
+#pragma unroll
+    for (int e = 0; e < VC; e += 4) {
+      const float4 y = *(const float4*)(a.acc + rec * KD + c0 + e);
+      x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
+    }
+    const float top = fmaxf(m, ml.x), base = base_of(top);
+    const float f0 = rk::fast_exp2(m - base), f1 = rk::fast_exp2(ml.x - base);
+    l = l * f0 + ml.y * f1;
+#pragma unroll
+    for (int e = 0; e < VC; ++e) o[e] = o[e] * f0 + x[e] * f1;
+    m = top;
+  }
+#pragma unroll
+  for (int e = 0; e < VC; ++e) s_acc[grp][c0 + e] = o[e];
+  if ((threadIdx.x & 15) == 0) {
+    s_ml[grp][0] = m;
+    s_ml[grp][1] = l;
+  }
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (c >= a.D) return;
+  float top = kNone, sum = 0.f, y = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, s_ml[i][0]);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float f = rk::fast_exp2(s_ml[i][0] - base_of(top));
+    sum += f * s_ml[i][1];
+    y += f * s_acc[i][c];
+  }
+  dst[c * a.o_sd] = DT::from_f32(sum > 0.f || sum != sum ? y / sum : 0.f);
+}
+
+// ------------------------------------------------------------------- host
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Call {
+  const rk_tensor *q, *out;
+  const rk_pages* pages;        // or
+  const rk_tensor *k, *v;       // plain rows, with
+  const int32_t* lens;          // their lengths
+  const int32_t* starts;
+  int64_t groups, window, sinks;
+};
+
+struct Plan {
+  int64_t B, rows;         // requests; output rows (new tokens times query heads)
+  bool single;             // one new token a request
+  size_t acc, ml, total;   // workspace
+};
+
+// Checks a call and forms its arguments and workspace; no HIP calls.
+int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
+  memset(a, 0, sizeof(*a));
+  memset(p, 0, sizeof(*p));
+  int st;
+  const bool plain = c.pages == nullptr;
+  if (!c.q || (plain && (!c.k || !c.v))) return RK_ERR_NULL;
+  const int rank = plain ? 4 : 3;
+  if ((st = rk::check_desc(c.q, rank))) return st;
+  const rk_tensor *k = plain ? c.k : &c.pages->k, *v = plain ? c.v : &c.pages->v;
+  int64_t cap = 0;
+  if (plain) {
+    if ((st = rk::check_desc(k, 4)) || (st = rk::check_desc(v, 4))) return st;
+    for (int i = 0; i < 4; ++i)
+      if (k->shape[i] != v->shape[i]) return RK_ERR_SHAPE;
+    if (k->shape[0] != c.q->shape[0]) return RK_ERR_SHAPE;
+    cap = k->shape[2];
+    if (cap >= (INT64_C(1) << 30) || k->shape[0] >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+    p->B = k->shape[0];
+    a->map.lens = c.lens;
+    a->map.B = a->map.pages = (int32_t)p->B;
+    a->map.per = 1;
+    a->map.shift = 31;
+    a->map.cap = (int32_t)cap;
+  } else {
+    if ((st = rk::set_pages(c.pages, &a->map, &p->B, &cap))) return st;
+    if (cap >= (INT64_C(1) << 30)) return RK_ERR_SHAPE;
+    if (!c.starts && c.q->shape[0] != p->B) return RK_ERR_SHAPE;
+  }
+  a->map.starts = c.starts;
+  if (!rk::is_half(c.q->dtype) || k->dtype != c.q->dtype || v->dtype != c.q->dtype) return RK_ERR_DTYPE;
+  const int64_t D = c.q->shape[rank - 1], Hq = c.q->shape[1], H = k->shape[1];
+  if (D < 8 || D > 128 || D % 8 || k->shape[3] != D) return RK_ERR_HEAD_DIM;
+  if (c.groups < 1 || H < 1 || H > (1 << 20) || c.groups > (1 << 20) || Hq != H * c.groups) return RK_ERR_HEADS;
+  if (!rk::vec_ok(k) || !rk::vec_ok(v)) return RK_ERR_STRIDE;
+  if (c.window < 0 || c.sinks < 0) return RK_ERR_ARG;
+  if (c.out) {
+    if ((st = rk::check_desc(c.out, rank))) return st;
+    if (c.out->dtype != c.q->dtype) return RK_ERR_DTYPE;
+    for (int i = 0; i < rank; ++i) {
+      if (c.out->shape[i] != c.q->shape[i]) return RK_ERR_SHAPE;
+      if (c.out->shape[i] > 1 && c.out->stride[i] == 0) return RK_ERR_STRIDE;
+    }
+  }
+  const int64_t T = plain ? c.q->shape[2] : c.starts ? 0 : 1;
+  const int64_t N = plain ? p->B * T : c.q->shape[0];
+  if (T >= (INT64_C(1) << 30) || N >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+  p->rows = N * Hq;
+  p->single = T == 1;
+  if (p->rows >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+  a->map.each = (int32_t)T;
+  a->N = N;
+  a->T = (int32_t)T;
+  a->Hq = (int32_t)Hq; a->H = (int32_t)H; a->G = (int32_t)c.groups; a->D = (int32_t)D;
+  a->window = c.window == 0 || c.window > INT_MAX ? INT_MAX : (int32_t)c.window;
+  a->sinks = (int32_t)std::min<int64_t>(c.sinks, INT_MAX);
+  a->scale_log2 = rk::kLog2e / sqrtf((float)D);
+  auto q_strides = [&](const rk_tensor* t, int64_t* sb, int64_t* st_, int64_t* sh, int64_t* sd) {
+    *sh = t->stride[1];
+    *sb = c.starts ? 0 : t->stride[0];
+    *st_ = plain ? t->stride[2] : t->stride[0];
+    *sd = t->stride[rank - 1];
+  };
+  a->q = c.q->data;
+  q_strides(c.q, &a->q_sb, &a->q_st, &a->q_sh, &a->q_sd);
+  a->q_vec = rk::vec_ok(c.q);
+  if (c.out) {
+    a->out = c.out->data;
+    q_strides(c.out, &a->o_sb, &a->o_st, &a->o_sh, &a->o_sd);
+    a->o_vec = rk::vec_ok(c.out);
+  }
+  a->k = k->data;
+  a->k_sp = k->stride[0]; a->k_sh = k->stride[1]; a->k_ss = k->stride[2];
+  a->v = v->data;
+  a->v_sp = v->stride[0]; a->v_sh = v->stride[1]; a->v_ss = v->stride[2];
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) & ~size_t(255);
+    return here;
+  };
+  if (p->single) {
+    const int64_t KD = D <= 64 ? 64 : 128;
+    // two workgroups a CU: what their registers allow
+    const int64_t pieces = p->B * H * cdiv(c.groups, kRows) * (cdiv(cap, kBlock) + 1);
+    if (pieces >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+    a->workers = (int32_t)std::max<int64_t>(std::min<int64_t>(2 * (int64_t)cus, pieces), 1);
+    const size_t records = (size_t)a->workers * 2 * kRows;
+    p->acc = take(records * KD * 4);
+    p->ml = take(records * 8);
+  } else if (p->rows > 0) {
+    // cut the tokens where the rows alone leave CUs empty, into parts of 256 or more
+    const int64_t grid = rk::window_slots(*a) * H;
+    a->splits = (int32_t)std::max<int64_t>(std::min(2 * (int64_t)cus / std::max<int64_t>(grid, 1), cap / 256), 1);
+    if (grid * a->splits >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+    if (a->splits > 1) {
+      p->acc = take((size_t)p->rows * a->splits * cdiv(D, 32) * 128);
+      p->ml = take((size_t)p->rows * a->splits * 8);
+    }
+  }
+  p->total = at;
+  return RK_OK;
+}
+
+int null_data(const Call& c, const PagedArgs& a) {
+  if (!a.q || !a.out) return RK_ERR_NULL;
+  if (a.map.pages > 0 && a.map.cap > 0 && (!a.k || !a.v)) return RK_ERR_NULL;
+  if (c.pages && (!a.map.lens || (a.map.cap > 0 && !a.map.table))) return RK_ERR_NULL;
+  return RK_OK;
+}
+
+int resolve_cus(int num_cus, int* st) {
+  *st = RK_OK;
+  if (num_cus > 0) return num_cus;
+  const int cus = num_cus < 0 ? 0 : rk::current_device_cus(nullptr);
+  if (cus <= 0) *st = num_cus < 0 ? RK_ERR_ARG : RK_ERR_NO_DEVICE;
+  return cus;
+}
+
+template <class F>
+int by_shape(int dtype, int D, F&& f) {
+  auto on = [&](auto dt) { D <= 64 ? f(dt, std::integral_constant<int, 2>{}) : f(dt, std::integral_constant<int, 4>{}); };
+  dtype == RK_F16 ? on(rk::F16{}) : on(rk::BF16{});
+  return hipGetLastError() == hipSuccess ? RK_OK : RK_ERR_HIP;
+}
+
+int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
+  PagedArgs a;
+  Plan p;
+  // everything but the split is checked before a device is asked for
+  int st = make_plan(c, 1, &a, &p);
+  if (st) return st;
+  if (!c.out) return RK_ERR_NULL;
+  if (p.rows == 0 || p.B == 0) return RK_OK;
+  if ((st = null_data(c, a))) return st;
+  const int cus = resolve_cus(0, &st);
+  if (st) return st;
+  if ((st = make_plan(c, cus, &a, &p))) return st;
+  if (p.total && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.total)) return RK_ERR_WORKSPACE;
+  a.acc = (float*)((char*)workspace + p.acc);
+  a.ml = (float*)((char*)workspace + p.ml);
+  const hipStream_t s = (hipStream_t)stream;
+  if (!p.single) return rk::window_launch(a, c.q->dtype, s);
+  return by_shape(c.q->dtype, a.D, [&](auto dt, auto kf) {
+    hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value>), dim3((unsigned)a.workers),
+                       dim3(kPagedThreads), 0, s, a);
+    hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value>), dim3((unsigned)p.rows),
+                       dim3(kPagedThreads), 0, s, a);
+  });
+}
+
+int check_call(const Call& c, int32_t num_cus, size_t* bytes) {
+  PagedArgs a;
+  Plan p;
+  int st = make_plan(c, 1, &a, &p);
+  if (st) return st;
+  const int cus = resolve_cus(num_cus, &st);
+  if (st) return st;
+  if ((st = make_plan(c, cus, &a, &p))) return st;
+  if (bytes) *bytes = p.total;
+  return RK_OK;
+}
+
+}  // namespace
+
+extern "C" int rk_paged_attention_check(const rk_tensor* q, const int32_t* starts, const rk_pages* pages,
+                                        int64_t num_kv_groups, int64_t window, int64_t sinks, const rk_tensor* out,
+                                        int32_t num_cus, size_t* workspace_bytes) {
+  if (!pages) return RK_ERR_NULL;
+  return check_call({q, out, pages, nullptr, nullptr, nullptr, starts, num_kv_groups, window, sinks}, num_cus,
+                    workspace_bytes);
+}
+
+extern "C" int rk_paged_attention(const rk_tensor* q, const int32_t* starts, const rk_pages* pages,
+                                  int64_t num_kv_groups, int64_t window, int64_t sinks, const rk_tensor* out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (!pages) return RK_ERR_NULL;
+  return run({q, out, pages, nullptr, nullptr, nullptr, starts, num_kv_groups, window, sinks}, workspace,
+             workspace_bytes, stream);
+}
+
+extern "C" int rk_window_attention_check(const rk_tensor* q, const rk_tensor* k, const rk_tensor* v,
+                                         const int32_t* lens, int64_t num_kv_groups, int64_t window, int64_t sinks,
+                                         const rk_tensor* out, int32_t num_cus, size_t* workspace_bytes) {
+  return check_call({q, out, nullptr, k, v, lens, nullptr, num_kv_groups, window, sinks}, num_cus, workspace_bytes);
+}
+
+extern "C" int rk_window_attention(const rk_tensor* q, const rk_tensor* k, const rk_tensor* v, const int32_t* lens,
+                                   int64_t num_kv_groups, int64_t window, int64_t sinks, const rk_tensor* out,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  return run({q, out, nullptr, k, v, lens, nullptr, num_kv_groups, window, sinks}, workspace, workspace_bytes, stream);
+}

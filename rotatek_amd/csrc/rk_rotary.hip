@@ -1,0 +1,400 @@
+// rk_rotary.hip -- rotation by position and the append to a paged cache on
+// MI355X (gfx950): rk_rotary, rk_paged_append of rotatek_hip.h.
+//
+// Mathematics.  Pair i of a head (channels i and i + P) turns by
+// a = pos[axis(i)] f[i].  pos f is formed in 64 bits, where it is exact to
+// 2^-53, and so are its turns a / 2 pi, of which only the fraction is kept: at
+// position 10^5 an angle in 32 bits is off by 2^-8.  The fraction's sine and
+// cosine are 32-bit; a pair is rounded once, as it is stored.
+//
+// A workgroup takes a few tokens.  Each pair's sine and cosine are formed once
+// for all heads of the token and go through LDS; then every lane turns a
+// vector of pairs (16 bytes from either half of the head) of one head.  In an
+// append the same pass writes Keys and Values to their pages.
+#include <hip/hip_runtime.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "rk_common.h"
+#include "rk_host.h"
+#include "rk_paged.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 4;  // tokens of a workgroup
+constexpr int kMaxPairs = 64;
+constexpr int kMaxAxes = 4;
+
+enum { kQ = 0, kK = 1, kV = 2, kParts = 3 };
+
+struct Part {
+  const void* x;
+  void* y;
+  int64_t x_sb, x_sh, x_ss, x_sd;  // elements; token (b, t)
+  int64_t y_sb, y_sh, y_ss, y_sd;  // ... of a page, a head, a row where the token goes to its page
+  int32_t heads;
+};
+
+struct RotaryArgs {
+  Part part[kParts];
+  const void* pos;  // null: nothing turns
+  const float* freq;
+  int64_t p_sa, p_sb, p_st, f_s;
+  uint32_t axis[4];  // two bits a pair
+  int32_t pos64;
+  float sign;
+  int32_t P, D;
+  int32_t T;  // tokens of a batch row
+  int64_t N;  // tokens
+  int32_t tokens;  // of a workgroup
+  // the pages (paged)
+  rk::PageMap map;
+};
+
+// cos and sin of 2 pi f for the fraction of turns f in [-1/2, 1/2].
+__device__ __forceinline__ float2 turn_of(double turns) {
+  const float f = (float)(turns - __builtin_rint(turns));
+  float s, c;
+  sincospif(2.f * f, &s, &c);
+  return make_float2(c, s);
+}
+
+// A pair turned.  The products are told apart (one rounded, one fused), so that
+// every path gives the same bits.
+__device__ __forceinline__ float2 turn(float lo, float hi, float2 cs) {
+  return make_float2(__builtin_fmaf(lo, cs.x, -(hi * cs.y)), __builtin_fmaf(hi, cs.x, lo * cs.y));
+}
+
+// VEC: 16 bytes of channels at a time.  PAGED: K and V go to their pages.
+template <class DT, bool VEC, bool PAGED>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
+  constexpr int E = VEC ? 16 / DT::kBytes : 1;  // elements of a step
+  using word = typename std::conditional<DT::kBytes == 4, uint32_t, uint16_t>::type;
+  __shared__ float2 s_turn[kMaxTokens * kMaxPairs];
+  __shared__ int64_t s_page[kMaxTokens];  // page number and row of a token, or -1
+  __shared__ int32_t s_row[kMaxTokens];
+  const int tid = threadIdx.x;
+  const int64_t n0 = (int64_t)blockIdx.x * a.tokens;
+  const int tokens = (int)min((int64_t)a.tokens, a.N - n0);
+  if (a.pos) {
+    for (int i = tid; i < tokens * a.P; i += kThreads) {
+      const int tok = i / a.P, p = i - tok * a.P;
+      const int64_t n = n0 + tok, b = n / a.T, t = n - b * a.T;
+      const int axis = (a.axis[p >> 4] >> (2 * (p & 15))) & 3;
+      const int64_t at = axis * a.p_sa + b * a.p_sb + t * a.p_st;
+      const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
+      float2 cs = turn_of(pos * (double)a.freq[p * a.f_s] * 0.15915494309189533577);
+      cs.y *= a.sign;
+      s_turn[tok * kMaxPairs + p] = cs;
+    }
+  }
+  if constexpr (PAGED) {
+    if (tid < tokens) {
+      int row = 0;
+      s_page[tid] = rk::place_of(a.map, n0 + tid, &row);
+      s_row[tid] = row;
+    }
+  }
+  __syncthreads();
+  // steps of a head: turned pairs, then copied channels
+  const int turned = a.pos ? a.P / E : 0;
+  const int copied = (a.D - (a.pos ? 2 * a.P : 0)) / E;
+  const int per = turned + copied, all = a.D / E;
+  const int nq = a.part[kQ].heads * per, nk = a.part[kK].heads * per, nv = a.part[kV].heads * all;
+  const int per_token = nq + nk + nv;
+  for (int i = tid; i < tokens * per_token; i += kThreads) {
+    const int tok = i / per_token;
+    int u = i - tok * per_token;
+    const int which = u < nq ? kQ : u < nq + nk ? kK : kV;
+    u -= which == kQ ? 0 : which == kK ? nq : nq + nk;
+    const Part& p = a.part[which];
+    const int steps = which == kV ? all : per;
+    const int h = u / steps, step = u - h * steps;
+    const int64_t n = n0 + tok, b = n / a.T, t = n - b * a.T;
+    const int64_t xo = b * p.x_sb + h * p.x_sh + t * p.x_ss;
+    int64_t yo;
+    if (PAGED && which != kQ) {
+      if (s_page[tok] < 0) continue;
+      yo = s_page[tok] * p.y_sb + h * p.y_sh + s_row[tok] * p.y_ss;
+    } else {
+      yo = b * p.y_sb + h * p.y_sh + t * p.y_ss;
+    }
+    const word* x = (const word*)p.x + xo;
+    word* y = (word*)p.y + yo;
+    const bool turns = which != kV && step < turned;
+    const int c = which == kV ? step * E : turns ? step * E : 2 * (a.pos ? a.P : 0) + (step - turned) * E;
+    if constexpr (VEC) {
+      const uint4 lo = *(const uint4*)(x + c);
+      if (!turns) {
+        *(uint4*)(y + c) = lo;
+        continue;
+      }
+      const uint4 hi = *(const uint4*)(x + c + a.P);
+      uint4 ylo, yhi;
+      const float2* cs = s_turn + tok * kMaxPairs + c;
+      if constexpr (DT::kBytes == 4) {
+        uint32_t l[4], m[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 y2 = turn(DT::to_f32(rk::word(lo, e)), DT::to_f32(rk::word(hi, e)), cs[e]);
+          l[e] = DT::from_f32(y2.x);
+          m[e] = DT::from_f32(y2.y);
+        }
+        ylo = make_uint4(l[0], l[1], l[2], l[3]);
+        yhi = make_uint4(m[0], m[1], m[2], m[3]);
+      } else {
+        uint32_t l[4], m[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t wl = rk::word(lo, e), wh = rk::word(hi, e);
+          const float2 y0 = turn(DT::to_f32((uint16_t)wl), DT::to_f32((uint16_t)wh), cs[2 * e]);
+          const float2 y1 = turn(DT::to_f32((uint16_t)(wl >> 16)), DT::to_f32((uint16_t)(wh >> 16)), cs[2 * e + 1]);
+          l[e] = DT::pack2(y0.x, y1.x);
+          m[e] = DT::pack2(y0.y, y1.y);
+        }
+        ylo = make_uint4(l[0], l[1], l[2], l[3]);
+        yhi = make_uint4(m[0], m[1], m[2], m[3]);
+      }
+      *(uint4*)(y + c) = ylo;
+      *(uint4*)(y + c + a.P) = yhi;
+    } else {
+      const word lo = x[c * p.x_sd];
+      if (!turns) {
+        y[c * p.y_sd] = lo;
+        continue;
+      }
+      const float2 y2 = turn(DT::to_f32(lo), DT::to_f32(x[(c + a.P) * p.x_sd]), s_turn[tok * kMaxPairs + c]);
+      y[c * p.y_sd] = DT::from_f32(y2.x);
+      y[(c + a.P) * p.y_sd] = DT::from_f32(y2.y);
+    }
+  }
+}
+
+// The rotation's arguments: positions [A,B,T] or [A,N], frequencies [P], pairs
+// of each axis.
+int set_rotation(RotaryArgs* a, const rk_tensor* pos, const rk_tensor* freq, const int32_t* sections, int32_t axes,
+                 int32_t interleaved, int32_t inverse, int64_t B, int64_t T, bool flat) {
+  if (!pos || !freq || !sections) return RK_ERR_NULL;
+  int st;
+  if ((st = rk::check_desc(pos, flat ? 2 : 3)) || (st = rk::check_desc(freq, 1))) return st;
+  if (pos->dtype != RK_I32 && pos->dtype != RK_I64) return RK_ERR_DTYPE;
+  if (freq->dtype != RK_F32) return RK_ERR_DTYPE;
+  if (axes < 1 || axes > kMaxAxes) return RK_ERR_ARG;
+  if (interleaved < 0 || interleaved > 1 || inverse < 0 || inverse > 1) return RK_ERR_ARG;
+  if (pos->shape[0] != axes) return RK_ERR_SHAPE;
+  if (flat ? pos->shape[1] != T : pos->shape[1] != B || pos->shape[2] != T) return RK_ERR_SHAPE;
+  const int64_t P = freq->shape[0];
+  if (P < 1 || P > kMaxPairs || 2 * P > a->D) return RK_ERR_SHAPE;
+  int64_t sum = 0;
+  int32_t left[kMaxAxes];
+  for (int i = 0; i < axes; ++i) {
+    if (sections[i] < 0 || sections[i] > P) return RK_ERR_ARG;
+    left[i] = sections[i];
+    sum += sections[i];
+  }
+  if (sum != P) return RK_ERR_ARG;
+  int axis = 0;
+  for (int i = 0; i < P; ++i) {
+    while (!left[axis]) axis = (axis + 1) % axes;  // ends: P pairs are left in all
+    a->axis[i >> 4] |= (uint32_t)axis << (2 * (i & 15));
+    --left[axis];
+    if (interleaved) axis = (axis + 1) % axes;
+  }
+  a->pos = pos->data;
+  a->pos64 = pos->dtype == RK_I64;
+  a->p_sa = pos->stride[0];
+  a->p_sb = flat ? 0 : pos->stride[1];
+  a->p_st = pos->stride[flat ? 1 : 2];
+  a->freq = (const float*)freq->data;
+  a->f_s = freq->stride[0];
+  a->P = (int32_t)P;
+  a->sign = inverse ? -1.f : 1.f;
+  return RK_OK;
+}
+
+// Strides of [B,H,T,D], or of [N,H,D] as one batch row.
+struct Strides {
+  int64_t sb, sh, ss, sd;
+};
+Strides strides_of(const rk_tensor* t) {
+  if (t->ndim == 4) return {t->stride[0], t->stride[1], t->stride[2], t->stride[3]};
+  return {0, t->stride[1], t->stride[0], t->stride[2]};
+}
+
+void set_in(Part* p, const rk_tensor* x) {
+  const Strides s = strides_of(x);
+  p->x = x->data;
+  p->x_sb = s.sb; p->x_sh = s.sh; p->x_ss = s.ss; p->x_sd = s.sd;
+  p->heads = (int32_t)x->shape[1];
+}
+void set_out(Part* p, void* y, const Strides& s) {
+  p->y = y;
+  p->y_sb = s.sb; p->y_sh = s.sh; p->y_ss = s.ss; p->y_sd = s.sd;
+}
+
+bool vec16(const rk_tensor* t) {
+  const int n = 16 / rk::dtype_size(t->dtype);
+  if (t->stride[t->ndim - 1] != 1 && t->shape[t->ndim - 1] > 1) return false;
+  for (int i = 0; i < t->ndim - 1; ++i)
+    if (t->shape[i] > 1 && t->stride[i] % n) return false;
+  return ((uintptr_t)t->data & 15) == 0;
+}
+
+// What a call writes must not repeat by a stride of 0.
+bool distinct(const rk_tensor* t) {
+  for (int i = 0; i < t->ndim; ++i)
+    if (t->shape[i] > 1 && t->stride[i] == 0) return false;
+  return true;
+}
+
+int check_x(const rk_tensor* x, int rank) {
+  if (int st = rk::check_desc(x, rank)) return st;
+  if (!rk::is_float_param(x->dtype)) return RK_ERR_DTYPE;
+  const int64_t D = x->shape[rank - 1];
+  if (D < 1 || D > 128) return RK_ERR_HEAD_DIM;
+  return x->shape[1] >= (1 << 20) ? RK_ERR_HEADS : RK_OK;
+}
+
+bool same_shape(const rk_tensor* a, const rk_tensor* b) {
+  if (a->ndim != b->ndim) return false;
+  for (int i = 0; i < a->ndim; ++i)
+    if (a->shape[i] != b->shape[i]) return false;
+  return true;
+}
+
+// The same tokens and channels (heads may differ).
+bool same_tokens(const rk_tensor* a, const rk_tensor* b) {
+  if (a->ndim != b->ndim) return false;
+  for (int i = 0; i < a->ndim; ++i)
+    if (i != 1 && a->shape[i] != b->shape[i]) return false;
+  return true;
+}
+
+template <class F>
+int by_type(int dtype, bool vec, F&& f) {
+  auto on = [&](auto dt) { vec ? f(dt, std::true_type{}) : f(dt, std::false_type{}); };
+  if (dtype == RK_F16)
+    on(rk::F16{});
+  else if (dtype == RK_BF16)
+    on(rk::BF16{});
+  else
+    on(rk::F32{});
+  return hipGetLastError() == hipSuccess ? RK_OK : RK_ERR_HIP;
+}
+
+template <bool PAGED>
+int launch(RotaryArgs& a, int dtype, bool vec, void* stream) {
+  const int E = vec ? 16 / rk::dtype_size(dtype) : 1;
+  if (E > 1 && (a.D % E || (a.pos && a.P % E))) vec = false;
+  a.tokens = a.N >= 2048 ? kMaxTokens : 1;
+  const int64_t grid = (a.N + a.tokens - 1) / a.tokens;
+  if (grid >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+  return by_type(dtype, vec, [&](auto dt, auto v) {
+    hipLaunchKernelGGL((rotary_kernel<decltype(dt), decltype(v)::value, PAGED>), dim3((unsigned)grid), dim3(kThreads),
+                       0, (hipStream_t)stream, a);
+  });
+}
+
+}  // namespace
+
+extern "C" int rk_rotary(const rk_tensor* q, const rk_tensor* k, const rk_tensor* positions,
+                         const rk_tensor* inv_freq, const int32_t* sections, int32_t axes, int32_t interleaved,
+                         int32_t inverse, const rk_tensor* q_out, const rk_tensor* k_out, void* stream) {
+  if (!q || !q_out || (k == nullptr) != (k_out == nullptr)) return RK_ERR_NULL;
+  const int rank = q->ndim;
+  if (rank != 3 && rank != 4) return RK_ERR_RANK;
+  RotaryArgs a;
+  memset(&a, 0, sizeof(a));
+  bool vec = true;
+  for (const rk_tensor* t : {q, q_out, k, k_out}) {
+    if (!t) continue;
+    if (int st = check_x(t, rank)) return st;
+    if (t->dtype != q->dtype) return RK_ERR_DTYPE;
+    if (!same_tokens(t, q)) return RK_ERR_SHAPE;
+    vec = vec && vec16(t);
+  }
+  if (!same_shape(q, q_out) || (k && !same_shape(k, k_out))) return RK_ERR_SHAPE;
+  for (const rk_tensor* t : {q_out, k_out})
+    if (t && !distinct(t)) return RK_ERR_STRIDE;
+  a.D = (int32_t)q->shape[rank - 1];
+  const int64_t B = rank == 4 ? q->shape[0] : 1, T = rank == 4 ? q->shape[2] : q->shape[0];
+  if (T >= (INT64_C(1) << 31) || (T > 0 && B >= (INT64_C(1) << 40) / T)) return RK_ERR_SHAPE;
+  if (int st = set_rotation(&a, positions, inv_freq, sections, axes, interleaved, inverse, B, T, rank == 3)) return st;
+  a.T = (int32_t)T;
+  a.N = B * T;
+  set_in(&a.part[kQ], q);
+  set_out(&a.part[kQ], q_out->data, strides_of(q_out));
+  if (k) {
+    set_in(&a.part[kK], k);
+    set_out(&a.part[kK], k_out->data, strides_of(k_out));
+  }
+  if (a.N == 0 || a.part[kQ].heads + a.part[kK].heads == 0) return RK_OK;
+  for (const Part& p : a.part)
+    if (p.heads && (!p.x || !p.y)) return RK_ERR_NULL;
+  if (!a.pos || !a.freq) return RK_ERR_NULL;
+  return launch<false>(a, q->dtype, vec, stream);
+}
+
+extern "C" int rk_paged_append(const rk_tensor* k_new, const rk_tensor* v_new, const rk_pages* pages,
+                               const int32_t* starts, const rk_tensor* q, const rk_tensor* q_out,
+                               const rk_tensor* positions, const rk_tensor* inv_freq, const int32_t* sections,
+                               int32_t axes, int32_t interleaved, void* stream) {
+  if (!k_new || !v_new || !pages || (q == nullptr) != (q_out == nullptr)) return RK_ERR_NULL;
+  if (q && !positions) return RK_ERR_NULL;
+  const int rank = k_new->ndim;
+  if (rank != 3 && rank != 4) return RK_ERR_RANK;
+  RotaryArgs a;
+  memset(&a, 0, sizeof(a));
+  int64_t B = 0, cap = 0;
+  int st = rk::set_pages(pages, &a.map, &B, &cap);
+  if (st) return st;
+  bool vec = vec16(&pages->k) && vec16(&pages->v);
+  for (const rk_tensor* t : {k_new, v_new, q, q_out}) {
+    if (!t) continue;
+    if ((st = check_x(t, rank))) return st;
+    if (t->dtype != k_new->dtype) return RK_ERR_DTYPE;
+    if (!same_tokens(t, k_new)) return RK_ERR_SHAPE;
+    vec = vec && vec16(t);
+  }
+  if (!same_shape(k_new, v_new) || (q && !same_shape(q, q_out))) return RK_ERR_SHAPE;
+  if (pages->k.dtype != k_new->dtype) return RK_ERR_DTYPE;
+  if (pages->k.shape[1] != k_new->shape[1]) return RK_ERR_HEADS;
+  if (pages->k.shape[3] != k_new->shape[rank - 1]) return RK_ERR_HEAD_DIM;
+  for (const rk_tensor* t : {&pages->k, &pages->v, q_out})
+    if (t && !distinct(t)) return RK_ERR_STRIDE;
+  // whole requests of one length, or tokens one after the other with starts
+  if (rank == 4 ? starts != nullptr || k_new->shape[0] != B : starts == nullptr && k_new->shape[0] != B)
+    return RK_ERR_SHAPE;
+  a.D = (int32_t)k_new->shape[rank - 1];
+  const int64_t T = rank == 4 ? k_new->shape[2] : k_new->shape[0];
+  if (T >= (INT64_C(1) << 31) || B >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+  const int64_t rows = rank == 4 ? B : 1;
+  if (T > 0 && rows >= (INT64_C(1) << 40) / T) return RK_ERR_SHAPE;
+  if (positions) {
+    st = set_rotation(&a, positions, inv_freq, sections, axes, interleaved, 0, rows, T, rank == 3);
+    if (st) return st;
+  }
+  a.T = (int32_t)T;
+  a.N = rows * T;
+  a.map.starts = starts;
+  a.map.each = rank == 4 ? (int32_t)T : 1;
+  if (q) {
+    set_in(&a.part[kQ], q);
+    set_out(&a.part[kQ], q_out->data, strides_of(q_out));
+  }
+  set_in(&a.part[kK], k_new);
+  set_in(&a.part[kV], v_new);
+  for (int i : {kK, kV}) {
+    const rk_tensor& t = i == kK ? pages->k : pages->v;
+    set_out(&a.part[i], t.data, {t.stride[0], t.stride[1], t.stride[2], t.stride[3]});
+  }
+  if (a.N == 0 || a.part[kQ].heads + a.part[kK].heads == 0) return RK_OK;
+  if (a.part[kQ].heads && (!a.part[kQ].x || !a.part[kQ].y)) return RK_ERR_NULL;
+  for (int i : {kK, kV})
+    if (a.part[i].heads && (!a.part[i].x || (a.map.pages > 0 && !a.part[i].y))) return RK_ERR_NULL;
+  if (B > 0 && (!a.map.lens || (cap > 0 && !a.map.table))) return RK_ERR_NULL;
+  if (positions && (!a.pos || !a.freq)) return RK_ERR_NULL;
+  return launch<true>(a, k_new->dtype, vec, stream);
+}

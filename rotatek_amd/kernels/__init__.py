@@ -10,7 +10,9 @@ at import and anything else raises ``ValueError``, as in the reference.
 
 The decodes over quantised rows (``rotatek_decode_quantized``,
 ``full_channel_decode_quantized``) and over a prefix that the batch shares
-(``shared_prefix_decode``) have one decomposition whatever the variable says.
+(``shared_prefix_decode``), and the attention over pages and windows
+(``paged_decode``, ``paged_prefill``, ``window_attention``), have one
+decomposition whatever the variable says.
 """
 import os
 
@@ -34,8 +36,10 @@ def _pick():
 
 rotatek_decode, full_channel_decode = _pick()
 
+from rotatek_amd.kernels.paged_attention import paged_decode, paged_prefill, window_attention  # noqa: E402
 from rotatek_amd.kernels.quantized_decode import full_channel_decode_quantized, rotatek_decode_quantized  # noqa: E402
 from rotatek_amd.kernels.shared_prefix import shared_prefix_decode  # noqa: E402
 
 __all__ = ["ROTATEK_KERNEL", "rotatek_decode", "full_channel_decode", "rotatek_decode_quantized",
-           "full_channel_decode_quantized", "shared_prefix_decode"]
+           "full_channel_decode_quantized", "shared_prefix_decode", "paged_decode", "paged_prefill",
+           "window_attention"]
