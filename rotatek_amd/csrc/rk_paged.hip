@@ -364,6 +364,8 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
   if (D < 8 || D > 128 || D % 8 || k->shape[3] != D) return RK_ERR_HEAD_DIM;
   if (c.groups < 1 || H < 1 || H > (1 << 20) || c.groups > (1 << 20) || Hq != H * c.groups) return RK_ERR_HEADS;
   if (!rk::vec_ok(k) || !rk::vec_ok(v)) return RK_ERR_STRIDE;
+  // eight rows within 32 bits of bytes
+  if (k->stride[2] >= (INT64_C(1) << 27) || v->stride[2] >= (INT64_C(1) << 27)) return RK_ERR_STRIDE;
   if (c.window < 0 || c.sinks < 0) return RK_ERR_ARG;
   if (c.out) {
     if ((st = rk::check_desc(c.out, rank))) return st;

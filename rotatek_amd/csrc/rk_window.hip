@@ -30,10 +30,17 @@ using rk::PagedArgs;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds4;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(1))) void* global_ptr;
 
 constexpr int kTile = 64;               // tokens
 constexpr int kWaveRows = 32;
 constexpr int kRows = kWaveRows * kPagedWaves;
+constexpr float kSlack = 8.f;           // log2 of what weights may grow to
+constexpr float kFar = 16384.f;         // a base that is rounded by 2^-11 at most
+
+// The wave's loads to LDS have arrived.
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <class DT>
 __device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
@@ -43,6 +50,16 @@ __device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(rk::bf16x8, a),
                                                    __builtin_bit_cast(rk::bf16x8, b), c, 0, 0, 0);
+}
+
+// Where the pieces of a row of Keys or Values lie in LDS: piece c at c ^ swap.
+template <int CH>
+__device__ __forceinline__ int key_swap(int row) {
+  return CH == 16 ? row & 15 : (row >> 1) & 7;
+}
+template <int CH>
+__device__ __forceinline__ int value_swap(int row) {
+  return CH == 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
 }
 
 // New tokens of request b: first and how many.
@@ -57,7 +74,8 @@ __device__ __forceinline__ Queries queries_of(const PagedArgs& a, int b) {
 }
 
 // One row by one wave, two channels a lane, over the tokens that it sees alone
-// (m: its maximum): any cost, for Values that are not finite.
+// (m: the score that weights are against): any cost, for Values that are not
+// finite.
 template <class DT>
 __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, rk::Seen<kTile> seen, int i0, int i1, int h,
                                      int row, int p0, int split, int KD, float m) {
@@ -82,7 +100,7 @@ __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, r
       float s = on ? q0 * DT::to_f32(k[c]) + q1 * DT::to_f32(k[c + 1]) : 0.f;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) s += rk::shfl_xor(s, d);
-      const float w = rk::fast_exp2(s * a.scale_log2 - base);
+      const float w = rk::fast_exp2((s - base) * a.scale_log2);
       l += w;
       if (on) {
         y0 += w * DT::to_f32(v[c]);
@@ -94,7 +112,7 @@ __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, r
   if (a.splits > 1) {
     const int64_t rec = (int64_t)split * a.N * a.Hq + (b * (int64_t)a.T + qs.first + t) * a.Hq + hq;
     *(float2*)(a.acc + rec * KD + c) = make_float2(y0, y1);
-    if (c == 0) *(float2*)(a.ml + 2 * rec) = make_float2(m, l);
+    if (c == 0) *(float2*)(a.ml + 2 * rec) = make_float2(m * a.scale_log2, l);
     return;
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -107,10 +125,11 @@ template <class DT, int NB>
 __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArgs a) {
   constexpr int CH = NB <= 2 ? 8 : 16;        // 16-byte pieces of a row in LDS
   constexpr int Pitch = CH * 16;              // bytes
-  constexpr int Passes = kTile * CH / kPagedThreads;
-  __shared__ __align__(16) char s_k[2][kTile * Pitch], s_v[2][kTile * Pitch];
+  constexpr int Passes = kTile * CH / kPagedThreads;  // loads of a wave for a tile's Keys
+  // two tiles; arrays of their own, so that reads of one do not wait for loads into the other
+  __shared__ __align__(16) char s_k0[kTile * Pitch], s_k1[kTile * Pitch], s_v0[kTile * Pitch], s_v1[kTile * Pitch];
   __shared__ int s_wave[kPagedWaves], s_found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, col = lane & 31;
   const int h = blockIdx.x % a.H;
   const int rest = blockIdx.x / a.H;
@@ -164,49 +183,73 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
 
   const uint16_t* kb = (const uint16_t*)a.k + h * a.k_sh;
   const uint16_t* vb = (const uint16_t*)a.v + h * a.v_sh;
-  // staging: piece `pc` of rows srow + i * (rows of a pass)
-  const int pc = tid % CH, srow = tid / CH;
-  uint4 kr[Passes], vr[Passes];
-  // lane l holds the page of token l of a tile; one past the pool where it is not seen by any row
+  // lane l holds the page of token l of a tile; one past the pool where no row sees it
   auto page_at = [&](int i) {
     const int j = seen.token(i) + lane;
     return i < i1 && j <= hi_p ? rk::page_of(a.map, b, j) : 0xffffffffu;
   };
-  auto load = [&](int i, uint32_t page) {
-    const int t0 = seen.token(i);
+  // A wave loads 16 rows of a tile straight to LDS, a lane 16 bytes: lane l's go
+  // to the l-th place of the load's part of the tile, so it asks for the piece
+  // that belongs there.  Pieces are swapped about in each row, so that the 16
+  // lanes of a read of Keys (one piece of 16 rows) and of Values (four rows of
+  // four pieces) meet different banks.  The rows lie in one page, or in two of
+  // eight rows.
+  constexpr int PerLoad = 64 / CH;  // rows
+  const int lrow = lane / CH, lpc = lane % CH;
+  uint32_t k_off[Passes];  // bytes
+#pragma unroll
+  for (int s = 0; s < Passes; ++s)
+    k_off[s] = 2 * (lrow * (uint32_t)a.k_ss + 8 * (lpc ^ key_swap<CH>(PerLoad * s + lrow)));
+  const uint32_t v_off = 2 * (lrow * (uint32_t)a.v_ss + 8 * (lpc ^ value_swap<CH>(lrow)));
+  const bool full = a.D == 8 * CH;
+  auto stage = [&](char* sk, char* sv, int i, uint32_t page, uint64_t there) {
+    const int first = 16 * wave, t0 = seen.token(i) + first;
+    const bool all = full && ((there >> first) & 0xffff) == 0xffff;
+    const char *kp[Passes], *vp[Passes];
 #pragma unroll
     for (int s = 0; s < Passes; ++s) {
-      const int row = srow + s * (kPagedThreads / CH);
-      const uint32_t pg = (uint32_t)__shfl((int)page, row, 64);
-      const int64_t at = (t0 + row) & ((1u << a.map.shift) - 1);
-      const bool ok = pg < (uint32_t)a.map.pages && 8 * pc < a.D;
-      kr[s] = ok ? *(const uint4*)(kb + (int64_t)pg * a.k_sp + at * a.k_ss + 8 * pc) : make_uint4(0, 0, 0, 0);
-      vr[s] = ok ? *(const uint4*)(vb + (int64_t)pg * a.v_sp + at * a.v_ss + 8 * pc) : make_uint4(0, 0, 0, 0);
+      const uint32_t pg = (uint32_t)__builtin_amdgcn_readlane((int)page, first + (PerLoad * s & 8));
+      const int64_t at = (t0 + PerLoad * s) & ((1u << a.map.shift) - 1);
+      kp[s] = (const char*)(kb + pg * a.k_sp + at * a.k_ss);
+      vp[s] = (const char*)(vb + pg * a.v_sp + at * a.v_ss);
     }
-  };
-  auto fk = [](int row) { return CH == 16 ? row & 15 : (row >> 1) & 7; };
-  auto fv = [](int row) { return CH == 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; };
-  auto store = [&](int buf) {
+    sk += first * Pitch;
+    sv += first * Pitch;
+    if (all) {
+#pragma unroll
+      for (int s = 0; s < Passes; ++s) {
+        __builtin_amdgcn_global_load_lds((global_ptr)(kp[s] + k_off[s]), (lds_ptr)(sk + s * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((global_ptr)(vp[s] + v_off), (lds_ptr)(sv + s * 1024), 16, 0, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int s = 0; s < Passes; ++s) {
-      const int row = srow + s * (kPagedThreads / CH);
-      *(uint4*)(s_k[buf] + row * Pitch + ((pc ^ fk(row)) << 4)) = kr[s];
-      *(uint4*)(s_v[buf] + row * Pitch + ((pc ^ fv(row)) << 4)) = vr[s];
+      const int row = PerLoad * s + lrow;
+      if (there >> (first + row) & 1) {
+        if (8 * (lpc ^ key_swap<CH>(row)) < a.D)
+          __builtin_amdgcn_global_load_lds((global_ptr)(kp[s] + k_off[s]), (lds_ptr)(sk + s * 1024), 16, 0, 0);
+        if (8 * (lpc ^ value_swap<CH>(row)) < a.D)
+          __builtin_amdgcn_global_load_lds((global_ptr)(vp[s] + v_off), (lds_ptr)(sv + s * 1024), 16, 0, 0);
+      } else {
+        *(uint4*)(sk + s * 1024 + 16 * lane) = make_uint4(0, 0, 0, 0);
+        *(uint4*)(sv + s * 1024 + 16 * lane) = make_uint4(0, 0, 0, 0);
+      }
     }
   };
-  uint32_t page = page_at(i0), page_next = page_at(i0 + 1);
-  if (i0 < i1) load(i0, page);
-  for (int i = i0; i < i1; ++i) {
-    const int buf = (i - i0) & 1;
-    store(buf);
-    __syncthreads();
-    const uint64_t there = __ballot(page < (uint32_t)a.map.pages);
-    page = page_next;
-    if (i + 1 < i1) load(i + 1, page);
-    page_next = page_at(i + 2);
+  int k_at[2 * NB], v_at[NB];  // of this lane's reads of a tile
+#pragma unroll
+  for (int c = 0; c < 2 * NB; ++c) k_at[c] = col * Pitch + (((2 * c + hi) ^ key_swap<CH>(col)) << 4);
+#pragma unroll
+  for (int c = 0; c < NB; ++c) {
+    // lane i of 16 addresses row i / 4, four channels from 4 (i % 4), and gets channel i of four rows
+    const int row = (lane & 15) >> 2, piece = 4 * c + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    v_at[c] = (4 * hi + row) * Pitch + ((piece ^ value_swap<CH>(row)) << 4) + 8 * (lane & 1);
+  }
+  auto multiply = [&](const char* sk, const char* sv, int i, uint64_t there) {
     const int t0 = seen.token(i);
     // tiles that no row of the wave sees
-    if (t0 > w_hi || (t0 + kTile - 1 <= w_lo - a.window && t0 >= a.sinks)) continue;
+    if (t0 > w_hi || (t0 + kTile - 1 <= w_lo - a.window && t0 >= a.sinks)) return;
     float x[2][16];
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb) {
@@ -215,21 +258,22 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
       for (int e = 0; e < 16; ++e) sc[e] = 0.f;
 #pragma unroll
       for (int c = 0; c < 2 * NB; ++c) {
-        const int row = 32 * tb + col;
-        const uint4 kf = *(const uint4*)(s_k[buf] + row * Pitch + (((2 * c + hi) ^ fk(row)) << 4));
+        const uint4 kf = *(const uint4*)(sk + k_at[c] + 32 * tb * Pitch);
         sc = mfma32<DT>(kf, q[c], sc);
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[tb][e] = sc[e] * a.scale_log2;
+      for (int e = 0; e < 16; ++e) x[tb][e] = sc[e];
     }
     const bool whole = there == ~0ull && t0 + kTile - 1 <= w_lo && (w_hi - t0 < a.window || t0 + kTile <= a.sinks);
     if (!whole) {
+      asm volatile("");  // a branch: most tiles are whole, and the masks cost more than the scores
+      const uint64_t mine_there = there >> (4 * hi);
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int k = 32 * tb + 8 * (e >> 2) + 4 * hi + (e & 3);
-          const bool on = rk::sees(p, t0 + k, a.window, a.sinks) && (there >> k & 1);
+          const int k = 32 * tb + 8 * (e >> 2) + (e & 3);
+          const bool on = rk::sees(p, t0 + 4 * hi + k, a.window, a.sinks) && (mine_there >> k & 1);
           x[tb][e] = on ? x[tb][e] : kNone;
         }
     }
@@ -239,19 +283,33 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, x[tb][e]);
     top = fmaxf(top, rk::shfl_xor(top, 32));
-    const float m_new = fmaxf(m, top), base = base_of(m_new);
-    const float keep = rk::fast_exp2(m - base);
-    m = m_new;
-    l *= keep;
+    // Weights are taken against an earlier maximum while they stay below 2^8: any
+    // base gives the same quotient, and few tiles raise the maximum by as much.
+    if (__any((top - m) * a.scale_log2 > kSlack)) {
+      const float m_new = fmaxf(m, top), keep = rk::fast_exp2((m - base_of(m_new)) * a.scale_log2);
+      m = m_new;
+      l *= keep;
 #pragma unroll
-    for (int c = 0; c < NB; ++c)
+      for (int c = 0; c < NB; ++c)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[c][e] *= keep;
+        for (int e = 0; e < 16; ++e) o[c][e] *= keep;
+    }
+    // Scale and base in one product, whose base is rounded: all of a row's weights
+    // take the same factor 2^(2^-24 base) from it, which far scores would make large.
+    float base = base_of(m) * a.scale_log2;
+    if (__any(fabsf(base) > kFar)) {
+      asm volatile("");
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[tb][e] -= base_of(m);
+      base = 0.f;
+    }
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        x[tb][e] = rk::fast_exp2(x[tb][e] - base);
+        x[tb][e] = rk::fast_exp2(__builtin_fmaf(x[tb][e], a.scale_log2, -base));
         l += x[tb][e];
       }
 #pragma unroll
@@ -261,18 +319,43 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
         const float* y = x[tb] + 8 * u;
         const uint4 w = make_uint4(DT::pack2(y[0], y[1]), DT::pack2(y[2], y[3]), DT::pack2(y[4], y[5]),
                                    DT::pack2(y[6], y[7]));
-        // lane i of 16 addresses row i / 4, four channels from 4 (i % 4), and gets channel i of four rows
-        const int row = 32 * tb + 16 * u + 4 * hi + ((lane & 15) >> 2);
 #pragma unroll
         for (int c = 0; c < NB; ++c) {
-          const int piece = 4 * c + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-          const char* at = s_v[buf] + row * Pitch + ((piece ^ fv(row)) << 4) + 8 * (lane & 1);
+          const char* at = sv + v_at[c] + (32 * tb + 16 * u) * Pitch;
           const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
           const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * Pitch));
           const uint2 u0 = __builtin_bit_cast(uint2, v0), u1 = __builtin_bit_cast(uint2, v1);
           o[c] = mfma32<DT>(make_uint4(u0.x, u0.y, u1.x, u1.y), w, o[c]);
         }
       }
+  };
+  if (i0 < i1) {
+    // pieces past D are never loaded: they stay zero
+    if (a.D < 8 * CH) {
+      for (int at = 16 * tid; at < kTile * Pitch; at += 16 * kPagedThreads) {
+        *(uint4*)(s_k0 + at) = *(uint4*)(s_k1 + at) = *(uint4*)(s_v0 + at) = *(uint4*)(s_v1 + at) =
+            make_uint4(0, 0, 0, 0);
+      }
+      __syncthreads();
+    }
+    auto is_there = [&](uint32_t page) { return (uint64_t)__ballot(page < (uint32_t)a.map.pages); };
+    uint32_t page = page_at(i0), page_next = page_at(i0 + 1);
+    uint64_t there = is_there(page);
+    stage(s_k0, s_v0, i0, page, there);
+    auto step = [&](int i, const char* sk, const char* sv, char* next_k, char* next_v) {
+      loads_done();
+      __syncthreads();  // this tile is there for all waves, and the last one has been read by all
+      const uint64_t here = there;
+      page = page_next;
+      there = is_there(page);
+      page_next = page_at(i + 2);
+      if (i + 1 < i1) stage(next_k, next_v, i + 1, page, there);
+      multiply(sk, sv, i, here);
+    };
+    for (int i = i0; i < i1; i += 2) {
+      step(i, s_k0, s_v0, s_k1, s_v1);
+      if (i + 1 < i1) step(i + 1, s_k1, s_v1, s_k0, s_v0);
+    }
   }
   l += rk::shfl_xor(l, 32);
   // Weight 0 times an infinity or a NaN is a NaN: a tile's Values reach rows
@@ -301,7 +384,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
         *(float4*)(dst + 32 * c + 2 * e + 4 * hi) = make_float4(o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]);
-    if (hi == 0) *(float2*)(a.ml + 2 * rec) = make_float2(m, l);
+    if (hi == 0) *(float2*)(a.ml + 2 * rec) = make_float2(m * a.scale_log2, l);
     return;
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
