@@ -39,6 +39,9 @@ constexpr int kRows = kWaveRows * kPagedWaves;
 constexpr float kSlack = 8.f;           // log2 of what weights may grow to
 constexpr float kFar = 16384.f;         // a base that is rounded by 2^-11 at most
 
+// Instructions stay on their side.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
 // The wave's loads to LDS have arrived.
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -50,6 +53,14 @@ __device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(rk::bf16x8, a),
                                                    __builtin_bit_cast(rk::bf16x8, b), c, 0, 0, 0);
+}
+
+// The values of this lane and of lane ^ 32, in some order.
+__device__ __forceinline__ float2 both_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x),
+                                                  false, false);
+  const uint32_t one = r[0], two = r[1];  // (bit_cast of a vector's element takes the first)
+  return make_float2(__builtin_bit_cast(float, one), __builtin_bit_cast(float, two));
 }
 
 // Where the pieces of a row of Keys or Values lie in LDS: piece c at c ^ swap.
@@ -121,7 +132,8 @@ __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, r
   dst[(c + 1) * a.o_sd] = DT::from_f32(y1 * inv);
 }
 
-template <class DT, int NB>
+// NB: blocks of 32 channels.  FULL: all pieces of a row in LDS hold channels.
+template <class DT, int NB, bool FULL>
 __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArgs a) {
   constexpr int CH = NB <= 2 ? 8 : 16;        // 16-byte pieces of a row in LDS
   constexpr int Pitch = CH * 16;              // bytes
@@ -154,7 +166,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
   const int lo_p = max(p0 + row0 / a.G, 0), hi_p = p0 + (row0 + rows - 1) / a.G;
   const rk::Seen<kTile> seen(lo_p, hi_p, a.window, a.sinks);
   const int i0 = (int)((int64_t)seen.blocks * split / a.splits);
-  const int i1 = (int)((int64_t)seen.blocks * (split + 1) / a.splits);
+  const int i1 = a.map.pages > 0 ? (int)((int64_t)seen.blocks * (split + 1) / a.splits) : i0;
 
   // the wave's rows: this lane's query and its position
   const int r = wave * kWaveRows + col;
@@ -183,59 +195,72 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
 
   const uint16_t* kb = (const uint16_t*)a.k + h * a.k_sh;
   const uint16_t* vb = (const uint16_t*)a.v + h * a.v_sh;
-  // lane l holds the page of token l of a tile; one past the pool where no row sees it
-  auto page_at = [&](int i) {
-    const int j = seen.token(i) + lane;
-    return i < i1 && j <= hi_p ? rk::page_of(a.map, b, j) : 0xffffffffu;
+  // lane l holds the page of token l of a tile, of the last token for those behind it
+  auto page_at = [&](int i) { return i < i1 ? rk::page_of(a.map, b, min(seen.token(i) + lane, hi_p)) : 0u; };
+  auto there_of = [&](int i, uint32_t page) {
+    return (uint64_t)__ballot(page < (uint32_t)a.map.pages && seen.token(i) + lane <= hi_p);
   };
   // A wave loads 16 rows of a tile straight to LDS, a lane 16 bytes: lane l's go
   // to the l-th place of the load's part of the tile, so it asks for the piece
   // that belongs there.  Pieces are swapped about in each row, so that the 16
   // lanes of a read of Keys (one piece of 16 rows) and of Values (four rows of
-  // four pieces) meet different banks.  The rows lie in one page, or in two of
-  // eight rows.
-  constexpr int PerLoad = 64 / CH;  // rows
+  // four pieces) meet different banks.  Eight rows lie in one page: one scalar
+  // address for them, and the lanes' offsets, which stay from tile to tile.  Behind
+  // the last token its row is loaded again (its weight is zero there), and where
+  // there is no page the pool's first row.
+  constexpr int PerLoad = 64 / CH;   // rows
+  constexpr int Loads = Passes / 2;  // of eight rows
   const int lrow = lane / CH, lpc = lane % CH;
-  uint32_t k_off[Passes];  // bytes
+  uint32_t k_off[Passes], v_off[Passes];  // bytes
+  int k_piece[Passes], v_piece;
 #pragma unroll
-  for (int s = 0; s < Passes; ++s)
-    k_off[s] = 2 * (lrow * (uint32_t)a.k_ss + 8 * (lpc ^ key_swap<CH>(PerLoad * s + lrow)));
-  const uint32_t v_off = 2 * (lrow * (uint32_t)a.v_ss + 8 * (lpc ^ value_swap<CH>(lrow)));
-  const bool full = a.D == 8 * CH;
-  auto stage = [&](char* sk, char* sv, int i, uint32_t page, uint64_t there) {
-    const int first = 16 * wave, t0 = seen.token(i) + first;
-    const bool all = full && ((there >> first) & 0xffff) == 0xffff;
-    const char *kp[Passes], *vp[Passes];
+  for (int s = 0; s < Passes; ++s) k_piece[s] = lpc ^ key_swap<CH>(PerLoad * s + lrow);
+  v_piece = lpc ^ value_swap<CH>(lrow);
+  // (the offsets of tile i: those behind its last token count in the last tile alone)
+  auto row_of = [&](int i, int s) {
+    const int last = hi_p - seen.token(i) - 16 * wave - (s < Loads ? 0 : 8);
+    return (uint32_t)min(PerLoad * (s % Loads) + lrow, max(last, 0));
+  };
+  auto k_offsets = [&](int i) {
 #pragma unroll
-    for (int s = 0; s < Passes; ++s) {
-      const uint32_t pg = (uint32_t)__builtin_amdgcn_readlane((int)page, first + (PerLoad * s & 8));
-      const int64_t at = (t0 + PerLoad * s) & ((1u << a.map.shift) - 1);
-      kp[s] = (const char*)(kb + pg * a.k_sp + at * a.k_ss);
-      vp[s] = (const char*)(vb + pg * a.v_sp + at * a.v_ss);
-    }
-    sk += first * Pitch;
-    sv += first * Pitch;
-    if (all) {
+    for (int s = 0; s < Passes; ++s) k_off[s] = 2 * (row_of(i, s) * (uint32_t)a.k_ss + 8 * k_piece[s]);
+  };
+  auto v_offsets = [&](int i) {
 #pragma unroll
-      for (int s = 0; s < Passes; ++s) {
-        __builtin_amdgcn_global_load_lds((global_ptr)(kp[s] + k_off[s]), (lds_ptr)(sk + s * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((global_ptr)(vp[s] + v_off), (lds_ptr)(sv + s * 1024), 16, 0, 0);
+    for (int s = 0; s < Passes; ++s) v_off[s] = 2 * (row_of(i, s) * (uint32_t)a.v_ss + 8 * v_piece);
+  };
+  struct Eight {
+    const char* at[2];
+  };
+  auto rows_at = [&](int i, uint32_t page, const uint16_t* src, int64_t sp, int64_t ss) {
+    const int t0 = seen.token(i) + 16 * wave;
+    Eight r;
+    if (t0 + 15 <= hi_p && a.map.shift > 3) {
+      const uint32_t pg = (uint32_t)__builtin_amdgcn_readlane((int)page, 16 * wave);
+      const int64_t row = t0 & ((1u << a.map.shift) - 1);
+      const bool ok = pg < (uint32_t)a.map.pages;
+      r.at[0] = (const char*)(src + (ok ? pg : 0u) * sp + (ok ? row : 0) * ss);
+      r.at[1] = r.at[0] + 16 * ss;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t pg = (uint32_t)__builtin_amdgcn_readlane((int)page, 16 * wave + 8 * e);
+        const int64_t row = min(t0 + 8 * e, hi_p) & ((1u << a.map.shift) - 1);
+        const bool ok = pg < (uint32_t)a.map.pages;
+        r.at[e] = (const char*)(src + (ok ? pg : 0u) * sp + (ok ? row : 0) * ss);
       }
-      return;
     }
-#pragma unroll
-    for (int s = 0; s < Passes; ++s) {
-      const int row = PerLoad * s + lrow;
-      if (there >> (first + row) & 1) {
-        if (8 * (lpc ^ key_swap<CH>(row)) < a.D)
-          __builtin_amdgcn_global_load_lds((global_ptr)(kp[s] + k_off[s]), (lds_ptr)(sk + s * 1024), 16, 0, 0);
-        if (8 * (lpc ^ value_swap<CH>(row)) < a.D)
-          __builtin_amdgcn_global_load_lds((global_ptr)(vp[s] + v_off), (lds_ptr)(sv + s * 1024), 16, 0, 0);
-      } else {
-        *(uint4*)(sk + s * 1024 + 16 * lane) = make_uint4(0, 0, 0, 0);
-        *(uint4*)(sv + s * 1024 + 16 * lane) = make_uint4(0, 0, 0, 0);
-      }
-    }
+    return r;
+  };
+  auto load_k = [&](char* dst, const Eight& r, int s) {
+    if (FULL || 8 * k_piece[s] < a.D)
+      __builtin_amdgcn_global_load_lds((global_ptr)(r.at[s / Loads] + k_off[s]),
+                                       (lds_ptr)(dst + 16 * wave * Pitch + s * 1024), 16, 0, 0);
+  };
+  auto load_v = [&](char* dst, const Eight& r, int s) {
+    if (FULL || 8 * v_piece < a.D)
+      __builtin_amdgcn_global_load_lds((global_ptr)(r.at[s / Loads] + v_off[s]),
+                                       (lds_ptr)(dst + 16 * wave * Pitch + s * 1024), 16, 0, 0);
   };
   int k_at[2 * NB], v_at[NB];  // of this lane's reads of a tile
 #pragma unroll
@@ -246,46 +271,52 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
     const int row = (lane & 15) >> 2, piece = 4 * c + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     v_at[c] = (4 * hi + row) * Pitch + ((piece ^ value_swap<CH>(row)) << 4) + 8 * (lane & 1);
   }
-  auto multiply = [&](const char* sk, const char* sv, int i, uint64_t there) {
-    const int t0 = seen.token(i);
-    // tiles that no row of the wave sees
-    if (t0 > w_hi || (t0 + kTile - 1 <= w_lo - a.window && t0 >= a.sinks)) return;
-    float x[2][16];
+  // Scores of a tile: products of two chains, reads a few products ahead.
+  auto scores = [&](const char* sk, f32x16 (&n)[2]) {
 #pragma unroll
-    for (int tb = 0; tb < 2; ++tb) {
-      f32x16 sc;
+    for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+      for (int e = 0; e < 16; ++e) n[tb][e] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2 * NB; ++c) {
-        const uint4 kf = *(const uint4*)(sk + k_at[c] + 32 * tb * Pitch);
-        sc = mfma32<DT>(kf, q[c], sc);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[tb][e] = sc[e];
-    }
-    const bool whole = there == ~0ull && t0 + kTile - 1 <= w_lo && (w_hi - t0 < a.window || t0 + kTile <= a.sinks);
-    if (!whole) {
-      asm volatile("");  // a branch: most tiles are whole, and the masks cost more than the scores
-      const uint64_t mine_there = there >> (4 * hi);
+    for (int c = 0; c < 2 * NB; ++c)
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb)
+        n[tb] = mfma32<DT>(*(const uint4*)(sk + k_at[c] + 32 * tb * Pitch), q[c], n[tb]);
+  };
+  // -inf where a row does not see the token.
+  auto mask = [&](int i, uint32_t page, f32x16 (&n)[2]) {
+    const int t0 = seen.token(i);
+    const uint64_t there = there_of(i, page);
+    if (there == ~0ull && t0 + kTile - 1 <= w_lo && (w_hi - t0 < a.window || t0 + kTile <= a.sinks)) return;
+    asm volatile("");  // a branch: most tiles are whole, and the masks cost more than the scores
+    const uint64_t mine_there = there >> (4 * hi);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int k = 32 * tb + 8 * (e >> 2) + (e & 3);
-          const bool on = rk::sees(p, t0 + 4 * hi + k, a.window, a.sinks) && (mine_there >> k & 1);
-          x[tb][e] = on ? x[tb][e] : kNone;
-        }
-    }
+    for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int k = 32 * tb + 8 * (e >> 2) + (e & 3);
+        const bool on = rk::sees(p, t0 + 4 * hi + k, a.window, a.sinks) && (mine_there >> k & 1);
+        n[tb][e] = on ? n[tb][e] : kNone;
+      }
+  };
+  float base = 0.f;  // what the weights are against, scaled
+  auto top_of = [&](const f32x16 (&n)[2]) {
     float top = kNone;
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, x[tb][e]);
-    top = fmaxf(top, rk::shfl_xor(top, 32));
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, n[tb][e]);
+    return top;
+  };
+  // The next tile's scores are known: what weights are against, and the sums so far
+  // against that.
+  auto rebase = [&](float top, f32x16 (&n)[2]) {
+    const float2 tops = both_halves(top);
+    top = fmaxf(tops.x, tops.y);
     // Weights are taken against an earlier maximum while they stay below 2^8: any
     // base gives the same quotient, and few tiles raise the maximum by as much.
     if (__any((top - m) * a.scale_log2 > kSlack)) {
+      asm volatile("");
       const float m_new = fmaxf(m, top), keep = rk::fast_exp2((m - base_of(m_new)) * a.scale_log2);
       m = m_new;
       l *= keep;
@@ -296,68 +327,167 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
     }
     // Scale and base in one product, whose base is rounded: all of a row's weights
     // take the same factor 2^(2^-24 base) from it, which far scores would make large.
-    float base = base_of(m) * a.scale_log2;
+    base = base_of(m) * a.scale_log2;
     if (__any(fabsf(base) > kFar)) {
       asm volatile("");
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[tb][e] -= base_of(m);
+        for (int e = 0; e < 16; ++e) n[tb][e] -= base_of(m);
       base = 0.f;
     }
-#pragma unroll
-    for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        x[tb][e] = rk::fast_exp2(__builtin_fmaf(x[tb][e], a.scale_log2, -base));
-        l += x[tb][e];
-      }
-#pragma unroll
-    for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float* y = x[tb] + 8 * u;
-        const uint4 w = make_uint4(DT::pack2(y[0], y[1]), DT::pack2(y[2], y[3]), DT::pack2(y[4], y[5]),
-                                   DT::pack2(y[6], y[7]));
-#pragma unroll
-        for (int c = 0; c < NB; ++c) {
-          const char* at = sv + v_at[c] + (32 * tb + 16 * u) * Pitch;
-          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
-          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * Pitch));
-          const uint2 u0 = __builtin_bit_cast(uint2, v0), u1 = __builtin_bit_cast(uint2, v1);
-          o[c] = mfma32<DT>(make_uint4(u0.x, u0.y, u1.x, u1.y), w, o[c]);
-        }
-      }
+  };
+  // Weight k of a tile's 32 in this lane, pairs of them in the products' type.
+  auto weight = [&](const f32x16 (&n)[2], float (&y)[32], uint32_t (&w)[16], int k) {
+    y[k] = rk::fast_exp2(__builtin_fmaf(n[k >> 4][k & 15], a.scale_log2, -base));
+    l += y[k];
+    if (k & 1) {
+      w[k >> 1] = DT::pack2(y[k - 1], y[k]);
+      asm volatile("" : "+v"(w[k >> 1]), "+v"(l));  // here, and not where it is used
+    }
+  };
+  auto value_at = [&](const char* sv, int g, int c) {  // 16 tokens by 32 channels
+    const char* at = sv + v_at[c] + 16 * g * Pitch;
+    const uint2 u0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at));
+    const uint2 u1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * Pitch)));
+    return make_uint4(u0.x, u0.y, u1.x, u1.y);
   };
   if (i0 < i1) {
-    // pieces past D are never loaded: they stay zero
-    if (a.D < 8 * CH) {
+    if (!FULL) {  // pieces past D are never loaded: they stay zero
       for (int at = 16 * tid; at < kTile * Pitch; at += 16 * kPagedThreads) {
         *(uint4*)(s_k0 + at) = *(uint4*)(s_k1 + at) = *(uint4*)(s_v0 + at) = *(uint4*)(s_v1 + at) =
             make_uint4(0, 0, 0, 0);
       }
       __syncthreads();
     }
-    auto is_there = [&](uint32_t page) { return (uint64_t)__ballot(page < (uint32_t)a.map.pages); };
-    uint32_t page = page_at(i0), page_next = page_at(i0 + 1);
-    uint64_t there = is_there(page);
-    stage(s_k0, s_v0, i0, page, there);
-    auto step = [&](int i, const char* sk, const char* sv, char* next_k, char* next_v) {
+    // pages of tiles i + 1 (Values to come), i + 2 (Keys to come) and i + 3
+    const int end = i1 - 1;
+    uint32_t page0 = page_at(i0), page1 = page_at(min(i0 + 1, end)), page2 = page_at(min(i0 + 2, end));
+    f32x16 s[2];
+    {
+      k_offsets(i0);
+      const Eight k0 = rows_at(i0, page0, kb, a.k_sp, a.k_ss), v0 = rows_at(i0, page0, vb, a.v_sp, a.v_ss);
+#pragma unroll
+      for (int r = 0; r < Passes; ++r) load_k(s_k0, k0, r);
+      v_offsets(i0);
+#pragma unroll
+      for (int r = 0; r < Passes; ++r) load_v(s_v0, v0, r);
       loads_done();
-      __syncthreads();  // this tile is there for all waves, and the last one has been read by all
-      const uint64_t here = there;
-      page = page_next;
-      there = is_there(page);
-      page_next = page_at(i + 2);
-      if (i + 1 < i1) stage(next_k, next_v, i + 1, page, there);
-      multiply(sk, sv, i, here);
+      __syncthreads();
+      k_offsets(min(i0 + 1, end));
+      const Eight k1 = rows_at(min(i0 + 1, end), page1, kb, a.k_sp, a.k_ss);
+#pragma unroll
+      for (int r = 0; r < Passes; ++r) load_k(s_k1, k1, r);
+      scores(s_k0, s);
+      mask(i0, page0, s);
+      rebase(top_of(s), s);
+    }
+    // Tile i's weights and products with Values, beside the products of tile i + 1's
+    // scores and the loads of what the next step takes.
+    auto step = [&](int i, const char* next_k, const char* sv, char* k_to, char* v_to, auto last) {
+      constexpr bool kLast = decltype(last)::value;
+      loads_done();
+      __syncthreads();  // these tiles are there for all waves, and the last ones have been read by all
+      const int ik = min(i + 2, end);
+      uint32_t page3 = 0;
+      Eight rk_, rv;
+      if (!kLast) {
+        page3 = page_at(min(i + 3, end));
+        if (ik == end) {
+          asm volatile("");  // a branch
+          k_offsets(ik);
+          if (i + 1 == end) v_offsets(end);
+        }
+        rk_ = rows_at(ik, page2, kb, a.k_sp, a.k_ss);
+        rv = rows_at(i + 1, page1, vb, a.v_sp, a.v_ss);
+      }
+      f32x16 n[2];
+      float y[32];
+      uint32_t w[16];
+      // Two products at a time, and what the other units do meanwhile: a product
+      // takes the matrix unit 32 cycles, an exponential its own 16.  The fences keep
+      // the mixture as it is written.
+      constexpr int kPairs = 2 * NB;
+      if (!kLast) {
+        uint4 k0[kPairs], k1[kPairs];
+        auto read = [&](int c) {
+          k0[c] = *(const uint4*)(next_k + k_at[c]);
+          k1[c] = *(const uint4*)(next_k + k_at[c] + 32 * Pitch);
+        };
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) n[tb][e] = 0.f;
+        read(0);
+        if (kPairs > 1) read(1);
+        fence();
+#pragma unroll
+        for (int c = 0; c < kPairs; ++c) {
+          if (c + 2 < kPairs) read(c + 2);
+          n[0] = mfma32<DT>(k0[c], q[c], n[0]);
+          n[1] = mfma32<DT>(k1[c], q[c], n[1]);
+#pragma unroll
+          for (int r = 0; r < 2 * Passes; ++r)
+            if (r * kPairs / (2 * Passes) == c) r & 1 ? load_k(k_to, rk_, r >> 1) : load_v(v_to, rv, r >> 1);
+#pragma unroll
+          for (int k = 0; k < 24; ++k)
+            if (k * kPairs / 24 == c) weight(s, y, w, k);
+          fence();
+        }
+        mask(i + 1, page1, n);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 24; ++k) weight(s, y, w, k);
+      }
+      float top = kNone;
+      {
+        constexpr int kProducts = 4 * NB;  // (g, c): g 16 tokens, c 32 channels
+        uint4 v[kProducts];
+        auto read = [&](int j) { v[j] = value_at(sv, j / NB, j % NB); };
+#pragma unroll
+        for (int j = 0; j < 4; ++j) read(j);
+        fence();
+#pragma unroll
+        for (int j = 0; j < kProducts; j += 2) {
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            if (j + d + 4 < kProducts) read(j + d + 4);
+            const int g = (j + d) / NB, c = (j + d) % NB;
+            o[c] = mfma32<DT>(v[j + d], make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]), o[c]);
+          }
+#pragma unroll
+          for (int k = 24; k < 32; ++k)
+            if ((k - 24) * (3 * NB / 2) / 8 == j / 2) weight(s, y, w, k);
+          if (!kLast) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (k * (kProducts / 2) / 32 == j / 2) top = fmaxf(top, n[k >> 4][k & 15]);
+          }
+          fence();
+        }
+      }
+      if (!kLast) {
+        rebase(top, n);
+        s[0] = n[0];
+        s[1] = n[1];
+      }
+      page1 = page2;
+      page2 = page3;
     };
-    for (int i = i0; i < i1; i += 2) {
-      step(i, s_k0, s_v0, s_k1, s_v1);
-      if (i + 1 < i1) step(i + 1, s_k1, s_v1, s_k0, s_v0);
+    int i = i0;
+    for (; i + 2 < i1; i += 2) {
+      step(i, s_k1, s_v0, s_k0, s_v1, std::false_type{});
+      step(i + 1, s_k0, s_v1, s_k1, s_v0, std::false_type{});
+    }
+    if (i + 1 < i1) {
+      step(i, s_k1, s_v0, s_k0, s_v1, std::false_type{});
+      step(i + 1, s_k0, s_v1, s_k1, s_v0, std::true_type{});
+    } else {
+      step(i, s_k1, s_v0, s_k0, s_v1, std::true_type{});
     }
   }
-  l += rk::shfl_xor(l, 32);
+  const float2 sums = both_halves(l);
+  l = sums.x + sums.y;
   // Weight 0 times an infinity or a NaN is a NaN: a tile's Values reach rows
   // that do not see them.  Rows that are not finite are summed again from what
   // they see.
@@ -453,19 +583,21 @@ int64_t window_slots(const PagedArgs& a) {
 int window_launch(const PagedArgs& a, int32_t dtype, hipStream_t s) {
   const int64_t grid = window_slots(a) * a.H * a.splits, rows = a.N * a.Hq;
   const int NB = (a.D + 31) / 32;
-  auto on = [&](auto dt, auto nb) {
-    hipLaunchKernelGGL((window_kernel<decltype(dt), decltype(nb)::value>), dim3((unsigned)grid), dim3(kPagedThreads),
-                       0, s, a);
+  auto on = [&](auto dt, auto nb, auto full) {
+    hipLaunchKernelGGL((window_kernel<decltype(dt), decltype(nb)::value, decltype(full)::value>), dim3((unsigned)grid),
+                       dim3(kPagedThreads), 0, s, a);
     if (a.splits > 1)
       hipLaunchKernelGGL((window_join_kernel<decltype(dt)>), dim3((unsigned)((rows + kPagedWaves - 1) / kPagedWaves)),
                          dim3(kPagedThreads), 0, s, a, 32 * NB);
   };
   auto by_dim = [&](auto dt) {
+    if (a.D == 128) return on(dt, std::integral_constant<int, 4>{}, std::true_type{});
+    if (a.D == 64) return on(dt, std::integral_constant<int, 2>{}, std::true_type{});
     switch (NB) {
-      case 1: on(dt, std::integral_constant<int, 1>{}); break;
-      case 2: on(dt, std::integral_constant<int, 2>{}); break;
-      case 3: on(dt, std::integral_constant<int, 3>{}); break;
-      default: on(dt, std::integral_constant<int, 4>{});
+      case 1: return on(dt, std::integral_constant<int, 1>{}, std::false_type{});
+      case 2: return on(dt, std::integral_constant<int, 2>{}, std::false_type{});
+      case 3: return on(dt, std::integral_constant<int, 3>{}, std::false_type{});
+      default: return on(dt, std::integral_constant<int, 4>{}, std::false_type{});
     }
   };
   dtype == RK_F16 ? by_dim(F16{}) : by_dim(BF16{});
