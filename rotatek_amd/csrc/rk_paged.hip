@@ -43,7 +43,7 @@ constexpr int kRows = 16;                     // queries of a unit
 
 // Pieces of one request and KV head.
 __device__ __forceinline__ int pieces_of(const PagedArgs& a, int b) {
-  const int p = rk::len_of(a.map, b) - 1;
+  const int p = a.map.pages > 0 ? rk::len_of(a.map, b) - 1 : -1;
   const rk::Seen<kStep> s(max(p, 0), p, a.window, a.sinks);
   return (s.blocks + kPagedWaves - 1) / kPagedWaves;
 }
@@ -62,16 +62,46 @@ __device__ __forceinline__ Shares shares_of(const PagedArgs& a, int per_request,
   return s;
 }
 
-// KF: blocks of 32 channels (2 or 4).
-template <class DT, int KF>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_split_kernel(const PagedArgs a) {
+// Bytes that are used once.
+template <class V>
+__device__ __forceinline__ V load_once(const void* p) {
+  return __builtin_nontemporal_load((const V*)p);
+}
+
+// The largest over the four lanes n, 16 + n, 32 + n, 48 + n.
+__device__ __forceinline__ float column_max(float x) {
+  uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t r0 = r[0], r1 = r[1];
+  x = fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+  u = __builtin_bit_cast(uint32_t, x);
+  const auto t = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t t0 = t[0], t1 = t[1];
+  return fmaxf(__builtin_bit_cast(float, t0), __builtin_bit_cast(float, t1));
+}
+
+// Pages of a wave's 32 tokens.  Lane (g, n) has Keys of tokens n and 16 + n,
+// channels 32 c + 8 g, and Values of tokens 4 g + 0..3 and 16 + 4 g + 0..3,
+// channels VC n.  Sixteen neighbouring tokens lie in one page, unless pages have
+// eight rows.
+struct Pages {
+  uint32_t k[2], v[2];
+};
+
+// Workgroups of a CU: what their registers allow.
+constexpr int per_cu(int KF) { return KF == 4 ? 2 : 3; }
+
+// KF: blocks of 32 channels (2 or 4).  EIGHT: pages of eight rows.
+template <class DT, int KF, bool EIGHT>
+__global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(const PagedArgs a) {
   constexpr int KD = 32 * KF;      // channels, stored ones up to D
   constexpr int VC = KD / 16;      // channels of a Value piece: 4 or 8
   constexpr int AccPitch = KD + 4;
+  typedef unsigned int piece __attribute__((ext_vector_type(KF)));
   __shared__ int s_wave[kPagedWaves], s_found[2];
   __shared__ float s_acc[kPagedWaves][kRows][AccPitch];
   __shared__ float s_ml[kPagedWaves][kRows][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int blocks = (a.G + kRows - 1) / kRows;
   const int units = a.H * blocks;  // of a request
@@ -120,85 +150,181 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_split_kernel(const Pag
 #pragma unroll
     for (int j = 0; j < VC; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int last = min(kPagedWaves * (off + take), seen.blocks);
-    for (int i = kPagedWaves * off + wave; i < last; i += kPagedWaves) {
+    const uint32_t in_page = (1u << a.map.shift) - 1;
+    // Bytes from a row group's first row to this lane's piece.  Behind the last
+    // token its row is read again, and channels past D are the first ones again:
+    // they count for nothing (`part`).
+    uint32_t k_off[2], v_off[2][4];
+    auto offsets = [&](int left) {  // tokens of the step that are there
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int end = max(left - 16 * s, 1) - 1;
+        const uint32_t row = EIGHT ? 0 : min(n, end);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t at = (EIGHT ? min(4 * g + e, end) - min(4 * g, end) : min(4 * g + e, end));
+          v_off[s][e] = 2 * (at * (uint32_t)a.v_ss + (VC * n < a.D ? VC * n : 0));
+        }
+        k_off[s] = 2 * (row * (uint32_t)a.k_ss);
+      }
+    };
+    offsets(kStep);
+    auto pages_at = [&](int i) {  // (past the last step: the last one's again)
+      const int t0 = seen.token(min(i, last - 1));
+      Pages x;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        x.k[s] = rk::page_of(a.map, b, min(t0 + 16 * s + (EIGHT ? n : 0), p));
+        x.v[s] = EIGHT ? rk::page_of(a.map, b, min(t0 + 16 * s + 4 * g, p)) : 0;
+      }
+      return x;
+    };
+    // The tokens of step i that the queries see and that have a page.
+    auto there_of = [&](int i, const Pages& at) {
       const int t0 = seen.token(i);
-      // Keys: token t0 + n (+ 16); Values: tokens t0 + 4 g + 0..3 (+ 16)
-      uint4 k[2][KF];
       uint32_t there = 0;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int j = t0 + 16 * s + n;
-        uint32_t page = 0;
-        bool ok = rk::sees(p, j, a.window, a.sinks);
-        if (ok) {
-          page = rk::page_of(a.map, b, j);
-          ok = page < (uint32_t)a.map.pages;
-        }
+        const bool ok = at.k[s] < (uint32_t)a.map.pages && rk::sees(p, t0 + 16 * s + n, a.window, a.sinks);
         there |= (uint32_t)(__ballot(ok) & 0xffff) << (16 * s);
-        const uint16_t* row = kb + (int64_t)page * a.k_sp + (int64_t)(j & ((1u << a.map.shift) - 1)) * a.k_ss;
-#pragma unroll
-        for (int c = 0; c < KF; ++c)
-          k[s][c] = ok && 32 * c + 8 * g < a.D ? *(const uint4*)(row + 32 * c + 8 * g) : make_uint4(0, 0, 0, 0);
       }
-      uint32_t v[8][VC / 2];
+      return there;
+    };
+    // First rows of either sixteen tokens (the pool's first row where there is no page).
+    auto rows_at = [&](int i, const uint32_t (&page)[2], int first, const uint16_t* src, int64_t sp, int64_t ss,
+                       const char* (&at)[2]) {
+      const int t0 = seen.token(i);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int j = t0 + 16 * s + 4 * g;
-        uint32_t page = 0;
-        const uint32_t mine = (there >> (16 * s + 4 * g)) & 15;
-        if (mine) page = rk::page_of(a.map, b, j);
-        const uint16_t* row = vb + (int64_t)page * a.v_sp + (int64_t)(j & ((1u << a.map.shift) - 1)) * a.v_ss + VC * n;
+        uint32_t pg = page[s];
+        if (!EIGHT) pg = (uint32_t)__builtin_amdgcn_readfirstlane((int)pg);
+        const bool ok = pg < (uint32_t)a.map.pages;
+        const int64_t row = min(t0 + 16 * s + (EIGHT ? first : 0), p) & in_page;
+        at[s] = (const char*)(src + (ok ? pg : 0u) * sp + (ok ? row : 0) * ss);
+      }
+    };
+    rk::u32x4 k[2][KF];
+    uint32_t v[8][KF];
+    auto load_k = [&](int i, const Pages& x) {
+      const char* at[2];
+      rows_at(i, x.k, n, kb, a.k_sp, a.k_ss, at);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int c = 0; c < KF; ++c) {
+          const int ch = 32 * c + 8 * g;
+          k[s][c] = load_once<rk::u32x4>(at[s] + k_off[s] + 2 * (KD == a.D || ch < a.D ? ch : 0));
+        }
+    };
+    auto load_v = [&](int i, const Pages& x) {
+      const char* at[2];
+      rows_at(i, EIGHT ? x.v : x.k, 4 * g, vb, a.v_sp, a.v_ss, at);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool ok = (mine >> e & 1) && VC * n < a.D;
-          if constexpr (VC == 8) {
-            const uint4 x = ok ? *(const uint4*)(row + e * a.v_ss) : make_uint4(0, 0, 0, 0);
-            v[4 * s + e][0] = x.x; v[4 * s + e][1] = x.y; v[4 * s + e][2] = x.z; v[4 * s + e][3] = x.w;
-          } else {
-            const uint2 x = ok ? *(const uint2*)(row + e * a.v_ss) : make_uint2(0, 0);
-            v[4 * s + e][0] = x.x; v[4 * s + e][1] = x.y;
+          const piece y = load_once<piece>(at[s] + v_off[s][e]);
+#pragma unroll
+          for (int d = 0; d < KF; ++d) v[4 * s + e][d] = y[d];
+        }
+    };
+    // Scores of the Keys at hand.  Then these registers take the next step's rows.
+    const int i0 = kPagedWaves * off + wave;
+    if (i0 < last) {
+      Pages now = pages_at(i0), next = pages_at(i0 + kPagedWaves);
+      auto cut = [&](int i) {  // the step that tokens end in is the last one
+        if (seen.token(i) + kStep - 1 > p) {
+          asm volatile("");
+          offsets(p + 1 - seen.token(i));
+        }
+      };
+      cut(i0);
+      load_k(i0, now);
+      load_v(i0, now);
+      for (int i = i0; i < last; i += kPagedWaves) {
+        const int then = i + kPagedWaves, t0 = seen.token(i);
+        // A CU's older workgroup goes first wherever both could, and ends early; by
+        // turns they end together (32 requests of 16000 tokens: 344 us, 338 so).
+        if (((i / kPagedWaves) ^ (2 * blockIdx.x >= gridDim.x ? 1 : 0)) & 1)
+          __builtin_amdgcn_s_setprio(2);
+        else
+          __builtin_amdgcn_s_setprio(0);
+        const bool part = a.D != KD || t0 + kStep - 1 > p || (p - t0 >= a.window && t0 + kStep > a.sinks) ||
+                          !__all(now.k[0] < (uint32_t)a.map.pages && now.k[1] < (uint32_t)a.map.pages);
+        uint32_t there = ~0u;
+        if (part) {
+          asm volatile("");  // a branch: most steps are whole
+          there = there_of(i, now);
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int c = 0; c < KF; ++c)
+              if (32 * c + 8 * g >= a.D) k[s][c] = rk::u32x4{0, 0, 0, 0};
+        }
+        f32x4 sc[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KF; ++c)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) sc[s] = DT::mfma(__builtin_bit_cast(uint4, k[s][c]), q[c], sc[s]);
+        if (then < last) {
+          cut(then);
+          load_k(then, next);
+        }
+        if (part) {
+          asm volatile("");
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool on = there >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1;
+            sc[e >> 2][e & 3] = on ? sc[e >> 2][e & 3] : kNone;
+#pragma unroll
+            for (int d = 0; d < KF; ++d) v[e][d] = on ? v[e][d] : 0;
           }
         }
-      }
-      f32x4 sc[2];
+        float top = kNone;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, sc[e >> 2][e & 3]);
+        top = column_max(top);
+        // against an earlier maximum while weights stay below 2^8, as any base gives
+        // the same quotient
+        if (__any((top - m) * a.scale_log2 > rk::kSlack)) {
+          asm volatile("");
+          const float m_new = fmaxf(m, top), keep = rk::fast_exp2((m - base_of(m_new)) * a.scale_log2);
+          m = m_new;
+          l *= keep;
 #pragma unroll
-        for (int c = 0; c < KF; ++c) sc[s] = DT::mfma(k[s][c], q[c], sc[s]);
-      }
-      float x[8];
-      float top = kNone;
+          for (int j = 0; j < VC; ++j) acc[j] *= keep;
+        }
+        float base = base_of(m) * a.scale_log2;
+        if (__any(fabsf(base) > rk::kFar)) {
+          asm volatile("");
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int bit = 16 * (e >> 2) + 4 * g + (e & 3);
-        x[e] = there >> bit & 1 ? sc[e >> 2][e & 3] * a.scale_log2 : kNone;
-        top = fmaxf(top, x[e]);
-      }
-      top = fmaxf(top, rk::shfl_xor(top, 16));
-      top = fmaxf(top, rk::shfl_xor(top, 32));
-      const float m_new = fmaxf(m, top), base = base_of(m_new);
-      const float keep = rk::fast_exp2(m - base);
-      m = m_new;
-      l *= keep;
+          for (int s = 0; s < 2; ++s) sc[s] -= base_of(m);
+          base = 0.f;
+        }
+        float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = rk::fast_exp2(x[e] - base);
-        l += x[e];
-      }
-      uint4 hi, lo;
-      DT::split8(x, hi, lo);
+        for (int e = 0; e < 8; ++e) {
+          x[e] = rk::fast_exp2(__builtin_fmaf(sc[e >> 2][e & 3], a.scale_log2, -base));
+          l += x[e];
+        }
+        uint4 hi, lo;
+        DT::split8(x, hi, lo);
 #pragma unroll
-      for (int j = 0; j < VC; ++j) {
-        uint32_t t[4];
+        for (int j = 0; j < VC; ++j) {
+          uint32_t t[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          t[e] = j & 1 ? rk::pack_hi(v[2 * e][j >> 1], v[2 * e + 1][j >> 1])
-                       : rk::pack_lo(v[2 * e][j >> 1], v[2 * e + 1][j >> 1]);
-        const uint4 vt = make_uint4(t[0], t[1], t[2], t[3]);
-        acc[j] *= keep;
-        acc[j] = DT::mfma(vt, hi, acc[j]);
-        acc[j] = DT::mfma(vt, lo, acc[j]);
+          for (int e = 0; e < 4; ++e)
+            t[e] = j & 1 ? rk::pack_hi(v[2 * e][j >> 1], v[2 * e + 1][j >> 1])
+                         : rk::pack_lo(v[2 * e][j >> 1], v[2 * e + 1][j >> 1]);
+          const uint4 vt = make_uint4(t[0], t[1], t[2], t[3]);
+          acc[j] = DT::mfma(vt, hi, acc[j]);
+          acc[j] = DT::mfma(vt, lo, acc[j]);
+        }
+        if (then < last) load_v(then, next);
+        now = next;
+        next = pages_at(then + kPagedWaves);
       }
     }
     l += rk::shfl_xor(l, 16);
@@ -209,7 +335,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_split_kernel(const Pag
 #pragma unroll
       for (int j = 0; j < VC; ++j) s_acc[wave][n][VC * (4 * g + i) + j] = acc[j][i];
     if (g == 0) {
-      s_ml[wave][n][0] = m;
+      s_ml[wave][n][0] = m * a.scale_log2;
       s_ml[wave][n][1] = l;
     }
     __syncthreads();
@@ -414,10 +540,9 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
   };
   if (p->single) {
     const int64_t KD = D <= 64 ? 64 : 128;
-    // two workgroups a CU: what their registers allow
     const int64_t pieces = p->B * H * cdiv(c.groups, kRows) * (cdiv(cap, kBlock) + 1);
     if (pieces >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
-    a->workers = (int32_t)std::max<int64_t>(std::min<int64_t>(2 * (int64_t)cus, pieces), 1);
+    a->workers = (int32_t)std::max<int64_t>(std::min<int64_t>(per_cu(D <= 64 ? 2 : 4) * (int64_t)cus, pieces), 1);
     const size_t records = (size_t)a->workers * 2 * kRows;
     p->acc = take(records * KD * 4);
     p->ml = take(records * 8);
@@ -475,8 +600,12 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
   const hipStream_t s = (hipStream_t)stream;
   if (!p.single) return rk::window_launch(a, c.q->dtype, s);
   return by_shape(c.q->dtype, a.D, [&](auto dt, auto kf) {
-    hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value>), dim3((unsigned)a.workers),
-                       dim3(kPagedThreads), 0, s, a);
+    if (a.map.shift == 3)
+      hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value, true>), dim3((unsigned)a.workers),
+                         dim3(kPagedThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value, false>), dim3((unsigned)a.workers),
+                         dim3(kPagedThreads), 0, s, a);
     hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value>), dim3((unsigned)p.rows),
                        dim3(kPagedThreads), 0, s, a);
   });

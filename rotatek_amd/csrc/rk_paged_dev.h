@@ -11,6 +11,8 @@ namespace rk {
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = 4;
 constexpr float kNone = -__builtin_inff();
+constexpr float kSlack = 8.f;    // log2 of what weights may grow to
+constexpr float kFar = 16384.f;  // a base of scores, in log2, that is rounded by 2^-11 at most
 
 // 2^(x - m), and the maximum to subtract where nothing counted yet: -inf - -inf
 // would be NaN.

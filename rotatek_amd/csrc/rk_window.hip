@@ -22,9 +22,11 @@
 namespace {
 
 using rk::base_of;
+using rk::kFar;
 using rk::kNone;
 using rk::kPagedThreads;
 using rk::kPagedWaves;
+using rk::kSlack;
 using rk::PagedArgs;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -36,8 +38,6 @@ typedef const __attribute__((address_space(1))) void* global_ptr;
 constexpr int kTile = 64;               // tokens
 constexpr int kWaveRows = 32;
 constexpr int kRows = kWaveRows * kPagedWaves;
-constexpr float kSlack = 8.f;           // log2 of what weights may grow to
-constexpr float kFar = 16384.f;         // a base that is rounded by 2^-11 at most
 
 // Instructions stay on their side.
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
