@@ -47,6 +47,7 @@ struct PagedArgs {
   int64_t q_sb, q_st, q_sh, q_sd, o_sb, o_st, o_sh, o_sd;
   int64_t k_sp, k_sh, k_ss, v_sp, v_sh, v_ss;
   float *acc, *ml;  // partial records
+  int2* span;       // one new token each: first and last share of a unit
   int64_t N;        // new tokens in all
   int32_t Hq, H, G, D, T;  // T: new tokens of each request (0: starts)
   int32_t window, sinks;   // window INT_MAX: none

@@ -90,6 +90,8 @@ struct Pages {
 
 // Workgroups of a CU: what their registers allow.
 constexpr int per_cu(int KF) { return KF == 4 ? 2 : 3; }
+// Steps whose rows are in registers or on their way there.
+constexpr int ring(int KF) { return KF == 4 ? 1 : 1; }
 
 // KF: blocks of 32 channels (2 or 4).  EIGHT: pages of eight rows.
 template <class DT, int KF, bool EIGHT>
@@ -97,6 +99,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
   constexpr int KD = 32 * KF;      // channels, stored ones up to D
   constexpr int VC = KD / 16;      // channels of a Value piece: 4 or 8
   constexpr int AccPitch = KD + 4;
+  constexpr int kRing = ring(KF);
   typedef unsigned int piece __attribute__((ext_vector_type(KF)));
   __shared__ int s_wave[kPagedWaves], s_found[2];
   __shared__ float s_acc[kPagedWaves][kRows][AccPitch];
@@ -203,9 +206,13 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
         at[s] = (const char*)(src + (ok ? pg : 0u) * sp + (ok ? row : 0) * ss);
       }
     };
-    rk::u32x4 k[2][KF];
-    uint32_t v[8][KF];
-    auto load_k = [&](int i, const Pages& x) {
+    struct Keys {
+      rk::u32x4 at[2][KF];
+    } keys[kRing];
+    struct Values {
+      uint32_t at[8][KF];
+    } values[kRing];
+    auto load_k = [&](int i, const Pages& x, Keys& y) {
       const char* at[2];
       rows_at(i, x.k, n, kb, a.k_sp, a.k_ss, at);
 #pragma unroll
@@ -213,10 +220,10 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
 #pragma unroll
         for (int c = 0; c < KF; ++c) {
           const int ch = 32 * c + 8 * g;
-          k[s][c] = load_once<rk::u32x4>(at[s] + k_off[s] + 2 * (KD == a.D || ch < a.D ? ch : 0));
+          y.at[s][c] = load_once<rk::u32x4>(at[s] + k_off[s] + 2 * (KD == a.D || ch < a.D ? ch : 0));
         }
     };
-    auto load_v = [&](int i, const Pages& x) {
+    auto load_v = [&](int i, const Pages& x, Values& z) {
       const char* at[2];
       rows_at(i, EIGHT ? x.v : x.k, 4 * g, vb, a.v_sp, a.v_ss, at);
 #pragma unroll
@@ -225,24 +232,36 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
         for (int e = 0; e < 4; ++e) {
           const piece y = load_once<piece>(at[s] + v_off[s][e]);
 #pragma unroll
-          for (int d = 0; d < KF; ++d) v[4 * s + e][d] = y[d];
+          for (int d = 0; d < KF; ++d) z.at[4 * s + e][d] = y[d];
         }
     };
-    // Scores of the Keys at hand.  Then these registers take the next step's rows.
+    // A ring of steps: as soon as a step's Keys (Values) have been used, their
+    // registers take those of the step kRing on.
     const int i0 = kPagedWaves * off + wave;
     if (i0 < last) {
-      Pages now = pages_at(i0), next = pages_at(i0 + kPagedWaves);
       auto cut = [&](int i) {  // the step that tokens end in is the last one
         if (seen.token(i) + kStep - 1 > p) {
           asm volatile("");
           offsets(p + 1 - seen.token(i));
         }
       };
-      cut(i0);
-      load_k(i0, now);
-      load_v(i0, now);
-      for (int i = i0; i < last; i += kPagedWaves) {
-        const int then = i + kPagedWaves, t0 = seen.token(i);
+      constexpr int kOn = kRing * kPagedWaves;
+      Pages pages[kRing], next;
+#pragma unroll
+      for (int d = 0; d < kRing; ++d) pages[d] = pages_at(i0 + d * kPagedWaves);
+      next = pages_at(i0 + kOn);
+#pragma unroll
+      for (int d = 0; d < kRing; ++d) {
+        const int i = i0 + d * kPagedWaves;
+        if (i >= last) break;
+        cut(i);
+        load_k(i, pages[d], keys[d]);
+        load_v(i, pages[d], values[d]);
+      }
+      auto step = [&](int i, Pages& now, Keys& key, Values& value) {
+        const int then = i + kOn, t0 = seen.token(i);
+        auto& k = key.at;
+        auto& v = value.at;
         // A CU's older workgroup goes first wherever both could, and ends early; by
         // turns they end together (32 requests of 16000 tokens: 344 us, 338 so).
         if (((i / kPagedWaves) ^ (2 * blockIdx.x >= gridDim.x ? 1 : 0)) & 1)
@@ -270,7 +289,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
           for (int s = 0; s < 2; ++s) sc[s] = DT::mfma(__builtin_bit_cast(uint4, k[s][c]), q[c], sc[s]);
         if (then < last) {
           cut(then);
-          load_k(then, next);
+          load_k(then, next, key);
         }
         if (part) {
           asm volatile("");
@@ -322,9 +341,16 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
           acc[j] = DT::mfma(vt, hi, acc[j]);
           acc[j] = DT::mfma(vt, lo, acc[j]);
         }
-        if (then < last) load_v(then, next);
+        if (then < last) load_v(then, next, value);
         now = next;
         next = pages_at(then + kPagedWaves);
+      };
+      for (int i = i0; i < last; i += kOn) {
+#pragma unroll
+        for (int d = 0; d < kRing; ++d) {
+          if (i + d * kPagedWaves >= last) break;
+          step(i + d * kPagedWaves, pages[d], keys[d], values[d]);
+        }
       }
     }
     l += rk::shfl_xor(l, 16);
@@ -368,73 +394,94 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
         if (n == 0) *(float2*)(a.ml + 2 * rec) = make_float2(top, sum);
       }
     }
+    // the shares that the unit lies in, for the launch that joins them
+    if (off == 0 && threadIdx.x == 0) {
+      const int64_t begin = at - take;
+      a.span[b * units + unit] = make_int2(w, sh.of(begin + pieces - 1));
+    }
     __syncthreads();
   }
 }
 
-// Joins the records of one query, or clears it where it sees nothing.
-template <class DT, int KF>
+// Joins the records of a query, by W waves, or clears it where it sees nothing.
+template <class DT, int KF, int W>
 __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedArgs a) {
   constexpr int KD = 32 * KF;
-  constexpr int VC = KD / 16;
-  __shared__ int s_wave[kPagedWaves];
-  __shared__ float s_acc[16][KD + 4], s_ml[16][2];
-  const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq;
+  constexpr int C = KD / 64;  // channels of a lane
+  constexpr int kAhead = 4;
+  __shared__ float s_acc[kPagedWaves][KD], s_ml[kPagedWaves][2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
+  const int64_t row = (int64_t)blockIdx.x * (kPagedWaves / W) + wave / W;
+  const bool mine = row < a.N * a.Hq;
+  const int b = mine ? (int)(row / a.Hq) : 0, hq = mine ? (int)(row - (int64_t)b * a.Hq) : 0;
   const int h = hq / a.G, r = hq - h * a.G;
   const int blocks = (a.G + kRows - 1) / kRows;
-  const int units = a.H * blocks;
-  const int pieces = pieces_of(a, b);
+  const int2 span = a.span[(int64_t)b * a.H * blocks + h * blocks + r / kRows];  // (not written where there is nothing)
+  const bool none = pieces_of(a, b) == 0;
+  if (W == 1 && !mine) return;
+  if (!none && span.x == span.y) return;  // the split launch wrote it (all waves of a row)
   uint16_t* dst = (uint16_t*)a.out + b * a.o_sb + (int64_t)hq * a.o_sh;
-  if (pieces == 0) {
-    for (int c = threadIdx.x; c < a.D; c += kPagedThreads) dst[c * a.o_sd] = 0;
+  const int c0 = C * lane;
+  if (none) {
+    if (part == 0)
+#pragma unroll
+      for (int e = 0; e < C; ++e)
+        if (c0 + e < a.D) dst[(c0 + e) * a.o_sd] = 0;
     return;
   }
-  auto count = [&](int i) { return pieces_of(a, i); };
-  auto count_before = [&](int i) { return i < b ? pieces_of(a, i) : 0; };
-  const Shares sh = shares_of(a, rk::pieces_of_all(a.map.B, count, s_wave), units);
-  const int before = rk::pieces_of_all(a.map.B, count_before, s_wave);
-  const int64_t first = (int64_t)before * units + (int64_t)(h * blocks + r / kRows) * pieces;
-  const int w0 = sh.of(first), w1 = sh.of(first + pieces - 1);
-  if (w0 == w1) return;  // the split launch wrote it
-  const int grp = threadIdx.x >> 4, c0 = VC * (threadIdx.x & 15);
-  float m = kNone, l = 0.f, o[VC];
+  float m = kNone, l = 0.f, o[C];
 #pragma unroll
-  for (int e = 0; e < VC; ++e) o[e] = 0.f;
-  for (int w = w0 + grp; w <= w1; w += 16) {
-    const int64_t rec = ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * kRows + (r & (kRows - 1));
-    const float2 ml = *(const float2*)(a.ml + 2 * rec);
-    float x[VC];
+  for (int e = 0; e < C; ++e) o[e] = 0.f;
+  for (int w0 = span.x + part; w0 <= span.y; w0 += W * kAhead) {
+    float2 ml[kAhead];
+    float x[kAhead][C];
 #pragma unroll
-    for (int e = 0; e < VC; e += 4) {
-      const float4 y = *(const float4*)(a.acc + rec * KD + c0 + e);
-      x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
+    for (int k = 0; k < kAhead; ++k) {
+      const int w = min(w0 + k * W, span.y);
+      const int64_t rec = ((int64_t)w * 2 + (w == span.x ? 1 : 0)) * kRows + (r & (kRows - 1));
+      ml[k] = *(const float2*)(a.ml + 2 * rec);
+#pragma unroll
+      for (int e = 0; e < C; ++e) x[k][e] = a.acc[rec * KD + c0 + e];
     }
-    const float top = fmaxf(m, ml.x), base = base_of(top);
-    const float f0 = rk::fast_exp2(m - base), f1 = rk::fast_exp2(ml.x - base);
-    l = l * f0 + ml.y * f1;
 #pragma unroll
-    for (int e = 0; e < VC; ++e) o[e] = o[e] * f0 + x[e] * f1;
-    m = top;
+    for (int k = 0; k < kAhead; ++k) {
+      if (w0 + k * W > span.y) break;
+      const float top = fmaxf(m, ml[k].x), base = base_of(top);
+      const float f0 = rk::fast_exp2(m - base), f1 = rk::fast_exp2(ml[k].x - base);
+      l = l * f0 + ml[k].y * f1;
+#pragma unroll
+      for (int e = 0; e < C; ++e) o[e] = o[e] * f0 + x[k][e] * f1;
+      m = top;
+    }
   }
+  if constexpr (W > 1) {
+    static_assert(W == kPagedWaves, "one row a workgroup");
 #pragma unroll
-  for (int e = 0; e < VC; ++e) s_acc[grp][c0 + e] = o[e];
-  if ((threadIdx.x & 15) == 0) {
-    s_ml[grp][0] = m;
-    s_ml[grp][1] = l;
+    for (int e = 0; e < C; ++e) s_acc[wave][c0 + e] = o[e];
+    if (lane == 0) {
+      s_ml[wave][0] = m;
+      s_ml[wave][1] = l;
+    }
+    __syncthreads();
+    if (wave) return;
+    float top = kNone;
+#pragma unroll
+    for (int i = 0; i < W; ++i) top = fmaxf(top, s_ml[i][0]);
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < C; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float f = rk::fast_exp2(s_ml[i][0] - base_of(top));
+      l += f * s_ml[i][1];
+#pragma unroll
+      for (int e = 0; e < C; ++e) o[e] += f * s_acc[i][c0 + e];
+    }
   }
-  __syncthreads();
-  const int c = threadIdx.x;
-  if (c >= a.D) return;
-  float top = kNone, sum = 0.f, y = 0.f;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = fmaxf(top, s_ml[i][0]);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float f = rk::fast_exp2(s_ml[i][0] - base_of(top));
-    sum += f * s_ml[i][1];
-    y += f * s_acc[i][c];
-  }
-  dst[c * a.o_sd] = DT::from_f32(sum > 0.f || sum != sum ? y / sum : 0.f);
+  for (int e = 0; e < C; ++e)
+    if (c0 + e < a.D) dst[(c0 + e) * a.o_sd] = DT::from_f32(o[e] * inv);
 }
 
 // ------------------------------------------------------------------- host
@@ -452,7 +499,8 @@ struct Call {
 struct Plan {
   int64_t B, rows;         // requests; output rows (new tokens times query heads)
   bool single;             // one new token a request
-  size_t acc, ml, total;   // workspace
+  size_t acc, ml, span, total;  // workspace
+  int join;                     // waves that join a row
 };
 
 // Checks a call and forms its arguments and workspace; no HIP calls.
@@ -546,6 +594,10 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
     const size_t records = (size_t)a->workers * 2 * kRows;
     p->acc = take(records * KD * 4);
     p->ml = take(records * 8);
+    const int64_t units = p->B * H * cdiv(c.groups, kRows);
+    p->span = take((size_t)units * 8);
+    // records of a unit, where requests are of one length
+    p->join = a->workers > 8 * units ? kPagedWaves : 1;
   } else if (p->rows > 0) {
     // cut the tokens where the rows alone leave CUs empty, into parts of 256 or more
     const int64_t grid = rk::window_slots(*a) * H;
@@ -597,6 +649,7 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
   if (p.total && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.total)) return RK_ERR_WORKSPACE;
   a.acc = (float*)((char*)workspace + p.acc);
   a.ml = (float*)((char*)workspace + p.ml);
+  a.span = (int2*)((char*)workspace + p.span);
   const hipStream_t s = (hipStream_t)stream;
   if (!p.single) return rk::window_launch(a, c.q->dtype, s);
   return by_shape(c.q->dtype, a.D, [&](auto dt, auto kf) {
@@ -606,8 +659,12 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
     else
       hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value, false>), dim3((unsigned)a.workers),
                          dim3(kPagedThreads), 0, s, a);
-    hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value>), dim3((unsigned)p.rows),
-                       dim3(kPagedThreads), 0, s, a);
+    const dim3 grid((unsigned)cdiv(p.rows, kPagedWaves / p.join));
+    if (p.join == 1)
+      hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value, 1>), grid, dim3(kPagedThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value, kPagedWaves>), grid,
+                         dim3(kPagedThreads), 0, s, a);
   });
 }
 
