@@ -552,17 +552,26 @@ __global__ __launch_bounds__(kPagedThreads) void window_join_kernel(const PagedA
     t = n - b * a.T;
   }
   const int c = 2 * (threadIdx.x & 63);
+  constexpr int kAhead = 4;
   float m = kNone, l = 0.f, y0 = 0.f, y1 = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t rec = s * rows + row;
-    const float2 ml = *(const float2*)(a.ml + 2 * rec);
-    const float2 x = c < a.D ? *(const float2*)(a.acc + rec * KD + c) : make_float2(0.f, 0.f);
-    const float top = fmaxf(m, ml.x), base = base_of(top);
-    const float f0 = rk::fast_exp2(m - base), f1 = rk::fast_exp2(ml.x - base);
-    l = l * f0 + ml.y * f1;
-    y0 = y0 * f0 + x.x * f1;
-    y1 = y1 * f0 + x.y * f1;
-    m = top;
+  for (int s0 = 0; s0 < a.splits; s0 += kAhead) {
+    float2 ml[kAhead], x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t rec = min(s0 + k, a.splits - 1) * rows + row;
+      ml[k] = *(const float2*)(a.ml + 2 * rec);
+      x[k] = c < a.D ? *(const float2*)(a.acc + rec * KD + c) : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (s0 + k >= a.splits) break;
+      const float top = fmaxf(m, ml[k].x), base = base_of(top);
+      const float f0 = rk::fast_exp2(m - base), f1 = rk::fast_exp2(ml[k].x - base);
+      l = l * f0 + ml[k].y * f1;
+      y0 = y0 * f0 + x[k].x * f1;
+      y1 = y1 * f0 + x[k].y * f1;
+      m = top;
+    }
   }
   if (c >= a.D) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
