@@ -49,22 +49,21 @@ RK_EVERYWHERE int request_of(const int32_t* starts, int B, int64_t n) {
   return low;
 }
 
-// Page and row that new token n goes to; a negative page where it goes nowhere.
-RK_EVERYWHERE int64_t place_of(const PageMap& m, int64_t n, int* row) {
-  int64_t b, i, each = m.each;
+// Page and row that new token n goes to, b: request_of it (where there are
+// starts); a negative page where it goes nowhere.
+RK_EVERYWHERE int64_t place_of(const PageMap& m, int64_t n, int64_t b, int* row) {
   if (m.B <= 0) return -1;
+  int64_t s, e;  // the request's new tokens
   if (m.starts) {
-    b = request_of(m.starts, m.B, n);
-    const int64_t s = m.starts[b], e = m.starts[b + 1];
-    if (n < s || n >= e) return -1;
-    i = n - s;
-    each = e - s;
+    s = m.starts[b];
+    e = m.starts[b + 1];
   } else {
-    b = n / each;
-    i = n - b * each;
+    b = n / m.each;
+    s = b * m.each;
+    e = s + m.each;
   }
-  const int64_t p = (int64_t)m.lens[b] - each + i;
-  if (p < 0 || p >= m.cap) return -1;
+  const int64_t len = m.lens[b], p = len - e + n;
+  if (n < s || n >= e || p < 0 || p >= m.cap) return -1;
   const uint32_t page = page_of(m, (int)b, (int)p);
   if (page >= (uint32_t)m.pages) return -1;
   *row = (int)p & ((1 << m.shift) - 1);

@@ -60,7 +60,7 @@ using namespace rk;
 extern "C" void place(const int32_t* table, long t_sb, const int32_t* lens, const int32_t* starts, int B, int per,
                       int pages, int shift, int each, long n, long* page, int* row) {
   PageMap m{table, lens, starts, t_sb, B, per, pages, each, shift, per << shift};
-  *page = place_of(m, n, row);
+  *page = place_of(m, n, starts ? request_of(starts, B, n) : 0, row);
 }
 extern "C" int length(const int32_t* lens, int b, int cap) {
   PageMap m{nullptr, lens, nullptr, 0, 0, 0, 0, 0, 31, cap};
