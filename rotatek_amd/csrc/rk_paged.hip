@@ -109,12 +109,13 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
   const int blocks = (a.G + kRows - 1) / kRows;
   const int units = a.H * blocks;  // of a request
   auto count = [&](int b) { return pieces_of(a, b); };
-  const Shares sh = shares_of(a, rk::pieces_of_all(a.map.B, count, s_wave), units);
+  rk::Line<decltype(count)> line(a.map.B, count, s_wave, s_found);
+  const Shares sh = shares_of(a, line.total, units);
   const int w = blockIdx.x;
   if (w >= sh.workers) return;
   int64_t at = sh.begin(w);
   const int64_t end = sh.begin(w + 1);
-  const rk::Found found = rk::request_at(a.map.B, count, (int)(at / units), s_wave, s_found);
+  const rk::Found found = line.find((int)(at / units));
   int b = found.b;
   int64_t first = (int64_t)found.before * units;  // first piece of request b
   while (at < end) {

@@ -40,39 +40,67 @@ __device__ __forceinline__ int scan_before(int n, int* s_wave, int* total) {
   return before;
 }
 
-// Work of requests 0 .. B - 1, count(b) pieces each, laid end to end: their
-// sum.
-template <class F>
-__device__ __forceinline__ int pieces_of_all(int B, F count, int* s_wave) {
-  int sum = 0;
-  for (int b = threadIdx.x; b < B; b += kPagedThreads) sum += count(b);
-  int total;
-  scan_before(sum, s_wave, &total);
-  return total;
+// Sum over the wave's lanes up to this one.
+__device__ __forceinline__ int wave_sum_to(int n) {
+  n += __builtin_amdgcn_update_dpp(0, n, 0x111, 0xf, 0xf, true);  // one lane of the row before, then two, ..
+  n += __builtin_amdgcn_update_dpp(0, n, 0x112, 0xf, 0xf, true);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x114, 0xf, 0xf, true);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x118, 0xf, 0xf, true);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x142, 0xa, 0xf, false);  // the last lane of the row before, to rows 1 and 3
+  n += __builtin_amdgcn_update_dpp(0, n, 0x143, 0xc, 0xf, false);  // of the first half, to the second
+  return n;
 }
 
 struct Found {
-  int b, before;  // the request, and the pieces before it
+  int b, before;  // a request, and the pieces before it
 };
 
-// The request that piece `at` (below the sum) belongs to.
+// Work of requests 0 .. B - 1, count(b) pieces each, laid end to end: the sum, and
+// the request that a piece belongs to.  Up to 64 requests every wave looks for
+// itself, without a barrier.
 template <class F>
-__device__ __forceinline__ Found request_at(int B, F count, int at, int* s_wave, int* s_found) {
-  int before = 0;
-  for (int b0 = 0; b0 < B; b0 += kPagedThreads) {
-    const int b = b0 + threadIdx.x;
-    const int n = b < B ? count(b) : 0;
-    int total;
-    const int mine = before + scan_before(n, s_wave, &total);
-    if (at >= mine && at < mine + n) {
-      s_found[0] = b;
-      s_found[1] = mine;
+struct Line {
+  F count;
+  int B, total;
+  int mine, to;  // up to 64 requests: the lane's pieces, and those up to them
+  int *s_wave, *s_found;
+
+  __device__ __forceinline__ Line(int B, F count, int* s_wave, int* s_found)
+      : count(count), B(B), s_wave(s_wave), s_found(s_found) {
+    if (B <= 64) {
+      const int lane = threadIdx.x & 63;
+      mine = lane < B ? count(lane) : 0;
+      to = wave_sum_to(mine);
+      total = __builtin_amdgcn_readlane(to, 63);
+    } else {
+      int sum = 0;
+      for (int b = threadIdx.x; b < B; b += kPagedThreads) sum += count(b);
+      scan_before(sum, s_wave, &total);
     }
-    before += total;
-    if (at < before) break;
   }
-  __syncthreads();
-  return {s_found[0], s_found[1]};
-}
+
+  // `at` below the sum.
+  __device__ __forceinline__ Found find(int at) {
+    if (B <= 64) {
+      const int b = __builtin_ctzll(__ballot(at < to));
+      return {b, __builtin_amdgcn_readlane(to - mine, b)};
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < B; b0 += kPagedThreads) {
+      const int b = b0 + threadIdx.x;
+      const int n = b < B ? count(b) : 0;
+      int sum;
+      const int first = before + scan_before(n, s_wave, &sum);
+      if (at >= first && at < first + n) {
+        s_found[0] = b;
+        s_found[1] = first;
+      }
+      before += sum;
+      if (at < before) break;
+    }
+    __syncthreads();
+    return {s_found[0], s_found[1]};
+  }
+};
 
 }  // namespace rk

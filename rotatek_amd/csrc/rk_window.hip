@@ -149,9 +149,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
   int b, tile;
   if (a.map.starts) {
     auto count = [&](int i) { return (queries_of(a, i).n * a.G + kRows - 1) / kRows; };
-    const int tiles = rk::pieces_of_all(a.map.B, count, s_wave);
-    if (slot >= tiles) return;
-    const rk::Found f = rk::request_at(a.map.B, count, slot, s_wave, s_found);
+    rk::Line<decltype(count)> line(a.map.B, count, s_wave, s_found);
+    if (slot >= line.total) return;
+    const rk::Found f = line.find(slot);
     b = f.b;
     tile = count(b) - 1 - (slot - f.before);
   } else {
