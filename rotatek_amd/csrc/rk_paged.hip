@@ -90,8 +90,6 @@ struct Pages {
 
 // Workgroups of a CU: what their registers allow.
 constexpr int per_cu(int KF) { return KF == 4 ? 2 : 3; }
-// Steps whose rows are in registers or on their way there.
-constexpr int ring(int KF) { return KF == 4 ? 1 : 1; }
 
 // KF: blocks of 32 channels (2 or 4).  EIGHT: pages of eight rows.
 template <class DT, int KF, bool EIGHT>
@@ -99,7 +97,6 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
   constexpr int KD = 32 * KF;      // channels, stored ones up to D
   constexpr int VC = KD / 16;      // channels of a Value piece: 4 or 8
   constexpr int AccPitch = KD + 4;
-  constexpr int kRing = ring(KF);
   typedef unsigned int piece __attribute__((ext_vector_type(KF)));
   __shared__ int s_wave[kPagedWaves], s_found[2];
   __shared__ float s_acc[kPagedWaves][kRows][AccPitch];
@@ -207,13 +204,9 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
         at[s] = (const char*)(src + (ok ? pg : 0u) * sp + (ok ? row : 0) * ss);
       }
     };
-    struct Keys {
-      rk::u32x4 at[2][KF];
-    } keys[kRing];
-    struct Values {
-      uint32_t at[8][KF];
-    } values[kRing];
-    auto load_k = [&](int i, const Pages& x, Keys& y) {
+    rk::u32x4 k[2][KF];
+    uint32_t v[8][KF];
+    auto load_k = [&](int i, const Pages& x) {
       const char* at[2];
       rows_at(i, x.k, n, kb, a.k_sp, a.k_ss, at);
 #pragma unroll
@@ -221,10 +214,10 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
 #pragma unroll
         for (int c = 0; c < KF; ++c) {
           const int ch = 32 * c + 8 * g;
-          y.at[s][c] = load_once<rk::u32x4>(at[s] + k_off[s] + 2 * (KD == a.D || ch < a.D ? ch : 0));
+          k[s][c] = load_once<rk::u32x4>(at[s] + k_off[s] + 2 * (KD == a.D || ch < a.D ? ch : 0));
         }
     };
-    auto load_v = [&](int i, const Pages& x, Values& z) {
+    auto load_v = [&](int i, const Pages& x) {
       const char* at[2];
       rows_at(i, EIGHT ? x.v : x.k, 4 * g, vb, a.v_sp, a.v_ss, at);
 #pragma unroll
@@ -233,11 +226,11 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
         for (int e = 0; e < 4; ++e) {
           const piece y = load_once<piece>(at[s] + v_off[s][e]);
 #pragma unroll
-          for (int d = 0; d < KF; ++d) z.at[4 * s + e][d] = y[d];
+          for (int d = 0; d < KF; ++d) v[4 * s + e][d] = y[d];
         }
     };
-    // A ring of steps: as soon as a step's Keys (Values) have been used, their
-    // registers take those of the step kRing on.
+    // As soon as a step's Keys (Values) have been used, their registers take the
+    // next step's; the page numbers of the one behind it are on their way too.
     const int i0 = kPagedWaves * off + wave;
     if (i0 < last) {
       auto cut = [&](int i) {  // the step that tokens end in is the last one
@@ -246,23 +239,12 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
           offsets(p + 1 - seen.token(i));
         }
       };
-      constexpr int kOn = kRing * kPagedWaves;
-      Pages pages[kRing], next;
-#pragma unroll
-      for (int d = 0; d < kRing; ++d) pages[d] = pages_at(i0 + d * kPagedWaves);
-      next = pages_at(i0 + kOn);
-#pragma unroll
-      for (int d = 0; d < kRing; ++d) {
-        const int i = i0 + d * kPagedWaves;
-        if (i >= last) break;
-        cut(i);
-        load_k(i, pages[d], keys[d]);
-        load_v(i, pages[d], values[d]);
-      }
-      auto step = [&](int i, Pages& now, Keys& key, Values& value) {
-        const int then = i + kOn, t0 = seen.token(i);
-        auto& k = key.at;
-        auto& v = value.at;
+      Pages now = pages_at(i0), next = pages_at(i0 + kPagedWaves);
+      cut(i0);
+      load_k(i0, now);
+      load_v(i0, now);
+      for (int i = i0; i < last; i += kPagedWaves) {
+        const int then = i + kPagedWaves, t0 = seen.token(i);
         // A CU's older workgroup goes first wherever both could, and ends early; by
         // turns they end together (32 requests of 16000 tokens: 344 us, 338 so).
         if (((i / kPagedWaves) ^ (2 * blockIdx.x >= gridDim.x ? 1 : 0)) & 1)
@@ -290,7 +272,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
           for (int s = 0; s < 2; ++s) sc[s] = DT::mfma(__builtin_bit_cast(uint4, k[s][c]), q[c], sc[s]);
         if (then < last) {
           cut(then);
-          load_k(then, next, key);
+          load_k(then, next);
         }
         if (part) {
           asm volatile("");
@@ -342,16 +324,9 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
           acc[j] = DT::mfma(vt, hi, acc[j]);
           acc[j] = DT::mfma(vt, lo, acc[j]);
         }
-        if (then < last) load_v(then, next, value);
+        if (then < last) load_v(then, next);
         now = next;
         next = pages_at(then + kPagedWaves);
-      };
-      for (int i = i0; i < last; i += kOn) {
-#pragma unroll
-        for (int d = 0; d < kRing; ++d) {
-          if (i + d * kPagedWaves >= last) break;
-          step(i + d * kPagedWaves, pages[d], keys[d], values[d]);
-        }
       }
     }
     l += rk::shfl_xor(l, 16);
@@ -555,7 +530,7 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
   if (T >= (INT64_C(1) << 30) || N >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
   p->rows = N * Hq;
   p->single = T == 1;
-  if (p->rows >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+  if (p->rows >= (INT64_C(1) << 30)) return RK_ERR_SHAPE;
   a->map.each = (int32_t)T;
   a->N = N;
   a->T = (int32_t)T;
