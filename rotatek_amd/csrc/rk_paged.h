@@ -52,6 +52,7 @@ struct PagedArgs {
   int32_t Hq, H, G, D, T;  // T: new tokens of each request (0: starts)
   int32_t window, sinks;   // window INT_MAX: none
   int32_t workers;         // one new token each: workgroups of the split launch
+  int32_t direct;          // ... a unit each, no shares and no join
   int32_t splits;          // many: parts that a row's tokens are cut into
   int32_t q_vec, o_vec;
   float scale_log2;  // log2(e) / sqrt(D)

@@ -40,6 +40,16 @@ using rk::PagedArgs;
 constexpr int kStep = 32;                     // tokens of a wave's step
 constexpr int kBlock = kStep * kPagedWaves;  // tokens of a piece of work
 constexpr int kRows = 16;                     // queries of a unit
+// Pieces of a unit up to which a workgroup takes all of it, for units that fill the
+// CUs and for fewer: one launch instead of two, no records, but the longest unit
+// ends last (bf16, 4 query heads to each of 8 KV heads of 128; shared and not: 32
+// requests of 500 tokens 19.9 and 18.2 us, 64 of 1000 49.4 and 46.7, 64 of up to
+// 2000 74.6 and 69.1; 1 of 1000 13.3 and 18.1, 8 of 1000 with 4 KV heads 14.7 and
+// 26.1, 1 of 500 11.4 and 12.0).
+constexpr int kDirectMany = 16, kDirectFew = 2;
+// Waves that join a query of many records (one wave reads four at a time): one text
+// of 32000 tokens, 8 query heads to its KV head: 31.3 us in all with 4, 17.8 with 16.
+constexpr int kJoinWaves = 16;
 
 // Pieces of one request and KV head.
 __device__ __forceinline__ int pieces_of(const PagedArgs& a, int b) {
@@ -106,15 +116,31 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
   const int blocks = (a.G + kRows - 1) / kRows;
   const int units = a.H * blocks;  // of a request
   auto count = [&](int b) { return pieces_of(a, b); };
-  rk::Line<decltype(count)> line(a.map.B, count, s_wave, s_found);
-  const Shares sh = shares_of(a, line.total, units);
   const int w = blockIdx.x;
-  if (w >= sh.workers) return;
-  int64_t at = sh.begin(w);
-  const int64_t end = sh.begin(w + 1);
-  const rk::Found found = line.find((int)(at / units));
-  int b = found.b;
-  int64_t first = (int64_t)found.before * units;  // first piece of request b
+  Shares sh;
+  int64_t at, end, first = 0;  // pieces; the first one of request b
+  int b;
+  if (a.direct) {  // a unit each
+    b = w / units;
+    const int unit = w - b * units, pieces = pieces_of(a, b);
+    at = (int64_t)unit * pieces;
+    end = at + pieces;
+    if (pieces == 0) {
+      const int h = unit / blocks, row0 = (unit - h * blocks) * kRows;
+      for (int r = wave; r < min(a.G - row0, kRows); r += kPagedWaves)
+        for (int c = lane; c < a.D; c += 64)
+          ((uint16_t*)a.out)[b * a.o_sb + (int64_t)(h * a.G + row0 + r) * a.o_sh + c * a.o_sd] = 0;
+    }
+  } else {
+    rk::Line<decltype(count)> line(a.map.B, count, s_wave, s_found);
+    sh = shares_of(a, line.total, units);
+    if (w >= sh.workers) return;
+    at = sh.begin(w);
+    end = sh.begin(w + 1);
+    const rk::Found found = line.find((int)(at / units));
+    b = found.b;
+    first = (int64_t)found.before * units;
+  }
   while (at < end) {
     const int pieces = pieces_of(a, b);
     if (at >= first + (int64_t)pieces * units) {
@@ -251,18 +277,20 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
           __builtin_amdgcn_s_setprio(2);
         else
           __builtin_amdgcn_s_setprio(0);
-        const bool part = a.D != KD || t0 + kStep - 1 > p || (p - t0 >= a.window && t0 + kStep > a.sinks) ||
+        const bool part = t0 + kStep - 1 > p || (p - t0 >= a.window && t0 + kStep > a.sinks) ||
                           !__all(now.k[0] < (uint32_t)a.map.pages && now.k[1] < (uint32_t)a.map.pages);
         uint32_t there = ~0u;
         if (part) {
           asm volatile("");  // a branch: most steps are whole
           there = there_of(i, now);
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int c = 0; c < KF; ++c)
-              if (32 * c + 8 * g >= a.D) k[s][c] = rk::u32x4{0, 0, 0, 0};
         }
+#pragma unroll
+        for (int c = 0; c < KF; ++c)
+          if (32 * c + 32 > a.D) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+              if (32 * c + 8 * g >= a.D) k[s][c] = rk::u32x4{0, 0, 0, 0};
+          }
         f32x4 sc[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -371,7 +399,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
       }
     }
     // the shares that the unit lies in, for the launch that joins them
-    if (off == 0 && threadIdx.x == 0) {
+    if (!a.direct && off == 0 && threadIdx.x == 0) {
       const int64_t begin = at - take;
       a.span[b * units + unit] = make_int2(w, sh.of(begin + pieces - 1));
     }
@@ -379,15 +407,16 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
   }
 }
 
-// Joins the records of a query, by W waves, or clears it where it sees nothing.
+// Joins the records of a query, by W waves, or clears it where it sees nothing: four
+// queries a workgroup, or one of many records.
 template <class DT, int KF, int W>
-__global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(W == 1 ? kPagedThreads : 64 * W) void paged_join_kernel(const PagedArgs a) {
   constexpr int KD = 32 * KF;
   constexpr int C = KD / 64;  // channels of a lane
   constexpr int kAhead = 4;
-  __shared__ float s_acc[kPagedWaves][KD], s_ml[kPagedWaves][2];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
-  const int64_t row = (int64_t)blockIdx.x * (kPagedWaves / W) + wave / W;
+  __shared__ float s_acc[W][KD], s_ml[W][2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = W == 1 ? 0 : wave;
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * kPagedWaves + wave : blockIdx.x;
   const bool mine = row < a.N * a.Hq;
   const int b = mine ? (int)(row / a.Hq) : 0, hq = mine ? (int)(row - (int64_t)b * a.Hq) : 0;
   const int h = hq / a.G, r = hq - h * a.G;
@@ -431,7 +460,6 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedAr
     }
   }
   if constexpr (W > 1) {
-    static_assert(W == kPagedWaves, "one row a workgroup");
 #pragma unroll
     for (int e = 0; e < C; ++e) s_acc[wave][c0 + e] = o[e];
     if (lane == 0) {
@@ -462,6 +490,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(const PagedAr
 
 // ------------------------------------------------------------------- host
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Pieces of the longest request that a table reaches.
+int64_t pieces_of_longest(int64_t cap, int64_t window, int64_t sinks) {
+  const int64_t seen = cdiv(std::min(window, cap), kStep) + 1 + cdiv(std::min(sinks, cap), kStep);
+  return cdiv(std::min(cdiv(cap, kStep), seen), kPagedWaves);
+}
 
 struct Call {
   const rk_tensor *q, *out;
@@ -564,16 +598,19 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
   };
   if (p->single) {
     const int64_t KD = D <= 64 ? 64 : 128;
-    const int64_t pieces = p->B * H * cdiv(c.groups, kRows) * (cdiv(cap, kBlock) + 1);
-    if (pieces >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
-    a->workers = (int32_t)std::max<int64_t>(std::min<int64_t>(per_cu(D <= 64 ? 2 : 4) * (int64_t)cus, pieces), 1);
-    const size_t records = (size_t)a->workers * 2 * kRows;
-    p->acc = take(records * KD * 4);
-    p->ml = take(records * 8);
-    const int64_t units = p->B * H * cdiv(c.groups, kRows);
-    p->span = take((size_t)units * 8);
-    // records of a unit, where requests are of one length
-    p->join = a->workers > 8 * units ? kPagedWaves : 1;
+    const int64_t units = p->B * H * cdiv(c.groups, kRows), longest = pieces_of_longest(a->map.cap, a->window, a->sinks);
+    if (units * (cdiv(cap, kBlock) + 1) >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+    a->direct = longest <= (units >= cus ? kDirectMany : kDirectFew);
+    a->workers = (int32_t)(a->direct ? units : std::max<int64_t>(
+        std::min<int64_t>(per_cu(D <= 64 ? 2 : 4) * (int64_t)cus, units * longest), 1));
+    if (!a->direct) {
+      const size_t records = (size_t)a->workers * 2 * kRows;
+      p->acc = take(records * KD * 4);
+      p->ml = take(records * 8);
+      p->span = take((size_t)units * 8);
+      // records of a unit, where requests are of one length
+      p->join = a->workers > 8 * units ? kJoinWaves : 1;
+    }
   } else if (p->rows > 0) {
     // Cut the tokens where the rows alone leave CUs empty.  A part saves its share
     // of the tiles, about a microsecond each, and costs its records, written and
@@ -640,12 +677,13 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
     else
       hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value, false>), dim3((unsigned)a.workers),
                          dim3(kPagedThreads), 0, s, a);
-    const dim3 grid((unsigned)cdiv(p.rows, kPagedWaves / p.join));
+    if (a.direct) return;
     if (p.join == 1)
-      hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value, 1>), grid, dim3(kPagedThreads), 0, s, a);
+      hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value, 1>),
+                         dim3((unsigned)cdiv(p.rows, kPagedWaves)), dim3(kPagedThreads), 0, s, a);
     else
-      hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value, kPagedWaves>), grid,
-                         dim3(kPagedThreads), 0, s, a);
+      hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value, kJoinWaves>), dim3((unsigned)p.rows),
+                         dim3(64 * kJoinWaves), 0, s, a);
   });
 }
 
