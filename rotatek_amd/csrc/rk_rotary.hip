@@ -23,7 +23,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 4;  // tokens of a workgroup, a wave each where their places are found
+constexpr int kMaxTokens = 2;  // tokens of a workgroup, a wave each where their places are found
 constexpr int kMaxPairs = 64;
 constexpr int kMaxAxes = 4;
 
@@ -37,8 +37,24 @@ struct Part {
   int32_t heads;
 };
 
+// i / d for the i that occur: by a product where that is exact.
+struct Divisor {
+  uint32_t d, magic;
+  __device__ __forceinline__ int quotient(int i) const {
+    return magic ? (int)__umulhi((uint32_t)i, magic) : (int)((uint32_t)i / d);
+  }
+};
+Divisor divisor_of(int64_t d, int64_t below) {
+  // 2^32 / d rounded up, by m: i m / 2^32 is off by less than i d / 2^32 of 1 / d
+  return {(uint32_t)d, d > 1 && below * d < (INT64_C(1) << 32) ? (uint32_t)((INT64_C(1) << 32) / d + 1) : 0u};
+}
+
 struct RotaryArgs {
   Part part[kParts];
+  // Work of a token: for each head items of two vectors, `turned` that turn (from
+  // either half of the pairs) and the others that are copied.
+  int32_t turned, copied, all, nq, nk;
+  Divisor token, head[kParts];
   const void* pos;  // null: nothing turns
   const float* freq;
   int64_t p_sa, p_sb, p_st, f_s;
@@ -81,28 +97,37 @@ __device__ __forceinline__ int request_of_wave(const rk::PageMap& m, int64_t n) 
   return low;
 }
 
-// What passes through leaves the caches to others: 3 x 32 heads x 2304 tokens of
-// 80 channels in fp32 (142 MB in all) take 26.7 us (a copy of as much 25.7), 37.6
-// with ordinary stores.
-__device__ __forceinline__ void store_once(void* p, uint4 v) {
-  __builtin_nontemporal_store(rk::u32x4{v.x, v.y, v.z, v.w}, (rk::u32x4*)p);
+// Token n is t of batch row b.
+__device__ __forceinline__ void batch_row(const RotaryArgs& a, int64_t n, int64_t* b, int64_t* t) {
+  *b = a.N >> 31 ? n / a.T : (uint32_t)n / (uint32_t)a.T;
+  *t = n - *b * a.T;
 }
 
-// VEC: 16 bytes of channels at a time.  PAGED: K and V go to their pages.
-template <class DT, bool VEC, bool PAGED>
+// The part's of three (by selects: an indexed argument is a load of its own).
+template <class V>
+__device__ __forceinline__ V of(int which, V q, V k, V v) {
+  return which == kQ ? q : which == kK ? k : v;
+}
+
+// E: elements at a time, up to 16 bytes.  PAGED: K and V go to their pages.
+// ONCE: past the caches.
+template <class DT, int E, bool PAGED, bool ONCE>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
-  constexpr int E = VEC ? 16 / DT::kBytes : 1;  // elements of a step
+  constexpr bool VEC = E > 1;
+  constexpr int W = VEC ? E * DT::kBytes / 4 : 1;  // words of a vector
+  typedef uint32_t vec __attribute__((ext_vector_type(W)));
   using word = typename std::conditional<DT::kBytes == 4, uint32_t, uint16_t>::type;
   __shared__ float2 s_turn[kMaxTokens * kMaxPairs];
-  __shared__ int64_t s_page[kMaxTokens];  // page number and row of a token, or -1
-  __shared__ int32_t s_row[kMaxTokens];
+  __shared__ const word* s_x[kMaxTokens][kParts];  // a token's first element
+  __shared__ word* s_y[kMaxTokens][kParts];        // null: nowhere
   const int tid = threadIdx.x;
   const int64_t n0 = (int64_t)blockIdx.x * a.tokens;
   const int tokens = (int)min((int64_t)a.tokens, a.N - n0);
   if (a.pos) {
     for (int i = tid; i < tokens * a.P; i += kThreads) {
       const int tok = i / a.P, p = i - tok * a.P;
-      const int64_t n = n0 + tok, b = n / a.T, t = n - b * a.T;
+      int64_t b, t;
+      batch_row(a, n0 + tok, &b, &t);
       const int axis = (a.axis[p >> 4] >> (2 * (p & 15))) & 3;
       const int64_t at = axis * a.p_sa + b * a.p_sb + t * a.p_st;
       const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
@@ -119,82 +144,80 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
       int row = 0;
       const int64_t page = rk::place_of(a.map, n0 + tok, a.map.starts ? request_of_wave(a.map, n0 + tok) : 0, &row);
       if ((tid & 63) == 0) {
-        s_page[tok] = page;
-        s_row[tok] = row;
+        for (int which : {kK, kV})
+          s_y[tok][which] = page < 0 ? nullptr : (word*)a.part[which].y + page * a.part[which].y_sb + row * a.part[which].y_ss;
       }
     }
   }
-  __syncthreads();
-  // steps of a head: turned pairs, then copied channels
-  const int turned = a.pos ? a.P / E : 0;
-  const int copied = (a.D - (a.pos ? 2 * a.P : 0)) / E;
-  const int per = turned + copied, all = a.D / E;
-  const int nq = a.part[kQ].heads * per, nk = a.part[kK].heads * per, nv = a.part[kV].heads * all;
-  const int per_token = nq + nk + nv;
-  for (int i = tid; i < tokens * per_token; i += kThreads) {
-    const int tok = i / per_token;
-    int u = i - tok * per_token;
-    const int which = u < nq ? kQ : u < nq + nk ? kK : kV;
-    u -= which == kQ ? 0 : which == kK ? nq : nq + nk;
+  if (tid < tokens * kParts) {
+    const int tok = tid / kParts, which = tid - tok * kParts;
     const Part& p = a.part[which];
-    const int steps = which == kV ? all : per;
-    const int h = u / steps, step = u - h * steps;
-    const int64_t n = n0 + tok, b = n / a.T, t = n - b * a.T;
-    const int64_t xo = b * p.x_sb + h * p.x_sh + t * p.x_ss;
-    int64_t yo;
-    if (PAGED && which != kQ) {
-      if (s_page[tok] < 0) continue;
-      yo = s_page[tok] * p.y_sb + h * p.y_sh + s_row[tok] * p.y_ss;
-    } else {
-      yo = b * p.y_sb + h * p.y_sh + t * p.y_ss;
-    }
-    const word* x = (const word*)p.x + xo;
-    word* y = (word*)p.y + yo;
-    const bool turns = which != kV && step < turned;
-    const int c = which == kV ? step * E : turns ? step * E : 2 * (a.pos ? a.P : 0) + (step - turned) * E;
+    int64_t b, t;
+    batch_row(a, n0 + tok, &b, &t);
+    s_x[tok][which] = (const word*)p.x + b * p.x_sb + t * p.x_ss;
+    if (!PAGED || which == kQ) s_y[tok][which] = (word*)p.y + b * p.y_sb + t * p.y_ss;
+  }
+  __syncthreads();
+  // (addresses that come from LDS: which memory they are in has to be said)
+  typedef __attribute__((address_space(1))) word global_word;
+  typedef __attribute__((address_space(1))) vec global_vec;
+  const int per_token = a.token.d;
+  for (int i = tid; i < tokens * per_token; i += kThreads) {
+    const int tok = a.token.quotient(i);
+    int u = i - tok * per_token;
+    const int which = u < a.nq ? kQ : u < a.nq + a.nk ? kK : kV;
+    u -= which == kQ ? 0 : which == kK ? a.nq : a.nq + a.nk;
+    const Part &pq = a.part[kQ], &pk = a.part[kK], &pv = a.part[kV];
+    const Divisor d = which == kV ? a.head[kV] : a.head[kQ];
+    const int h = d.quotient(u), item = u - h * (int)d.d;
+    if (PAGED && !s_y[tok][which]) continue;
+    global_word* y = (global_word*)s_y[tok][which] + h * of(which, pq.y_sh, pk.y_sh, pv.y_sh);
+    const global_word* x = (const global_word*)s_x[tok][which] + h * of(which, pq.x_sh, pk.x_sh, pv.x_sh);
+    const bool turns = which != kV && item < a.turned;
+    // the item's vectors: channels c and c2 (copied: if that is below D)
+    const int first = which == kV ? 0 : a.turned, n = which == kV ? a.all : a.copied, half = (n + 1) / 2;
+    const int base = which == kV || !a.pos ? 0 : 2 * a.P;
+    const int c = turns ? item * E : base + (item - first) * E;
+    const int c2 = turns ? c + a.P : c + half * E;
+    const bool two = turns || item - first + half < n;
     if constexpr (VEC) {
-      const uint4 lo = *(const uint4*)(x + c);
-      if (!turns) {
-        store_once(y + c, lo);
-        continue;
-      }
-      const uint4 hi = *(const uint4*)(x + c + a.P);
-      uint4 ylo, yhi;
-      const float2* cs = s_turn + tok * kMaxPairs + c;
-      if constexpr (DT::kBytes == 4) {
-        uint32_t l[4], m[4];
+      vec lo = *(const global_vec*)(x + c), hi = lo;
+      if (two) hi = *(const global_vec*)(x + c2);
+      if (turns) {
+        const float2* cs = s_turn + tok * kMaxPairs + c;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 y2 = turn(DT::to_f32(rk::word(lo, e)), DT::to_f32(rk::word(hi, e)), cs[e]);
-          l[e] = DT::from_f32(y2.x);
-          m[e] = DT::from_f32(y2.y);
+        for (int e = 0; e < W; ++e) {
+          const uint32_t wl = lo[e], wh = hi[e];
+          if constexpr (DT::kBytes == 4) {
+            const float2 y2 = turn(DT::to_f32(wl), DT::to_f32(wh), cs[e]);
+            lo[e] = DT::from_f32(y2.x);
+            hi[e] = DT::from_f32(y2.y);
+          } else {
+            const float2 y0 = turn(DT::to_f32((uint16_t)wl), DT::to_f32((uint16_t)wh), cs[2 * e]);
+            const float2 y1 = turn(DT::to_f32((uint16_t)(wl >> 16)), DT::to_f32((uint16_t)(wh >> 16)), cs[2 * e + 1]);
+            lo[e] = DT::pack2(y0.x, y1.x);
+            hi[e] = DT::pack2(y0.y, y1.y);
+          }
         }
-        ylo = make_uint4(l[0], l[1], l[2], l[3]);
-        yhi = make_uint4(m[0], m[1], m[2], m[3]);
+      }
+      if constexpr (ONCE) {
+        __builtin_nontemporal_store(lo, (global_vec*)(y + c));
+        if (two) __builtin_nontemporal_store(hi, (global_vec*)(y + c2));
       } else {
-        uint32_t l[4], m[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t wl = rk::word(lo, e), wh = rk::word(hi, e);
-          const float2 y0 = turn(DT::to_f32((uint16_t)wl), DT::to_f32((uint16_t)wh), cs[2 * e]);
-          const float2 y1 = turn(DT::to_f32((uint16_t)(wl >> 16)), DT::to_f32((uint16_t)(wh >> 16)), cs[2 * e + 1]);
-          l[e] = DT::pack2(y0.x, y1.x);
-          m[e] = DT::pack2(y0.y, y1.y);
-        }
-        ylo = make_uint4(l[0], l[1], l[2], l[3]);
-        yhi = make_uint4(m[0], m[1], m[2], m[3]);
+        *(global_vec*)(y + c) = lo;
+        if (two) *(global_vec*)(y + c2) = hi;
       }
-      store_once(y + c, ylo);
-      store_once(y + c + a.P, yhi);
     } else {
-      const word lo = x[c * p.x_sd];
-      if (!turns) {
-        y[c * p.y_sd] = lo;
-        continue;
+      const int64_t x_sd = of(which, pq.x_sd, pk.x_sd, pv.x_sd), y_sd = of(which, pq.y_sd, pk.y_sd, pv.y_sd);
+      word lo = x[c * x_sd], hi = lo;
+      if (two) hi = x[c2 * x_sd];
+      if (turns) {
+        const float2 y2 = turn(DT::to_f32(lo), DT::to_f32(hi), s_turn[tok * kMaxPairs + c]);
+        lo = DT::from_f32(y2.x);
+        hi = DT::from_f32(y2.y);
       }
-      const float2 y2 = turn(DT::to_f32(lo), DT::to_f32(x[(c + a.P) * p.x_sd]), s_turn[tok * kMaxPairs + c]);
-      y[c * p.y_sd] = DT::from_f32(y2.x);
-      y[(c + a.P) * p.y_sd] = DT::from_f32(y2.y);
+      y[c * y_sd] = lo;
+      if (two) y[c2 * y_sd] = hi;
     }
   }
 }
@@ -261,12 +284,19 @@ void set_out(Part* p, void* y, const Strides& s) {
   p->y_sb = s.sb; p->y_sh = s.sh; p->y_ss = s.ss; p->y_sd = s.sd;
 }
 
-bool vec16(const rk_tensor* t) {
-  const int n = 16 / rk::dtype_size(t->dtype);
-  if (t->stride[t->ndim - 1] != 1 && t->shape[t->ndim - 1] > 1) return false;
+// Elements that lie together and aligned in every row, up to 16 bytes of them.
+int vector_of(const rk_tensor* t) {
+  const int size = rk::dtype_size(t->dtype);
+  int64_t n = 16 / size;
+  if (t->stride[t->ndim - 1] != 1 && t->shape[t->ndim - 1] > 1) return 1;
+  auto cut = [&](int64_t x) {
+    while (n > 1 && x % n) n /= 2;
+  };
+  cut(t->shape[t->ndim - 1]);
   for (int i = 0; i < t->ndim - 1; ++i)
-    if (t->shape[i] > 1 && t->stride[i] % n) return false;
-  return ((uintptr_t)t->data & 15) == 0;
+    if (t->shape[i] > 1) cut(t->stride[i]);
+  while (n > 1 && (uintptr_t)t->data % (n * size)) n /= 2;
+  return n * size < 4 ? 1 : (int)n;
 }
 
 // What a call writes must not repeat by a stride of 0.
@@ -300,8 +330,14 @@ bool same_tokens(const rk_tensor* a, const rk_tensor* b) {
 }
 
 template <class F>
-int by_type(int dtype, bool vec, F&& f) {
-  auto on = [&](auto dt) { vec ? f(dt, std::true_type{}) : f(dt, std::false_type{}); };
+int by_type(int dtype, int e, F&& f) {
+  auto on = [&](auto dt) {
+    constexpr int most = 16 / decltype(dt)::kBytes;
+    if (e == most) return f(dt, std::integral_constant<int, most>{});
+    if (e == most / 2) return f(dt, std::integral_constant<int, most / 2>{});
+    if (e == most / 4 && most / 4 > 1) return f(dt, std::integral_constant<int, most / 4>{});
+    f(dt, std::integral_constant<int, 1>{});
+  };
   if (dtype == RK_F16)
     on(rk::F16{});
   else if (dtype == RK_BF16)
@@ -311,16 +347,42 @@ int by_type(int dtype, bool vec, F&& f) {
   return hipGetLastError() == hipSuccess ? RK_OK : RK_ERR_HIP;
 }
 
+// e: what all tensors allow.
 template <bool PAGED>
-int launch(RotaryArgs& a, int dtype, bool vec, void* stream) {
-  const int E = vec ? 16 / rk::dtype_size(dtype) : 1;
-  if (E > 1 && (a.D % E || (a.pos && a.P % E))) vec = false;
+int launch(RotaryArgs& a, int dtype, int e, void* stream) {
+  while (a.pos && a.P % e) e /= 2;
+  if (e * rk::dtype_size(dtype) < 4) e = 1;
   a.tokens = a.N >= 2048 ? kMaxTokens : 1;
+  a.turned = a.pos ? a.P / e : 0;
+  a.copied = (a.D - (a.pos ? 2 * a.P : 0)) / e;
+  a.all = a.D / e;
+  const int64_t per = a.turned + (a.copied + 1) / 2, half = (a.all + 1) / 2;
+  const int64_t heads[kParts] = {a.part[kQ].heads, a.part[kK].heads, a.part[kV].heads};
+  a.nq = (int32_t)(heads[kQ] * per);
+  a.nk = (int32_t)(heads[kK] * per);
+  const int64_t items = a.nq + a.nk + heads[kV] * half;
+  a.token = divisor_of(items, kMaxTokens * items);
+  a.head[kQ] = a.head[kK] = divisor_of(per, std::max(heads[kQ], heads[kK]) * per);
+  a.head[kV] = divisor_of(half, heads[kV] * half);
+  // Stores of whole lines leave the caches to others: 3 x 32 heads x 2304 tokens of
+  // 80 channels in fp32 (142 MB in all) take 27 us (a copy of as much 26), 39 with
+  // ordinary stores; 17 prompts of up to 4097 tokens into pages 177 and 183.  Lines
+  // that two stores share have to meet in a cache: 23205 tokens of 96 heads of 96
+  // channels in fp16 take 227 us with 48 pairs, 253 past the caches.
+  const int size = rk::dtype_size(dtype), run = (a.pos ? a.P : a.D) * size;
+  const bool once = e * size == 16 && run >= 128 && run % 32 == 0 && a.D * size % 32 == 0;
   const int64_t grid = (a.N + a.tokens - 1) / a.tokens;
   if (grid >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
-  return by_type(dtype, vec, [&](auto dt, auto v) {
-    hipLaunchKernelGGL((rotary_kernel<decltype(dt), decltype(v)::value, PAGED>), dim3((unsigned)grid), dim3(kThreads),
-                       0, (hipStream_t)stream, a);
+  return by_type(dtype, e, [&](auto dt, auto n) {
+    constexpr int E = decltype(n)::value;
+    if constexpr (E * decltype(dt)::kBytes == 16)
+      if (once) {
+        hipLaunchKernelGGL((rotary_kernel<decltype(dt), E, PAGED, true>), dim3((unsigned)grid), dim3(kThreads), 0,
+                           (hipStream_t)stream, a);
+        return;
+      }
+    hipLaunchKernelGGL((rotary_kernel<decltype(dt), E, PAGED, false>), dim3((unsigned)grid), dim3(kThreads), 0,
+                       (hipStream_t)stream, a);
   });
 }
 
@@ -334,13 +396,13 @@ extern "C" int rk_rotary(const rk_tensor* q, const rk_tensor* k, const rk_tensor
   if (rank != 3 && rank != 4) return RK_ERR_RANK;
   RotaryArgs a;
   memset(&a, 0, sizeof(a));
-  bool vec = true;
+  int vec = 8;
   for (const rk_tensor* t : {q, q_out, k, k_out}) {
     if (!t) continue;
     if (int st = check_x(t, rank)) return st;
     if (t->dtype != q->dtype) return RK_ERR_DTYPE;
     if (!same_tokens(t, q)) return RK_ERR_SHAPE;
-    vec = vec && vec16(t);
+    vec = std::min(vec, vector_of(t));
   }
   if (!same_shape(q, q_out) || (k && !same_shape(k, k_out))) return RK_ERR_SHAPE;
   for (const rk_tensor* t : {q_out, k_out})
@@ -377,13 +439,13 @@ extern "C" int rk_paged_append(const rk_tensor* k_new, const rk_tensor* v_new, c
   int64_t B = 0, cap = 0;
   int st = rk::set_pages(pages, &a.map, &B, &cap);
   if (st) return st;
-  bool vec = vec16(&pages->k) && vec16(&pages->v);
+  int vec = std::min(vector_of(&pages->k), vector_of(&pages->v));
   for (const rk_tensor* t : {k_new, v_new, q, q_out}) {
     if (!t) continue;
     if ((st = check_x(t, rank))) return st;
     if (t->dtype != k_new->dtype) return RK_ERR_DTYPE;
     if (!same_tokens(t, k_new)) return RK_ERR_SHAPE;
-    vec = vec && vec16(t);
+    vec = std::min(vec, vector_of(t));
   }
   if (!same_shape(k_new, v_new) || (q && !same_shape(q, q_out))) return RK_ERR_SHAPE;
   if (pages->k.dtype != k_new->dtype) return RK_ERR_DTYPE;
