@@ -63,14 +63,29 @@ __device__ __forceinline__ float2 both_halves(float x) {
   return make_float2(__builtin_bit_cast(float, one), __builtin_bit_cast(float, two));
 }
 
-// Where the pieces of a row of Keys or Values lie in LDS: piece c at c ^ swap.
+// Where piece c of row r of a tile of Keys or Values lies in its row of CH pieces in
+// LDS, and which piece lies at a place.  Rows are 16 CH bytes apart, so the rows that
+// meet the same banks are every 4th, 2nd or each; they are moved apart by a rotation
+// or an exclusive or, so that the 16 lanes of a read of Keys (one piece of 16 rows)
+// and of Values (four rows of four pieces) have banks of their own.
 template <int CH>
-__device__ __forceinline__ int key_swap(int row) {
-  return CH == 16 ? row & 15 : (row >> 1) & 7;
+__device__ __forceinline__ int key_place(int c, int r) {
+  if (CH == 12) return (c + (r >> 2 & 3)) % 12;
+  return c ^ (CH == 16 ? r & 15 : CH == 8 ? r >> 1 & 7 : r >> 2 & 3);
 }
 template <int CH>
-__device__ __forceinline__ int value_swap(int row) {
-  return CH == 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+__device__ __forceinline__ int key_piece(int at, int r) {
+  if (CH == 12) return (at + 12 - (r >> 2 & 3)) % 12;
+  return key_place<CH>(at, r);
+}
+template <int CH>
+__device__ __forceinline__ int value_place(int c, int r) {
+  if (CH == 12) return key_place<CH>(c, r);
+  return c ^ (CH == 16 ? (r & 3) << 2 : CH == 8 ? (r >> 1 & 1) << 2 : 0);
+}
+template <int CH>
+__device__ __forceinline__ int value_piece(int at, int r) {
+  return CH == 12 ? key_piece<CH>(at, r) : value_place<CH>(at, r);
 }
 
 // New tokens of request b: first and how many.
@@ -132,12 +147,17 @@ __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, r
   dst[(c + 1) * a.o_sd] = DT::from_f32(y1 * inv);
 }
 
-// NB: blocks of 32 channels.  FULL: all pieces of a row in LDS hold channels.
-template <class DT, int NB, bool FULL>
-__global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArgs a) {
-  constexpr int CH = NB <= 2 ? 8 : 16;        // 16-byte pieces of a row in LDS
+// Waves of a SIMD: what the accumulators of the channels leave room for (64
+// channels, 8192 tokens: 277 us with two, 262 with three).
+constexpr int waves_of(int KC) { return KC <= 4 ? 3 : 2; }
+
+// KC: blocks of 16 channels.
+template <class DT, int KC>
+__global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(const PagedArgs a) {
+  constexpr int NB = (KC + 1) / 2;     // blocks of 32 channels
+  constexpr int CH = 4 * NB;           // 16-byte pieces of a row in LDS
   constexpr int Pitch = CH * 16;              // bytes
-  constexpr int Passes = kTile * CH / kPagedThreads;  // loads of a wave for a tile's Keys
+  constexpr int Loads = NB;  // of a wave for a tile's Keys
   // two tiles; arrays of their own, so that reads of one do not wait for loads into the other
   __shared__ __align__(16) char s_k0[kTile * Pitch], s_k1[kTile * Pitch], s_v0[kTile * Pitch], s_v1[kTile * Pitch];
   __shared__ int s_wave[kPagedWaves], s_found[2];
@@ -176,9 +196,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
   const int w_last = min(wave * kWaveRows + kWaveRows, rows) - 1;  // the wave's last row
   const int w_lo = max(p0 + (row0 + wave * kWaveRows) / a.G, 0);
   const int w_hi = w_last < wave * kWaveRows ? -1 : p0 + (row0 + w_last) / a.G;
-  uint4 q[2 * NB];
+  uint4 q[KC];
 #pragma unroll
-  for (int c = 0; c < 2 * NB; ++c) {
+  for (int c = 0; c < KC; ++c) {
     const int ch = 16 * c + 8 * hi;
     q[c] = make_uint4(0, 0, 0, 0);
     if (mine && ch < a.D) {
@@ -202,32 +222,25 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
   };
   // A wave loads 16 rows of a tile straight to LDS, a lane 16 bytes: lane l's go
   // to the l-th place of the load's part of the tile, so it asks for the piece
-  // that belongs there.  Pieces are swapped about in each row, so that the 16
-  // lanes of a read of Keys (one piece of 16 rows) and of Values (four rows of
-  // four pieces) meet different banks.  Eight rows lie in one page: one scalar
-  // address for them, and the lanes' offsets, which stay from tile to tile.  Behind
-  // the last token its row is loaded again (its weight is zero there), and where
-  // there is no page the pool's first row.
-  constexpr int PerLoad = 64 / CH;   // rows
-  constexpr int Loads = Passes / 2;  // of eight rows
-  const int lrow = lane / CH, lpc = lane % CH;
-  uint32_t k_off[Passes], v_off[Passes];  // bytes
-  int k_piece[Passes], v_piece;
-#pragma unroll
-  for (int s = 0; s < Passes; ++s) k_piece[s] = lpc ^ key_swap<CH>(PerLoad * s + lrow);
-  v_piece = lpc ^ value_swap<CH>(lrow);
-  // (the offsets of tile i: those behind its last token count in the last tile alone)
-  auto row_of = [&](int i, int s) {
-    const int last = hi_p - seen.token(i) - 16 * wave - (s < Loads ? 0 : 8);
-    return (uint32_t)min(PerLoad * (s % Loads) + lrow, max(last, 0));
+  // that belongs there (past D: the first one again; queries are zero there, and
+  // those channels of the output are not written).  Eight rows lie in one page: one
+  // scalar address for them, and the lanes' offsets, which stay from tile to tile.
+  // Behind the last token its row is loaded again (its weight is zero there), and
+  // where there is no page the pool's first row.
+  auto row_of = [&](int s) { return (64 * s + lane) / CH; };
+  auto place_of = [&](int s) { return (64 * s + lane) % CH; };
+  uint32_t k_off[Loads], v_off[Loads];  // bytes
+  auto offset = [&](int i, int s, int piece, int64_t ss) {
+    const int row = row_of(s), last = hi_p - seen.token(i) - 16 * wave - (row & 8);
+    return 2 * ((uint32_t)min(row & 7, max(last, 0)) * (uint32_t)ss + 8 * (8 * piece < a.D ? piece : 0));
   };
   auto k_offsets = [&](int i) {
 #pragma unroll
-    for (int s = 0; s < Passes; ++s) k_off[s] = 2 * (row_of(i, s) * (uint32_t)a.k_ss + 8 * k_piece[s]);
+    for (int s = 0; s < Loads; ++s) k_off[s] = offset(i, s, key_piece<CH>(place_of(s), row_of(s)), a.k_ss);
   };
   auto v_offsets = [&](int i) {
 #pragma unroll
-    for (int s = 0; s < Passes; ++s) v_off[s] = 2 * (row_of(i, s) * (uint32_t)a.v_ss + 8 * v_piece);
+    for (int s = 0; s < Loads; ++s) v_off[s] = offset(i, s, value_piece<CH>(place_of(s), row_of(s)), a.v_ss);
   };
   struct Eight {
     const char* at[2];
@@ -252,24 +265,24 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
     }
     return r;
   };
-  auto load_k = [&](char* dst, const Eight& r, int s) {
-    if (FULL || 8 * k_piece[s] < a.D)
-      __builtin_amdgcn_global_load_lds((global_ptr)(r.at[s / Loads] + k_off[s]),
-                                       (lds_ptr)(dst + 16 * wave * Pitch + s * 1024), 16, 0, 0);
+  auto load = [&](char* dst, const Eight& r, int s, uint32_t off) {
+    constexpr int Half = 8 * CH;  // lanes of eight rows
+    const char* from = 64 * s >= Half ? r.at[1] : r.at[0];
+    if (64 * s < Half && 64 * s + 64 > Half) from = 64 * s + lane < Half ? r.at[0] : r.at[1];
+    __builtin_amdgcn_global_load_lds((global_ptr)(from + off), (lds_ptr)(dst + 16 * wave * Pitch + s * 1024), 16, 0, 0);
   };
-  auto load_v = [&](char* dst, const Eight& r, int s) {
-    if (FULL || 8 * v_piece < a.D)
-      __builtin_amdgcn_global_load_lds((global_ptr)(r.at[s / Loads] + v_off[s]),
-                                       (lds_ptr)(dst + 16 * wave * Pitch + s * 1024), 16, 0, 0);
-  };
-  int k_at[2 * NB], v_at[NB];  // of this lane's reads of a tile
+  auto load_k = [&](char* dst, const Eight& r, int s) { load(dst, r, s, k_off[s]); };
+  auto load_v = [&](char* dst, const Eight& r, int s) { load(dst, r, s, v_off[s]); };
+  int k_at[KC], v_at[NB][2];  // of this lane's reads of a tile; Values: eight rows on
 #pragma unroll
-  for (int c = 0; c < 2 * NB; ++c) k_at[c] = col * Pitch + (((2 * c + hi) ^ key_swap<CH>(col)) << 4);
+  for (int c = 0; c < KC; ++c) k_at[c] = col * Pitch + (key_place<CH>(2 * c + hi, col) << 4);
 #pragma unroll
   for (int c = 0; c < NB; ++c) {
     // lane i of 16 addresses row i / 4, four channels from 4 (i % 4), and gets channel i of four rows
-    const int row = (lane & 15) >> 2, piece = 4 * c + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    v_at[c] = (4 * hi + row) * Pitch + ((piece ^ value_swap<CH>(row)) << 4) + 8 * (lane & 1);
+    const int row = 4 * hi + ((lane & 15) >> 2), piece = 4 * c + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    v_at[c][0] = row * Pitch + (value_place<CH>(piece, row) << 4) + 8 * (lane & 1);
+    v_at[c][1] = CH == 12 ? (row + 8) * Pitch + (value_place<CH>(piece, row + 8) << 4) + 8 * (lane & 1)
+                          : v_at[c][0] + 8 * Pitch;
   }
   // Scores of a tile: products of two chains, reads a few products ahead.
   auto scores = [&](const char* sk, f32x16 (&n)[2]) {
@@ -278,7 +291,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
 #pragma unroll
       for (int e = 0; e < 16; ++e) n[tb][e] = 0.f;
 #pragma unroll
-    for (int c = 0; c < 2 * NB; ++c)
+    for (int c = 0; c < KC; ++c)
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb)
         n[tb] = mfma32<DT>(*(const uint4*)(sk + k_at[c] + 32 * tb * Pitch), q[c], n[tb]);
@@ -347,19 +360,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
     }
   };
   auto value_at = [&](const char* sv, int g, int c) {  // 16 tokens by 32 channels
-    const char* at = sv + v_at[c] + 16 * g * Pitch;
-    const uint2 u0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at));
-    const uint2 u1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * Pitch)));
+    const char* at = sv + 16 * g * Pitch;
+    const uint2 u0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + v_at[c][0])));
+    const uint2 u1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + v_at[c][1])));
     return make_uint4(u0.x, u0.y, u1.x, u1.y);
   };
   if (i0 < i1) {
-    if (!FULL) {  // pieces past D are never loaded: they stay zero
-      for (int at = 16 * tid; at < kTile * Pitch; at += 16 * kPagedThreads) {
-        *(uint4*)(s_k0 + at) = *(uint4*)(s_k1 + at) = *(uint4*)(s_v0 + at) = *(uint4*)(s_v1 + at) =
-            make_uint4(0, 0, 0, 0);
-      }
-      __syncthreads();
-    }
     // pages of tiles i + 1 (Values to come), i + 2 (Keys to come) and i + 3
     const int end = i1 - 1;
     uint32_t page0 = page_at(i0), page1 = page_at(min(i0 + 1, end)), page2 = page_at(min(i0 + 2, end));
@@ -368,16 +374,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
       k_offsets(i0);
       const Eight k0 = rows_at(i0, page0, kb, a.k_sp, a.k_ss), v0 = rows_at(i0, page0, vb, a.v_sp, a.v_ss);
 #pragma unroll
-      for (int r = 0; r < Passes; ++r) load_k(s_k0, k0, r);
+      for (int r = 0; r < Loads; ++r) load_k(s_k0, k0, r);
       v_offsets(i0);
 #pragma unroll
-      for (int r = 0; r < Passes; ++r) load_v(s_v0, v0, r);
+      for (int r = 0; r < Loads; ++r) load_v(s_v0, v0, r);
       loads_done();
       __syncthreads();
       k_offsets(min(i0 + 1, end));
       const Eight k1 = rows_at(min(i0 + 1, end), page1, kb, a.k_sp, a.k_ss);
 #pragma unroll
-      for (int r = 0; r < Passes; ++r) load_k(s_k1, k1, r);
+      for (int r = 0; r < Loads; ++r) load_k(s_k1, k1, r);
       scores(s_k0, s);
       mask(i0, page0, s);
       rebase(top_of(s), s);
@@ -407,9 +413,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
       // Two products at a time, and what the other units do meanwhile: a product
       // takes the matrix unit 32 cycles, an exponential its own 16.  The fences keep
       // the mixture as it is written.
-      constexpr int kPairs = 2 * NB;
       if (!kLast) {
-        uint4 k0[kPairs], k1[kPairs];
+        uint4 k0[KC], k1[KC];
         auto read = [&](int c) {
           k0[c] = *(const uint4*)(next_k + k_at[c]);
           k1[c] = *(const uint4*)(next_k + k_at[c] + 32 * Pitch);
@@ -419,19 +424,19 @@ __global__ __launch_bounds__(kPagedThreads, 2) void window_kernel(const PagedArg
 #pragma unroll
           for (int e = 0; e < 16; ++e) n[tb][e] = 0.f;
         read(0);
-        if (kPairs > 1) read(1);
+        if (KC > 1) read(1);
         fence();
 #pragma unroll
-        for (int c = 0; c < kPairs; ++c) {
-          if (c + 2 < kPairs) read(c + 2);
+        for (int c = 0; c < KC; ++c) {
+          if (c + 2 < KC) read(c + 2);
           n[0] = mfma32<DT>(k0[c], q[c], n[0]);
           n[1] = mfma32<DT>(k1[c], q[c], n[1]);
 #pragma unroll
-          for (int r = 0; r < 2 * Passes; ++r)
-            if (r * kPairs / (2 * Passes) == c) r & 1 ? load_k(k_to, rk_, r >> 1) : load_v(v_to, rv, r >> 1);
+          for (int r = 0; r < 2 * Loads; ++r)
+            if (r * KC / (2 * Loads) == c) r & 1 ? load_k(k_to, rk_, r >> 1) : load_v(v_to, rv, r >> 1);
 #pragma unroll
           for (int k = 0; k < 24; ++k)
-            if (k * kPairs / 24 == c) weight(s, y, w, k);
+            if (k * KC / 24 == c) weight(s, y, w, k);
           fence();
         }
         mask(i + 1, page1, n);
@@ -591,22 +596,23 @@ int64_t window_slots(const PagedArgs& a) {
 
 int window_launch(const PagedArgs& a, int32_t dtype, hipStream_t s) {
   const int64_t grid = window_slots(a) * a.H * a.splits, rows = a.N * a.Hq;
-  const int NB = (a.D + 31) / 32;
-  auto on = [&](auto dt, auto nb, auto full) {
-    hipLaunchKernelGGL((window_kernel<decltype(dt), decltype(nb)::value, decltype(full)::value>), dim3((unsigned)grid),
-                       dim3(kPagedThreads), 0, s, a);
+  auto on = [&](auto dt, auto kc) {
+    constexpr int KC = decltype(kc)::value;
+    hipLaunchKernelGGL((window_kernel<decltype(dt), KC>), dim3((unsigned)grid), dim3(kPagedThreads), 0, s, a);
     if (a.splits > 1)
       hipLaunchKernelGGL((window_join_kernel<decltype(dt)>), dim3((unsigned)((rows + kPagedWaves - 1) / kPagedWaves)),
-                         dim3(kPagedThreads), 0, s, a, 32 * NB);
+                         dim3(kPagedThreads), 0, s, a, 32 * ((KC + 1) / 2));
   };
   auto by_dim = [&](auto dt) {
-    if (a.D == 128) return on(dt, std::integral_constant<int, 4>{}, std::true_type{});
-    if (a.D == 64) return on(dt, std::integral_constant<int, 2>{}, std::true_type{});
-    switch (NB) {
-      case 1: return on(dt, std::integral_constant<int, 1>{}, std::false_type{});
-      case 2: return on(dt, std::integral_constant<int, 2>{}, std::false_type{});
-      case 3: return on(dt, std::integral_constant<int, 3>{}, std::false_type{});
-      default: return on(dt, std::integral_constant<int, 4>{}, std::false_type{});
+    switch ((a.D + 15) / 16) {
+      case 1: return on(dt, std::integral_constant<int, 1>{});
+      case 2: return on(dt, std::integral_constant<int, 2>{});
+      case 3: return on(dt, std::integral_constant<int, 3>{});
+      case 4: return on(dt, std::integral_constant<int, 4>{});
+      case 5: return on(dt, std::integral_constant<int, 5>{});
+      case 6: return on(dt, std::integral_constant<int, 6>{});
+      case 7: return on(dt, std::integral_constant<int, 7>{});
+      default: return on(dt, std::integral_constant<int, 8>{});
     }
   };
   dtype == RK_F16 ? by_dim(F16{}) : by_dim(BF16{});

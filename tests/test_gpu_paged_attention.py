@@ -215,11 +215,12 @@ def test_window_layouts():
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("where", ["k", "v"])
 @pytest.mark.parametrize("T, S, window, sinks, at", [(200, 200, None, 0, 150), (200, 200, 40, 3, 20), (4, 900, None, 0, 898)])
-def test_what_is_not_seen_does_not_matter(bad, where, T, S, window, sinks, at):
+@pytest.mark.parametrize("D", [64, 80, 40])
+def test_what_is_not_seen_does_not_matter(bad, where, T, S, window, sinks, at, D):
     """One odd value at a token: queries that do not see it are as without it, the
     others as the formula says (a NaN there is a NaN here)."""
     dt, g = torch.bfloat16, torch.Generator().manual_seed(5)
-    q, k, v = (torch.randn(1, h, n, 64, generator=g).to(dt) for h, n in ((4, T), (2, S), (2, S)))
+    q, k, v = (torch.randn(1, h, n, D, generator=g).to(dt) for h, n in ((4, T), (2, S), (2, S)))
     if where == "k":
         q[..., 7] = q[..., 7].abs() + 0.5       # inf times it keeps its sign
     clean = window_attention(q.cuda(), k.cuda(), v.cuda(), 2, window, sinks).cpu()
@@ -230,7 +231,7 @@ def test_what_is_not_seen_does_not_matter(bad, where, T, S, window, sinks, at):
     assert sees.any() and not sees.all()
     assert torch.equal(got[:, :2], clean[:, :2])
     same = [7] if where == "v" else []
-    rest = [c for c in range(64) if c not in same]
+    rest = [c for c in range(D) if c not in same]
     blind = got[0, 2:, ~sees]
     # summed in another order where a neighbour is not finite
     torch.testing.assert_close(blind.float(), clean[0, 2:, ~sees].float(), rtol=2.0 ** -6, atol=2.0 ** -6)
