@@ -613,7 +613,7 @@ int rk_shared_prefix_decode(const rk_tensor* q, const rk_tensor* R_partial, cons
  * q [B,Hq,T,D], k [B,Hkv,T,D] (or NULL), positions [axes,B,T]; or q [N,Hq,D],
  * k [N,Hkv,D], positions [axes,N].  F16, BF16 or F32 alike; positions I32 or
  * I64; any strides, and an output may be its input itself (not a view of it
- * that lies otherwise). */
+ * that lies otherwise).  Fewer than 2^25 tokens (RK_ERR_SHAPE). */
 int rk_rotary(const rk_tensor* q, const rk_tensor* k, const rk_tensor* positions, const rk_tensor* inv_freq,
               const int32_t* sections, int32_t axes, int32_t interleaved, int32_t inverse, const rk_tensor* q_out,
               const rk_tensor* k_out, void* stream);
@@ -650,7 +650,9 @@ int rk_paged_append(const rk_tensor* k_new, const rk_tensor* v_new, const rk_pag
  * with starts as above (rows that no request has stay as they are).  F16 or
  * BF16 alike; D a multiple of 8, up to 128; pages with unit last stride, other
  * strides multiples of 8 and a 16-byte aligned base (RK_ERR_STRIDE); q and out
- * any strides.  Workspace and capture as for the quantised decode. */
+ * any strides.  Fewer than 2^26 rows (new tokens times query heads) of single
+ * tokens, and as many workgroups as a launch takes (RK_ERR_SHAPE).  Workspace and
+ * capture as for the quantised decode. */
 int rk_paged_attention_check(const rk_tensor* q, const int32_t* starts, const rk_pages* pages,
                              int64_t num_kv_groups, int64_t window, int64_t sinks, const rk_tensor* out,
                              int32_t num_cus, size_t* workspace_bytes);

@@ -11,6 +11,10 @@
 
 namespace rk {
 
+// Workgroups of 256 threads that a launch has less than: its threads are counted in
+// 32 bits.
+constexpr int64_t kMostGroups = INT64_C(1) << 24;
+
 // Checks a pool and its table; *B requests, *cap tokens each at most.
 inline int set_pages(const rk_pages* p, PageMap* m, int64_t* B, int64_t* cap) {
   int st;

@@ -600,6 +600,7 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
     const int64_t KD = D <= 64 ? 64 : 128;
     const int64_t units = p->B * H * cdiv(c.groups, kRows), longest = pieces_of_longest(a->map.cap, a->window, a->sinks);
     if (units * (cdiv(cap, kBlock) + 1) >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+    if (units >= rk::kMostGroups || cdiv(p->rows, kPagedWaves) >= rk::kMostGroups) return RK_ERR_SHAPE;
     a->direct = longest <= (units >= cus ? kDirectMany : kDirectFew);
     a->workers = (int32_t)(a->direct ? units : std::max<int64_t>(
         std::min<int64_t>(per_cu(D <= 64 ? 2 : 4) * (int64_t)cus, units * longest), 1));
@@ -620,7 +621,7 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
     const double tiles = cap / 64.0, record = (double)p->rows * cdiv(D, 32) * 128 * 2 / 3.1e6;
     const int64_t most = std::min(2 * (int64_t)cus / std::max<int64_t>(grid, 1), cdiv(cap, 128));
     a->splits = (int32_t)std::max<int64_t>(std::min<int64_t>(most, (int64_t)sqrt(tiles / record)), 1);
-    if (grid * a->splits >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+    if (grid * a->splits >= rk::kMostGroups) return RK_ERR_SHAPE;
     if (a->splits > 1) {
       p->acc = take((size_t)p->rows * a->splits * cdiv(D, 32) * 128);
       p->ml = take((size_t)p->rows * a->splits * 8);

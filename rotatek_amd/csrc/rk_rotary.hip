@@ -372,7 +372,7 @@ int launch(RotaryArgs& a, int dtype, int e, void* stream) {
   const int size = rk::dtype_size(dtype), run = (a.pos ? a.P : a.D) * size;
   const bool once = e * size == 16 && run >= 128 && run % 32 == 0 && a.D * size % 32 == 0;
   const int64_t grid = (a.N + a.tokens - 1) / a.tokens;
-  if (grid >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
+  if (grid >= rk::kMostGroups) return RK_ERR_SHAPE;
   return by_type(dtype, e, [&](auto dt, auto n) {
     constexpr int E = decltype(n)::value;
     if constexpr (E * decltype(dt)::kBytes == 16)

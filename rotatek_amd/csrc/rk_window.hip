@@ -99,41 +99,107 @@ __device__ __forceinline__ Queries queries_of(const PagedArgs& a, int b) {
   return {s, (int)max(e - s, (int64_t)0)};
 }
 
-// One row by one wave, two channels a lane, over the tokens that it sees alone
-// (m: the score that weights are against): any cost, for Values that are not
-// finite.
+// Whether rows of a wave (positions lo_p .. hi_p) may be not finite for what they do
+// not see in its tiles: a token without a page, one that some row does not see with a
+// Value that is not finite, or a Key that is not among the first eight channels, which
+// are read again past D where D is no multiple of 16.
+template <class DT>
+__device__ __forceinline__ bool odd_unseen(const PagedArgs& a, int b, rk::Seen<kTile> seen, int i0, int i1, int h, int lo_p,
+                                     int hi_p, int last) {
+  constexpr uint32_t kExponent = std::is_same<DT, rk::F16>::value ? 0x7c00 : 0x7f80;
+  auto odd_piece = [](const uint16_t* x) {
+    const uint4 y = *(const uint4*)x;
+    bool odd = false;
+    for (const uint32_t w : {y.x, y.y, y.z, y.w})
+      odd |= (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
+    return odd;
+  };
+  for (int i = i0; i < i1; ++i) {
+    const int j = seen.token(i) + (threadIdx.x & 63);
+    bool odd = false;
+    if (j <= last) {
+      const uint32_t page = rk::page_of(a.map, b, j);
+      const int64_t at = j & ((1u << a.map.shift) - 1);
+      odd = page >= (uint32_t)a.map.pages;
+      if (!odd && a.D % 16) odd = odd_piece((const uint16_t*)a.k + h * a.k_sh + (int64_t)page * a.k_sp + at * a.k_ss);
+      if (!odd && !(j <= lo_p && (hi_p - j < a.window || j < a.sinks))) {
+        const uint16_t* v = (const uint16_t*)a.v + h * a.v_sh + (int64_t)page * a.v_sp + at * a.v_ss;
+        for (int c = 0; c < a.D; c += 8) odd |= odd_piece(v + c);
+      }
+    }
+    if (__any(odd)) return true;
+  }
+  return false;
+}
+
+// One row by one wave, over the tokens that it sees alone (m: the score that weights
+// are against): for Values that are not finite, until all its channels are NaN.  A
+// lane forms the weight of one token of a tile, and sums two channels over all of them.
 template <class DT>
 __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, rk::Seen<kTile> seen, int i0, int i1, int h,
                                      int row, int p0, int split, int KD, float m) {
+  const int lane = threadIdx.x & 63;
   const int t = row / a.G, hq = h * a.G + row - t * a.G, p = p0 + t;
-  const int c = 2 * (threadIdx.x & 63);
+  const int c = 2 * lane;
   const bool on = c < a.D;
   const uint16_t* q = (const uint16_t*)a.q + b * a.q_sb + (qs.first + t) * a.q_st + hq * a.q_sh;
   const uint16_t* kb = (const uint16_t*)a.k + h * a.k_sh;
   const uint16_t* vb = (const uint16_t*)a.v + h * a.v_sh;
   const float q0 = on ? DT::to_f32(q[c * a.q_sd]) : 0.f, q1 = on ? DT::to_f32(q[(c + 1) * a.q_sd]) : 0.f;
+  auto lane_of = [](float x, int i) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), i));
+  };
   const float base = base_of(m);
   float l = 0.f, y0 = 0.f, y1 = 0.f;
   for (int i = i0; i < i1; ++i) {
-    const int t0 = seen.token(i);
-    for (int j = t0; j < t0 + kTile; ++j) {
-      if (!rk::sees(p, j, a.window, a.sinks)) continue;
-      const uint32_t page = rk::page_of(a.map, b, j);
-      if (page >= (uint32_t)a.map.pages) continue;
-      const int64_t at = j & ((1u << a.map.shift) - 1);
-      const uint16_t* k = kb + (int64_t)page * a.k_sp + at * a.k_ss;
-      const uint16_t* v = vb + (int64_t)page * a.v_sp + at * a.v_ss;
-      float s = on ? q0 * DT::to_f32(k[c]) + q1 * DT::to_f32(k[c + 1]) : 0.f;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) s += rk::shfl_xor(s, d);
-      const float w = rk::fast_exp2((s - base) * a.scale_log2);
-      l += w;
-      if (on) {
-        y0 += w * DT::to_f32(v[c]);
-        y1 += w * DT::to_f32(v[c + 1]);
-      }
+    const int t0 = seen.token(i), j = t0 + lane;
+    bool there = rk::sees(p, j, a.window, a.sinks);
+    uint32_t page = 0;
+    float w = 0.f;
+    if (there) {
+      page = rk::page_of(a.map, b, j);
+      there = page < (uint32_t)a.map.pages;
     }
+    const int64_t at = j & ((1u << a.map.shift) - 1);
+    if (there) {
+      const uint16_t* k = kb + (int64_t)page * a.k_sp + at * a.k_ss;
+      float s = 0.f;
+      for (int d = 0; d < a.D; d += 8) {
+        const uint4 x = *(const uint4*)(k + d);
+        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s = __builtin_fmaf(lane_of(q0, d / 2 + e), DT::to_f32((uint16_t)u[e]), s);
+          s = __builtin_fmaf(lane_of(q1, d / 2 + e), DT::to_f32((uint16_t)(u[e] >> 16)), s);
+        }
+      }
+      w = rk::fast_exp2((s - base) * a.scale_log2);
+    }
+    l += w;
+    const uint64_t bits = __ballot(there);
+    constexpr int kAhead = 8;
+    for (int j0 = 0; j0 < kTile; j0 += kAhead) {
+      uint32_t v[kAhead];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        v[e] = 0;
+        if ((bits >> (j0 + e) & 1) && on) {
+          const uint32_t pg = (uint32_t)__builtin_amdgcn_readlane((int)page, j0 + e);
+          v[e] = *(const uint32_t*)(vb + (int64_t)pg * a.v_sp + ((t0 + j0 + e) & ((1u << a.map.shift) - 1)) * a.v_ss + c);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e)
+        if (bits >> (j0 + e) & 1) {
+          const float x = lane_of(w, j0 + e);
+          y0 = __builtin_fmaf(x, DT::to_f32((uint16_t)v[e]), y0);
+          y1 = __builtin_fmaf(x, DT::to_f32((uint16_t)(v[e] >> 16)), y1);
+        }
+    }
+    if (__all(!on || (y0 != y0 && y1 != y1))) break;
   }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) l += rk::shfl_xor(l, d);
   if (!on) return;
   if (a.splits > 1) {
     const int64_t rec = (int64_t)split * a.N * a.Hq + (b * (int64_t)a.T + qs.first + t) * a.Hq + hq;
@@ -494,8 +560,8 @@ __global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(con
   const float2 sums = both_halves(l);
   l = sums.x + sums.y;
   // Weight 0 times an infinity or a NaN is a NaN: a tile's Values reach rows
-  // that do not see them.  Rows that are not finite are summed again from what
-  // they see.
+  // that do not see them.  Where there are such, rows that are not finite are summed
+  // again from what they see.
   float probe = l * 0.f;
 #pragma unroll
   for (int c = 0; c < NB; ++c)
@@ -503,6 +569,7 @@ __global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(con
     for (int e = 0; e < 16; ++e) probe += o[c][e] * 0.f;
   const uint64_t odd = __ballot(mine && probe != 0.f);
   uint32_t again = (uint32_t)odd | (uint32_t)(odd >> 32);
+  if (again && !odd_unseen<DT>(a, b, seen, i0, i1, h, p0 + (row0 + wave * kWaveRows) / a.G, w_hi, hi_p)) again = 0;
   const bool done = again >> col & 1;
   while (again) {
     const int rr = __builtin_ctz(again);

@@ -247,6 +247,62 @@ def test_what_is_not_seen_does_not_matter(bad, where, T, S, window, sinks, at, D
         assert torch.isnan(got[0, 2:, sees]).all()
 
 
+@pytest.mark.parametrize("dtype", HALF)
+def test_values_that_are_not_finite(dtype):
+    """Rows ahead of the text see nothing, whatever token 0 holds; all NaN gives NaN;
+    an infinity that all rows see stays in its channel."""
+    dt, g = DTYPES[dtype], torch.Generator().manual_seed(6)
+    q, k, v = (torch.randn(1, h, n, 64, generator=g).to(dt) for h, n in ((2, 300), (1, 270), (1, 270)))
+    clean = window_attention(q.cuda(), k.cuda(), v.cuda(), 2).cpu()
+    v[0, 0, 0, 3] = float("inf")
+    got = window_attention(q.cuda(), k.cuda(), v.cuda(), 2).cpu()
+    assert (got[:, :, :30] == 0).all() and (got[:, :, 30:, 3] == float("inf")).all()
+    got[..., 3] = clean[..., 3]
+    # (in a wave whose rows do not all see it, sums are formed in another order)
+    torch.testing.assert_close(got.float(), clean.float(), rtol=2.0 ** -6, atol=2.0 ** -6)
+    assert torch.equal(got[:, :, 96:], clean[:, :, 96:])
+    v[:] = float("nan")
+    got = window_attention(q.cuda(), k.cuda(), v.cuda(), 2).cpu()
+    assert (got[:, :, :30] == 0).all() and torch.isnan(got[:, :, 30:]).all()
+
+
+@pytest.mark.parametrize("per, window", [(2, None), (40, None), (40, 70)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [2, 1, 30]])
+def test_captured_calls(per, window, new):
+    """Every form in a graph (a launch or two, tokens cut or not), replayed with other
+    lengths, queries and pages, against the eager call, with eager work between."""
+    dt, page, H, G, D = torch.float16, 16, 2, 3, 64
+    torch.manual_seed(7)
+    k, v = (torch.randn(3 * per + 2, H, page, D, device="cuda").to(dt) for _ in range(2))
+    table = torch.randperm(3 * per + 2, device="cuda")[:3 * per].to(torch.int32).view(3, per)
+    lens = torch.full((3,), 30, dtype=torch.int32, device="cuda")
+    q, starts = torch.randn(sum(new), H * G, D, device="cuda").to(dt), starts_of(new)
+
+    def call():
+        if max(new) == 1:
+            return paged_decode(q, k, v, table, lens, G, window, 3)[:, 0]
+        return paged_prefill(q, starts, k, v, table, lens, G, window, 3)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(12):
+        lens.copy_(torch.randint(0, per * page + 3, (3,)))
+        q.copy_(torch.randn(q.shape, device="cuda").to(dt))
+        table.copy_(torch.randperm(3 * per + 2, device="cuda")[:3 * per].to(torch.int32).view(3, per))
+        want = call().clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+
+
 def test_decode_is_its_prefill():
     """The same tokens through both: within both's bounds of each other."""
     dt, lens = torch.bfloat16, [1, 77, 640]

@@ -214,6 +214,7 @@ def test_attention_takes():
     (dict(p=pool(table_stride=(1, 3))), _lib.RK_ERR_STRIDE),
     (dict(p=pool(stride=(2048, 1024, 64, 2))), _lib.RK_ERR_STRIDE),
     (dict(p=pool(stride=(2112, 1056, 66, 1))), _lib.RK_ERR_STRIDE),
+    (dict(p=pool(stride=(1 << 32, 1 << 31, 1 << 27, 1))), _lib.RK_ERR_STRIDE),  # eight rows past 32 bits of bytes
     (dict(window=-1), _lib.RK_ERR_ARG),
     (dict(sinks=-1), _lib.RK_ERR_ARG),
     (dict(out=desc((3, 4, 72))), _lib.RK_ERR_SHAPE),
@@ -222,6 +223,22 @@ def test_attention_takes():
 ])
 def test_attention_refuses(call, status):
     assert attention(**call) == status
+
+
+def test_attention_refuses_more_than_a_launch():
+    """A launch's threads are counted in 32 bits: 2^24 workgroups of 256 are too many."""
+    most = 1 << 24
+
+    def single(B, H, groups, tokens=16):
+        return window(q=(B, H * groups, 1, 64), k=(B, H, tokens, 64), groups=groups)
+
+    assert single(most - 1, 1, 1) == 0
+    assert single(most, 1, 1) == _lib.RK_ERR_SHAPE
+    assert single(most // 8, 8, 4) == _lib.RK_ERR_SHAPE
+    assert single(most // 8 - 1, 8, 4) == 0
+    assert single(most // 2, 1, 8, 16) == _lib.RK_ERR_SHAPE          # rows to join, four a workgroup
+    assert window(q=(most - 1, 1, 2, 64), k=(most - 1, 1, 16, 64), groups=1) == 0
+    assert window(q=(most, 1, 2, 64), k=(most, 1, 16, 64), groups=1) == _lib.RK_ERR_SHAPE
 
 
 def test_attention_without_a_pool_or_output():
@@ -282,6 +299,12 @@ def rotary(q=None, k=None, pos=None, freq=None, sections=(32,), axes=1, interlea
 ])
 def test_rotary_refuses(call, status):
     assert rotary(**call) == status
+
+
+def test_rotary_refuses_more_than_a_launch():
+    most = 1 << 25
+    assert rotary(q=desc((1, 1, most, 64)), pos=desc((1, 1, most), _lib.RK_I32)) == _lib.RK_ERR_SHAPE
+    assert append(k=desc((3, 2, most, 64))) == _lib.RK_ERR_SHAPE
 
 
 def append(k=None, v=None, p=None, starts=None, q=None, qo=None, pos=None, freq=None):
