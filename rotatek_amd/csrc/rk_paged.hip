@@ -19,6 +19,11 @@
 // come straight from memory in 16-byte pieces; a lane's eight Value rows by
 // eight channels are turned by v_perm.  Weights enter the products as two
 // 16-bit terms (2^-16 of a weight in all).
+//
+// 32 requests of 16000 tokens, 32/8 heads of 128, fp16: 320 us, 6.6 TB/s, where a
+// plain read runs at 7.1 (one workgroup a CU 411 and with rows five steps ahead
+// 386, of a form of two that took 373).  One of 2400 tokens: 8 us, three memory
+// latencies behind each other (length, table, rows), and 4 for the join.
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <math.h>

@@ -11,6 +11,8 @@
 // for all heads of the token and go through LDS; then every lane turns a
 // vector of pairs (16 bytes from either half of the head) of one head.  In an
 // append the same pass writes Keys and Values to their pages.
+//
+// The bytes bound it: 1.6 GB of video heads in 300 us, 5.3 TB/s, as a copy.
 #include <hip/hip_runtime.h>
 #include <string.h>
 

@@ -12,6 +12,12 @@
 // V^T is read by the transposing LDS load.  Weights are rounded to the inputs'
 // type (2^-9 of each in bf16, as much as the output's own rounding); maxima,
 // sums and accumulators are 32-bit.
+//
+// 8192 tokens, 32/8 heads of 128, window 4096, bf16: 405 us, 1.02 PFLOP/s (a large
+// matrix product 1.34).  Power bounds it: the matrix units are busy half of the
+// cycles, and the clock falls from 2.35 GHz to 1.75; waits for loads, barriers or
+// LDS taken away leave the time as it is, the loads of tiles themselves 353.  64
+// rows a wave, which read LDS half as often, leave one wave a SIMD: 487.
 #include <hip/hip_runtime.h>
 #include <limits.h>
 
