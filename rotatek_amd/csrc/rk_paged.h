@@ -58,6 +58,7 @@ struct PagedArgs {
   int32_t workers;         // one new token each: workgroups of the split launch
   int32_t direct;          // ... a unit each, no shares and no join
   int32_t splits;          // many: parts that a row's tokens are cut into
+  int32_t round;           // ... workgroups of a KV head that CUs take one each of, where all begin at once (0: not)
   int32_t q_vec, o_vec;
   float scale_log2;  // log2(e) / sqrt(D)
 };
@@ -65,6 +66,7 @@ struct PagedArgs {
 // The launches over many new tokens a request (rk_window.hip); a status.
 // Slots: workgroups of a KV head and split.
 int64_t window_slots(const PagedArgs& a);
+int window_per_cu(const PagedArgs& a);  // workgroups that a CU holds
 int window_launch(const PagedArgs& a, int32_t dtype, hipStream_t s);
 
 }  // namespace rk

@@ -627,6 +627,12 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
     const int64_t most = std::min(2 * (int64_t)cus / std::max<int64_t>(grid, 1), cdiv(cap, 128));
     a->splits = (int32_t)std::max<int64_t>(std::min<int64_t>(most, (int64_t)sqrt(tiles / record)), 1);
     if (grid * a->splits >= rk::kMostGroups) return RK_ERR_SHAPE;
+    // One round, of more than a workgroup a CU: long and short ones on each (causal, 3 x
+    // 1018 tokens, 16 query heads to each of 2 of 64: 40.8 us, 29.8 so; 8 x 600, 8 heads
+    // of 128: 27.5 and 25.1; requests of equal windows: as long).  More rounds even out by
+    // themselves, and keep a request's tiles together.
+    if (grid * a->splits > cus && grid * a->splits <= rk::window_per_cu(*a) * cus)
+      a->round = (int32_t)std::max<int64_t>(cus / H, 1);
     if (a->splits > 1) {
       p->acc = take((size_t)p->rows * a->splits * cdiv(D, 32) * 128);
       p->ml = take((size_t)p->rows * a->splits * 8);

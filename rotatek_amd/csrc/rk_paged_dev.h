@@ -79,6 +79,25 @@ struct Line {
     }
   }
 
+  // Up to 64 requests, the first piece of each before the second ones: the request of
+  // piece `at`, and how many of its own come before it.
+  __device__ __forceinline__ Found across(int at) const {
+    auto within = [&](int n) { return __builtin_amdgcn_readlane(wave_sum_to(min(mine, n)), 63); };  // the first n of each
+    int low = 0, high = 1;
+    while (within(high) <= at) {
+      low = high;
+      high *= 2;
+    }
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (within(mid) <= at) low = mid; else high = mid;
+    }
+    const int left = at - within(low);  // (by all lanes, ahead of any condition)
+    const uint64_t more = __ballot(mine > low);
+    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(more >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)more, 0));
+    return {__builtin_ctzll(__ballot((mine > low) & (rank == left))), low};
+  }
+
   // `at` below the sum.
   __device__ __forceinline__ Found find(int at) {
     if (B <= 64) {

@@ -167,20 +167,19 @@ __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, r
       there = page < (uint32_t)a.map.pages;
     }
     const int64_t at = j & ((1u << a.map.shift) - 1);
-    if (there) {
-      const uint16_t* k = kb + (int64_t)page * a.k_sp + at * a.k_ss;
-      float s = 0.f;
-      for (int d = 0; d < a.D; d += 8) {
-        const uint4 x = *(const uint4*)(k + d);
-        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    const uint16_t* k = kb + (int64_t)page * a.k_sp + at * a.k_ss;
+    float s = 0.f;
+    for (int d = 0; d < a.D; d += 8) {  // (by all lanes: a lane's channels of q are read by the others)
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (there) x = *(const uint4*)(k + d);
+      const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s = __builtin_fmaf(lane_of(q0, d / 2 + e), DT::to_f32((uint16_t)u[e]), s);
-          s = __builtin_fmaf(lane_of(q1, d / 2 + e), DT::to_f32((uint16_t)(u[e] >> 16)), s);
-        }
+      for (int e = 0; e < 4; ++e) {
+        s = __builtin_fmaf(lane_of(q0, d / 2 + e), DT::to_f32((uint16_t)u[e]), s);
+        s = __builtin_fmaf(lane_of(q1, d / 2 + e), DT::to_f32((uint16_t)(u[e] >> 16)), s);
       }
-      w = rk::fast_exp2((s - base) * a.scale_log2);
     }
+    if (there) w = rk::fast_exp2((s - base) * a.scale_log2);
     l += w;
     const uint64_t bits = __ballot(there);
     constexpr int kAhead = 8;
@@ -189,9 +188,9 @@ __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, r
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
         v[e] = 0;
-        if ((bits >> (j0 + e) & 1) && on) {
+        if (bits >> (j0 + e) & 1) {
           const uint32_t pg = (uint32_t)__builtin_amdgcn_readlane((int)page, j0 + e);
-          v[e] = *(const uint32_t*)(vb + (int64_t)pg * a.v_sp + ((t0 + j0 + e) & ((1u << a.map.shift) - 1)) * a.v_ss + c);
+          if (on) v[e] = *(const uint32_t*)(vb + (int64_t)pg * a.v_sp + ((t0 + j0 + e) & ((1u << a.map.shift) - 1)) * a.v_ss + c);
         }
       }
 #pragma unroll
@@ -236,20 +235,34 @@ __global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(con
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, col = lane & 31;
   const int h = blockIdx.x % a.H;
-  const int rest = blockIdx.x / a.H;
-  const int split = rest % a.splits, slot = rest / a.splits;
-  int b, tile;
+  // The last tokens see the most, so they begin first.  Where all workgroups begin at
+  // once, the tiles are taken from all requests in turn, and every second workgroup of a
+  // CU counts from the other end.
+  int rest = blockIdx.x / a.H;
+  const auto snake = [&](int n) {
+    if (!a.round) return;
+    const int turn = rest / a.round;
+    if (turn & 1) rest = turn * a.round + min((turn + 1) * a.round, n) - 1 - rest;
+  };
+  int b, tile, split;
   if (a.map.starts) {
     auto count = [&](int i) { return (queries_of(a, i).n * a.G + kRows - 1) / kRows; };
     rk::Line<decltype(count)> line(a.map.B, count, s_wave, s_found);
-    if (slot >= line.total) return;
-    const rk::Found f = line.find(slot);
+    if (rest >= line.total * a.splits) return;
+    snake(line.total * a.splits);
+    split = rest % a.splits;
+    const int slot = rest / a.splits;
+    const bool across = a.round && a.map.B <= 64;
+    const rk::Found f = across ? line.across(slot) : line.find(slot);
     b = f.b;
-    tile = count(b) - 1 - (slot - f.before);
+    tile = count(b) - 1 - (across ? f.before : slot - f.before);
   } else {
     const int tiles = (a.T * a.G + kRows - 1) / kRows;
-    b = slot / tiles;
-    tile = tiles - 1 - (slot - b * tiles);  // the last tokens see the most: they begin first
+    snake(gridDim.x / a.H);
+    split = rest % a.splits;
+    const int slot = rest / a.splits;
+    b = a.round ? slot % a.map.B : slot / tiles;
+    tile = tiles - 1 - (a.round ? slot / a.map.B : slot - b * tiles);
   }
   const Queries qs = queries_of(a, b);
   const int len = rk::len_of(a.map, b);
@@ -666,6 +679,8 @@ int64_t window_slots(const PagedArgs& a) {
   if (a.map.starts) return (a.N * a.G + kRows - 1) / kRows + a.map.B;
   return a.map.B * (((int64_t)a.T * a.G + kRows - 1) / kRows);
 }
+
+int window_per_cu(const PagedArgs& a) { return waves_of((a.D + 15) / 16); }
 
 int window_launch(const PagedArgs& a, int32_t dtype, hipStream_t s) {
   const int64_t grid = window_slots(a) * a.H * a.splits, rows = a.N * a.Hq;

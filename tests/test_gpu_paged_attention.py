@@ -140,6 +140,30 @@ def test_prefill(dtype, lens, new, H, G, D, page, window, sinks):
     prefill_check(pool, q, new, G, window, sinks, got, dt)
 
 
+@pytest.mark.parametrize("new, H, D", [
+    ([300, 0, 130, 5, 260], 40, 16),                    # 360 workgroups: two a CU, tiles of all requests in turn
+    ([300, 0, 130, 5, 260, 0], 64, 16),                 # 576: three
+    ([int(n) for n in (np.arange(70) * 37) % 140], 4, 8),  # more requests than a wave has lanes
+    ([0, 0, 1, 0] * 16, 20, 80),                        # one token each, the others none
+])
+def test_prefill_of_one_round(new, H, D):
+    dt, lens = torch.bfloat16, [n + 9 * (i % 3) for i, n in enumerate(new)]
+    pool = Pool(lens, H, D, 16, dt, seed=H).cuda()
+    q = torch.randn(sum(new), H, D, device="cuda").to(dt)
+    got = paged_prefill(q, starts_of(new), pool.dk, pool.dv, pool.dtable, pool.dlens, 1, 200, 3)
+    prefill_check(pool, q, new, 1, 200, 3, got, dt)
+
+
+@pytest.mark.parametrize("B, H, T, D", [(3, 40, 300, 16), (2, 24, 700, 72)])
+def test_window_of_one_round(B, H, T, D):
+    dt, g = torch.float16, torch.Generator().manual_seed(T)
+    q, k, v = (torch.randn(B, H, T, D, generator=g).to(dt) for _ in range(3))
+    got = window_attention(q.cuda(), k.cuda(), v.cuda(), 1)
+    for b in range(B):
+        want, amp, big = op.attend(f64(q[b]).swapaxes(0, 1), f64(k[b]), f64(v[b]), np.ones(T, bool), 0, 1, None, 0)
+        check(got[b].transpose(0, 1), want, attention_bound(want, amp, big, T, dt, False))
+
+
 @pytest.mark.parametrize("splits", [False, True])
 def test_rows_of_no_request_stay(splits):
     dt, lens = torch.float16, [600, 90]
