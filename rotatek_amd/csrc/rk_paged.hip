@@ -621,10 +621,12 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
     // Cut the tokens where the rows alone leave CUs empty.  A part saves its share
     // of the tiles, about a microsecond each, and costs its records, written and
     // read: the two are equal at the square root (3 x 77 queries on 1077 tokens, 8
-    // heads of 80: 18.9 us in 4 parts, 16.7 in 6, 17.7 in 9, 20.5 in 17).
+    // heads of 80: 18.9 us in 4 parts, 16.7 in 6, 17.7 in 9, 20.5 in 17; 512 on 8000,
+    // 32/8 heads of 128: 30.3 us whole with a window of 1024, 33.3 in 3).
     const int64_t grid = rk::window_slots(*a) * H;
-    const double tiles = cap / 64.0, record = (double)p->rows * cdiv(D, 32) * 128 * 2 / 3.1e6;
-    const int64_t most = std::min(2 * (int64_t)cus / std::max<int64_t>(grid, 1), cdiv(cap, 128));
+    const int64_t seen = std::min(cap, std::min<int64_t>(a->window, cap) + std::min<int64_t>(a->sinks, cap) + 128 / c.groups);
+    const double tiles = seen / 64.0, record = (double)p->rows * cdiv(D, 32) * 128 * 2 / 3.1e6;
+    const int64_t most = std::min(2 * (int64_t)cus / std::max<int64_t>(grid, 1), cdiv(seen, 128));
     a->splits = (int32_t)std::max<int64_t>(std::min<int64_t>(most, (int64_t)sqrt(tiles / record)), 1);
     if (grid * a->splits >= rk::kMostGroups) return RK_ERR_SHAPE;
     // One round, of more than a workgroup a CU: long and short ones on each (causal, 3 x
