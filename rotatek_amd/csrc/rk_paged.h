@@ -56,7 +56,7 @@ struct PagedArgs {
   int32_t Hq, H, G, D, T;  // T: new tokens of each request (0: starts)
   int32_t window, sinks;   // window INT_MAX: none
   int32_t workers;         // one new token each: workgroups of the split launch
-  int32_t direct;          // ... a unit each, no shares and no join
+  int32_t direct;          // ... waves of one that takes a unit by itself (0: shares and a join)
   int32_t splits;          // many: parts that a row's tokens are cut into
   int32_t round;           // ... workgroups of a KV head that CUs take one each of, where all begin at once (0: not)
   int32_t q_vec, o_vec;

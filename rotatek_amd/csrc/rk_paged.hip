@@ -45,13 +45,10 @@ using rk::PagedArgs;
 constexpr int kStep = 32;                     // tokens of a wave's step
 constexpr int kBlock = kStep * kPagedWaves;  // tokens of a piece of work
 constexpr int kRows = 16;                     // queries of a unit
-// Pieces of a unit up to which a workgroup takes all of it, for units that fill the
-// CUs and for fewer: one launch instead of two, no records, but the longest unit
-// ends last (bf16, 4 query heads to each of 8 KV heads of 128; shared and not: 32
-// requests of 500 tokens 19.9 and 18.2 us, 64 of 1000 49.4 and 46.7, 64 of up to
-// 2000 74.6 and 69.1; 1 of 1000 13.3 and 18.1, 8 of 1000 with 4 KV heads 14.7 and
-// 26.1, 1 of 500 11.4 and 12.0).
-constexpr int kDirectMany = 16, kDirectFew = 2;
+// Pieces of a unit up to which a workgroup may take all of it: one launch instead of
+// two and no records, but the longest unit ends last.
+constexpr int kMostAlone = 16;
+constexpr int kAloneWaves = 8;  // of such a workgroup, where each CU has one at most
 // Waves that join a query of many records (one wave reads four at a time): one text
 // of 32000 tokens, 8 query heads to its KV head: 31.3 us in all with 4, 17.8 with 16.
 constexpr int kJoinWaves = 16;
@@ -106,16 +103,18 @@ struct Pages {
 // Workgroups of a CU: what their registers allow.
 constexpr int per_cu(int KF) { return KF == 4 ? 2 : 3; }
 
-// KF: blocks of 32 channels (2 or 4).  EIGHT: pages of eight rows.
-template <class DT, int KF, bool EIGHT>
-__global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(const PagedArgs a) {
+// KF: blocks of 32 channels (2 or 4).  EIGHT: pages of eight rows.  W: waves; more
+// than kPagedWaves of them for a unit each alone.
+template <class DT, int KF, bool EIGHT, int W>
+__global__ __launch_bounds__(64 * W, W == kPagedWaves ? per_cu(KF) : 2) void paged_split_kernel(const PagedArgs a) {
+  constexpr bool kAlone = W != kPagedWaves;
   constexpr int KD = 32 * KF;      // channels, stored ones up to D
   constexpr int VC = KD / 16;      // channels of a Value piece: 4 or 8
   constexpr int AccPitch = KD + 4;
   typedef unsigned int piece __attribute__((ext_vector_type(KF)));
   __shared__ int s_wave[kPagedWaves], s_found[2];
-  __shared__ float s_acc[kPagedWaves][kRows][AccPitch];
-  __shared__ float s_ml[kPagedWaves][kRows][2];
+  __shared__ float s_acc[W][kRows][AccPitch];
+  __shared__ float s_ml[W][kRows][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int blocks = (a.G + kRows - 1) / kRows;
@@ -125,14 +124,14 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
   Shares sh;
   int64_t at, end, first = 0;  // pieces; the first one of request b
   int b;
-  if (a.direct) {  // a unit each
+  if (kAlone || a.direct) {  // a unit each
     b = w / units;
     const int unit = w - b * units, pieces = pieces_of(a, b);
     at = (int64_t)unit * pieces;
     end = at + pieces;
     if (pieces == 0) {
       const int h = unit / blocks, row0 = (unit - h * blocks) * kRows;
-      for (int r = wave; r < min(a.G - row0, kRows); r += kPagedWaves)
+      for (int r = wave; r < min(a.G - row0, kRows); r += W)
         for (int c = lane; c < a.D; c += 64)
           ((uint16_t*)a.out)[b * a.o_sb + (int64_t)(h * a.G + row0 + r) * a.o_sh + c * a.o_sd] = 0;
     }
@@ -270,15 +269,15 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
           offsets(p + 1 - seen.token(i));
         }
       };
-      Pages now = pages_at(i0), next = pages_at(i0 + kPagedWaves);
+      Pages now = pages_at(i0), next = pages_at(i0 + W);
       cut(i0);
       load_k(i0, now);
       load_v(i0, now);
-      for (int i = i0; i < last; i += kPagedWaves) {
-        const int then = i + kPagedWaves, t0 = seen.token(i);
+      for (int i = i0; i < last; i += W) {
+        const int then = i + W, t0 = seen.token(i);
         // A CU's older workgroup goes first wherever both could, and ends early; by
         // turns they end together (32 requests of 16000 tokens: 344 us, 338 so).
-        if (((i / kPagedWaves) ^ (2 * blockIdx.x >= gridDim.x ? 1 : 0)) & 1)
+        if (((i / W) ^ (2 * blockIdx.x >= gridDim.x ? 1 : 0)) & 1)
           __builtin_amdgcn_s_setprio(2);
         else
           __builtin_amdgcn_s_setprio(0);
@@ -359,7 +358,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
         }
         if (then < last) load_v(then, next);
         now = next;
-        next = pages_at(then + kPagedWaves);
+        next = pages_at(then + W);
       }
     }
     l += rk::shfl_xor(l, 16);
@@ -378,18 +377,18 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
     if (r < rows) {
       float top = kNone;
 #pragma unroll
-      for (int v = 0; v < kPagedWaves; ++v) top = fmaxf(top, s_ml[v][r][0]);
+      for (int v = 0; v < W; ++v) top = fmaxf(top, s_ml[v][r][0]);
       float sum = 0.f, o[VC];
 #pragma unroll
       for (int e = 0; e < VC; ++e) o[e] = 0.f;
 #pragma unroll
-      for (int v = 0; v < kPagedWaves; ++v) {
+      for (int v = 0; v < W; ++v) {
         const float f = rk::fast_exp2(s_ml[v][r][0] - base_of(top));
         sum += f * s_ml[v][r][1];
 #pragma unroll
         for (int e = 0; e < VC; ++e) o[e] += f * s_acc[v][r][c0 + e];
       }
-      if (take == pieces) {
+      if (kAlone || take == pieces) {
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
         uint16_t* dst = (uint16_t*)a.out + b * a.o_sb + (int64_t)(h * a.G + row0 + r) * a.o_sh;
 #pragma unroll
@@ -404,7 +403,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(KF)) void paged_split_kernel(
       }
     }
     // the shares that the unit lies in, for the launch that joins them
-    if (!a.direct && off == 0 && threadIdx.x == 0) {
+    if (!kAlone && !a.direct && off == 0 && threadIdx.x == 0) {
       const int64_t begin = at - take;
       a.span[b * units + unit] = make_int2(w, sh.of(begin + pieces - 1));
     }
@@ -606,7 +605,16 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
     const int64_t units = p->B * H * cdiv(c.groups, kRows), longest = pieces_of_longest(a->map.cap, a->window, a->sinks);
     if (units * (cdiv(cap, kBlock) + 1) >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
     if (units >= rk::kMostGroups || cdiv(p->rows, kPagedWaves) >= rk::kMostGroups) return RK_ERR_SHAPE;
-    a->direct = longest <= (units >= cus ? kDirectMany : kDirectFew);
+    // A unit to a workgroup, or all of them shared out evenly with a join: the first
+    // saves about 4 us and takes its pieces on the fullest CU, 2.1 us each, the second
+    // all CUs' average of them, 2.6 us each (128 channels; 1.3 and 1.6 with 64), less
+    // where requests differ.  32 queries on 8 KV heads of 128, shared and alone: 1
+    // request of 380 tokens 10.6 and 9.7 us, of 760 12.4 and 16.8; 16 of 760 19.8 and
+    // 18.5, of 1000 20.6 and 22.7; 28 of 1500 40.5 and 34.0; 40 of 500 27.5 and 23.5, of
+    // 1500 51.2 and 56.2; 64 of up to 2000 74.6 and 69.1.
+    const int64_t fullest = cdiv(units, cus);
+    const bool alone = longest <= kMostAlone && longest * (40 * (fullest * cus - units) + 3 * cus) <= 140 * cus;
+    a->direct = !alone ? 0 : fullest > 1 ? kPagedWaves : kAloneWaves;
     a->workers = (int32_t)(a->direct ? units : std::max<int64_t>(
         std::min<int64_t>(per_cu(D <= 64 ? 2 : 4) * (int64_t)cus, units * longest), 1));
     if (!a->direct) {
@@ -685,12 +693,19 @@ int run(const Call& c, void* workspace, size_t workspace_bytes, void* stream) {
   const hipStream_t s = (hipStream_t)stream;
   if (!p.single) return rk::window_launch(a, c.q->dtype, s);
   return by_shape(c.q->dtype, a.D, [&](auto dt, auto kf) {
-    if (a.map.shift == 3)
-      hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value, true>), dim3((unsigned)a.workers),
-                         dim3(kPagedThreads), 0, s, a);
+    const auto split = [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      if (a.map.shift == 3)
+        hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value, true, W>), dim3((unsigned)a.workers),
+                           dim3(64 * W), 0, s, a);
+      else
+        hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value, false, W>), dim3((unsigned)a.workers),
+                           dim3(64 * W), 0, s, a);
+    };
+    if (a.direct == kAloneWaves)
+      split(std::integral_constant<int, kAloneWaves>{});
     else
-      hipLaunchKernelGGL((paged_split_kernel<decltype(dt), decltype(kf)::value, false>), dim3((unsigned)a.workers),
-                         dim3(kPagedThreads), 0, s, a);
+      split(std::integral_constant<int, kPagedWaves>{});
     if (a.direct) return;
     if (p.join == 1)
       hipLaunchKernelGGL((paged_join_kernel<decltype(dt), decltype(kf)::value, 1>),
