@@ -38,6 +38,8 @@ class PagedCache(Cache):
             raise ValueError(f"page must be a power of two from 8 on, got {page}")
         if min(layers, heads_kv, head_dim, pages, requests) < 1:
             raise ValueError("layers, heads_kv, head_dim, pages and requests must be at least 1")
+        if dtype not in (torch.float16, torch.bfloat16) or head_dim % 8 or head_dim > 128:
+            raise ValueError(f"pages hold fp16 or bf16, head_dim a multiple of 8 up to 128; got {dtype}, {head_dim}")
         most = pages * page if max_tokens is None else max_tokens
         if most < 1:
             raise ValueError("max_tokens must be at least 1")

@@ -388,7 +388,8 @@ def test_cache_counts_and_pages():
         c.attend(0, torch.zeros(3, 4, 16), 2)
 
 
-@pytest.mark.parametrize("args", [dict(page=12), dict(page=4), dict(pages=0), dict(requests=0), dict(max_tokens=0)])
+@pytest.mark.parametrize("args", [dict(page=12), dict(page=4), dict(pages=0), dict(requests=0), dict(max_tokens=0),
+                                  dict(dtype=torch.float32), dict(head_dim=20), dict(head_dim=136)])
 def test_cache_refuses(args):
     with pytest.raises(ValueError):
         PagedCache(**{**dict(layers=1, heads_kv=1, head_dim=16, pages=2, device="cpu"), **args})
