@@ -13,6 +13,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/Dtype.h>
@@ -352,9 +353,17 @@ bool needs_grad(T... o) {
   return false;
 }
 
+// A new tensor, from the allocator of a given one: what at::empty does behind its two
+// dispatches (a rotation of one token's queries and Keys 7.1 us with them, 5.9 so).
+at::Tensor fresh(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+  c10::Allocator* const from = like.storage().allocator();
+  if (!from || !like.is_cuda()) return at::empty(sizes, on(like, type));
+  return at::detail::empty_generic(sizes, from, c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
+
 // A new tensor like t, and its descriptor.
 int make_like(const at::Tensor& t, int64_t device, at::Tensor* out, Arg* d) {
-  *out = at::empty(t.sizes(), on(t, t.scalar_type()));
+  *out = fresh(t, t.sizes(), t.scalar_type());
   d->p = &d->d;
   return describe(*out, device, &d->d, kWrite);
 }
@@ -482,21 +491,34 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// Output, workspace and launch of an attention call: `out` or a status.
+// Output, workspace and launch of an attention call: `out` or a status.  A new output
+// for q [B, H, D] of single tokens is [B, 1, H, D].
 template <class Check, class Launch>
-PyObject* attend(PyObject* out_arg, const at::Tensor& q, int64_t dev, Check check, Launch launch) {
+PyObject* attend(PyObject* out_arg, const at::Tensor& q, bool single, int64_t dev, Check check, Launch launch) {
   Arg out;
   at::Tensor made;
   int st = out.set(out_arg, dev, kWrite);
-  if (!st && !out.p) st = make_like(q, dev, &made, &out);
+  if (!st && !out.p && single && q.dim() == 3) {
+    made = fresh(q, {q.size(0), 1, q.size(1), q.size(2)}, q.scalar_type());
+    st = describe(made, dev, &out.d, kWrite);
+    for (int i = 1; i < 3; ++i) {
+      out.d.shape[i] = out.d.shape[i + 1];
+      out.d.stride[i] = out.d.stride[i + 1];
+    }
+    out.d.ndim = 3;
+    out.p = &out.d;
+  } else if (!st && !out.p) {
+    st = make_like(q, dev, &made, &out);
+  }
   if (st) return status(st);
   size_t bytes = 0;
   if ((st = check(out.p, &bytes))) return status(st);
   // the call's own: torch's allocator hands it on in the stream's order
-  const at::Tensor ws = at::empty({(int64_t)(bytes > 0 ? bytes : 256)}, on(q, at::kByte));
+  const at::Tensor ws = bytes > 0 ? fresh(q, {(int64_t)bytes}, at::kByte) : at::Tensor();
+  void* const scratch = bytes > 0 ? ws.data_ptr() : nullptr;
   {
     const Unlocked unlocked;
-    st = launch(out.p, ws.data_ptr(), (size_t)ws.numel());
+    st = launch(out.p, scratch, bytes);
   }
   if (st) return status(st);
   return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(out_arg);
@@ -522,7 +544,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = stream_of(a[10]);
   if (st || PyErr_Occurred()) return status(st);
   return attend(
-      a[9], t, dev,
+      a[9], t, starts == nullptr, dev,
       [&](const rk_tensor* out, size_t* bytes) {
         return g_entry.paged_check(q.p, starts, &pages.d, groups, window, sinks, out, 0, bytes);
       },
@@ -551,7 +573,7 @@ PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = stream_of(a[8]);
   if (st || PyErr_Occurred()) return status(st);
   return attend(
-      a[7], t, dev,
+      a[7], t, false, dev,
       [&](const rk_tensor* out, size_t* bytes) {
         return g_entry.window_check(q.p, k.p, v.p, lens, groups, window, sinks, out, 0, bytes);
       },

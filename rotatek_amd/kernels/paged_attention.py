@@ -52,8 +52,8 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     [B, 1, H_q, D] (``out``: [B, H_q, D] to write to)."""
     if q.dim() != 3:
         raise ValueError(f"q needs 3 dims [B, H_q, D], got shape {tuple(q.shape)}")
-    return _paged("paged_decode", q, None, k_pages, v_pages, table, lens, num_kv_groups, window, sinks,
-                  out).unsqueeze(1)
+    r = _paged("paged_decode", q, None, k_pages, v_pages, table, lens, num_kv_groups, window, sinks, out)
+    return r if out is None else r.unsqueeze(1)
 
 
 def paged_prefill(q: torch.Tensor, starts: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
