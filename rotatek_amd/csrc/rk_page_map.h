@@ -49,8 +49,18 @@ RK_EVERYWHERE int request_of(const int32_t* starts, int B, int64_t n) {
   return low;
 }
 
-// Page and row that new token n goes to, b: request_of it (where there are
-// starts); a negative page where it goes nowhere.
+// Page and row that new token n of request b's s .. e - 1 goes to, which holds `len`
+// with them; a negative page where it goes nowhere.
+RK_EVERYWHERE int64_t place_in(const PageMap& m, int64_t n, int64_t b, int64_t s, int64_t e, int64_t len, int* row) {
+  const int64_t p = len - e + n;
+  if (n < s || n >= e || p < 0 || p >= m.cap) return -1;
+  const uint32_t page = page_of(m, (int)b, (int)p);
+  if (page >= (uint32_t)m.pages) return -1;
+  *row = (int)p & ((1 << m.shift) - 1);
+  return page;
+}
+
+// The same, b: request_of n (where there are starts).
 RK_EVERYWHERE int64_t place_of(const PageMap& m, int64_t n, int64_t b, int* row) {
   if (m.B <= 0) return -1;
   int64_t s, e;  // the request's new tokens
@@ -62,12 +72,7 @@ RK_EVERYWHERE int64_t place_of(const PageMap& m, int64_t n, int64_t b, int* row)
     s = b * m.each;
     e = s + m.each;
   }
-  const int64_t len = m.lens[b], p = len - e + n;
-  if (n < s || n >= e || p < 0 || p >= m.cap) return -1;
-  const uint32_t page = page_of(m, (int)b, (int)p);
-  if (page >= (uint32_t)m.pages) return -1;
-  *row = (int)p & ((1 << m.shift) - 1);
-  return page;
+  return place_in(m, n, b, s, e, m.lens[b], row);
 }
 
 // The tokens that queries at positions lo_p .. hi_p (lo_p from 0 on) see, as
