@@ -380,7 +380,8 @@ int launch(RotaryArgs& a, int dtype, int e, void* stream) {
   a.head[kV] = divisor_of(half, heads[kV] * half);
   // Stores of whole lines leave the caches to others: 3 x 32 heads x 2304 tokens of
   // 80 channels in fp32 (142 MB in all) take 27 us (a copy of as much 26), 39 with
-  // ordinary stores; 17 prompts of up to 4097 tokens into pages 177 and 183.  Lines
+  // ordinary stores; 17 prompts of up to 4097 tokens into pages 177 and
+  // 183 (with places found behind the angles).  Lines
   // that two stores share have to meet in a cache: 23205 tokens of 96 heads of 96
   // channels in fp16 take 227 us with 48 pairs, 253 past the caches.
   const int size = rk::dtype_size(dtype), run = (a.pos ? a.P : a.D) * size;

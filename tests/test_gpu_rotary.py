@@ -209,3 +209,17 @@ def test_rounding_is_to_nearest():
         x = torch.randn(3, 2, 64, device="cuda").to(dt)
         y, _ = apply_rotary(x, None, torch.zeros(3, dtype=torch.int64, device="cuda"), inverse_frequencies(64))
         assert torch.equal(x, y) and half(dt) > 0
+
+
+def test_tensors_that_others_allocated():
+    """Inference mode, and tensors whose memory is not from torch's allocator."""
+    dt = torch.bfloat16
+    q, k = torch.randn(5, 4, 64, device="cuda").to(dt), torch.randn(5, 2, 64, device="cuda").to(dt)
+    pos, freq = torch.arange(5, device="cuda"), inverse_frequencies(64)
+    want = apply_rotary(q, k, pos, freq)
+    for x, y in ((torch.from_dlpack(q), torch.from_dlpack(k)), (q.view(torch.int16).view(dt), k[:, :, :])):
+        assert all(torch.equal(a, b) for a, b in zip(apply_rotary(x, y, pos, freq), want))
+    with torch.inference_mode():
+        got = apply_rotary(q.clone(), k.clone(), pos, freq)
+        assert all(a.is_inference() for a in got)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
