@@ -107,8 +107,9 @@ __device__ __forceinline__ Queries queries_of(const PagedArgs& a, int b) {
 
 // Whether rows of a wave (positions lo_p .. hi_p) may be not finite for what they do
 // not see in its tiles: a token without a page, one that some row does not see with a
-// Value that is not finite, or a Key that is not among the first eight channels, which
-// are read again past D where D is no multiple of 16.
+// Value that is not finite, or a Key that is not finite among the first eight channels,
+// which are read again past D where D is no multiple of 16.  The tiles' last token
+// stands behind itself too, in the rest of its tile, where nobody sees it.
 template <class DT>
 __device__ __forceinline__ bool odd_unseen(const PagedArgs& a, int b, rk::Seen<kTile> seen, int i0, int i1, int h, int lo_p,
                                      int hi_p, int last) {
@@ -128,7 +129,9 @@ __device__ __forceinline__ bool odd_unseen(const PagedArgs& a, int b, rk::Seen<k
       const int64_t at = j & ((1u << a.map.shift) - 1);
       odd = page >= (uint32_t)a.map.pages;
       if (!odd && a.D % 16) odd = odd_piece((const uint16_t*)a.k + h * a.k_sh + (int64_t)page * a.k_sp + at * a.k_ss);
-      if (!odd && !(j <= lo_p && (hi_p - j < a.window || j < a.sinks))) {
+      const bool seen_by_all = j <= lo_p && (hi_p - j < a.window || j < a.sinks);
+      const bool repeated = j == last && (last + 1) % kTile != 0;
+      if (!odd && (!seen_by_all || repeated)) {
         const uint16_t* v = (const uint16_t*)a.v + h * a.v_sh + (int64_t)page * a.v_sp + at * a.v_ss;
         for (int c = 0; c < a.D; c += 8) odd |= odd_piece(v + c);
       }

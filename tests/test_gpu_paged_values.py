@@ -1,0 +1,58 @@
+"""Values that are not finite, at tokens that are seen: the formula's answer in
+every kernel (oracle.paged.attend: an infinity times its weight)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as op
+from rotatek_amd.kernels import paged_decode, paged_prefill, window_attention
+from tests.paged import DTYPES, Pool, attention_bound, f64
+
+pytestmark = pytest.mark.gpu
+HALF = ["bf16", "fp16"]
+INF, NAN = float("inf"), float("nan")
+
+
+def check_odd(got, want, amp, big, S, dt, single):
+    """Where the formula is not finite, the same infinity or a NaN; elsewhere within its bound."""
+    got, odd = f64(got), ~np.isfinite(want)
+    np.testing.assert_array_equal(got[odd], want[odd])
+    bound = attention_bound(np.where(odd, 0.0, want), np.where(odd, 0.0, amp), big, S, dt, single)
+    off = np.abs(np.where(odd, 0.0, got) - np.where(odd, 0.0, want))
+    assert (off <= bound)[~odd].all(), np.argwhere(~(off <= bound) & ~odd)[:4].tolist()
+
+
+def starts_of(new):
+    return torch.tensor([0] + list(np.cumsum(new)), dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+@pytest.mark.parametrize("T, S, G, D", [(33, 100, 1, 64), (33, 33, 1, 80), (2, 1000, 1, 128), (9, 77, 32, 40), (65, 128, 1, 16)])
+def test_window_with_an_odd_last_token(dtype, bad, T, S, G, D):
+    """Rows of a wave that all stand at the last token, and others."""
+    dt, g = DTYPES[dtype], torch.Generator().manual_seed(T + S)
+    q, k, v = (torch.randn(1, h, n, D, generator=g).to(dt) for h, n in ((2 * G, T), (2, S), (2, S)))
+    v[0, 1, S - 1, 5] = bad
+    got = window_attention(q.cuda(), k.cuda(), v.cuda(), G)
+    want, amp, big = op.attend(f64(q[0]).swapaxes(0, 1), f64(k[0]), f64(v[0]), np.ones(S, bool), S - T, G)
+    check_odd(got[0].transpose(0, 1), want, amp, big, S, dt, False)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+@pytest.mark.parametrize("window, sinks", [(None, 0), (20, 2)])
+def test_prefill_with_an_odd_last_token(dtype, bad, window, sinks):
+    """A request of one new token among others: all its rows see the last one."""
+    dt, lens, new, G = DTYPES[dtype], [50, 1, 90, 700], [1, 1, 40, 1], 3
+    pool = Pool(lens, 2, 64, 16, dt, seed=3)
+    for b, n in enumerate(lens):
+        pool.v[int(pool.table[b, (n - 1) // 16]), 0, (n - 1) % 16, 9] = bad
+    pool.cuda()
+    q = torch.randn(sum(new), 2 * G, 64, device="cuda").to(dt)
+    got = paged_prefill(q, starts_of(new), pool.dk, pool.dv, pool.dtable, pool.dlens, G, window, sinks)
+    at = 0
+    for b, n in enumerate(new):
+        want, amp, big = pool.want(b, q[at:at + n].cpu(), G, window, sinks)
+        check_odd(got[at:at + n], want, amp, big, 700, dt, False)
+        at += n
