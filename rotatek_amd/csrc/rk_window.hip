@@ -105,20 +105,22 @@ __device__ __forceinline__ Queries queries_of(const PagedArgs& a, int b) {
   return {s, (int)max(e - s, (int64_t)0)};
 }
 
-// Whether rows of a wave (positions lo_p .. hi_p) may be not finite for what they do
-// not see in its tiles: a token without a page, one that some row does not see with a
-// Value that is not finite, or a Key that is not finite among the first eight channels,
-// which are read again past D where D is no multiple of 16.  The tiles' last token
-// stands behind itself too, in the rest of its tile, where nobody sees it.
+// Whether rows of a wave (positions lo_p .. hi_p) may be NaN for what the products of
+// its tiles added to what the formula says, a weight of zero times something that is not
+// finite: a token without a page; one that some row does not see, with such a Value; an
+// infinite Value whose weight is zero in 16 bits alone; a Key that is not finite among
+// the first eight channels, which are read again past D where D is no multiple of 16.
+// The tiles' last token stands behind itself too, in the rest of its tile, where nobody
+// sees it.
 template <class DT>
-__device__ __forceinline__ bool odd_unseen(const PagedArgs& a, int b, rk::Seen<kTile> seen, int i0, int i1, int h, int lo_p,
-                                     int hi_p, int last) {
+__device__ __forceinline__ bool nan_by_zero(const PagedArgs& a, int b, rk::Seen<kTile> seen, int i0, int i1, int h, int lo_p,
+                                      int hi_p, int last) {
   constexpr uint32_t kExponent = std::is_same<DT, rk::F16>::value ? 0x7c00 : 0x7f80;
-  auto odd_piece = [](const uint16_t* x) {
+  auto odd_piece = [](const uint16_t* x, bool infinite) {  // of eight: not finite, or infinite
     const uint4 y = *(const uint4*)x;
+    const uint32_t bits = infinite ? 0x7fff : kExponent;
     bool odd = false;
-    for (const uint32_t w : {y.x, y.y, y.z, y.w})
-      odd |= (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
+    for (const uint32_t w : {y.x, y.y, y.z, y.w}) odd |= (w & bits) == kExponent || (w >> 16 & bits) == kExponent;
     return odd;
   };
   for (int i = i0; i < i1; ++i) {
@@ -128,12 +130,12 @@ __device__ __forceinline__ bool odd_unseen(const PagedArgs& a, int b, rk::Seen<k
       const uint32_t page = rk::page_of(a.map, b, j);
       const int64_t at = j & ((1u << a.map.shift) - 1);
       odd = page >= (uint32_t)a.map.pages;
-      if (!odd && a.D % 16) odd = odd_piece((const uint16_t*)a.k + h * a.k_sh + (int64_t)page * a.k_sp + at * a.k_ss);
+      if (!odd && a.D % 16) odd = odd_piece((const uint16_t*)a.k + h * a.k_sh + (int64_t)page * a.k_sp + at * a.k_ss, false);
       const bool seen_by_all = j <= lo_p && (hi_p - j < a.window || j < a.sinks);
       const bool repeated = j == last && (last + 1) % kTile != 0;
-      if (!odd && (!seen_by_all || repeated)) {
+      if (!odd) {
         const uint16_t* v = (const uint16_t*)a.v + h * a.v_sh + (int64_t)page * a.v_sp + at * a.v_ss;
-        for (int c = 0; c < a.D; c += 8) odd |= odd_piece(v + c);
+        for (int c = 0; c < a.D; c += 8) odd |= odd_piece(v + c, seen_by_all && !repeated);
       }
     }
     if (__any(odd)) return true;
@@ -581,17 +583,17 @@ __global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(con
   }
   const float2 sums = both_halves(l);
   l = sums.x + sums.y;
-  // Weight 0 times an infinity or a NaN is a NaN: a tile's Values reach rows
-  // that do not see them.  Where there are such, rows that are not finite are summed
-  // again from what they see.
-  float probe = l * 0.f;
+  // Weight 0 times an infinity or a NaN is a NaN: a tile's Values reach rows that do
+  // not see them, or by a weight that is too small for 16 bits.  Where there are such,
+  // rows that are NaN are summed again from what they see.
+  bool nan = l != l;
 #pragma unroll
   for (int c = 0; c < NB; ++c)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) probe += o[c][e] * 0.f;
-  const uint64_t odd = __ballot(mine && probe != 0.f);
+    for (int e = 0; e < 16; ++e) nan |= o[c][e] != o[c][e];
+  const uint64_t odd = __ballot(mine && nan);
   uint32_t again = (uint32_t)odd | (uint32_t)(odd >> 32);
-  if (again && !odd_unseen<DT>(a, b, seen, i0, i1, h, p0 + (row0 + wave * kWaveRows) / a.G, w_hi, hi_p)) again = 0;
+  if (again && !nan_by_zero<DT>(a, b, seen, i0, i1, h, p0 + (row0 + wave * kWaveRows) / a.G, w_hi, hi_p)) again = 0;
   const bool done = again >> col & 1;
   while (again) {
     const int rr = __builtin_ctz(again);

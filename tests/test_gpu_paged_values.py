@@ -56,3 +56,17 @@ def test_prefill_with_an_odd_last_token(dtype, bad, window, sinks):
         want, amp, big = pool.want(b, q[at:at + n].cpu(), G, window, sinks)
         check_odd(got[at:at + n], want, amp, big, 700, dt, False)
         at += n
+
+
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+@pytest.mark.parametrize("T, S, at", [(40, 300, 100), (40, 300, 259), (4, 900, 3)])
+def test_window_with_an_odd_token_of_little_weight(bad, T, S, at):
+    """A weight of 2^-50 is none in fp16; times an infinity it is one all the same."""
+    dt, g = torch.float16, torch.Generator().manual_seed(S)
+    q, k, v = (torch.randn(1, h, n, 64, generator=g).to(dt) for h, n in ((2, T), (1, S), (1, S)))
+    q[..., 0], k[..., 0] = 16.0, 0.0
+    k[0, 0, at, 0] = -20.0      # 16 * 20 / 8 log2(e) = 57.7 below the others
+    v[0, 0, at, 5] = bad
+    got = window_attention(q.cuda(), k.cuda(), v.cuda(), 2)
+    want, amp, big = op.attend(f64(q[0]).swapaxes(0, 1), f64(k[0]), f64(v[0]), np.ones(S, bool), S - T, 2)
+    check_odd(got[0].transpose(0, 1), want, amp, big, S, dt, False)
