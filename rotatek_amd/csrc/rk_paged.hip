@@ -54,6 +54,8 @@ constexpr int kAloneWaves = 8;  // of such a workgroup, where each CU has one at
 // 8 records a row: 12.9 with one wave, 11.3 with 16, 4 records as long.
 constexpr int kJoinWaves = 16;
 
+constexpr float kAlike = 0x1p-14f;  // weight of tokens whose Values only have to show what is not finite
+
 // Pieces of one request and KV head.
 __device__ __forceinline__ int pieces_of(const PagedArgs& a, int b) {
   const int p = a.map.pages > 0 ? rk::len_of(a.map, b) - 1 : -1;
@@ -260,6 +262,41 @@ __global__ __launch_bounds__(64 * W, W == kPagedWaves ? per_cu(KF) : 2) void pag
           for (int d = 0; d < KF; ++d) v[4 * s + e][d] = y[d];
         }
     };
+    // Scores of the step whose Keys are there.
+    auto score = [&](f32x4 (&sc)[2]) {
+#pragma unroll
+      for (int c = 0; c < KF; ++c)
+        if (32 * c + 32 > a.D) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            if (32 * c + 8 * g >= a.D) k[s][c] = rk::u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KF; ++c)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) sc[s] = DT::mfma(__builtin_bit_cast(uint4, k[s][c]), q[c], sc[s]);
+    };
+    // Nothing of the tokens that are not there: scores -inf, Values zero.
+    auto only = [&](uint32_t there, f32x4 (&sc)[2]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool on = there >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1;
+        sc[e >> 2][e & 3] = on ? sc[e >> 2][e & 3] : kNone;
+#pragma unroll
+        for (int d = 0; d < KF; ++d) v[e][d] = on ? v[e][d] : 0;
+      }
+    };
+    // Channels VC n + j of the step's Values, eight tokens.
+    auto turned = [&](int j) {
+      uint32_t t[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        t[e] = j & 1 ? rk::pack_hi(v[2 * e][j >> 1], v[2 * e + 1][j >> 1])
+                     : rk::pack_lo(v[2 * e][j >> 1], v[2 * e + 1][j >> 1]);
+      return make_uint4(t[0], t[1], t[2], t[3]);
+    };
     // As soon as a step's Keys (Values) have been used, their registers take the
     // next step's; the page numbers of the one behind it are on their way too.
     const int i0 = kPagedWaves * off + wave;
@@ -289,33 +326,15 @@ __global__ __launch_bounds__(64 * W, W == kPagedWaves ? per_cu(KF) : 2) void pag
           asm volatile("");  // a branch: most steps are whole
           there = there_of(i, now);
         }
-#pragma unroll
-        for (int c = 0; c < KF; ++c)
-          if (32 * c + 32 > a.D) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-              if (32 * c + 8 * g >= a.D) k[s][c] = rk::u32x4{0, 0, 0, 0};
-          }
         f32x4 sc[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KF; ++c)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) sc[s] = DT::mfma(__builtin_bit_cast(uint4, k[s][c]), q[c], sc[s]);
+        score(sc);
         if (then < last) {
           cut(then);
           load_k(then, next);
         }
         if (part) {
           asm volatile("");
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const bool on = there >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1;
-            sc[e >> 2][e & 3] = on ? sc[e >> 2][e & 3] : kNone;
-#pragma unroll
-            for (int d = 0; d < KF; ++d) v[e][d] = on ? v[e][d] : 0;
-          }
+          only(there, sc);
         }
         float top = kNone;
 #pragma unroll
@@ -348,12 +367,7 @@ __global__ __launch_bounds__(64 * W, W == kPagedWaves ? per_cu(KF) : 2) void pag
         DT::split8(x, hi, lo);
 #pragma unroll
         for (int j = 0; j < VC; ++j) {
-          uint32_t t[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            t[e] = j & 1 ? rk::pack_hi(v[2 * e][j >> 1], v[2 * e + 1][j >> 1])
-                         : rk::pack_lo(v[2 * e][j >> 1], v[2 * e + 1][j >> 1]);
-          const uint4 vt = make_uint4(t[0], t[1], t[2], t[3]);
+          const uint4 vt = turned(j);
           acc[j] = DT::mfma(vt, hi, acc[j]);
           acc[j] = DT::mfma(vt, lo, acc[j]);
         }
@@ -364,6 +378,43 @@ __global__ __launch_bounds__(64 * W, W == kPagedWaves ? per_cu(KF) : 2) void pag
     }
     l += rk::shfl_xor(l, 16);
     l += rk::shfl_xor(l, 32);
+    // A weight is above zero, and an infinity or a NaN times it is one.  Its two terms are
+    // not both: the second is often zero or below, and both are zero where 16 bits hold no
+    // less.  So channels that are not finite are summed again with all weights alike, and
+    // become what that gives (rows whose sum of weights is NaN are all NaN anyhow).
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < VC; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) odd |= !(fabsf(acc[j][i]) < __builtin_inff());
+    if (__any(odd)) {
+      f32x4 kind[VC];
+#pragma unroll
+      for (int j = 0; j < VC; ++j) kind[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      offsets(kStep);
+      for (int i = i0; i < last; i += W) {
+        const Pages now = pages_at(i);
+        if (seen.token(i) + kStep - 1 > p) offsets(p + 1 - seen.token(i));
+        load_k(i, now);
+        load_v(i, now);
+        const uint32_t there = there_of(i, now);
+        f32x4 sc[2];
+        score(sc);
+        only(there, sc);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = sc[e >> 2][e & 3] == kNone ? 0.f : kAlike;
+        uint4 hi, lo;
+        DT::split8(x, hi, lo);
+#pragma unroll
+        for (int j = 0; j < VC; ++j) kind[j] = DT::mfma(turned(j), hi, kind[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < VC; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(fabsf(acc[j][i]) < __builtin_inff()) && !(fabsf(kind[j][i]) < __builtin_inff())) acc[j][i] = kind[j][i];
+    }
     // ---- the waves' parts: lane (g, n) holds channels VC (4 g + i) + j of query n
 #pragma unroll
     for (int i = 0; i < 4; ++i)

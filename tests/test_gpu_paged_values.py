@@ -70,3 +70,47 @@ def test_window_with_an_odd_token_of_little_weight(bad, T, S, at):
     got = window_attention(q.cuda(), k.cuda(), v.cuda(), 2)
     want, amp, big = op.attend(f64(q[0]).swapaxes(0, 1), f64(k[0]), f64(v[0]), np.ones(S, bool), S - T, 2)
     check_odd(got[0].transpose(0, 1), want, amp, big, S, dt, False)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("lens, H, G, D, page, per_more, window, sinks", [
+    ([1, 2, 33, 700], 2, 7, 128, 16, 1, None, 0),       # a workgroup to a unit
+    ([1, 40, 129], 1, 20, 80, 8, 1, None, 0),
+    ([1, 300, 2500], 2, 3, 64, 64, 1, None, 0),         # shares and a join
+    ([64, 2200], 1, 1, 128, 8, 1, 2100, 5),
+    ([90, 500], 2, 4, 40, 16, 1, 30, 3),
+])
+def test_decode_with_odd_tokens(dtype, lens, H, G, D, page, per_more, window, sinks):
+    """+inf, -inf, NaN and both infinities at tokens that are seen, each in a channel
+    of its own, at the ends and in the middle; one that is not seen."""
+    dt = DTYPES[dtype]
+    pool = Pool(lens, H, D, page, dt, seed=D + G, per_more=per_more)
+
+    def put(b, t, c, x):
+        pool.v[int(pool.table[b, t // page]), H - 1, t % page, c] = x
+    for b, n in enumerate(lens):
+        put(b, n - 1, 0, INF)
+        put(b, 0, 1, -INF)
+        put(b, n // 2, 2, NAN)
+        put(b, n - 1, 3, INF)
+        put(b, max(n - 2, 0), 3, -INF)
+        put(b, max(n - 20, 0), 4, -INF)
+    pool.cuda()
+    q = torch.randn(len(lens), H * G, D, device="cuda").to(dt)
+    got = paged_decode(q, pool.dk, pool.dv, pool.dtable, pool.dlens, G, window, sinks)
+    for b in range(len(lens)):
+        want, amp, big = pool.want(b, q[b:b + 1].cpu(), G, window, sinks)
+        check_odd(got[b], want, amp, big, 4096, dt, True)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_single_row_with_odd_tokens(dtype):
+    """window_attention of one new token, weights of 2^-50 among them."""
+    dt, S, g = DTYPES[dtype], 200, torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(1, h, n, 64, generator=g).to(dt) for h, n in ((4, 1), (2, S), (2, S)))
+    q[..., 0], k[..., 0] = 16.0, 0.0
+    k[0, :, 50, 0] = -20.0
+    v[0, 0, 50, 5], v[0, 1, S - 1, 6], v[0, 1, 50, 7] = INF, -INF, NAN
+    got = window_attention(q.cuda(), k.cuda(), v.cuda(), 2)
+    want, amp, big = op.attend(f64(q[0]).swapaxes(0, 1), f64(k[0]), f64(v[0]), np.ones(S, bool), S - 1, 2)
+    check_odd(got[0].transpose(0, 1), want, amp, big, S, dt, True)
