@@ -18,7 +18,8 @@
 // O^T = V^T P^T wants them: no weight moves between lanes.  Keys and Values
 // come straight from memory in 16-byte pieces; a lane's eight Value rows by
 // eight channels are turned by v_perm.  Weights enter the products as two
-// 16-bit terms (2^-16 of a weight in all).
+// 16-bit terms: bf16 leaves 2^-17 of a weight, fp16 2^-23 or, of a weight below
+// 2^-9 of the row's largest, 2^-32 of that.
 //
 // 32 requests of 16000 tokens, 32/8 heads of 128, fp16: 320 us, 6.6 TB/s, where a
 // plain read runs at 7.1 (one workgroup a CU 411 and with rows five steps ahead
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(64 * W, W == kPagedWaves ? per_cu(KF) : 2) void pag
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = rk::fast_exp2(__builtin_fmaf(sc[e >> 2][e & 3], a.scale_log2, -base));
+          x[e] = rk::fast_exp2(__builtin_fmaf(sc[e >> 2][e & 3], a.scale_log2, rk::kLift<DT> - base));
           l += x[e];
         }
         uint4 hi, lo;

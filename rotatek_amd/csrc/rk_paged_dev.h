@@ -3,6 +3,8 @@
 // different lengths is divided.
 #pragma once
 
+#include <type_traits>
+
 #include "rk_common.h"
 #include "rk_paged.h"
 
@@ -13,6 +15,12 @@ constexpr int kPagedWaves = 4;
 constexpr float kNone = -__builtin_inff();
 constexpr float kSlack = 8.f;    // log2 of what weights may grow to
 constexpr float kFar = 16384.f;  // a base of scores, in log2, that is rounded by 2^-11 at most
+
+// log2 of what all weights are raised by, which the quotient does not show.  fp16 ends
+// at 2^-24, so a weight loses up to 2^-25 whatever its size; weights are 2^kSlack at
+// most, so another 2^7 fit below 65504, and the loss is 2^-32 of the largest weight.
+template <class DT>
+constexpr float kLift = std::is_same<DT, F16>::value ? 7.f : 0.f;
 
 // 2^(x - m), and the maximum to subtract where nothing counted yet: -inf - -inf
 // would be NaN.

@@ -10,8 +10,8 @@
 // product) leaves each lane the scores of one row, eight of 16 tokens in the
 // order in which O^T = V^T P^T takes them, so that weights stay where they are;
 // V^T is read by the transposing LDS load.  Weights are rounded to the inputs'
-// type (2^-9 of each in bf16, as much as the output's own rounding); maxima,
-// sums and accumulators are 32-bit.
+// type (2^-8 of each in bf16 at most, as much as the output's own rounding; fp16
+// 2^-11, or 2^-32 of the row's largest); maxima, sums and accumulators are 32-bit.
 //
 // 8192 tokens, 32/8 heads of 128, window 4096, bf16: 405 us, 1.02 PFLOP/s (a large
 // matrix product 1.34).  Power bounds it: the matrix units are busy half of the
@@ -184,7 +184,7 @@ __device__ __forceinline__ void sum_row(const PagedArgs& a, int b, Queries qs, r
         s = __builtin_fmaf(lane_of(q1, d / 2 + e), DT::to_f32((uint16_t)(u[e] >> 16)), s);
       }
     }
-    if (there) w = rk::fast_exp2((s - base) * a.scale_log2);
+    if (there) w = rk::fast_exp2((s - base) * a.scale_log2 + rk::kLift<DT>);
     l += w;
     const uint64_t bits = __ballot(there);
     constexpr int kAhead = 8;
@@ -439,6 +439,7 @@ __global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(con
         for (int e = 0; e < 16; ++e) n[tb][e] -= base_of(m);
       base = 0.f;
     }
+    base -= rk::kLift<DT>;
   };
   // Weight k of a tile's 32 in this lane, pairs of them in the products' type.
   auto weight = [&](const f32x16 (&n)[2], float (&y)[32], uint32_t (&w)[16], int k) {
