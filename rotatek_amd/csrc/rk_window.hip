@@ -11,7 +11,9 @@
 // order in which O^T = V^T P^T takes them, so that weights stay where they are;
 // V^T is read by the transposing LDS load.  Weights are rounded to the inputs'
 // type (2^-8 of each in bf16 at most, as much as the output's own rounding; fp16
-// 2^-11, or 2^-32 of the row's largest); maxima, sums and accumulators are 32-bit.
+// 2^-11, or 2^-32 of the row's largest), and the sum that divides takes them rounded,
+// so Values that are alike come back as they are; maxima, sums and accumulators are
+// 32-bit.
 //
 // 8192 tokens, 32/8 heads of 128, window 4096, bf16: 405 us, 1.02 PFLOP/s (a large
 // matrix product 1.34).  Power bounds it: the matrix units are busy half of the
@@ -59,6 +61,18 @@ __device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(rk::bf16x8, a),
                                                    __builtin_bit_cast(rk::bf16x8, b), c, 0, 0, 0);
+}
+
+// l and two packed numbers, summed in 32 bits.
+template <class DT>
+__device__ __forceinline__ float add2(uint32_t w, float l) {
+  if constexpr (std::is_same<DT, rk::F16>::value) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), h2{1, 1}, l, false);
+  } else {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.f, (__bf16)1.f}, l, false);
+  }
 }
 
 // The values of this lane and of lane ^ 32, in some order.
@@ -444,10 +458,9 @@ __global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(con
   // Weight k of a tile's 32 in this lane, pairs of them in the products' type.
   auto weight = [&](const f32x16 (&n)[2], float (&y)[32], uint32_t (&w)[16], int k) {
     y[k] = rk::fast_exp2(__builtin_fmaf(n[k >> 4][k & 15], a.scale_log2, -base));
-    l += y[k];
     if (k & 1) {
       w[k >> 1] = DT::pack2(y[k - 1], y[k]);
-      asm volatile("" : "+v"(w[k >> 1]), "+v"(l));  // here, and not where it is used
+      asm volatile("" : "+v"(w[k >> 1]));  // here, and not where it is used
     }
   };
   auto value_at = [&](const char* sv, int g, int c) {  // 16 tokens by 32 channels
@@ -554,6 +567,10 @@ __global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(con
 #pragma unroll
           for (int k = 24; k < 32; ++k)
             if ((k - 24) * (3 * NB / 2) / 8 == j / 2) weight(s, y, w, k);
+          // (here the sums take no time; beside the scores' products 3 % of it)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (k * (kProducts / 2) / 16 == j / 2) l = add2<DT>(w[k], l);
           if (!kLast) {
 #pragma unroll
             for (int k = 0; k < 32; ++k)

@@ -5,7 +5,7 @@ import torch
 
 from oracle import paged as op
 from rotatek_amd.kernels import window_attention
-from tests.paged import f64
+from tests.paged import DTYPES, f64
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,19 @@ def test_small_weights_in_fp16(below, T):
     err = np.abs(f64(got[0].transpose(0, 1)) - want)
     bound = np.abs(want) * (rel + 2.0 ** -11 * (1 + rel)) + 2.0 ** -25
     assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("raised", [0.3, 1.2, 5.0, 7.1])
+def test_equal_values_come_back(dtype, raised):
+    """All Values alike: whatever the weights, the output is that Value, as what the
+    Values are multiplied by is what is summed.  64 tokens first, against which
+    the others' weights are 2^raised: no 16-bit number.  A sum of S tokens is off by
+    S 2^-24 before it is rounded, far below half a step."""
+    dt, S, T, H = DTYPES[dtype], 400, 256, 40       # (one part: the first tokens are everybody's)
+    q, k = torch.zeros(1, H, T, 64), torch.zeros(1, H, S, 64)
+    q[..., 0] = 8.0
+    k[0, :, 64:, 0] = raised * float(np.log(2.0))
+    v = (2.0 - torch.finfo(dt).eps * torch.arange(1, 65)).expand(1, H, S, 64).contiguous()
+    got = window_attention(q.to(dt).cuda(), k.to(dt).cuda(), v.to(dt).cuda(), 1)
+    assert torch.equal(got.cpu(), v[:, :, :1].to(dt).expand(1, H, T, 64))
