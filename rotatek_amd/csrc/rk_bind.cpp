@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/Dtype.h>
@@ -344,12 +345,17 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- paged cache
 
-// Whether autograd would record one of these.
+// Whether autograd would record one of these, or follow its tangent (which it does
+// without recording too).
 template <class... T>
 bool needs_grad(T... o) {
-  if (!c10::GradMode::is_enabled()) return false;
-  for (PyObject* x : {o...})
-    if (THPVariable_Check(x) && THPVariable_Unpack(x).requires_grad()) return true;
+  const bool records = c10::GradMode::is_enabled();
+  const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (PyObject* x : {o...}) {
+    if (!THPVariable_Check(x)) continue;
+    const at::Tensor& t = THPVariable_Unpack(x);
+    if ((records && t.requires_grad()) || (tangents && t._fw_grad(0).defined())) return true;
+  }
   return false;
 }
 

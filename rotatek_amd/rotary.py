@@ -32,9 +32,10 @@ def inverse_frequencies(channels: int, base: float = 10000.0, device="cuda") -> 
 
 
 def no_grad_only(what: str, status: int) -> None:
-    """Raise for a call whose inputs autograd would follow."""
+    """Raise for a call whose inputs autograd would follow, backward or forward."""
     if status == _lib.bind().NEEDS_GRAD:
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+        raise RuntimeError(f"{what} has no gradient: call it on detached tensors or, where none has a tangent, under "
+                           "torch.no_grad()")
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
