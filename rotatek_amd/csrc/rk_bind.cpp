@@ -359,6 +359,17 @@ bool needs_grad(T... o) {
   return false;
 }
 
+// Marks tensors that a call has written (None among them), for autograd, which may have
+// saved them.  Those of inference mode have no count.
+template <class... T>
+void written(T... o) {
+  for (PyObject* x : {o...}) {
+    if (!THPVariable_Check(x)) continue;
+    const at::Tensor& t = THPVariable_Unpack(x);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
+}
+
 // A new tensor, from the allocator of a given one: what at::empty does behind its two
 // dispatches (a rotation of one token's queries and Keys 7.1 us with them, 5.9 so).
 at::Tensor fresh(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
@@ -431,6 +442,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     st = g_entry.rotary(q.p, k.p, pos.p, freq.p, sections.n, sections.axes, interleaved, inverse, qo.p, ko.p, stream);
   }
   if (st) return status(st);
+  written(a[7], a[8]);
   PyObject* x = new_q.defined() ? THPVariable_Wrap(new_q) : Py_NewRef(a[7]);
   PyObject* y = !x ? nullptr : new_k.defined() ? THPVariable_Wrap(new_k) : Py_NewRef(a[8]);
   PyObject* pair = y ? PyTuple_Pack(2, x, y) : nullptr;
@@ -493,6 +505,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                               interleaved, stream);
   }
   if (st) return status(st);
+  written(a[2], a[3], a[8]);
   return new_q.defined() ? THPVariable_Wrap(new_q) : Py_NewRef(a[8]);
   END_HANDLE_TH_ERRORS
 }
@@ -527,6 +540,7 @@ PyObject* attend(PyObject* out_arg, const at::Tensor& q, bool single, int64_t de
     st = launch(out.p, scratch, bytes);
   }
   if (st) return status(st);
+  written(out_arg);
   return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(out_arg);
 }
 

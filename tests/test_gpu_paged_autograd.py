@@ -54,3 +54,28 @@ def test_tangents_are_refused(name):
                 call()
             setattr(s, x, plain)
     call()
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_what_is_written_is_marked(name):
+    """Autograd has to see that a tensor it saved has changed since."""
+    s = Step()
+    call, reads, writes = s.calls()[name]
+    before = {x: getattr(s, x)._version for x in set(reads.split()) | set(writes.split()) | {"table", "lens"}}
+    call()
+    for x, v in before.items():
+        assert (getattr(s, x)._version > v) == (x in writes.split()), x
+    w = torch.ones(3, 4, 64, device="cuda", requires_grad=True)
+    y = (w * s.out).sum()       # saves out
+    call()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_what_is_written_in_inference_mode():
+    with torch.inference_mode():
+        s = Step()
+        for call, _, _ in s.calls().values():
+            call()
+    for call, _, _ in s.calls().values():       # (tensors of that mode have no count)
+        call()
