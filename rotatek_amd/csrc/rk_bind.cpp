@@ -416,7 +416,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!counts("rotary", n, 10)) return nullptr;
   if (!THPVariable_Check(a[0])) return status(RK_ERR_ARG);
-  if (needs_grad(a[0], a[1], a[3])) return status(kNeedsGrad);
+  if (needs_grad(a[0], a[1], a[3], a[7], a[8])) return status(kNeedsGrad);
   const at::Tensor& t = THPVariable_Unpack(a[0]);
   const int64_t dev = t.get_device();
   Arg q, k, pos, freq, qo, ko;
@@ -475,7 +475,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!counts("paged_append", n, 14)) return nullptr;
   if (!THPVariable_Check(a[0])) return status(RK_ERR_ARG);
-  if (needs_grad(a[0], a[1], a[2], a[3], a[7], a[10])) return status(kNeedsGrad);
+  if (needs_grad(a[0], a[1], a[2], a[3], a[7], a[8], a[10])) return status(kNeedsGrad);
   const at::Tensor& t = THPVariable_Unpack(a[0]);
   const int64_t dev = t.get_device();
   Arg k, v, q, qo, pos, freq;
@@ -550,7 +550,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!counts("paged_attention", n, 11)) return nullptr;
   if (!THPVariable_Check(a[0])) return status(RK_ERR_ARG);
-  if (needs_grad(a[0], a[2], a[3])) return status(kNeedsGrad);
+  if (needs_grad(a[0], a[2], a[3], a[9])) return status(kNeedsGrad);
   const at::Tensor& t = THPVariable_Unpack(a[0]);
   const int64_t dev = t.get_device();
   Arg q;
@@ -579,7 +579,7 @@ PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!counts("window_attention", n, 9)) return nullptr;
   if (!THPVariable_Check(a[0])) return status(RK_ERR_ARG);
-  if (needs_grad(a[0], a[1], a[2])) return status(kNeedsGrad);
+  if (needs_grad(a[0], a[1], a[2], a[7])) return status(kNeedsGrad);
   const at::Tensor& t = THPVariable_Unpack(a[0]);
   const int64_t dev = t.get_device();
   Arg q, k, v;

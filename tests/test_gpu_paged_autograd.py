@@ -79,3 +79,17 @@ def test_what_is_written_in_inference_mode():
             call()
     for call, _, _ in s.calls().values():       # (tensors of that mode have no count)
         call()
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_outputs_that_want_a_gradient_are_refused(name):
+    s = Step()
+    call, _, writes = s.calls()[name]
+    for x in writes.split():
+        plain = getattr(s, x)
+        setattr(s, x, plain.detach().clone().requires_grad_())
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        setattr(s, x, plain)
