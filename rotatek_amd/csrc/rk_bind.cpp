@@ -70,6 +70,7 @@ int describe(const at::Tensor& t, int64_t device, rk_tensor* d, Use use) {
   const int32_t code = dtype_code(t.scalar_type());
   if (nd > 4) return RK_ERR_RANK;
   if (code < 0) return RK_ERR_DTYPE;
+  if (t.is_neg()) return RK_ERR_ARG;  // its memory holds the negatives (the caller words it)
   memset(d, 0, sizeof(*d));
   d->data = t.numel() == 0 ? nullptr : use == kWrite ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
   d->dtype = code;

@@ -117,6 +117,8 @@ def refused(what: str, status: int, index: int, *tensors) -> None:
     """Raise for a call that the host path answered with ``status``."""
     if status == _lib.bind().OTHER_DEVICE:
         same_device(what, index, *tensors)
+    if any(isinstance(t, torch.Tensor) and t.is_neg() for t in tensors):
+        raise ValueError(f"{what}: a tensor is a view that torch negates when it is read; call resolve_neg() on it first")
     _lib.check(status, what)
 
 
