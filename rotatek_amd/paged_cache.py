@@ -15,7 +15,8 @@ reference.
 ``begin`` counts on the host and copies table, lengths and starts to the device
 without waiting; ``append`` and ``attend`` work on the device alone, with
 buffers that never move, so a step's layers may be captured in a HIP graph and
-replayed behind a ``begin`` of the same counts.
+replayed behind a ``begin`` of the same counts (``begin`` and ``free`` themselves
+may not be captured).
 """
 from __future__ import annotations
 
@@ -77,6 +78,14 @@ class PagedCache(Cache):
         """Tokens that a request holds, the present step's among them."""
         return self._held[request]
 
+    def _outside_capture(self) -> None:
+        """A copy that is captured would be replayed from pinned memory that others
+        have by then."""
+        if self.table.is_cuda:
+            with torch.cuda.device(self.table.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("begin and free count on the host: call them outside a capture, ahead of a replay")
+
     def _put(self, to: torch.Tensor, values) -> None:
         """Copy to the device in the current stream's order, without waiting (the
         pinned copy is kept by torch's allocator until it has been read)."""
@@ -95,6 +104,7 @@ class PagedCache(Cache):
         found for them.  Returns their sum N.  Where a request would pass
         ``max_tokens`` (ValueError) or pages run out (RuntimeError), nothing
         changes."""
+        self._outside_capture()
         counts = [int(n) for n in counts]
         if len(counts) != self.requests or min(counts) < 0:
             raise ValueError(f"counts must hold {self.requests} numbers from 0 on")
@@ -121,6 +131,7 @@ class PagedCache(Cache):
 
     def free(self, request: int) -> None:
         """A request is done: its pages go to the next ones that ask."""
+        self._outside_capture()
         self._free.extend(reversed(self._own[request]))
         self._own[request] = []
         self._held[request] = 0
