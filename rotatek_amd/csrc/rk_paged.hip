@@ -658,15 +658,24 @@ int make_plan(const Call& c, int cus, PagedArgs* a, Plan* p) {
     const int64_t units = p->B * H * cdiv(c.groups, kRows), longest = pieces_of_longest(a->map.cap, a->window, a->sinks);
     if (units * (cdiv(cap, kBlock) + 1) >= (INT64_C(1) << 31)) return RK_ERR_SHAPE;
     if (units >= rk::kMostGroups || cdiv(p->rows, kPagedWaves) >= rk::kMostGroups) return RK_ERR_SHAPE;
-    // A unit to a workgroup, or all of them shared out evenly with a join: the first
-    // saves about 4 us and takes its pieces on the fullest CU, 2.1 us each, the second
-    // all CUs' average of them, 2.6 us each (128 channels; 1.3 and 1.6 with 64), less
-    // where requests differ.  32 queries on 8 KV heads of 128, shared and alone: 1
-    // request of 380 tokens 10.6 and 9.7 us, of 760 12.4 and 16.8; 16 of 760 19.8 and
-    // 18.5, of 1000 20.6 and 22.7; 28 of 1500 40.5 and 34.0; 40 of 500 27.5 and 23.5, of
-    // 1500 51.2 and 56.2; 64 of up to 2000 74.6 and 69.1.
+    // A unit to a workgroup, or all of them shared out evenly with a join.  The first
+    // saves the join, its records and the search for shares, 5 us.  A piece of the
+    // longest unit takes it 1.85 us with eight waves, where each CU has one unit at most,
+    // and 4.3 with four, where units begin at once (128 channels; 1.1 and 2.6 with 64):
+    // the memory's latency, a step of a wave each.  All CUs together read a piece of as
+    // many units as CUs in 2.5 us (1.4), which bounds either form and is all that the
+    // shared one takes.  32 query heads on 8 KV heads of 128, alone and shared: 4 requests
+    // of 364 tokens 11.6 and 12.5 us, of 1004 21.2 and 12.9; 16 of 876 20.3 and 20.3; 32 of
+    // 2028 46.0 and 49.5; 40 of 492 23.5 and 27.3, of 2028 73.9 and 61.2.  Heads of 64: 4
+    // of 1004 13.4 and 10.7, 16 of them 14.6 and 16.7, 40 of them 24.7 and 25.2.  Where
+    // requests differ the first gains: 96 of 10 to 1004 47 and 58.
+    const bool narrow = D <= 64;
+    const double share = (double)units / cus;
+    const double all = (narrow ? 1.4 : 2.5) * share;
+    const double own = share <= 1 ? (narrow ? 1.1 : 1.85)
+                                  : (narrow ? 2.6 : 4.3) * std::max(1.0, share / per_cu(narrow ? 2 : 4));
+    const bool alone = longest <= kMostAlone && (double)longest * (std::max(own, all) - all) <= 5.0;
     const int64_t fullest = cdiv(units, cus);
-    const bool alone = longest <= kMostAlone && longest * (40 * (fullest * cus - units) + 3 * cus) <= 140 * cus;
     a->direct = !alone ? 0 : fullest > 1 ? kPagedWaves : kAloneWaves;
     a->workers = (int32_t)(a->direct ? units : std::max<int64_t>(
         std::min<int64_t>(per_cu(D <= 64 ? 2 : 4) * (int64_t)cus, units * longest), 1));
