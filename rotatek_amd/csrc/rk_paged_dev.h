@@ -60,7 +60,7 @@ __device__ __forceinline__ int wave_sum_to(int n) {
 }
 
 struct Found {
-  int b, before;  // a request, and the pieces before it
+  int b, before;  // a request (below zero: none), and the pieces before it
 };
 
 // Work of requests 0 .. B - 1, count(b) pieces each, laid end to end: the sum, and
@@ -106,12 +106,13 @@ struct Line {
     return {__builtin_ctzll(__ballot((mine > low) & (rank == left))), low};
   }
 
-  // `at` below the sum.
+  // `at` below the sum; none where counts of more than 64 requests add up to 2^31 or more.
   __device__ __forceinline__ Found find(int at) {
     if (B <= 64) {
       const int b = __builtin_ctzll(__ballot(at < to));
       return {b, __builtin_amdgcn_readlane(to - mine, b)};
     }
+    if (threadIdx.x == 0) s_found[0] = -1;  // (the scan's barriers stand between this and the next)
     int before = 0;
     for (int b0 = 0; b0 < B; b0 += kPagedThreads) {
       const int b = b0 + threadIdx.x;

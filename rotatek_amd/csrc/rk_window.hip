@@ -274,6 +274,7 @@ __global__ __launch_bounds__(kPagedThreads, waves_of(KC)) void window_kernel(con
     const bool across = a.round && a.map.B <= 64;
     const rk::Found f = across ? line.across(slot) : line.find(slot);
     b = f.b;
+    if (b < 0) return;  // starts that do not ascend may count each token for every request
     tile = count(b) - 1 - (across ? f.before : slot - f.before);
   } else {
     const int tiles = (a.T * a.G + kRows - 1) / kRows;
