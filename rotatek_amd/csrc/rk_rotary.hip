@@ -15,7 +15,8 @@
 // vector of pairs (16 bytes from either half of the head) of one head.  In an
 // append the same pass writes Keys and Values to their pages.
 //
-// The bytes bound it: 1.6 GB of video heads in 300 us, 5.3 TB/s, as a copy.
+// The bytes bound it: 1.6 GB of video heads in 300 us, 5.3 TB/s; a plain copy reaches
+// 6.3 at best (a piece of 16 bytes a thread), 5.8 with four pieces.
 #include <hip/hip_runtime.h>
 #include <string.h>
 
@@ -381,7 +382,7 @@ int launch(RotaryArgs& a, int dtype, int e, void* stream) {
   a.head[kQ] = a.head[kK] = divisor_of(per, std::max(heads[kQ], heads[kK]) * per);
   a.head[kV] = divisor_of(half, heads[kV] * half);
   // Stores of whole lines leave the caches to others: 3 x 32 heads x 2304 tokens of
-  // 80 channels in fp32 (142 MB in all) take 27 us (a copy of as much 26), 39 with
+  // 80 channels in fp32 (142 MB in all) take 26 us (a copy of as much 23 at best), 39 with
   // ordinary stores; 17 prompts of up to 4097 tokens into pages 177 and
   // 183 (with places found behind the angles).  Lines
   // that two stores share have to meet in a cache: 23205 tokens of 96 heads of 96

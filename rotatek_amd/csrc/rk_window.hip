@@ -15,11 +15,12 @@
 // so Values that are alike come back as they are; maxima, sums and accumulators are
 // 32-bit.
 //
-// 8192 tokens, 32/8 heads of 128, window 4096, bf16: 405 us, 1.02 PFLOP/s (a large
-// matrix product 1.34).  Power bounds it: the matrix units are busy half of the
-// cycles, and the clock falls from 2.35 GHz to 1.75; waits for loads, barriers or
-// LDS taken away leave the time as it is, the loads of tiles themselves 353.  64
-// rows a wave, which read LDS half as often, leave one wave a SIMD: 487.
+// 8192 tokens, 32/8 heads of 128, window 4096, bf16: 398 to 428 us by card, 0.96 to
+// 1.03 PFLOP/s (a large matrix product 1.34).  Power bounds it: the matrix units are
+// busy half of the cycles, and the clock falls from 2.35 GHz to 1.72; waits for loads,
+// barriers or LDS taken away leave the time as it is, the loads of tiles themselves
+// take off an eighth.  64 rows a wave, which read LDS half as often, leave one wave a
+// SIMD: a fifth longer.
 #include <hip/hip_runtime.h>
 #include <limits.h>
 

@@ -47,7 +47,8 @@ def append_pages(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor
     ascending: request b's tokens are ``starts[b] .. starts[b + 1] - 1``; None:
     one token each), or [B, H_kv, T, D], T tokens each.  ``k_pages`` /
     ``v_pages`` [pages, H_kv, page, D] of the same type (fp16, bf16 or fp32; any
-    strides; page a power of two from 8 on), ``table`` device int32 [B, per],
+    strides; page a power of two from 8 on; ``kernels``' attention takes fp16 and
+    bf16 pages alone), ``table`` device int32 [B, per],
     ``lens`` device int32 [B], new tokens counted.
 
     With ``positions`` ([axes, N] or [axes, B, T]) the Keys turn as in

@@ -17,6 +17,11 @@ without waiting; ``append`` and ``attend`` work on the device alone, with
 buffers that never move, so a step's layers may be captured in a HIP graph and
 replayed behind a ``begin`` of the same counts (``begin`` and ``free`` themselves
 may not be captured).
+
+``attend`` is planned for requests of ``max_tokens`` (see ``kernels.paged_attention``),
+and a ``begin`` that adds pages writes the table's rows anew: 0.8 ms where 32 requests
+of up to 32768 tokens come to a page's end at once, 13 of up to 10^6, 0.03 where none
+does.  So ``max_tokens`` should be no more than is needed.
 """
 from __future__ import annotations
 
