@@ -645,7 +645,8 @@ int rk_paged_append(const rk_tensor* k_new, const rk_tensor* v_new, const rk_pag
 /* Attention of new tokens over pages.  Request b's i-th new token of n stands
  * at position p = lens[b] - n + i and sees the tokens j <= p with j > p - window
  * (window 0: all of them) or j < sinks:
- *   out = sum w v / sum w,  w = exp(q . k / sqrt(D) - max),  0 where it sees none
+ *   out = sum w v / sum w,  w = exp(q . k / sqrt(D) - max),  0 where it sees none or
+ * all its scores are -inf
  * (a Value that is not finite counts so for those that see it and for no other; where
  * its weight is below 2^-126 of the largest, an infinity may give a NaN).
  * q, out [B,Hq,D] with starts NULL (one new token each: decode), or [N,Hq,D]

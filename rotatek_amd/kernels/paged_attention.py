@@ -3,9 +3,9 @@
 The queries of a request's new tokens stand at its last positions; the one at
 position p sees the tokens j <= p, with ``window`` only the last ``window`` of
 them (p among them) and the first ``sinks`` of the request.  Scores are
-q . k / sqrt(D); a query that sees nothing gives zeros.  No counterpart in the
-reference, whose prefill attention is a library's and whose caches are one
-tensor a layer.
+q . k / sqrt(D); a query that sees nothing, or whose scores are all -inf, gives
+zeros.  No counterpart in the reference, whose prefill attention is a library's and
+whose caches are one tensor a layer.
 
 fp16 and bf16, D a multiple of 8 up to 128.  Rows of Keys and Values lie in
 whole 16-byte pieces (unit last stride, other strides multiples of 8 elements,
